@@ -182,6 +182,68 @@ int k3d_moe_experts(float *out, const int *idx, const float *wt, const float *x,
                     int act, float b1, float b2, int prec, void *ws, size_t ws_bytes,
                     int *perm_out, int *offsets_out, int *drops_out, void *stream);
 
+/* ---- the operators of the layer around the routed experts -------------------------------
+ * No counterpart in the reference as single calls. Strides are in elements; nothing is allocated,
+ * nothing synchronises, and the calls can be captured in a HIP graph. The stream belongs to the
+ * current device. */
+
+/* Element types of the tensors below. */
+enum { K3D_F32 = 0, K3D_BF16 = 1 };
+
+/* Dense product with bias, activation and residual:
+ *   y[t][o] = act(sum_k x[t][k] W[o][k] + bias[o]) + res[t][o],   t < T, o < out, k < in.
+ * W bf16 [out][ldw], x [T][ldx] of x_type, bias fp32 [out] or NULL, res [T][ldr] of y_type or NULL
+ * (it may be y itself, with its stride), y [T][ldy] of y_type; rows and pointers at any alignment of
+ * their elements. fp32 x counts in full: cut into three bf16 terms that hold all 24 bits of it
+ * (an infinite weight then gives NaN where it meets a finite x). Sums, bias, activation and
+ * residual are formed in fp32 and rounded once to y_type. Which kernel runs, and with it the order
+ * of a sum, goes by the shape, the types and the alignment; a call's bits repeat. in, ldx and ldw up to
+ * K3D_LINEAR_MAX_LD. y must not overlap x, W, bias or ws. */
+enum { K3D_ACT_NONE = 0, K3D_ACT_RELU = 1, K3D_ACT_SILU = 2, K3D_ACT_GELU = 3 /* erf */, K3D_ACT_GELU_TANH = 4 };
+#define K3D_LINEAR_MAX_LD (1 << 22)
+size_t k3d_linear_ws(int T, int in, int out, int x_type);
+int k3d_linear(void *y, int y_type, long ldy, const void *x, int x_type, long ldx, int T, const uint16_t *W,
+               long ldw, int in, int out, const float *bias, int act, const void *res, long ldr, void *ws,
+               size_t ws_bytes, void *stream);
+
+/* Routing from logits [T][ld] (of `type`; k3d_linear's, say): idx/wt [T][topk], the form that
+ * k3d_moe_experts takes. Per token:
+ *   score[e]  = sigmoid(logit) (K3D_SCORE_SIGMOID) or softmax over the token's experts (K3D_SCORE_SOFTMAX);
+ *   choice[e] = score[e] + bias[e] (bias fp32 [n_experts] or NULL);
+ *   groups    : n_groups runs of n_experts / n_groups experts; a group's value is the sum of its
+ *               group_top (1 or 2) largest choices; the top_groups groups of largest value stay;
+ *   idx       : the topk largest choices among them, descending; wt their scores, divided by their
+ *               sum if renorm and topk > 1 (as k3_router does), times routed_scale.
+ * Equal values go to the lower index, of groups and of experts. Scores, choices, sums and
+ * comparisons are formed in 64 bits, wt is rounded once. A logit of -inf or NaN, or a choice of -inf or
+ * NaN, is an expert that cannot be taken (a masked one; a NaN logit is left out of the softmax too); a
+ * group has the value of those it can give, and one without any is never taken; where fewer than topk
+ * are left, the last slots get idx -1 and wt 0 (k3d_moe_experts skips them), and weights
+ * that sum to 0 are 0. Logits of +inf share a softmax among themselves.
+ * 1 <= n_experts <= 2048, n_groups <= 64 and a divisor of it, topk <= 64 and at most the experts of
+ * top_groups groups. */
+enum { K3D_SCORE_SIGMOID = 0, K3D_SCORE_SOFTMAX = 1 };
+int k3d_route(int *idx, float *wt, const void *logits, int type, long ld, int T, int n_experts, const float *bias,
+              int score, int n_groups, int top_groups, int group_top, int topk, int renorm, float routed_scale,
+              void *stream);
+
+/* RMSNorm of every query and key head, and the position rotation behind it. Head h of token t
+ * is the `dim` elements at q + t * ldq + h * hsq (k likewise); it goes to qo / ko in the same form,
+ * which may be the input itself (same pointer and strides), else must not overlap it.
+ *   u = v / sqrt(mean(v^2) + eps) * w     (w: qw or kw, fp32 [dim], or NULL for ones)
+ *   rotated over u[rot_off .. rot_off + rot): the pairs (i, i + rot/2) (K3D_ROT_HALVES) or
+ *   (2i, 2i + 1) (K3D_ROT_INTERLEAVED) turn by the angle pos[t] * inv_freq[i], i < rot/2, and are
+ *   multiplied by rot_scale; the rest of u stays as it is.
+ * Angles are formed and reduced in 64 bits (inv_freq fp64), so far positions lose nothing; the rest is fp32,
+ * rounded once. A token of negative position is padding: its rows of qo and ko are left as they were.
+ * hq or hk may be 0. 1 <= dim <= 1024; rot even (0: no rotation, pos may then be NULL: no padding);
+ * eps >= 0. */
+enum { K3D_ROT_HALVES = 0, K3D_ROT_INTERLEAVED = 1 };
+int k3d_qk_norm_rope(void *qo, long ldqo, long hsqo, void *ko, long ldko, long hsko, const void *q, long ldq, long hsq,
+                     const void *k, long ldk, long hsk, int type, int T, int hq, int hk, int dim, const float *qw,
+                     const float *kw, float eps, const int *pos, const double *inv_freq, int rot, int rot_off,
+                     int pairs, float rot_scale, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

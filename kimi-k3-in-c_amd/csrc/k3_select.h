@@ -10,6 +10,7 @@
 
 #include "k3_common.h"
 #include "k3_expf.h"
+#include "k3_wave.h"
 
 namespace {
 
@@ -137,30 +138,6 @@ __device__ __forceinline__ uint32_t choice_order(float v)
 {
     const uint32_t b = __float_as_uint(v == 0.0f ? 0.0f : v);
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-}
-
-/* 32-bit max / min of the wave by DPP, the same in every lane: pairs, quads (quad_perm),
- * 8 (row half mirror), 16 (row mirror), then rows 0-1 and 2-3 (row_bcast15 into rows 1,
- * 3) and rows 0-3 (row_bcast31 into rows 2, 3), so lane 63 holds the result. */
-/* (rows outside RM read the identity of the operation, so each step is one DPP max/min) */
-template <int CTRL, int RM, uint32_t ID>
-__device__ __forceinline__ uint32_t dpp_u32(uint32_t v)
-{
-    return (uint32_t)__builtin_amdgcn_update_dpp((int)ID, (int)v, CTRL, RM, 0xf, false);
-}
-
-template <bool MAX>
-__device__ __forceinline__ uint32_t wave_reduce_u32(uint32_t v)
-{
-    constexpr uint32_t ID = MAX ? 0u : 0xffffffffu;
-    auto op = [](uint32_t a, uint32_t b) { return MAX ? (a > b ? a : b) : (a < b ? a : b); };
-    v = op(v, dpp_u32<0xB1, 0xf, ID>(v));      /* quad_perm [1,0,3,2] */
-    v = op(v, dpp_u32<0x4E, 0xf, ID>(v));      /* quad_perm [2,3,0,1] */
-    v = op(v, dpp_u32<0x141, 0xf, ID>(v));     /* row_half_mirror */
-    v = op(v, dpp_u32<0x140, 0xf, ID>(v));     /* row_mirror */
-    v = op(v, dpp_u32<0x142, 0xa, ID>(v));     /* row_bcast15 */
-    v = op(v, dpp_u32<0x143, 0xc, ID>(v));     /* row_bcast31 */
-    return __builtin_amdgcn_readlane(v, 63);
 }
 
 /* Selection key (order-preserving bits of the choice) << 32 | ~expert: the largest key is

@@ -328,6 +328,49 @@ int k3k_rmsnorm(float *y, const float *x, const float *w, int n, int rows, float
 int k3k_axpy_rows(float *out, const float *add, size_t n, void *stream); /* out += add */
 int k3k_scale(float *out, const float *in, float s, size_t n, void *stream);
 
+/* ---- the operators around the routed experts (k3_linear.hip, k3_groute.hip, k3_heads.hip) ---- */
+/* The arguments of k3d_linear (k3_dev.h), checked; ws: k3k_linear_ws bytes. */
+typedef struct {
+    void *y;
+    const void *x, *res;
+    const uint16_t *W;
+    const float *bias;
+    long ldy, ldx, ldw, ldr;
+    int y_type, x_type, T, in, out, act;
+    void *ws;
+    size_t ws_bytes;
+} K3kLinear;
+size_t k3k_linear_ws(int T, int in, int out, int x_type);
+int k3k_linear(const K3kLinear *a, void *stream);
+
+/* The arguments of k3d_route, checked. */
+typedef struct {
+    int *idx;
+    float *wt;
+    const void *logits;
+    const float *bias;
+    long ld;
+    int type, T, n, score, n_groups, top_groups, group_top, topk, renorm;
+    float scale;
+} K3kRoute;
+int k3k_route(const K3kRoute *a, void *stream);
+
+/* The arguments of k3d_qk_norm_rope, checked; views[0]: queries, views[1]: keys. */
+typedef struct {
+    struct {
+        void *out;
+        const void *in;
+        const float *w;
+        long ldo, hso, ld, hs;
+        int heads;
+    } v[2];
+    int type, T, dim, rot, rot_off, pairs;
+    float eps, rot_scale;
+    const int *pos;
+    const double *freq;
+} K3kHeads;
+int k3k_heads(const K3kHeads *a, void *stream);
+
 /* ---- the allocation-free workspace (k3_static.hip) --------------------------------- */
 /* Looks up, once per device, the device address of the library's static workspace for the
  * current device (called by k3d_init). */

@@ -22,6 +22,10 @@ K3_WF32, K3_WBF16, K3_WI8 = 0, 1, 2
 K3_ACT_SITU, K3_ACT_SILU = 0, 1
 K3_MAX_TOPK = 64
 K3D_LAYOUT_ROWS, K3D_LAYOUT_TILED = 0, 1
+K3D_F32, K3D_BF16 = 0, 1
+K3D_ACT_NONE, K3D_ACT_RELU, K3D_ACT_SILU, K3D_ACT_GELU, K3D_ACT_GELU_TANH = 0, 1, 2, 3, 4
+K3D_SCORE_SIGMOID, K3D_SCORE_SOFTMAX = 0, 1
+K3D_ROT_HALVES, K3D_ROT_INTERLEAVED = 0, 1
 STAGES = ("begin", "router", "gather", "gateup", "down", "combine", "gemv", "shared")
 
 _lib = None
@@ -147,6 +151,11 @@ def _declare(L):
     d("k3d_shared_expert", I, P, I, P, I, P, P, P, I, I, I, F, F, I, P, SZ, P)
     d("k3d_mxfp4_tiled_size", I, I, I, P, P)
     d("k3d_mxfp4_tile", I, P, P, P, P, I, I, P)
+    LG = C.c_long
+    d("k3d_linear_ws", SZ, I, I, I, I)
+    d("k3d_linear", I, P, I, LG, P, I, LG, I, P, LG, I, I, P, I, P, LG, P, SZ, P)
+    d("k3d_route", I, P, P, P, I, LG, I, I, P, I, I, I, I, I, I, F, P)
+    d("k3d_qk_norm_rope", I, P, LG, LG, P, LG, LG, P, LG, LG, P, LG, LG, I, I, I, I, I, P, P, F, P, P, I, I, I, F, P)
     # generator
     d("k3g_u64", C.c_uint64, C.c_uint64, C.c_uint64)
     d("k3g_bytes", None, P, SZ, C.c_uint64)
