@@ -7,8 +7,14 @@
 #include "k3_dev.h"
 #include "k3k.h"
 
+#include <type_traits>
+
 namespace {
 
+constexpr int LIN_KS = 64;                      /* columns of a tile kernel's step */
+constexpr uint32_t LIN_OOB = 0x80000000u;       /* a buffer offset past any descriptor used here */
+
+/* ---- epilogue ------------------------------------------------------------------------ */
 __device__ __forceinline__ float act_of(float v, int act)
 {
     switch (act) {
@@ -20,65 +26,710 @@ __device__ __forceinline__ float act_of(float v, int act)
     }
 }
 
-__device__ __forceinline__ void put(const K3kLinear &a, int t, int o, float v)
+/* outputs o .. o + 3 of token t (those below a.out), from their sums; b: their bias */
+__device__ __forceinline__ void put4(const K3kLinear &a, int t, int o, float4 acc, const float (&b)[4])
 {
-    if (a.bias) v += a.bias[o];
-    v = act_of(v, a.act);
-    const size_t i = (size_t)t * a.ldy + o, r = (size_t)t * a.ldr + o;
+    if (t >= a.T || o >= a.out) return;
+    const size_t yi = (size_t)t * a.ldy + o, ri = (size_t)t * a.ldr + o;
+    const int n = min(4, a.out - o);
+    float v[4] = {acc.x + b[0], acc.y + b[1], acc.z + b[2], acc.w + b[3]};
+    if (a.act)
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = act_of(v[i], a.act);
     if (a.y_type == K3D_F32) {
-        if (a.res) v += ((const float *)a.res)[r];
-        ((float *)a.y)[i] = v;
+        float *y = (float *)a.y + yi;
+        const float *r = (const float *)a.res + ri;
+        if (a.res) {
+            if (n == 4 && ((uintptr_t)r & 15) == 0) {
+                const float4 q = *reinterpret_cast<const float4 *>(r);
+                v[0] += q.x, v[1] += q.y, v[2] += q.z, v[3] += q.w;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (i < n) v[i] += r[i];
+            }
+        }
+        if (n == 4 && ((uintptr_t)y & 15) == 0) {
+            *reinterpret_cast<float4 *>(y) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (i < n) y[i] = v[i];
+        }
     } else {
-        if (a.res) v += k3_bf16_to_f32(((const uint16_t *)a.res)[r]);
-        ((uint16_t *)a.y)[i] = k3_bf16_rne(v);
+        uint16_t *y = (uint16_t *)a.y + yi;
+        const uint16_t *r = (const uint16_t *)a.res + ri;
+        if (a.res) {
+            if (n == 4 && ((uintptr_t)r & 7) == 0) {
+                const uint2 q = *reinterpret_cast<const uint2 *>(r);
+                v[0] += __uint_as_float(q.x << 16), v[1] += __uint_as_float(q.x & 0xffff0000u);
+                v[2] += __uint_as_float(q.y << 16), v[3] += __uint_as_float(q.y & 0xffff0000u);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (i < n) v[i] += k3_bf16_to_f32(r[i]);
+            }
+        }
+        uint16_t h[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) h[i] = k3_bf16_rne(v[i]);
+        if (n == 4 && ((uintptr_t)y & 7) == 0) {
+            *reinterpret_cast<uint2 *>(y) = make_uint2((uint32_t)h[0] | (uint32_t)h[1] << 16, (uint32_t)h[2] | (uint32_t)h[3] << 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (i < n) y[i] = h[i];
+        }
     }
 }
 
-/* A wave per 16 rows of W and 16 tokens, operands element by element from memory. */
-__global__ __launch_bounds__(256) void linear_kernel(K3kLinear a)
+__device__ __forceinline__ void bias4(const K3kLinear &a, int o, float (&b)[4])
 {
+#pragma unroll
+    for (int i = 0; i < 4; i++) b[i] = a.bias && o + i < a.out ? a.bias[o + i] : 0.0f;
+}
+
+/* ---- operands ------------------------------------------------------------------------ */
+/* eight floats as three bf16 terms by truncation, x = h + m + l: each keeps the next 8 bits of the
+ * significand, so the three hold all 24 and every product with a weight is exact. Infinities and
+ * NaN are in the first term alone. */
+__device__ __forceinline__ void cut3(const float (&f)[8], uint32_t (&h)[4], uint32_t (&m)[4], uint32_t (&l)[4])
+{
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const uint32_t u = __float_as_uint(f[i]);
+        const bool fin = (u & 0x7f800000u) != 0x7f800000u;
+        const uint32_t uh = (u & 0xffff0000u) | (f[i] != f[i] ? 0x00400000u : 0u);
+        const float r1 = fin ? f[i] - __uint_as_float(uh) : 0.0f;
+        const uint32_t um = __float_as_uint(r1) & 0xffff0000u;
+        const uint32_t ul = __float_as_uint(r1 - __uint_as_float(um));
+        if (i & 1) {
+            h[i / 2] |= uh, m[i / 2] |= um, l[i / 2] |= ul & 0xffff0000u;
+        } else {
+            h[i / 2] = uh >> 16, m[i / 2] = um >> 16, l[i / 2] = ul >> 16;
+        }
+    }
+}
+
+__device__ __forceinline__ k3_bf16x8 as_frag(const uint32_t (&w)[4])
+{
+    return k3_as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
+}
+
+/* eight bf16 from an address aligned to them only (one load: the hardware takes any alignment) */
+__device__ __forceinline__ uint4 load8_any(const uint16_t *p)
+{
+    uint4 v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+}
+
+/* the first n of eight bf16 (n < 1: none), zeros behind */
+__device__ __forceinline__ uint4 load8_upto(const uint16_t *p, int n)
+{
+    uint64_t lo = 0, hi = 0;
+#pragma unroll 1
+    for (int i = min(n, 8) - 1; i >= 0; i--) {
+        hi = (hi << 16) | (lo >> 48);
+        lo = (lo << 16) | p[i];
+    }
+    return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
+}
+
+/* ---- few tokens: weights straight into registers ---------------------------------------- */
+/* A workgroup takes 16 RF rows of W and 16 NT tokens; its waves share the columns, each a run of
+ * 32-column steps, and their sums meet in LDS. A lane's weights (row lane % 16, columns 8 (lane / 16)
+ * ..+8 of a step) are an MFMA operand as loaded. Rows and tokens past the ends repeat the last one; only
+ * the last step can pass the end of a row (guarded, zeros behind). */
+template <int RF, int NT, int U, int MAXW, bool XF32, bool ALIGNED>
+__global__ __launch_bounds__(64 * MAXW) void lin_stream_kernel(K3kLinear a, int nw)
+{
+    extern __shared__ float4 part[];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, r16 = lane & 15, g = lane >> 4;
-    const int o0 = (blockIdx.x * 4 + wv) * 16, t0 = blockIdx.y * 16;
-    const int o = o0 + r16, t = t0 + r16;
-    k3_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int k0 = 0; k0 < a.in; k0 += 32) {
-        k3_bf16x8 w, x[3];
+    const int o0 = blockIdx.x * 16 * RF, t0 = blockIdx.y * 16 * NT;
+    const int steps = (a.in + 31) / 32, per = (steps + nw - 1) / nw;
+    const int s0 = wv * per, n = min(per, steps - s0);          /* (n < 1: nothing for this wave) */
+
+    const uint16_t *wp[RF];
+    const char *xp[NT];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int k = k0 + 8 * g + i;
-            const bool in = k < a.in;
-            const uint16_t wb = in && o < a.out ? a.W[(size_t)o * a.ldw + k] : (uint16_t)0;
-            float v = 0.0f;
-            if (in && t < a.T)
-                v = a.x_type == K3D_F32 ? ((const float *)a.x)[(size_t)t * a.ldx + k]
-                                        : k3_bf16_to_f32(((const uint16_t *)a.x)[(size_t)t * a.ldx + k]);
-            w[i] = __builtin_bit_cast(__bf16, wb);
-            const bool fin = (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u;
-            float r = v;
+    for (int i = 0; i < RF; i++) wp[i] = a.W + (size_t)min(o0 + 16 * i + r16, a.out - 1) * a.ldw + 8 * g;
 #pragma unroll
-            for (int s = 0; s < 3; s++) {
-                uint32_t u = __float_as_uint(r) & 0xffff0000u;
-                if (r != r) u |= 0x00400000u;
-                x[s][i] = __builtin_bit_cast(__bf16, (uint16_t)(u >> 16));
-                r = fin ? r - __uint_as_float(u) : 0.0f;
+    for (int j = 0; j < NT; j++)
+        xp[j] = (const char *)a.x + ((size_t)min(t0 + 16 * j + r16, a.T - 1) * a.ldx + 8 * g) * (XF32 ? 4 : 2);
+
+    k3_f32x4 acc[RF][NT];
+#pragma unroll
+    for (int i = 0; i < RF; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) acc[i][j] = k3_f32x4{0.f, 0.f, 0.f, 0.f};
+
+    struct Slot {
+        uint4 w[RF], x[NT][XF32 ? 2 : 1];
+    };
+    auto load = [&](Slot &s, int step) {
+        const int k = step * 32;
+#pragma unroll
+        for (int i = 0; i < RF; i++) s.w[i] = ALIGNED ? k3_ldg16(wp[i] + k) : load8_any(wp[i] + k);
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            const char *p = xp[j] + (size_t)k * (XF32 ? 4 : 2);
+            if (XF32) {
+                if (ALIGNED) {
+                    s.x[j][0] = k3_ldg16(p);
+                    s.x[j][XF32 ? 1 : 0] = k3_ldg16(p + 16);
+                } else {
+                    __builtin_memcpy(&s.x[j][0], p, 16);
+                    __builtin_memcpy(&s.x[j][XF32 ? 1 : 0], p + 16, 16);
+                }
+            } else {
+                s.x[j][0] = ALIGNED ? k3_ldg16(p) : load8_any((const uint16_t *)p);
             }
         }
+    };
+    /* the step that passes the end of the rows */
+    auto load_last = [&](Slot &s, int step) {
+        const int k = step * 32, left = a.in - k - 8 * g;
 #pragma unroll
-        for (int s = 2; s >= 0; s--) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x[s], acc, 0, 0, 0);
+        for (int i = 0; i < RF; i++) s.w[i] = load8_upto(wp[i] + k, left);
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            const char *p = xp[j] + (size_t)k * (XF32 ? 4 : 2);
+            if (XF32) {
+                float f[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) f[i] = i < left ? ((const float *)p)[i] : 0.0f;
+                __builtin_memcpy(&s.x[j][0], f, 16);
+                __builtin_memcpy(&s.x[j][XF32 ? 1 : 0], f + 4, 16);
+            } else {
+                s.x[j][0] = load8_upto((const uint16_t *)p, left);
+            }
+        }
+    };
+    auto use = [&](const Slot &s) {
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            if (XF32) {
+                float f[8];
+                uint32_t h[4], m[4], l[4];
+                __builtin_memcpy(f, &s.x[j][0], 16);
+                __builtin_memcpy(f + 4, &s.x[j][XF32 ? 1 : 0], 16);
+                cut3(f, h, m, l);
+                const k3_bf16x8 xl = as_frag(l), xm = as_frag(m), xh = as_frag(h);
+#pragma unroll
+                for (int i = 0; i < RF; i++) {
+                    const k3_bf16x8 w = k3_as_bf16x8(s.w[i]);
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, xl, acc[i][j], 0, 0, 0);
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, xm, acc[i][j], 0, 0, 0);
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, xh, acc[i][j], 0, 0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < RF; i++)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k3_as_bf16x8(s.w[i]), k3_as_bf16x8(s.x[j][0]), acc[i][j], 0, 0, 0);
+            }
+        }
+    };
+
+    /* whole steps through a ring of U slots (past the end the last one is requested again and goes unused) */
+    const int whole = min(n, a.in / 32 - s0);
+    if (whole > 0) {
+        Slot ring[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) load(ring[u], s0 + min(u, whole - 1));
+        int s = 0;
+        for (; s + U <= whole; s += U)
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                use(ring[u]);
+                load(ring[u], s0 + min(s + u + U, whole - 1));
+            }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (s + u < whole) use(ring[u]);
+    }
+    if (n > 0 && whole < n) {
+        Slot s;
+        load_last(s, s0 + n - 1);
+        use(s);
+    }
+
+#pragma unroll
+    for (int i = 0; i < RF; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+            part[(wv * RF * NT + i * NT + j) * 64 + lane] = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+    __syncthreads();
+    for (int q = wv; q < RF * NT; q += nw) {
+        const int o = o0 + 16 * (q / NT) + 4 * g;
+        float b[4];
+        bias4(a, o, b);
+        float4 s = part[q * 64 + lane];
+        for (int w = 1; w < nw; w++) {
+            const float4 v = part[(w * RF * NT + q) * 64 + lane];
+            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+        }
+        put4(a, t0 + 16 * (q % NT) + r16, o, s, b);
+    }
+}
+
+/* ---- x for the tile kernel: terms and padding ------------------------------------------- */
+/* xs[t][terms][kp] bf16, kp a multiple of 64: fp32 x as l, m, h; bf16 x as it is. Where the rows' length is
+ * no multiple of 64, the last block of 64 columns holds the rest with zeros behind it (over 0), or columns
+ * in - 64 .. in with zeros in place of those that the block before it holds (over 64 - in % 64). */
+template <bool XF32>
+__global__ __launch_bounds__(256) void lin_pack_kernel(uint16_t *xs, const void *x, long ldx, int T, int in, int kp, int over)
+{
+    const int per = kp / 8;
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    const int t = (int)(i / per), kb = (int)(i % per) * 8;
+    if (t >= T) return;
+    const int last = kp - LIN_KS, k = kb >= last ? kb - over : kb;      /* the first of the eight columns */
+    const bool whole = k >= (kb >= last ? last : 0) && k + 8 <= in;
+    if (XF32) {
+        const float *p = (const float *)x + (size_t)t * ldx;
+        float f[8];
+        if (whole && ((uintptr_t)(p + k) & 15) == 0) {
+            __builtin_memcpy(f, __builtin_assume_aligned(p + k, 16), 32);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) f[j] = k + j < in && (kb < last || k + j >= last) ? p[k + j] : 0.0f;
+        }
+        uint32_t h[4], m[4], l[4];
+        cut3(f, h, m, l);
+        uint16_t *q = xs + (size_t)t * 3 * kp + kb;
+        *reinterpret_cast<uint4 *>(q) = make_uint4(l[0], l[1], l[2], l[3]);
+        *reinterpret_cast<uint4 *>(q + kp) = make_uint4(m[0], m[1], m[2], m[3]);
+        *reinterpret_cast<uint4 *>(q + 2 * (size_t)kp) = make_uint4(h[0], h[1], h[2], h[3]);
+    } else {
+        const uint16_t *p = (const uint16_t *)x + (size_t)t * ldx;
+        uint4 v;
+        if (whole) {
+            v = load8_any(p + k);
+        } else {
+            uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (k + j < in && (kb < last || k + j >= last)) w[j / 2] |= (uint32_t)p[k + j] << (16 * (j & 1));
+            v = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        *reinterpret_cast<uint4 *>(xs + (size_t)t * kp + kb) = v;
+    }
+}
+
+/* ---- many tokens: tiles through LDS -------------------------------------------------------- */
+typedef struct {
+    K3kLinear a;
+    const uint16_t *x;      /* bf16 rows, 16-byte aligned, ldx % 8 == 0 */
+    long ldx;
+    int xcols;              /* columns of x: in, or all terms' padded ones */
+    int nks, steps;         /* steps of one term, of all */
+    int nt, no;             /* tiles over tokens and outputs */
+    int nsl, per;           /* slices of the steps, steps of one */
+    float *part;            /* [nsl][T][out] sums of the slices (nsl > 1) */
+} LinTile;
+
+/* Which token and output tile workgroup b takes. The dispatcher deals workgroups to the XCDs in turn; each XCD
+ * gets a run of tiles of its own, in blocks of 8 token tiles by all... */
+__device__ __forceinline__ void tile_of(const LinTile &p, int b, int &tt, int &to, int &sl)
+{
+    const int tiles = p.nt * p.no, all = tiles * p.nsl;
+    const int full = all / K3_NXCD * K3_NXCD;
+    int i = b;
+    if (b < full) i = (b % K3_NXCD) * (all / K3_NXCD) + b / K3_NXCD;
+    sl = i / tiles;
+    i -= sl * tiles;
+    constexpr int GT = 8;
+    const int blk = GT * p.no, q = i / blk, h = min(GT, p.nt - q * GT), r = i - q * blk;
+    to = r / h;
+    tt = q * GT + r % h;
+}
+
+template <int BT, int BO, int WT, int WO, int NST, bool WREG>
+__global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
+{
+    constexpr int NW = WT * WO, FT = BT / WT / 16, FO = BO / WO / 16;
+    constexpr int XD = BT / 8 / NW, WD = WREG ? 0 : BO / 8 / NW, DN = XD + WD;      /* DMAs of a wave per step */
+    constexpr int WR = WREG ? BO * 8 / (64 * NW) : 1;                                /* 16-byte pieces of W per thread */
+    constexpr int FG = FO % 4 == 0 ? 4 : FO % 2 == 0 ? 2 : 1;       /* fragments that share a run of outputs */
+    static_assert(XD >= 1 && (WREG || WD >= 1) && NST >= 2 && NST <= 4, "tile");
+    constexpr int SZ = (BT + BO) * LIN_KS;
+    __shared__ __attribute__((aligned(1024))) uint16_t S0[SZ], S1[SZ], S2[NST > 2 ? SZ : 8], S3[NST > 3 ? SZ : 8];
+
+    const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wt = wv % WT, wo = wv / WT;
+    int tt, to, sl;
+    tile_of(p, blockIdx.x, tt, to, sl);
+    const int t0 = tt * BT, o0 = to * BO;
+    const int k0 = sl * p.per, n = min(p.per, p.steps - k0);
+
+    /* Row swizzle of the LDS tiles: the 16-byte column c of row r lies in slot c ^ sw(r), so that the 16 rows of a
+     * fragment read (one column) fall on all 64 banks. x: fragment rows are consecutive. W: the
+     * rows of fragment q of FG are 4 FG j + 4 q + e (j: lane group, e: register of the result), so that a
+     * lane's results of FG fragments are 4 FG consecutive outputs. */
+    auto swx = [](int r) { return (r >> 1) & 7; };
+    auto sww = [](int r) { return FG == 1 ? (r >> 1) & 7 : (((r / (4 * FG)) & 3) << 1) | ((r >> 1) & 1); };
+
+    const int tn = min(BT, p.a.T - t0), on = min(BO, p.a.out - o0);
+    const k3_rsrc rx = k3_make_rsrc(p.x + (size_t)t0 * p.ldx, (uint32_t)(((size_t)(tn - 1) * p.ldx + p.xcols) * 2));
+    const k3_rsrc rw = k3_make_rsrc(p.a.W + (size_t)o0 * p.a.ldw, (uint32_t)(((size_t)(on - 1) * p.a.ldw + p.a.in) * 2));
+    /* DMA i of wave wv fills LDS rows 8 (NW i + wv) ..+8, a lane a 16-byte slot. Rows past the last one repeat
+     * it (their sums go unused), so every read lies in its matrix. */
+    uint32_t xo[XD], wo_[WD > 0 ? WD : 1];
+#pragma unroll
+    for (int i = 0; i < XD; i++) {
+        const int r = (i * NW + wv) * 8 + lane / 8;
+        xo[i] = (uint32_t)min(r, tn - 1) * (uint32_t)(p.ldx * 2) + ((lane & 7) ^ swx(r)) * 16;
     }
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-        if (t < a.T && o0 + 4 * g + i < a.out) put(a, t, o0 + 4 * g + i, acc[i]);
+    for (int i = 0; i < WD; i++) {
+        const int r = (i * NW + wv) * 8 + lane / 8;
+        wo_[i] = (uint32_t)min(r, on - 1) * (uint32_t)(p.a.ldw * 2) + ((lane & 7) ^ sww(r)) * 16;
+    }
+    auto buf_of = [&](auto slot) -> uint16_t * {
+        constexpr int S = decltype(slot)::value;
+        if constexpr (S == 0) return S0;
+        else if constexpr (S == 1) return S1;
+        else if constexpr (S == 2) return S2;
+        else return S3;
+    };
+    /* Stages are requested in order: step `xk` of x, which is column block `wk` of W (of a term), the last one
+     * of a row from where its 64 columns end with the row. Past the slice: zeros, so that every step requests
+     * as much and none is under a branch. */
+    int xk = k0, wk = k0 % p.nks;
+    const int kend = k0 + n;
+    auto issue = [&](auto slot) {
+        uint16_t *const b = buf_of(slot);
+        const uint32_t none = xk < kend ? 0u : LIN_OOB;
+        const uint32_t xs = (uint32_t)xk * (LIN_KS * 2), ws = (uint32_t)(wk == p.nks - 1 ? p.a.in - LIN_KS : wk * LIN_KS) * 2;
+#pragma unroll
+        for (int i = 0; i < XD; i++) k3_dma16(rx, b + (i * NW + wv) * 8 * LIN_KS, xo[i] | none, xs);
+#pragma unroll
+        for (int i = 0; i < WD; i++) k3_dma16(rw, b + (BT + (i * NW + wv) * 8) * LIN_KS, wo_[i] | none, ws);
+        xk++;
+        if (++wk == p.nks) wk = 0;
+    };
+    /* weights at any alignment: through registers */
+    uint4 wr[WR];
+    int gk = k0 % p.nks;
+    auto wload = [&]() {
+#pragma unroll
+        for (int i = 0; i < WR; i++) {
+            const int c = tid + 64 * NW * i, r = c >> 3, k = gk * LIN_KS + (c & 7) * 8, left = p.a.in - k;
+            const uint16_t *q = p.a.W + (size_t)(o0 + min(r, on - 1)) * p.a.ldw + k;
+            wr[i] = left >= 8 ? load8_any(q) : load8_upto(q, left);
+        }
+        if (++gk == p.nks) gk = 0;
+    };
+    auto wstore = [&](auto slot) {
+        uint16_t *const b = buf_of(slot);
+#pragma unroll
+        for (int i = 0; i < WR; i++) {
+            const int c = tid + 64 * NW * i, r = c >> 3;
+            *reinterpret_cast<uint4 *>(b + (BT + r) * LIN_KS + ((c & 7) ^ sww(r)) * 8) = wr[i];
+        }
+    };
+
+    /* where the lane's fragments lie: x row 16 j + r16 of the wave's tokens, W row as above (their swizzles are
+     * the same for every fragment); column 8 g of a half step */
+    const int xr = wt * (BT / WT) + r16, wr0 = wo * (BO / WO) + (r16 >> 2) * 4 * FG + (r16 & 3);
+    int xa[2], wa[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        xa[h] = xr * LIN_KS + (((4 * h + g) ^ swx(xr)) * 8);
+        wa[h] = (BT + wr0) * LIN_KS + (((4 * h + g) ^ sww(wr0)) * 8);
+    }
+    auto read = [&](const uint16_t *b, int half, k3_bf16x8 (&xf)[FT], k3_bf16x8 (&wf)[FO]) {
+#pragma unroll
+        for (int i = 0; i < FO; i++)
+            wf[i] = k3_as_bf16x8(*reinterpret_cast<const uint4 *>(b + wa[half] + ((i / FG) * 16 * FG + (i % FG) * 4) * LIN_KS));
+#pragma unroll
+        for (int j = 0; j < FT; j++) xf[j] = k3_as_bf16x8(*reinterpret_cast<const uint4 *>(b + xa[half] + 16 * j * LIN_KS));
+    };
+    k3_f32x4 acc[FO][FT];
+#pragma unroll
+    for (int i = 0; i < FO; i++)
+#pragma unroll
+        for (int j = 0; j < FT; j++) acc[i][j] = k3_f32x4{0.f, 0.f, 0.f, 0.f};
+    auto mma = [&](const k3_bf16x8 (&xf)[FT], const k3_bf16x8 (&wf)[FO]) {
+#pragma unroll
+        for (int i = 0; i < FO; i++)
+#pragma unroll
+            for (int j = 0; j < FT; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[i], xf[j], acc[i][j], 0, 0, 0);
+    };
+    /* issue order of a half: a fragment read of the other half behind each of the first MFMAs */
+    constexpr int NRD = FO + FT, NMF = FO * FT, GAP = NMF / NRD > 0 ? NMF / NRD : 1;
+    auto pin = [&]() {
+#pragma unroll
+        for (int i = 0; i < NRD; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, GAP, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, NMF, 0);
+    };
+    /* all but the last NST - 2 stages' requests (with weights through registers: all) */
+    constexpr int WAITN = WREG ? 0 : DN * (NST - 2);
+    constexpr int WAIT_STAGE = (WAITN & 15) | (7 << 4) | (15 << 8) | ((WAITN >> 4) << 14);
+    constexpr int WAIT_VM0 = (7 << 4) | (15 << 8);
+    k3_bf16x8 fx0[FT], fw0[FO], fx1[FT], fw1[FO];
+
+    /* Step k: its second half is read while the first is multiplied; then every wave is past its reads of
+     * buffer k % NST and stage k + 1 has landed (one barrier), so stage k + NST goes into that buffer and the
+     * next step's first half is read while the second is multiplied. */
+    auto step = [&](auto slot) {
+        constexpr int S = decltype(slot)::value;
+        uint16_t *const b = buf_of(slot);
+        uint16_t *const nb = buf_of(std::integral_constant<int, (S + 1) % NST>{});
+        read(b, 1, fx1, fw1);
+        mma(fx0, fw0);
+        pin();
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(WAIT_STAGE);
+        __syncthreads();
+        if (WREG) wstore(slot);
+        issue(slot);
+        if (WREG) wload();
+        __builtin_amdgcn_sched_barrier(0);
+        read(nb, 0, fx0, fw0);          /* (past the last step: what lies there, unused) */
+        mma(fx1, fw1);
+        pin();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto start = [&](auto slot) {
+        constexpr int S = decltype(slot)::value;
+        if constexpr (S < NST) {
+            if (WREG) {
+                wload();
+                wstore(slot);
+            }
+            issue(slot);
+        }
+    };
+    using C0 = std::integral_constant<int, 0>;
+    using C1 = std::integral_constant<int, 1>;
+    using C2 = std::integral_constant<int, 2>;
+    using C3 = std::integral_constant<int, 3>;
+    start(C0{});
+    start(C1{});
+    if constexpr (NST > 2) start(C2{});
+    if constexpr (NST > 3) start(C3{});
+    if (WREG) wload();
+    __builtin_amdgcn_s_waitcnt(WAIT_VM0);
+    __syncthreads();
+    read(S0, 0, fx0, fw0);
+    /* (whole rounds in the loop: a way out of its middle costs copies of the accumulators) */
+    int k = 0;
+    for (; k + NST <= n; k += NST) {
+        step(C0{});
+        step(C1{});
+        if constexpr (NST > 2) step(C2{});
+        if constexpr (NST > 3) step(C3{});
+    }
+    if (k < n) step(C0{});
+    if constexpr (NST > 2)
+        if (k + 1 < n) step(C1{});
+    if constexpr (NST > 3)
+        if (k + 2 < n) step(C2{});
+    __builtin_amdgcn_s_waitcnt(WAIT_VM0);      /* the last requests land before LDS is used again */
+
+    /* A lane holds token r16 of each token fragment and 4 FG consecutive outputs of FG fragments. The sums go
+     * through LDS (the stage buffers, a region per wave, JR token fragments at a time; 16-byte column c of row r
+     * in c ^ (r % 16)), so that a wave writes whole rows of its outputs, and the epilogue's code is there once. */
+    constexpr int WOUT = BO / WO, C = WOUT / 4, JR = FT <= 4 ? FT : FT / 2, RB = JR * 16 * WOUT * 4;
+    constexpr int PER = SZ * 2 / RB;        /* regions per stage buffer */
+    static_assert(PER >= 1 && PER * 2 >= NW && 64 % C == 0, "epilogue regions");
+    uint16_t *stage = S0;
+    if (PER < NW) stage = wv / PER == 0 ? S0 : S1;
+    float4 *const reg = reinterpret_cast<float4 *>(stage + (wv % PER) * (RB / 2));
+    const int c = lane % C, o = o0 + wo * WOUT + 4 * c;
+    float b[4];
+    bias4(p.a, p.nsl > 1 ? p.a.out : o, b);
+    __syncthreads();
+#pragma unroll
+    for (int j0 = 0; j0 < FT; j0 += JR) {
+#pragma unroll
+        for (int j = 0; j < JR; j++)
+#pragma unroll
+            for (int i = 0; i < FO; i++) {
+                const int oc = (i / FG) * 4 * FG + g * FG + i % FG, r = 16 * j + r16;
+                reg[r * C + (oc ^ (r16 & (C - 1)))] = make_float4(acc[i][j0 + j][0], acc[i][j0 + j][1], acc[i][j0 + j][2], acc[i][j0 + j][3]);
+            }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 2
+        for (int r = lane / C; r < 16 * JR; r += 64 / C) {
+            const float4 v = reg[r * C + (c ^ (r & 15 & (C - 1)))];
+            const int t = t0 + wt * (BT / WT) + 16 * j0 + r;
+            if (p.nsl == 1) {
+                put4(p.a, t, o, v, b);
+            } else if (t < p.a.T && o < p.a.out) {
+                float *q = p.part + ((size_t)sl * p.a.T + t) * p.a.out + o;
+                if (o + 4 <= p.a.out && ((uintptr_t)q & 15) == 0) {
+                    *reinterpret_cast<float4 *>(q) = v;
+                } else {
+                    const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (o + i < p.a.out) q[i] = e[i];
+                }
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+/* the slices' sums, in slice order, and the epilogue */
+__global__ __launch_bounds__(256) void lin_join_kernel(K3kLinear a, const float *part, int nsl)
+{
+    const int per = (a.out + 3) / 4;
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    const int t = (int)(i / per), o = (int)(i % per) * 4;
+    if (t >= a.T) return;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    const bool whole = a.out % 4 == 0;
+    for (int s = 0; s < nsl; s++) {
+        const float *q = part + ((size_t)s * a.T + t) * a.out + o;
+        if (whole) {
+            const float4 f = *reinterpret_cast<const float4 *>(q);
+            v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (o + e < a.out) v[e] += q[e];
+        }
+    }
+    float b[4];
+    bias4(a, o, b);
+    put4(a, t, o, make_float4(v[0], v[1], v[2], v[3]), b);
+}
+
+/* ---- launches -------------------------------------------------------------------------------- */
+constexpr int LIN_STREAM_T = 64;            /* tokens up to which the weights go straight into registers */
+constexpr int LIN_MAX_SLICES = 16;
+constexpr size_t LIN_PART_CAP = (size_t)32 << 20;
+
+int kpad(int in) { return (in + LIN_KS - 1) / LIN_KS * LIN_KS; }
+
+size_t pack_bytes(int T, int in, int x_type)
+{
+    return ((size_t)T * kpad(in) * (x_type == K3D_F32 ? 3 : 1) * 2 + 255) / 256 * 256;
+}
+
+/* the slices' sums of any batch up to T: a call takes slices only as far as they fit this */
+size_t part_bytes(int T, int out)
+{
+    const size_t most = (size_t)LIN_MAX_SLICES * T * out * 4;
+    return most < LIN_PART_CAP ? most : LIN_PART_CAP;
+}
+
+template <int RF, int NT, int U, int MAXW, bool XF32>
+void stream_go(const K3kLinear *a, int nw, bool aligned, hipStream_t st)
+{
+    const dim3 grid((a->out + 16 * RF - 1) / (16 * RF), (a->T + 16 * NT - 1) / (16 * NT));
+    const size_t lds = (size_t)nw * RF * NT * 1024;
+    if (aligned) lin_stream_kernel<RF, NT, U, MAXW, XF32, true><<<grid, 64 * nw, lds, st>>>(*a, nw);
+    else lin_stream_kernel<RF, NT, U, MAXW, XF32, false><<<grid, 64 * nw, lds, st>>>(*a, nw);
+}
+
+template <bool XF32>
+void stream_pick(const K3kLinear *a, bool aligned, hipStream_t st)
+{
+    const int nt = (a->T + 15) / 16, rf = nt == 1 ? 1 : 2;
+    const long wgs = (a->out + 16 * rf - 1) / (16 * rf);
+    const int steps = (a->in + 31) / 32, cus = k3k_cu_count();
+    /* waves that share a workgroup's columns: enough for the chip, each with a few steps */
+    int nw = 4;
+    if (wgs < 2 * cus) nw = 8;
+    if (wgs < cus / 2 && nt == 1) nw = 16;
+    while (nw > 1 && steps < 2 * nw) nw /= 2;
+    if (nt == 1) stream_go<1, 1, XF32 ? 4 : 8, 16, XF32>(a, nw, aligned, st);
+    else if (nt == 2) stream_go<2, 2, 4, 8, XF32>(a, nw, aligned, st);
+    else if (nt == 3) stream_go<2, 3, XF32 ? 2 : 4, 8, XF32>(a, nw, aligned, st);
+    else stream_go<2, 4, XF32 ? 2 : 4, 8, XF32>(a, nw, aligned, st);
+}
+
+template <int BT, int BO, int WT, int WO, int NST, bool WREG>
+void tile_go(LinTile *p, hipStream_t st)
+{
+    lin_tile_kernel<BT, BO, WT, WO, NST, WREG><<<p->nt * p->no * p->nsl, 64 * WT * WO, 0, st>>>(*p);
 }
 
 }  // namespace
 
-extern "C" size_t k3k_linear_ws(int T, int in, int out, int x_type) { return 0; }
+extern "C" size_t k3k_linear_ws(int T, int in, int out, int x_type)
+{
+    if (T <= LIN_STREAM_T) return 0;
+    return pack_bytes(T, in, x_type) + part_bytes(T, out);
+}
 
 extern "C" int k3k_linear(const K3kLinear *a, void *stream)
 {
-    const dim3 grid((a->out + 63) / 64, (a->T + 15) / 16);
-    linear_kernel<<<grid, 256, 0, (hipStream_t)stream>>>(*a);
+    hipStream_t st = (hipStream_t)stream;
+    const bool w16 = ((uintptr_t)a->W & 15) == 0 && a->ldw % 8 == 0;
+    if (a->T <= LIN_STREAM_T) {
+        const int xe = a->x_type == K3D_F32 ? 4 : 8;
+        const bool al = w16 && ((uintptr_t)a->x & 15) == 0 && a->ldx % xe == 0;
+        if (a->x_type == K3D_F32) stream_pick<true>(a, al, st);
+        else stream_pick<false>(a, al, st);
+        K3K_LAUNCH_CHECK("linear");
+        return 0;
+    }
+    LinTile p;
+    p.a = *a;
+    p.nks = (a->in + LIN_KS - 1) / LIN_KS;
+    p.steps = p.nks;
+    /* weights by DMA, or, at other alignments and in rows shorter than a step, through registers */
+    const bool dma = w16 && a->in % 8 == 0 && a->in >= LIN_KS;
+    const int kp = kpad(a->in);
+    if (a->x_type == K3D_F32 || ((uintptr_t)a->x & 15) || a->ldx % 8 || a->in % LIN_KS) {
+        const int f32 = a->x_type == K3D_F32, over = dma ? kp - a->in : 0;
+        const size_t n = (size_t)a->T * (kp / 8);
+        const unsigned grid = (unsigned)((n + 255) / 256);
+        if (f32) lin_pack_kernel<true><<<grid, 256, 0, st>>>((uint16_t *)a->ws, a->x, a->ldx, a->T, a->in, kp, over);
+        else lin_pack_kernel<false><<<grid, 256, 0, st>>>((uint16_t *)a->ws, a->x, a->ldx, a->T, a->in, kp, over);
+        K3K_LAUNCH_CHECK("linear: pack");
+        p.x = (const uint16_t *)a->ws;
+        p.steps *= f32 ? 3 : 1;
+        p.ldx = p.xcols = p.steps * LIN_KS;
+    } else {
+        p.x = (const uint16_t *)a->x;
+        p.ldx = a->ldx;
+        p.xcols = a->in;
+    }
+    p.part = (float *)((char *)a->ws + pack_bytes(a->T, a->in, a->x_type));
+    const long cus = k3k_cu_count();
+    /* the tile shape, and slices of the columns where the tiles cannot fill the chip */
+    const long t256 = (long)((a->T + 255) / 256) * ((a->out + 255) / 256);
+    const long t128 = (long)((a->T + 127) / 128) * ((a->out + 127) / 128);
+    const int shape = dma && t256 >= cus * 3 / 4 ? 256 : t128 >= cus ? 128 : 64;
+    p.nt = (a->T + shape - 1) / shape;
+    p.no = (a->out + shape - 1) / shape;
+    const long tiles = (long)p.nt * p.no;
+    int nsl = 1;
+    if (shape == 64) {
+        nsl = (int)(2 * cus / tiles);
+        const size_t cap = part_bytes(a->T, a->out) / ((size_t)a->T * a->out * 4);
+        if (nsl > p.steps / 4) nsl = p.steps / 4;
+        if (nsl > LIN_MAX_SLICES) nsl = LIN_MAX_SLICES;
+        if ((size_t)nsl > cap) nsl = (int)cap;
+        if (nsl < 1) nsl = 1;
+    }
+    p.per = (p.steps + nsl - 1) / nsl;
+    p.nsl = (p.steps + p.per - 1) / p.per;
+    if (shape == 256) {
+        tile_go<256, 256, 2, 4, 2, false>(&p, st);
+    } else if (shape == 128) {
+        if (dma) tile_go<128, 128, 2, 2, 2, false>(&p, st);
+        else tile_go<128, 128, 2, 2, 2, true>(&p, st);
+    } else {
+        if (dma) tile_go<64, 64, 2, 2, 4, false>(&p, st);
+        else tile_go<64, 64, 2, 2, 4, true>(&p, st);
+    }
     K3K_LAUNCH_CHECK("linear");
+    if (p.nsl > 1) {
+        const size_t n = (size_t)a->T * ((a->out + 3) / 4);
+        lin_join_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(*a, p.part, p.nsl);
+        K3K_LAUNCH_CHECK("linear: join");
+    }
     return 0;
 }
