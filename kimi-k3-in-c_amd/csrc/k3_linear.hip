@@ -12,6 +12,7 @@
 namespace {
 
 constexpr int LIN_KS = 64;                      /* columns of a tile kernel's step */
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));     /* (a load of uint4 loses what tells LDS arrays apart) */
 constexpr uint32_t LIN_OOB = 0x80000000u;       /* a buffer offset past any descriptor used here */
 
 /* ---- epilogue ------------------------------------------------------------------------ */
@@ -270,6 +271,173 @@ __global__ __launch_bounds__(64 * MAXW) void lin_stream_kernel(K3kLinear a, int 
             s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
         }
         put4(a, t0 + 16 * (q % NT) + r16, o, s, b);
+    }
+}
+
+/* ---- few tokens: a ring of LDS stages per wave ---------------------------------------------- */
+/* A workgroup takes 16 RW rows of W and all tokens (8 XD of them at most); its NW waves share the columns in
+ * runs of 64-column stages. Each wave fills a ring of NST stages of its own by DMA (8 lanes read a row's
+ * 128 contiguous bytes; the operand layout itself, read from memory, has 16 lanes in a row on 16 rows
+ * and a CU then takes in 10 bytes a cycle) and waits for its own requests alone, so there is no barrier until the
+ * waves' sums meet. x takes part as bf16 or, cut into its three terms as it is read, fp32. */
+template <int RW, int XD, int NW, int NST, bool XF32>
+__global__ __launch_bounds__(64 * NW) void lin_skinny_kernel(K3kLinear a)
+{
+    constexpr int NT = (XD + 1) / 2, XB = XF32 ? 2 : 1;         /* token fragments; 128-byte pieces of a row of x */
+    constexpr int WD = 2 * RW, DN = WD + XD * XB;               /* DMAs of a stage */
+    constexpr int STG = (WD + XD * XB) * 512;                   /* elements of a wave's stage */
+    static_assert(RW * NT * 512 <= STG, "the sums fit the wave's part of a stage");
+    __shared__ __attribute__((aligned(1024))) uint16_t S0[STG * NW], S1[STG * NW], S2[NST > 2 ? STG * NW : 8], S3[NST > 3 ? STG * NW : 8];
+    const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int o0 = blockIdx.x * 16 * RW;
+    const int nks = (a.in + LIN_KS - 1) / LIN_KS, k0 = (int)((long)nks * wv / NW), k1 = (int)((long)nks * (wv + 1) / NW);
+    const int on = min(16 * RW, a.out - o0);
+
+    /* 16-byte column c of an LDS row r lies in slot c ^ (r / 2 % 8): the rows of a fragment fall on all banks */
+    const k3_rsrc rw = k3_make_rsrc(a.W + (size_t)o0 * a.ldw, (uint32_t)(((size_t)(on - 1) * a.ldw + a.in) * 2));
+    const k3_rsrc rx = k3_make_rsrc(a.x, (uint32_t)(((size_t)(a.T - 1) * a.ldx + a.in) * (XF32 ? 4 : 2)));
+    uint32_t wo[WD], xo[XD];
+#pragma unroll
+    for (int i = 0; i < WD; i++) {
+        const int r = 8 * i + lane / 8;
+        wo[i] = (uint32_t)min(r, on - 1) * (uint32_t)(a.ldw * 2) + ((lane & 7) ^ ((r >> 1) & 7)) * 16;
+    }
+#pragma unroll
+    for (int i = 0; i < XD; i++) {
+        const int r = 8 * i + lane / 8;
+        xo[i] = (uint32_t)min(r, a.T - 1) * (uint32_t)(a.ldx * (XF32 ? 4 : 2)) + ((lane & 7) ^ ((r >> 1) & 7)) * 16;
+    }
+    auto buf_of = [&](auto slot) -> uint16_t * {
+        constexpr int S = decltype(slot)::value;
+        uint16_t *b;
+        if constexpr (S == 0) b = S0;
+        else if constexpr (S == 1) b = S1;
+        else if constexpr (S == 2) b = S2;
+        else b = S3;
+        return b + wv * STG;
+    };
+    /* the stage of column block xk; the last block of a row ends with it (columns of the block before come
+     * again, see `over`); past the wave's run: zeros, so that every stage requests as much */
+    int xk = k0;
+    auto issue = [&](auto slot) {
+        uint16_t *const b = buf_of(slot);
+        const uint32_t none = xk < k1 ? 0u : LIN_OOB;
+        const uint32_t c = xk == nks - 1 ? a.in - LIN_KS : xk * LIN_KS;
+#pragma unroll
+        for (int i = 0; i < WD; i++) k3_dma16(rw, b + i * 512, wo[i] | none, c * 2);
+#pragma unroll
+        for (int h = 0; h < XB; h++)
+#pragma unroll
+            for (int i = 0; i < XD; i++) k3_dma16(rx, b + (WD + h * XD + i) * 512, xo[i] | none, c * (XF32 ? 4 : 2) + h * 128);
+        xk++;
+    };
+    k3_f32x4 acc[RW][NT];
+#pragma unroll
+    for (int i = 0; i < RW; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) acc[i][j] = k3_f32x4{0.f, 0.f, 0.f, 0.f};
+    const int sw = (r16 >> 1) & 7, over = nks * LIN_KS - a.in;
+    constexpr int WAITN = DN * (NST - 1);
+    constexpr int WAIT_STAGE = (WAITN & 15) | (7 << 4) | (15 << 8) | ((WAITN >> 4) << 14);
+    constexpr int WAIT_LGKM0 = 15 | (7 << 4) | (0 << 8) | (3 << 14);
+    static_assert(WAITN < 64, "requests in flight");
+    int rk = k0;
+    auto step = [&](auto slot) {
+        const uint16_t *const b = buf_of(slot);
+        __builtin_amdgcn_s_waitcnt(WAIT_STAGE);
+        __builtin_amdgcn_sched_barrier(0);
+        u32x4 wf[2][RW], xf[2][NT][XB];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+#pragma unroll
+            for (int i = 0; i < RW; i++) wf[h][i] = *reinterpret_cast<const u32x4 *>(b + (16 * i + r16) * 64 + ((4 * h + g) ^ sw) * 8);
+            /* (a last fragment of 8 tokens: its upper lanes repeat the lower ones') */
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                const int r = 16 * j + (XD % 2 && j == NT - 1 ? r16 & 7 : r16), s = (r >> 1) & 7;
+                const uint16_t *q = b + (WD * 8 + r) * 64;
+                if constexpr (XF32) {      /* columns 8 g.. of half h: 16-byte pieces 2 g, 2 g + 1 of its 128 bytes */
+                    xf[h][j][0] = *reinterpret_cast<const u32x4 *>(q + h * XD * 512 + ((2 * g) ^ s) * 8);
+                    xf[h][j][1] = *reinterpret_cast<const u32x4 *>(q + h * XD * 512 + ((2 * g + 1) ^ s) * 8);
+                } else {
+                    xf[h][j][0] = *reinterpret_cast<const u32x4 *>(q + ((4 * h + g) ^ s) * 8);
+                }
+            }
+        }
+        __builtin_amdgcn_s_waitcnt(WAIT_LGKM0);
+        __builtin_amdgcn_sched_barrier(0);
+        issue(slot);
+        __builtin_amdgcn_sched_barrier(0);
+        const int skip = rk++ == nks - 1 ? over : 0;
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                const bool zero = 32 * h + 8 * g < skip;
+                if constexpr (XF32) {
+                    float f[8];
+                    uint32_t t[3][4];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) f[e] = zero ? 0.0f : __uint_as_float(xf[h][j][e / 4][e % 4]);
+                    cut3(f, t[2], t[1], t[0]);
+#pragma unroll
+                    for (int q = 0; q < 3; q++)
+#pragma unroll
+                        for (int i = 0; i < RW; i++)
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(k3_bf16x8, wf[h][i]), as_frag(t[q]), acc[i][j], 0, 0, 0);
+                } else {
+                    u32x4 v = xf[h][j][0];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[e] = zero ? 0u : v[e];
+#pragma unroll
+                    for (int i = 0; i < RW; i++)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(k3_bf16x8, wf[h][i]), __builtin_bit_cast(k3_bf16x8, v), acc[i][j], 0, 0, 0);
+                }
+            }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    using C0 = std::integral_constant<int, 0>;
+    using C1 = std::integral_constant<int, 1>;
+    using C2 = std::integral_constant<int, 2>;
+    using C3 = std::integral_constant<int, 3>;
+    issue(C0{});
+    issue(C1{});
+    if constexpr (NST > 2) issue(C2{});
+    if constexpr (NST > 3) issue(C3{});
+    const int n = k1 - k0;
+    int k = 0;
+    for (; k + NST <= n; k += NST) {
+        step(C0{});
+        step(C1{});
+        if constexpr (NST > 2) step(C2{});
+        if constexpr (NST > 3) step(C3{});
+    }
+    if (k < n) step(C0{});
+    if (k + 1 < n) step(C1{});
+    if constexpr (NST > 3)
+        if (k + 2 < n) step(C2{});
+    __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));      /* the last requests land before LDS is used again */
+
+    float4 *const mine = reinterpret_cast<float4 *>(S0 + wv * STG);
+#pragma unroll
+    for (int i = 0; i < RW; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+            mine[(i * NT + j) * 64 + lane] = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+    __syncthreads();
+    for (int q = wv; q < RW * NT; q += NW) {
+        const int o = o0 + 16 * (q / NT) + 4 * g, t = 16 * (q % NT) + r16;
+        float b[4];
+        bias4(a, o, b);
+        const float4 *p = reinterpret_cast<const float4 *>(S0) + q * 64 + lane;
+        float4 s = p[0];
+#pragma unroll
+        for (int w = 1; w < NW; w++) {
+            const float4 v = p[w * (STG / 8)];
+            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+        }
+        put4(a, t, o, s, b);
     }
 }
 
@@ -648,6 +816,35 @@ void stream_pick(const K3kLinear *a, bool aligned, hipStream_t st)
     else stream_go<2, 4, XF32 ? 2 : 4, 8, XF32>(a, nw, aligned, st);
 }
 
+template <int RW, int XD, int NW, int NST, bool XF32>
+void skinny_go(const K3kLinear *a, hipStream_t st)
+{
+    lin_skinny_kernel<RW, XD, NW, NST, XF32><<<(a->out + 16 * RW - 1) / (16 * RW), 64 * NW, 0, st>>>(*a);
+}
+
+template <int XD, bool XF32>
+void skinny_pick(const K3kLinear *a, hipStream_t st)
+{
+    constexpr int SB = 4 + XD * (XF32 ? 2 : 1);        /* KB of a wave's stage */
+    constexpr int NST = 16 * SB <= 160 ? 4 : 12 * SB <= 160 ? 3 : 2;
+    skinny_go<2, XD, 4, NST, XF32>(a, st);
+}
+
+template <bool XF32>
+void skinny(const K3kLinear *a, hipStream_t st)
+{
+    switch ((a->T + 7) / 8) {
+    case 1: return skinny_pick<1, XF32>(a, st);
+    case 2: return skinny_pick<2, XF32>(a, st);
+    case 3: return skinny_pick<3, XF32>(a, st);
+    case 4: return skinny_pick<4, XF32>(a, st);
+    case 5: return skinny_pick<5, XF32>(a, st);
+    case 6: return skinny_pick<6, XF32>(a, st);
+    case 7: return skinny_pick<7, XF32>(a, st);
+    default: return skinny_pick<8, XF32>(a, st);
+    }
+}
+
 template <int BT, int BO, int WT, int WO, int NST, bool WREG>
 void tile_go(LinTile *p, hipStream_t st)
 {
@@ -669,6 +866,12 @@ extern "C" int k3k_linear(const K3kLinear *a, void *stream)
     if (a->T <= LIN_STREAM_T) {
         const int xe = a->x_type == K3D_F32 ? 4 : 8;
         const bool al = w16 && ((uintptr_t)a->x & 15) == 0 && a->ldx % xe == 0;
+        if (al && a->in % 8 == 0 && a->in >= LIN_KS) {
+            if (a->x_type == K3D_F32) skinny<true>(a, st);
+            else skinny<false>(a, st);
+            K3K_LAUNCH_CHECK("linear");
+            return 0;
+        }
         if (a->x_type == K3D_F32) stream_pick<true>(a, al, st);
         else stream_pick<false>(a, al, st);
         K3K_LAUNCH_CHECK("linear");
