@@ -174,10 +174,11 @@ __device__ __forceinline__ uint32_t k3_bload1(k3_rsrc r, uint32_t off)
 /* 16 bytes per lane from a buffer straight into LDS (buffer_load_dwordx4 ... lds): lane L
  * writes lds_row + 16 L, where lds_row is wave-uniform; counts against vmcnt. The builtin
  * exists only for the device pass (in the host pass it would drop the kernel's stub). */
+template <int POL = K3_LD_DEFAULT>
 __device__ __forceinline__ void k3_dma16(k3_rsrc r, void *lds_row, uint32_t voff, uint32_t soff)
 {
 #if defined(__HIP_DEVICE_COMPILE__)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)lds_row, 16, voff, soff, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)lds_row, 16, voff, soff, 0, POL);
 #else
     (void)r; (void)lds_row; (void)voff; (void)soff;
 #endif

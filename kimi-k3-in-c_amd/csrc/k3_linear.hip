@@ -7,6 +7,7 @@
 #include "k3_dev.h"
 #include "k3k.h"
 
+#include <math.h>
 #include <type_traits>
 
 namespace {
@@ -15,14 +16,38 @@ constexpr int LIN_KS = 64;                      /* columns of a tile kernel's st
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));     /* (a load of uint4 loses what tells LDS arrays apart) */
 constexpr uint32_t LIN_OOB = 0x80000000u;       /* a buffer offset past any descriptor used here */
 
+/* f(0), f(1) .. f(N - 1), the numbers as constants */
+template <int S, int N, class F>
+__device__ __forceinline__ void each_stage(F &&f)
+{
+    if constexpr (S < N) {
+        f(std::integral_constant<int, S>{});
+        each_stage<S + 1, N>(f);
+    }
+}
+
 /* ---- epilogue ------------------------------------------------------------------------ */
+/* v / (1 + e^-z). e^-z as 2^t (1 + r ln 2), t = -z log2 e rounded and r what the rounding left: within 3 units in the last
+ * place, for a third of the instructions of expf and a division (silu of 4096 x 12288 outputs, bf16: 592 -> SILU_US us
+ * with the product). */
+__device__ __forceinline__ float over_1p_exp(float v, float z)
+{
+    const float t = -1.44269504f * z;
+    const float r = fmaf(z, -1.92596299e-8f, fmaf(z, -1.44269504f, -t));
+    const float e = __builtin_amdgcn_exp2f(t);
+    const float d = 1.0f + fmaf(e, r * 0.693147181f, e);
+    const float q = __builtin_amdgcn_rcpf(d);
+    const float w = v * q;
+    return __builtin_isinf(d) ? v / d : fmaf(fmaf(-d, w, v), q, w);
+}
+
 __device__ __forceinline__ float act_of(float v, int act)
 {
     switch (act) {
     case K3D_ACT_RELU: return v < 0.0f ? 0.0f : v;
-    case K3D_ACT_SILU: return v / (1.0f + expf(-v));
+    case K3D_ACT_SILU: return over_1p_exp(v, v);
     case K3D_ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678f));
-    case K3D_ACT_GELU_TANH: return v / (1.0f + expf(-1.5957691f * (v + 0.044715f * v * v * v)));
+    case K3D_ACT_GELU_TANH: return over_1p_exp(v, 1.59576912f * v * fmaf(0.044715f * v, v, 1.0f));
     default: return v;
     }
 }
@@ -142,7 +167,7 @@ __device__ __forceinline__ uint4 load8_upto(const uint16_t *p, int n)
  * 32-column steps, and their sums meet in LDS. A lane's weights (row lane % 16, columns 8 (lane / 16)
  * ..+8 of a step) are an MFMA operand as loaded. Rows and tokens past the ends repeat the last one; only
  * the last step can pass the end of a row (guarded, zeros behind). */
-template <int RF, int NT, int U, int MAXW, bool XF32, bool ALIGNED>
+template <int RF, int NT, int U, int MAXW, bool XF32>
 __global__ __launch_bounds__(64 * MAXW) void lin_stream_kernel(K3kLinear a, int nw)
 {
     extern __shared__ float4 part[];
@@ -171,20 +196,15 @@ __global__ __launch_bounds__(64 * MAXW) void lin_stream_kernel(K3kLinear a, int 
     auto load = [&](Slot &s, int step) {
         const int k = step * 32;
 #pragma unroll
-        for (int i = 0; i < RF; i++) s.w[i] = ALIGNED ? k3_ldg16(wp[i] + k) : load8_any(wp[i] + k);
+        for (int i = 0; i < RF; i++) s.w[i] = load8_any(wp[i] + k);
 #pragma unroll
         for (int j = 0; j < NT; j++) {
             const char *p = xp[j] + (size_t)k * (XF32 ? 4 : 2);
             if (XF32) {
-                if (ALIGNED) {
-                    s.x[j][0] = k3_ldg16(p);
-                    s.x[j][XF32 ? 1 : 0] = k3_ldg16(p + 16);
-                } else {
-                    __builtin_memcpy(&s.x[j][0], p, 16);
-                    __builtin_memcpy(&s.x[j][XF32 ? 1 : 0], p + 16, 16);
-                }
+                __builtin_memcpy(&s.x[j][0], p, 16);
+                __builtin_memcpy(&s.x[j][XF32 ? 1 : 0], p + 16, 16);
             } else {
-                s.x[j][0] = ALIGNED ? k3_ldg16(p) : load8_any((const uint16_t *)p);
+                s.x[j][0] = load8_any((const uint16_t *)p);
             }
         }
     };
@@ -280,18 +300,20 @@ __global__ __launch_bounds__(64 * MAXW) void lin_stream_kernel(K3kLinear a, int 
  * 128 contiguous bytes; the operand layout itself, read from memory, has 16 lanes in a row on 16 rows
  * and a CU then takes in 10 bytes a cycle) and waits for its own requests alone, so there is no barrier until the
  * waves' sums meet. x takes part as bf16 or, cut into its three terms as it is read, fp32. */
-template <int RW, int XD, int NW, int NST, bool XF32>
+template <int RW, int XR, int NW, int NST, bool XF32, int POL>
 __global__ __launch_bounds__(64 * NW) void lin_skinny_kernel(K3kLinear a)
 {
-    constexpr int NT = (XD + 1) / 2, XB = XF32 ? 2 : 1;         /* token fragments; 128-byte pieces of a row of x */
-    constexpr int WD = 2 * RW, DN = WD + XD * XB;               /* DMAs of a stage */
-    constexpr int STG = (WD + XD * XB) * 512;                   /* elements of a wave's stage */
+    constexpr int KS = LIN_KS, C = KS / 8, RD = 64 / C;         /* 16-byte columns of a row; rows of a DMA */
+    constexpr int NT = (XR + 1) / 2, XB = XF32 ? 2 : 1;         /* token fragments; pieces of KS * 2 bytes of a row of x */
+    constexpr int WD = 16 * RW / RD, XD = 8 * XR / RD, DN = WD + XD * XB;       /* DMAs of a stage */
+    constexpr int STG = DN * 512;                               /* elements of a wave's stage */
     static_assert(RW * NT * 512 <= STG, "the sums fit the wave's part of a stage");
     __shared__ __attribute__((aligned(1024))) uint16_t S0[STG * NW], S1[STG * NW], S2[NST > 2 ? STG * NW : 8], S3[NST > 3 ? STG * NW : 8];
     const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int o0 = blockIdx.x * 16 * RW;
-    const int nks = (a.in + LIN_KS - 1) / LIN_KS, k0 = (int)((long)nks * wv / NW), k1 = (int)((long)nks * (wv + 1) / NW);
+    auto swz = [](int r) { return (r >> 1) & 7; };
+    const int nks = (a.in + KS - 1) / KS, k0 = (int)((long)nks * wv / NW), k1 = (int)((long)nks * (wv + 1) / NW);
     const int on = min(16 * RW, a.out - o0);
 
     /* 16-byte column c of an LDS row r lies in slot c ^ (r / 2 % 8): the rows of a fragment fall on all banks */
@@ -300,13 +322,13 @@ __global__ __launch_bounds__(64 * NW) void lin_skinny_kernel(K3kLinear a)
     uint32_t wo[WD], xo[XD];
 #pragma unroll
     for (int i = 0; i < WD; i++) {
-        const int r = 8 * i + lane / 8;
-        wo[i] = (uint32_t)min(r, on - 1) * (uint32_t)(a.ldw * 2) + ((lane & 7) ^ ((r >> 1) & 7)) * 16;
+        const int r = RD * i + lane / C;
+        wo[i] = (uint32_t)min(r, on - 1) * (uint32_t)(a.ldw * 2) + ((lane & (C - 1)) ^ swz(r)) * 16;
     }
 #pragma unroll
     for (int i = 0; i < XD; i++) {
-        const int r = 8 * i + lane / 8;
-        xo[i] = (uint32_t)min(r, a.T - 1) * (uint32_t)(a.ldx * (XF32 ? 4 : 2)) + ((lane & 7) ^ ((r >> 1) & 7)) * 16;
+        const int r = RD * i + lane / C;
+        xo[i] = (uint32_t)min(r, a.T - 1) * (uint32_t)(a.ldx * (XF32 ? 4 : 2)) + ((lane & (C - 1)) ^ swz(r)) * 16;
     }
     auto buf_of = [&](auto slot) -> uint16_t * {
         constexpr int S = decltype(slot)::value;
@@ -323,13 +345,13 @@ __global__ __launch_bounds__(64 * NW) void lin_skinny_kernel(K3kLinear a)
     auto issue = [&](auto slot) {
         uint16_t *const b = buf_of(slot);
         const uint32_t none = xk < k1 ? 0u : LIN_OOB;
-        const uint32_t c = xk == nks - 1 ? a.in - LIN_KS : xk * LIN_KS;
+        const uint32_t c = xk == nks - 1 ? a.in - KS : xk * KS;
 #pragma unroll
-        for (int i = 0; i < WD; i++) k3_dma16(rw, b + i * 512, wo[i] | none, c * 2);
+        for (int i = 0; i < WD; i++) k3_dma16<POL>(rw, b + i * 512, wo[i] | none, c * 2);
 #pragma unroll
         for (int h = 0; h < XB; h++)
 #pragma unroll
-            for (int i = 0; i < XD; i++) k3_dma16(rx, b + (WD + h * XD + i) * 512, xo[i] | none, c * (XF32 ? 4 : 2) + h * 128);
+            for (int i = 0; i < XD; i++) k3_dma16(rx, b + (WD + h * XD + i) * 512, xo[i] | none, c * (XF32 ? 4 : 2) + h * KS * 2);
         xk++;
     };
     k3_f32x4 acc[RW][NT];
@@ -337,7 +359,7 @@ __global__ __launch_bounds__(64 * NW) void lin_skinny_kernel(K3kLinear a)
     for (int i = 0; i < RW; i++)
 #pragma unroll
         for (int j = 0; j < NT; j++) acc[i][j] = k3_f32x4{0.f, 0.f, 0.f, 0.f};
-    const int sw = (r16 >> 1) & 7, over = nks * LIN_KS - a.in;
+    const int sw = swz(r16), over = nks * KS - a.in;
     constexpr int WAITN = DN * (NST - 1);
     constexpr int WAIT_STAGE = (WAITN & 15) | (7 << 4) | (15 << 8) | ((WAITN >> 4) << 14);
     constexpr int WAIT_LGKM0 = 15 | (7 << 4) | (0 << 8) | (3 << 14);
@@ -347,19 +369,19 @@ __global__ __launch_bounds__(64 * NW) void lin_skinny_kernel(K3kLinear a)
         const uint16_t *const b = buf_of(slot);
         __builtin_amdgcn_s_waitcnt(WAIT_STAGE);
         __builtin_amdgcn_sched_barrier(0);
-        u32x4 wf[2][RW], xf[2][NT][XB];
+        u32x4 wf[KS / 32][RW], xf[KS / 32][NT][XB];
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
+        for (int h = 0; h < KS / 32; h++) {
 #pragma unroll
-            for (int i = 0; i < RW; i++) wf[h][i] = *reinterpret_cast<const u32x4 *>(b + (16 * i + r16) * 64 + ((4 * h + g) ^ sw) * 8);
+            for (int i = 0; i < RW; i++) wf[h][i] = *reinterpret_cast<const u32x4 *>(b + (16 * i + r16) * KS + ((4 * h + g) ^ sw) * 8);
             /* (a last fragment of 8 tokens: its upper lanes repeat the lower ones') */
 #pragma unroll
             for (int j = 0; j < NT; j++) {
-                const int r = 16 * j + (XD % 2 && j == NT - 1 ? r16 & 7 : r16), s = (r >> 1) & 7;
-                const uint16_t *q = b + (WD * 8 + r) * 64;
-                if constexpr (XF32) {      /* columns 8 g.. of half h: 16-byte pieces 2 g, 2 g + 1 of its 128 bytes */
-                    xf[h][j][0] = *reinterpret_cast<const u32x4 *>(q + h * XD * 512 + ((2 * g) ^ s) * 8);
-                    xf[h][j][1] = *reinterpret_cast<const u32x4 *>(q + h * XD * 512 + ((2 * g + 1) ^ s) * 8);
+                const int r = 16 * j + (XR % 2 && j == NT - 1 ? r16 & 7 : r16), s = swz(r), f = 8 * h + 2 * g;
+                const uint16_t *q = b + (WD * RD + r) * KS;
+                if constexpr (XF32) {      /* two 16-byte columns */
+                    xf[h][j][0] = *reinterpret_cast<const u32x4 *>(q + f / C * XD * 512 + ((f % C) ^ s) * 8);
+                    xf[h][j][1] = *reinterpret_cast<const u32x4 *>(q + f / C * XD * 512 + ((f % C + 1) ^ s) * 8);
                 } else {
                     xf[h][j][0] = *reinterpret_cast<const u32x4 *>(q + ((4 * h + g) ^ s) * 8);
                 }
@@ -371,7 +393,7 @@ __global__ __launch_bounds__(64 * NW) void lin_skinny_kernel(K3kLinear a)
         __builtin_amdgcn_sched_barrier(0);
         const int skip = rk++ == nks - 1 ? over : 0;
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+        for (int h = 0; h < KS / 32; h++)
 #pragma unroll
             for (int j = 0; j < NT; j++) {
                 const bool zero = 32 * h + 8 * g < skip;
@@ -397,26 +419,12 @@ __global__ __launch_bounds__(64 * NW) void lin_skinny_kernel(K3kLinear a)
             }
         __builtin_amdgcn_sched_barrier(0);
     };
-    using C0 = std::integral_constant<int, 0>;
-    using C1 = std::integral_constant<int, 1>;
-    using C2 = std::integral_constant<int, 2>;
-    using C3 = std::integral_constant<int, 3>;
-    issue(C0{});
-    issue(C1{});
-    if constexpr (NST > 2) issue(C2{});
-    if constexpr (NST > 3) issue(C3{});
-    const int n = k1 - k0;
-    int k = 0;
-    for (; k + NST <= n; k += NST) {
-        step(C0{});
-        step(C1{});
-        if constexpr (NST > 2) step(C2{});
-        if constexpr (NST > 3) step(C3{});
-    }
-    if (k < n) step(C0{});
-    if (k + 1 < n) step(C1{});
-    if constexpr (NST > 3)
-        if (k + 2 < n) step(C2{});
+    each_stage<0, NST>(issue);
+    int left = k1 - k0;
+    for (; left >= NST; left -= NST) each_stage<0, NST>(step);
+    each_stage<0, NST - 1>([&](auto slot) {
+        if (decltype(slot)::value < left) step(slot);
+    });
     __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));      /* the last requests land before LDS is used again */
 
     float4 *const mine = reinterpret_cast<float4 *>(S0 + wv * STG);
@@ -520,9 +528,10 @@ __global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
     constexpr int XD = BT / 8 / NW, WD = WREG ? 0 : BO / 8 / NW, DN = XD + WD;      /* DMAs of a wave per step */
     constexpr int WR = WREG ? BO * 8 / (64 * NW) : 1;                                /* 16-byte pieces of W per thread */
     constexpr int FG = FO % 4 == 0 ? 4 : FO % 2 == 0 ? 2 : 1;       /* fragments that share a run of outputs */
-    static_assert(XD >= 1 && (WREG || WD >= 1) && NST >= 2 && NST <= 4, "tile");
+    static_assert(XD >= 1 && (WREG || WD >= 1) && NST >= 2 && NST <= 8, "tile");
     constexpr int SZ = (BT + BO) * LIN_KS;
-    __shared__ __attribute__((aligned(1024))) uint16_t S0[SZ], S1[SZ], S2[NST > 2 ? SZ : 8], S3[NST > 3 ? SZ : 8];
+    __shared__ __attribute__((aligned(1024))) uint16_t S0[SZ], S1[SZ], S2[NST > 2 ? SZ : 8], S3[NST > 3 ? SZ : 8], S4[NST > 4 ? SZ : 8],
+        S5[NST > 5 ? SZ : 8], S6[NST > 6 ? SZ : 8], S7[NST > 7 ? SZ : 8];
 
     const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -560,7 +569,11 @@ __global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
         if constexpr (S == 0) return S0;
         else if constexpr (S == 1) return S1;
         else if constexpr (S == 2) return S2;
-        else return S3;
+        else if constexpr (S == 3) return S3;
+        else if constexpr (S == 4) return S4;
+        else if constexpr (S == 5) return S5;
+        else if constexpr (S == 6) return S6;
+        else return S7;
     };
     /* Stages are requested in order: step `xk` of x, which is column block `wk` of W (of a term), the last one
      * of a row from where its 64 columns end with the row. Past the slice: zeros, so that every step requests
@@ -626,19 +639,23 @@ __global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
 #pragma unroll
             for (int j = 0; j < FT; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[i], xf[j], acc[i][j], 0, 0, 0);
     };
-    /* issue order of a half: a fragment read of the other half behind each of the first MFMAs */
+    /* issue order of a half: a fragment read of the other half behind each of the first MFMAs, and, behind the
+     * barrier, the next stage's requests between them too (in a burst they keep the SIMD from its MFMAs for
+     * some hundred cycles) */
     constexpr int NRD = FO + FT, NMF = FO * FT, GAP = NMF / NRD > 0 ? NMF / NRD : 1;
-    auto pin = [&]() {
-#pragma unroll
-        for (int i = 0; i < NRD; i++) {
+    auto pin = [&](auto dma) {
+        each_stage<0, NRD>([&](auto at) {
+            constexpr int I = decltype(at)::value, ND = decltype(dma)::value, Q = (I + 1) * ND / NRD - I * ND / NRD;
             __builtin_amdgcn_sched_group_barrier(0x008, GAP, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        }
+            if constexpr (Q > 0) __builtin_amdgcn_sched_group_barrier(0x010, Q, 0);
+        });
         __builtin_amdgcn_sched_group_barrier(0x008, NMF, 0);
     };
     /* all but the last NST - 2 stages' requests (with weights through registers: all) */
     constexpr int WAITN = WREG ? 0 : DN * (NST - 2);
-    constexpr int WAIT_STAGE = (WAITN & 15) | (7 << 4) | (15 << 8) | ((WAITN >> 4) << 14);
+    constexpr int WAIT_STAGE = (WAITN & 15) | (7 << 4) | (0 << 8) | ((WAITN >> 4) << 14);       /* and LDS: none */
+    static_assert(WAITN < 64, "requests in flight");
     constexpr int WAIT_VM0 = (7 << 4) | (15 << 8);
     k3_bf16x8 fx0[FT], fw0[FO], fx1[FT], fw1[FO];
 
@@ -651,62 +668,48 @@ __global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
         uint16_t *const nb = buf_of(std::integral_constant<int, (S + 1) % NST>{});
         read(b, 1, fx1, fw1);
         mma(fx0, fw0);
-        pin();
+        pin(std::integral_constant<int, 0>{});
         __builtin_amdgcn_sched_barrier(0);
+        /* (__syncthreads would wait for every request) */
         __builtin_amdgcn_s_waitcnt(WAIT_STAGE);
-        __syncthreads();
+        asm volatile("s_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
         if (WREG) wstore(slot);
         issue(slot);
         if (WREG) wload();
-        __builtin_amdgcn_sched_barrier(0);
+        if (WREG) __builtin_amdgcn_sched_barrier(0);
         read(nb, 0, fx0, fw0);          /* (past the last step: what lies there, unused) */
         mma(fx1, fw1);
-        pin();
+        pin(std::integral_constant<int, WREG ? 0 : DN>{});
         __builtin_amdgcn_sched_barrier(0);
     };
     auto start = [&](auto slot) {
-        constexpr int S = decltype(slot)::value;
-        if constexpr (S < NST) {
-            if (WREG) {
-                wload();
-                wstore(slot);
-            }
-            issue(slot);
+        if (WREG) {
+            wload();
+            wstore(slot);
         }
+        issue(slot);
     };
-    using C0 = std::integral_constant<int, 0>;
-    using C1 = std::integral_constant<int, 1>;
-    using C2 = std::integral_constant<int, 2>;
-    using C3 = std::integral_constant<int, 3>;
-    start(C0{});
-    start(C1{});
-    if constexpr (NST > 2) start(C2{});
-    if constexpr (NST > 3) start(C3{});
+    each_stage<0, NST>(start);
     if (WREG) wload();
     __builtin_amdgcn_s_waitcnt(WAIT_VM0);
     __syncthreads();
     read(S0, 0, fx0, fw0);
     /* (whole rounds in the loop: a way out of its middle costs copies of the accumulators) */
-    int k = 0;
-    for (; k + NST <= n; k += NST) {
-        step(C0{});
-        step(C1{});
-        if constexpr (NST > 2) step(C2{});
-        if constexpr (NST > 3) step(C3{});
-    }
-    if (k < n) step(C0{});
-    if constexpr (NST > 2)
-        if (k + 1 < n) step(C1{});
-    if constexpr (NST > 3)
-        if (k + 2 < n) step(C2{});
+    int left = n;
+    for (; left >= NST; left -= NST) each_stage<0, NST>(step);
+    each_stage<0, NST - 1>([&](auto slot) {
+        if (decltype(slot)::value < left) step(slot);
+    });
     __builtin_amdgcn_s_waitcnt(WAIT_VM0);      /* the last requests land before LDS is used again */
 
     /* A lane holds token r16 of each token fragment and 4 FG consecutive outputs of FG fragments. The sums go
      * through LDS (the stage buffers, a region per wave, JR token fragments at a time; 16-byte column c of row r
      * in c ^ (r % 16)), so that a wave writes whole rows of its outputs, and the epilogue's code is there once. */
-    constexpr int WOUT = BO / WO, C = WOUT / 4, JR = FT <= 4 ? FT : FT / 2, RB = JR * 16 * WOUT * 4;
-    constexpr int PER = SZ * 2 / RB;        /* regions per stage buffer */
-    static_assert(PER >= 1 && PER * 2 >= NW && 64 % C == 0, "epilogue regions");
+    constexpr int WOUT = BO / WO, C = WOUT / 4;
+    constexpr int JR = SZ * 2 / (FT * 64 * WOUT) * 2 >= NW ? FT : SZ * 2 / (FT * 32 * WOUT) * 2 >= NW ? FT / 2 : FT / 4;
+    constexpr int RB = JR * 64 * WOUT, PER = SZ * 2 / RB;       /* bytes of a region; regions per stage buffer */
+    static_assert(JR >= 1 && FT % JR == 0 && PER >= 1 && PER * 2 >= NW && 64 % C == 0, "epilogue regions");
     uint16_t *stage = S0;
     if (PER < NW) stage = wv / PER == 0 ? S0 : S1;
     float4 *const reg = reinterpret_cast<float4 *>(stage + (wv % PER) * (RB / 2));
@@ -772,9 +775,11 @@ __global__ __launch_bounds__(256) void lin_join_kernel(K3kLinear a, const float 
 }
 
 /* ---- launches -------------------------------------------------------------------------------- */
-constexpr int LIN_STREAM_T = 64;            /* tokens up to which the weights go straight into registers */
 constexpr int LIN_MAX_SLICES = 16;
-constexpr size_t LIN_PART_CAP = (size_t)32 << 20;
+constexpr size_t LIN_PART_CAP = (size_t)64 << 20;
+/* weights that no cache keeps from one call to the next, from here on read past the caches (102 MB times 64
+ * tokens 30.6 -> 29.5 us, 176 MB times one 30.2 -> 26.8; but 51 MB times 16 12.4 -> 12.8, 29 MB times 32 10.2 -> 14.5) */
+constexpr size_t LIN_NT_BYTES = (size_t)96 << 20;
 
 int kpad(int in) { return (in + LIN_KS - 1) / LIN_KS * LIN_KS; }
 
@@ -790,109 +795,187 @@ size_t part_bytes(int T, int out)
     return most < LIN_PART_CAP ? most : LIN_PART_CAP;
 }
 
+/* ---- at any alignment, or rows shorter than a stage ---- */
 template <int RF, int NT, int U, int MAXW, bool XF32>
-void stream_go(const K3kLinear *a, int nw, bool aligned, hipStream_t st)
+void stream_go(const K3kLinear *a, int nw, hipStream_t st)
 {
     const dim3 grid((a->out + 16 * RF - 1) / (16 * RF), (a->T + 16 * NT - 1) / (16 * NT));
-    const size_t lds = (size_t)nw * RF * NT * 1024;
-    if (aligned) lin_stream_kernel<RF, NT, U, MAXW, XF32, true><<<grid, 64 * nw, lds, st>>>(*a, nw);
-    else lin_stream_kernel<RF, NT, U, MAXW, XF32, false><<<grid, 64 * nw, lds, st>>>(*a, nw);
+    lin_stream_kernel<RF, NT, U, MAXW, XF32><<<grid, 64 * nw, (size_t)nw * RF * NT * 1024, st>>>(*a, nw);
 }
 
 template <bool XF32>
-void stream_pick(const K3kLinear *a, bool aligned, hipStream_t st)
+void stream_pick(const K3kLinear *a, hipStream_t st)
 {
     const int nt = (a->T + 15) / 16, rf = nt == 1 ? 1 : 2;
     const long wgs = (a->out + 16 * rf - 1) / (16 * rf);
     const int steps = (a->in + 31) / 32, cus = k3k_cu_count();
     /* waves that share a workgroup's columns: enough for the chip, each with a few steps */
-    int nw = 4;
-    if (wgs < 2 * cus) nw = 8;
-    if (wgs < cus / 2 && nt == 1) nw = 16;
+    int nw = wgs < 2 * cus ? 8 : 4;
     while (nw > 1 && steps < 2 * nw) nw /= 2;
-    if (nt == 1) stream_go<1, 1, XF32 ? 4 : 8, 16, XF32>(a, nw, aligned, st);
-    else if (nt == 2) stream_go<2, 2, 4, 8, XF32>(a, nw, aligned, st);
-    else if (nt == 3) stream_go<2, 3, XF32 ? 2 : 4, 8, XF32>(a, nw, aligned, st);
-    else stream_go<2, 4, XF32 ? 2 : 4, 8, XF32>(a, nw, aligned, st);
+    if (nt == 1) stream_go<1, 1, XF32 ? 4 : 8, 8, XF32>(a, nw, st);
+    else if (nt == 2) stream_go<2, 2, 4, 8, XF32>(a, nw, st);
+    else if (nt == 3) stream_go<2, 3, XF32 ? 2 : 4, 8, XF32>(a, nw, st);
+    else stream_go<2, 4, XF32 ? 2 : 4, 8, XF32>(a, nw, st);
 }
 
-template <int RW, int XD, int NW, int NST, bool XF32>
+/* ---- few tokens ---- */
+constexpr int SK_NW = 4;
+constexpr int sk_kb(int rw, int xr, bool f32) { return 2 * rw + xr * (f32 ? 2 : 1); }      /* KB of a wave's stage */
+constexpr int sk_nst(int rw, int xr, bool f32)
+{
+    return 4 * SK_NW * sk_kb(rw, xr, f32) <= 160 ? 4 : 3 * SK_NW * sk_kb(rw, xr, f32) <= 160 ? 3 : 2 * SK_NW * sk_kb(rw, xr, f32) <= 160 ? 2 : 0;
+}
+/* tokens go in groups of 8, 16, 32, 48 and 64 (and no group past the last that fits the LDS) */
+constexpr int sk_group(int T) { return T <= 8 ? 1 : T <= 16 ? 2 : T <= 32 ? 4 : T <= 48 ? 6 : 8; }
+
+template <int RW, int XR, bool XF32>
 void skinny_go(const K3kLinear *a, hipStream_t st)
 {
-    lin_skinny_kernel<RW, XD, NW, NST, XF32><<<(a->out + 16 * RW - 1) / (16 * RW), 64 * NW, 0, st>>>(*a);
-}
-
-template <int XD, bool XF32>
-void skinny_pick(const K3kLinear *a, hipStream_t st)
-{
-    constexpr int SB = 4 + XD * (XF32 ? 2 : 1);        /* KB of a wave's stage */
-    constexpr int NST = 16 * SB <= 160 ? 4 : 12 * SB <= 160 ? 3 : 2;
-    skinny_go<2, XD, 4, NST, XF32>(a, st);
-}
-
-template <bool XF32>
-void skinny(const K3kLinear *a, hipStream_t st)
-{
-    switch ((a->T + 7) / 8) {
-    case 1: return skinny_pick<1, XF32>(a, st);
-    case 2: return skinny_pick<2, XF32>(a, st);
-    case 3: return skinny_pick<3, XF32>(a, st);
-    case 4: return skinny_pick<4, XF32>(a, st);
-    case 5: return skinny_pick<5, XF32>(a, st);
-    case 6: return skinny_pick<6, XF32>(a, st);
-    case 7: return skinny_pick<7, XF32>(a, st);
-    default: return skinny_pick<8, XF32>(a, st);
+    constexpr int NST = sk_nst(RW, XR, XF32);
+    if constexpr (NST > 0) {
+        const unsigned grid = (a->out + 16 * RW - 1) / (16 * RW);
+        if ((size_t)a->in * a->out * 2 >= LIN_NT_BYTES)
+            lin_skinny_kernel<RW, XR, SK_NW, NST, XF32, K3_LD_NT><<<grid, 64 * SK_NW, 0, st>>>(*a);
+        else
+            lin_skinny_kernel<RW, XR, SK_NW, NST, XF32, K3_LD_DEFAULT><<<grid, 64 * SK_NW, 0, st>>>(*a);
     }
 }
 
+template <int RW, bool XF32>
+void skinny_rows(const K3kLinear *a, hipStream_t st)
+{
+    switch (sk_group(a->T)) {
+    case 1: return skinny_go<RW, 1, XF32>(a, st);
+    case 2: return skinny_go<RW, 2, XF32>(a, st);
+    case 4: return skinny_go<RW, 4, XF32>(a, st);
+    case 6: return skinny_go<RW, 6, XF32>(a, st);
+    default: return skinny_go<RW, 8, XF32>(a, st);
+    }
+}
+
+template <bool XF32>
+void skinny(const K3kLinear *a, int rw, hipStream_t st)
+{
+    if (rw == 1) skinny_rows<1, XF32>(a, st);
+    else if (rw == 2) skinny_rows<2, XF32>(a, st);
+    else skinny_rows<4, XF32>(a, st);
+}
+
+/* Two limits of one time: neither hides all of the other. */
+float both(float a, float b) { return sqrtf(a * a + b * b); }
+
+/* Microseconds of lin_skinny_kernel: a CU takes in 82 KB/us while the chip's 17.8 GB/ms allow it (a workgroup's
+ * rows of W and all of x for them), the weights come at 5.9 GB/ms, fp32 x costs a wave 0.26 us to cut 8 tokens of a
+ * stage. The constants of this and of tile_cost are fitted to 40 shapes of 1 to 4096 tokens, each on every kernel: they are off by
+ * 10 % on average, and what they choose is 2.5 % slower than the best of them (16 % at 64 tokens of 7168 -> 576, 23 %
+ * at 1024 of 7168 -> 384 at the worst). 0: does not fit the LDS. */
+float skinny_cost(int T, int in, int out, bool f32, int rw, long cus)
+{
+    const int xr = sk_group(T);
+    if (sk_nst(rw, xr, f32) == 0) return 0.0f;
+    const long wgs = (out + 16 * rw - 1) / (16 * rw), rounds = (wgs + cus - 1) / cus;
+    const float kb = (float)in * 2.0f / 1024.0f * (16 * rw + 8 * xr * (f32 ? 2 : 1));
+    const float rate = fminf(82.0f, 17800.0f / (float)(wgs < cus ? wgs : cus));
+    const float cut = f32 ? (float)((in + LIN_KS - 1) / LIN_KS) / SK_NW * xr * 0.26f : 0.0f;
+    return 2.9f + both(rounds * fmaxf(kb / rate, cut), (float)in * out * 2.0f / 5.9e6f);
+}
+
+/* ---- many tokens ---- */
 template <int BT, int BO, int WT, int WO, int NST, bool WREG>
-void tile_go(LinTile *p, hipStream_t st)
+void tile_go(const LinTile *p, hipStream_t st)
 {
     lin_tile_kernel<BT, BO, WT, WO, NST, WREG><<<p->nt * p->no * p->nsl, 64 * WT * WO, 0, st>>>(*p);
+}
+
+/* Microseconds of a launch of lin_tile_kernel and, with slices, the join: rounds of as many workgroups as fit the chip, each
+ * of `per` steps; a step takes what a CU takes in at 74 KB/us and the chip at 35 GB/ms, or the matrix cores at
+ * 1.66 PFLOP/s of the chip; W and x come at 6.7 GB/ms. */
+struct Shape {
+    int bt, bo, per_cu;
+};
+constexpr Shape SHAPES[] = {{256, 256, 1}, {256, 128, 1}, {128, 128, 1}, {128, 64, 2}, {64, 128, 2}, {64, 64, 2}};
+constexpr int N_SHAPES = sizeof SHAPES / sizeof SHAPES[0];
+
+float tile_cost(const Shape &s, int T, int in, int out, int steps, int nsl, long cus)
+{
+    const long wgs = (long)((T + s.bt - 1) / s.bt) * ((out + s.bo - 1) / s.bo) * nsl, slots = cus * s.per_cu;
+    const int per = (steps + nsl - 1) / nsl;
+    const float kb = (s.bt + s.bo) * LIN_KS * 2.0f / 1024.0f, mfma = 2.0f * s.bt * s.bo * LIN_KS / 6.5e6f;
+    auto round = [&](long n) {
+        const float on = (float)((n + cus - 1) / cus);          /* workgroups of a CU */
+        return per * both(on * fmaxf(kb / 74.0f, mfma), kb * n / 35000.0f) + 1.1f + 0.08f * kb;
+    };
+    float t = (float)(wgs / slots) * round(slots) + (wgs % slots ? round(wgs % slots) : 0.0f);
+    t = 2.6f + both(t, ((float)out + T) * in * 2.0f / 6.7e6f);
+    if (nsl > 1) t += 2.1f + (nsl + 1.0f) * T * out * 4.0f / 4.7e6f;
+    return t;
 }
 
 }  // namespace
 
 extern "C" size_t k3k_linear_ws(int T, int in, int out, int x_type)
 {
-    if (T <= LIN_STREAM_T) return 0;
     return pack_bytes(T, in, x_type) + part_bytes(T, out);
 }
 
 extern "C" int k3k_linear(const K3kLinear *a, void *stream)
 {
     hipStream_t st = (hipStream_t)stream;
+    const long cus = k3k_cu_count();
+    const bool f32 = a->x_type == K3D_F32;
     const bool w16 = ((uintptr_t)a->W & 15) == 0 && a->ldw % 8 == 0;
-    if (a->T <= LIN_STREAM_T) {
-        const int xe = a->x_type == K3D_F32 ? 4 : 8;
-        const bool al = w16 && ((uintptr_t)a->x & 15) == 0 && a->ldx % xe == 0;
-        if (al && a->in % 8 == 0 && a->in >= LIN_KS) {
-            if (a->x_type == K3D_F32) skinny<true>(a, st);
-            else skinny<false>(a, st);
-            K3K_LAUNCH_CHECK("linear");
+    const bool x16 = ((uintptr_t)a->x & 15) == 0 && a->ldx % (f32 ? 4 : 8) == 0;
+    /* weights by DMA, or, at other alignments and in rows shorter than a stage, through registers */
+    const bool dma = w16 && a->in % 8 == 0 && a->in >= LIN_KS;
+    const int nks = (a->in + LIN_KS - 1) / LIN_KS, steps = nks * (f32 ? 3 : 1);
+    const bool pack = f32 || !x16 || a->in % LIN_KS;
+
+    /* the cheapest tile shape and number of slices */
+    float best = 0.0f;
+    int shape = 0, nsl = 1;
+    const size_t one = (size_t)a->T * a->out * 4, room = part_bytes(a->T, a->out);
+    for (int i = 0; i < N_SHAPES; i++) {
+        if (!dma && !(SHAPES[i].bt == SHAPES[i].bo && SHAPES[i].bt < 256)) continue;
+        for (int n : {1, 2, 3, 4, 6, 8, 12, LIN_MAX_SLICES}) {
+            if (n > 1 && (n * one > room || steps < 4 * n)) break;
+            const float t = tile_cost(SHAPES[i], a->T, a->in, a->out, steps, n, cus);
+            if (best == 0.0f || t < best) best = t, shape = i, nsl = n;
+        }
+    }
+    if (pack) best += 2.5f + (float)a->T * kpad(a->in) * (f32 ? 10 : 4) / 4e6f;
+    if (a->T <= 64) {
+        int rw = 0;
+        if (dma && x16)
+            for (int r = 1; r <= 4; r *= 2) {
+                const float t = skinny_cost(a->T, a->in, a->out, f32, r, cus);
+                if (t > 0.0f && t < best) best = t, rw = r;
+            }
+        if (rw) {
+            if (f32) skinny<true>(a, rw, st);
+            else skinny<false>(a, rw, st);
+            K3K_LAUNCH_CHECK("linear: few tokens");
             return 0;
         }
-        if (a->x_type == K3D_F32) stream_pick<true>(a, al, st);
-        else stream_pick<false>(a, al, st);
-        K3K_LAUNCH_CHECK("linear");
-        return 0;
+        if (!dma) {
+            if (f32) stream_pick<true>(a, st);
+            else stream_pick<false>(a, st);
+            K3K_LAUNCH_CHECK("linear: any alignment");
+            return 0;
+        }
     }
+
     LinTile p;
     p.a = *a;
-    p.nks = (a->in + LIN_KS - 1) / LIN_KS;
-    p.steps = p.nks;
-    /* weights by DMA, or, at other alignments and in rows shorter than a step, through registers */
-    const bool dma = w16 && a->in % 8 == 0 && a->in >= LIN_KS;
-    const int kp = kpad(a->in);
-    if (a->x_type == K3D_F32 || ((uintptr_t)a->x & 15) || a->ldx % 8 || a->in % LIN_KS) {
-        const int f32 = a->x_type == K3D_F32, over = dma ? kp - a->in : 0;
+    p.nks = nks;
+    p.steps = steps;
+    if (pack) {
+        const int kp = kpad(a->in), over = dma ? kp - a->in : 0;
         const size_t n = (size_t)a->T * (kp / 8);
         const unsigned grid = (unsigned)((n + 255) / 256);
         if (f32) lin_pack_kernel<true><<<grid, 256, 0, st>>>((uint16_t *)a->ws, a->x, a->ldx, a->T, a->in, kp, over);
         else lin_pack_kernel<false><<<grid, 256, 0, st>>>((uint16_t *)a->ws, a->x, a->ldx, a->T, a->in, kp, over);
         K3K_LAUNCH_CHECK("linear: pack");
         p.x = (const uint16_t *)a->ws;
-        p.steps *= f32 ? 3 : 1;
         p.ldx = p.xcols = p.steps * LIN_KS;
     } else {
         p.x = (const uint16_t *)a->x;
@@ -900,35 +983,25 @@ extern "C" int k3k_linear(const K3kLinear *a, void *stream)
         p.xcols = a->in;
     }
     p.part = (float *)((char *)a->ws + pack_bytes(a->T, a->in, a->x_type));
-    const long cus = k3k_cu_count();
-    /* the tile shape, and slices of the columns where the tiles cannot fill the chip */
-    const long t256 = (long)((a->T + 255) / 256) * ((a->out + 255) / 256);
-    const long t128 = (long)((a->T + 127) / 128) * ((a->out + 127) / 128);
-    const int shape = dma && t256 >= cus * 3 / 4 ? 256 : t128 >= cus ? 128 : 64;
-    p.nt = (a->T + shape - 1) / shape;
-    p.no = (a->out + shape - 1) / shape;
-    const long tiles = (long)p.nt * p.no;
-    int nsl = 1;
-    if (shape == 64) {
-        nsl = (int)(2 * cus / tiles);
-        const size_t cap = part_bytes(a->T, a->out) / ((size_t)a->T * a->out * 4);
-        if (nsl > p.steps / 4) nsl = p.steps / 4;
-        if (nsl > LIN_MAX_SLICES) nsl = LIN_MAX_SLICES;
-        if ((size_t)nsl > cap) nsl = (int)cap;
-        if (nsl < 1) nsl = 1;
-    }
-    p.per = (p.steps + nsl - 1) / nsl;
-    p.nsl = (p.steps + p.per - 1) / p.per;
-    if (shape == 256) {
-        tile_go<256, 256, 2, 4, 2, false>(&p, st);
-    } else if (shape == 128) {
-        if (dma) tile_go<128, 128, 2, 2, 2, false>(&p, st);
-        else tile_go<128, 128, 2, 2, 2, true>(&p, st);
+    p.nt = (a->T + SHAPES[shape].bt - 1) / SHAPES[shape].bt;
+    p.no = (a->out + SHAPES[shape].bo - 1) / SHAPES[shape].bo;
+    p.per = (steps + nsl - 1) / nsl;
+    p.nsl = (steps + p.per - 1) / p.per;
+    if (dma) {
+        switch (shape) {
+        case 0: tile_go<256, 256, 2, 4, 2, false>(&p, st); break;
+        case 1: tile_go<256, 128, 4, 2, 3, false>(&p, st); break;
+        case 2: tile_go<128, 128, 2, 2, 4, false>(&p, st); break;
+        case 3: tile_go<128, 64, 2, 2, 3, false>(&p, st); break;
+        case 4: tile_go<64, 128, 1, 4, 3, false>(&p, st); break;
+        default: tile_go<64, 64, 2, 2, 4, false>(&p, st); break;
+        }
+    } else if (shape == 2) {
+        tile_go<128, 128, 2, 2, 2, true>(&p, st);
     } else {
-        if (dma) tile_go<64, 64, 2, 2, 4, false>(&p, st);
-        else tile_go<64, 64, 2, 2, 4, true>(&p, st);
+        tile_go<64, 64, 2, 2, 4, true>(&p, st);
     }
-    K3K_LAUNCH_CHECK("linear");
+    K3K_LAUNCH_CHECK("linear: tiles");
     if (p.nsl > 1) {
         const size_t n = (size_t)a->T * ((a->out + 3) / 4);
         lin_join_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(*a, p.part, p.nsl);
