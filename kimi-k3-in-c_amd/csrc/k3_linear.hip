@@ -28,17 +28,17 @@ __device__ __forceinline__ void each_stage(F &&f)
 
 /* ---- epilogue ------------------------------------------------------------------------ */
 /* v / (1 + e^-z). e^-z as 2^t (1 + r ln 2), t = -z log2 e rounded and r what the rounding left: within 3 units in the last
- * place, for a third of the instructions of expf and a division (silu of 4096 x 12288 outputs, bf16: 592 -> SILU_US us
+ * place, for a third of the instructions of expf and a division (silu of 4096 x 12288 outputs, bf16: 592 -> 580 us
  * with the product). */
 __device__ __forceinline__ float over_1p_exp(float v, float z)
 {
     const float t = -1.44269504f * z;
-    const float r = fmaf(z, -1.92596299e-8f, fmaf(z, -1.44269504f, -t));
+    const float r = fabsf(t) < 127.0f ? fmaf(z, -1.92596299e-8f, fmaf(z, -1.44269504f, -t)) : 0.0f;
     const float e = __builtin_amdgcn_exp2f(t);
-    const float d = 1.0f + fmaf(e, r * 0.693147181f, e);
-    const float q = __builtin_amdgcn_rcpf(d);
-    const float w = v * q;
-    return __builtin_isinf(d) ? v / d : fmaf(fmaf(-d, w, v), q, w);
+    const float d1 = fmaf(e, fmaf(r, 0.693147181f, 1.0f), 1.0f);
+    const float k = d1 > 0x1p64f ? 0x1p-64f : 1.0f, d = d1 * k;     /* (the reciprocal stays normal) */
+    const float q = __builtin_amdgcn_rcpf(d), w = v * k * q, c = fmaf(fmaf(-d, w, v * k), q, w);
+    return c == c ? c : w;          /* (no correction where d or w is infinite) */
 }
 
 __device__ __forceinline__ float act_of(float v, int act)

@@ -47,7 +47,7 @@ def act64(v, act):
     if act == "gelu":
         return v * 0.5 * np.array([math.erfc(-a / math.sqrt(2.0)) for a in v.ravel()]).reshape(v.shape)
     if act == "gelu_tanh":
-        return 0.5 * v * (1.0 + np.tanh(math.sqrt(2.0 / math.pi) * (v + 0.044715 * v ** 3)))
+        return v / (1.0 + np.exp(-2.0 * math.sqrt(2.0 / math.pi) * (v + 0.044715 * v ** 3)))    # (1 + tanh z) / 2 without its cancellation
     return v
 
 

@@ -107,6 +107,35 @@ def test_nonfinite(gpu, k3, x_type, T, inn, out):
     assert torch.equal(y[2:][:, keep], clean[2:][:, keep])
 
 
+@pytest.mark.parametrize("act", lo.ACTS)
+def test_activation_range(gpu, k3, act):
+    """From subnormal to infinite arguments of the activations: one weight of 1, sums exact. v / (1 + e^-z) in fp32
+    is 0 once e^-z passes the largest fp32 number, at z < -88.73: there it is less than |v| 2^-128, which for
+    silu falls with v (|v| e^v) and for gelu_tanh is at |v| < 10 (z = 1.6 v (1 + .045 v^2)): 89 * 2^-128 at most."""
+    say(f"case: {act}")
+    m = torch.logspace(-40, 38.4, 3000, device="cuda", dtype=torch.float64).float()
+    v = torch.cat([m, -m, torch.linspace(-100, 100, 4001, device="cuda"), torch.tensor([0.0, -0.0, float("inf"), -float("inf"), float("nan")], device="cuda")])
+    x = torch.zeros(v.numel(), 64, device="cuda")
+    x[:, 0] = v
+    w = torch.zeros(1, 64, device="cuda", dtype=BF16)
+    w[0, 0] = 1
+    got = lo.f64(lo.linear(k3, x, w, act=act))[:, 0]
+    with np.errstate(all="ignore"):
+        want = lo.act64(lo.f64(v), act)
+    fin = np.isfinite(want)
+    size = np.abs(lo.f64(v) if act == "gelu" else want)[fin]
+    tol = 2.0 ** -21 * size + 2.0 ** -126 * 1.01
+    if act in ("silu", "gelu_tanh"):
+        tol = np.maximum(tol, 89 * 2.0 ** -128)
+    if act == "gelu_tanh":      # z comes out of three roundings, each of which moves e^-z by 2^-24 |z| of itself, |z| < 89 where it counts
+        tol = tol + 3 * 89 * 2.0 ** -24 * size
+    assert (np.abs(got[fin] - want[fin]) <= tol).all()
+    assert np.isnan(got[-1])
+    if act != "gelu" and act != "gelu_tanh" and act != "silu":
+        assert got[-2] == (0 if act == "relu" else -np.inf)
+    assert got[-3] == np.inf
+
+
 @pytest.mark.parametrize("T,inn,out", [(1, 512, 96), (24, 512, 96), (200, 2048, 260), (900, 512, 300)])
 def test_repeats_and_graph(gpu, k3, T, inn, out):
     """The same bits from call to call, on another stream and from a captured graph replayed on new inputs."""
