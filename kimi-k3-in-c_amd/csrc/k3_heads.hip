@@ -4,13 +4,14 @@
  *
  *   u = v / sqrt(mean(v^2) + eps) * w;  pairs of u turn by pos * freq.
  *
- * Bound by HBM: every head is read once and written once. A workgroup takes some tokens and
- * some of their heads; the tokens' cosines and sines, which all heads share, are formed once per
- * workgroup in LDS (per head they would cost more vector time than the rows take to move).
- * A head lies in L lanes of one wave, V elements of 16 bytes (or fewer where a row's
- * alignment, dim or the rotated range ask for it) per load; the other element of a pair (half the
- * rotated range away) is read a second time, out of the L1, rather than fetched from the lane that
- * holds it: the reads of a head all come before its writes, so a head may be written over itself.
+ * Bound by HBM: every head is read once and written once. A wave takes one token and a run of its
+ * heads, 64 >> lsh of them at a time, so nothing waits for another wave. It forms the token's cosines and sines
+ * once, in its part of LDS, and keeps, per element of its lane, the two factors that all heads share: an output is
+ *   r (x A + p B),   A = w cos, B = -+ w' sin (p, w': the pair's other element; A = w, B = 0 outside the rotation),
+ * seven vector instructions an element where the weights, cosines and sines read per head took over twenty.
+ * An element's other one (half the rotated range away) is read a second time, out of the L1, rather than
+ * fetched from the lane that holds it. The next heads' rows are requested before these are worked on; the
+ * reads of a head all come before its writes, so a head may be written over itself.
  */
 #include "k3_common.h"
 #include "k3_dev.h"
@@ -18,8 +19,7 @@
 
 namespace {
 
-constexpr int HD_THREADS = 256;
-constexpr int HD_MAXANG = 2048;          /* angles that fit a workgroup's table (16 KB) */
+constexpr int HD_WAVES = 4;              /* waves of a workgroup, each on its own */
 
 /* cos and sin of a = pos * freq: reduced in fp64 by multiples of pi/2 (taken from it as a sum of two
  * doubles), then the Taylor polynomials to x^15 / x^14 on [-pi/4, pi/4], whose next terms are
@@ -52,136 +52,149 @@ __device__ void turn(double a, float scale, float *c, float *s)
     *s = scale * (float)((k & 2) ? -si : si);
 }
 
+/* V elements as they lie in memory (one load), and as floats */
 template <int TYPE, int V>
 struct Chunk {
-    float f[V];
+    static constexpr int W = TYPE == K3D_F32 ? V : (V + 1) / 2;
+    uint32_t w[W];
+    __device__ __forceinline__ void zero()
+    {
+#pragma unroll
+        for (int i = 0; i < W; i++) w[i] = 0;
+    }
     __device__ __forceinline__ void load(const void *p, size_t i)
     {
-        if constexpr (TYPE == K3D_F32) {
-            if constexpr (V == 4) {
-                const float4 v = *reinterpret_cast<const float4 *>((const float *)p + i);
-                f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
-            } else if constexpr (V == 2) {
-                const float2 v = *reinterpret_cast<const float2 *>((const float *)p + i);
-                f[0] = v.x, f[1] = v.y;
-            } else {
-                f[0] = ((const float *)p)[i];
-            }
-        } else {
-            uint32_t w[(V + 1) / 2];
-            if constexpr (V == 8) {
-                const uint4 v = *reinterpret_cast<const uint4 *>((const uint16_t *)p + i);
-                w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-            } else if constexpr (V == 4) {
-                const uint2 v = *reinterpret_cast<const uint2 *>((const uint16_t *)p + i);
-                w[0] = v.x, w[1] = v.y;
-            } else if constexpr (V == 2) {
-                w[0] = *reinterpret_cast<const uint32_t *>((const uint16_t *)p + i);
-            } else {
-                w[0] = ((const uint16_t *)p)[i];
-            }
-#pragma unroll
-            for (int j = 0; j < V; j++) f[j] = __uint_as_float((j & 1) ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
-        }
+        if constexpr (TYPE == K3D_BF16 && V == 1) w[0] = ((const uint16_t *)p)[i];
+        else __builtin_memcpy(w, __builtin_assume_aligned((const char *)p + i * (TYPE == K3D_F32 ? 4 : 2), W * 4), W * 4);
     }
-    __device__ __forceinline__ void store(void *p, size_t i) const
+    __device__ __forceinline__ float get(int i) const
+    {
+        if constexpr (TYPE == K3D_F32) return __uint_as_float(w[i]);
+        else return __uint_as_float((i & 1) ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    }
+    __device__ __forceinline__ static void store(void *p, size_t i, const float (&f)[V])
     {
         if constexpr (TYPE == K3D_F32) {
-            if constexpr (V == 4) *reinterpret_cast<float4 *>((float *)p + i) = make_float4(f[0], f[1], f[2], f[3]);
-            else if constexpr (V == 2) *reinterpret_cast<float2 *>((float *)p + i) = make_float2(f[0], f[1]);
-            else ((float *)p)[i] = f[0];
+            __builtin_memcpy(__builtin_assume_aligned((float *)p + i, W * 4), f, W * 4);
         } else {
-            uint32_t w[(V + 1) / 2];
+            __bf16 h[V];
 #pragma unroll
-            for (int j = 0; j < V; j += 2)
-                w[j / 2] = (uint32_t)k3_bf16_rne(f[j]) | (j + 1 < V ? (uint32_t)k3_bf16_rne(f[j + 1 < V ? j + 1 : j]) << 16 : 0u);
-            if constexpr (V == 8) *reinterpret_cast<uint4 *>((uint16_t *)p + i) = make_uint4(w[0], w[1], w[2], w[3]);
-            else if constexpr (V == 4) *reinterpret_cast<uint2 *>((uint16_t *)p + i) = make_uint2(w[0], w[1]);
-            else if constexpr (V == 2) *reinterpret_cast<uint32_t *>((uint16_t *)p + i) = w[0];
-            else ((uint16_t *)p)[i] = (uint16_t)w[0];
+            for (int j = 0; j < V; j++) h[j] = (__bf16)f[j];
+            __builtin_memcpy(__builtin_assume_aligned((uint16_t *)p + i, V * 2), h, V * 2);
         }
     }
 };
 
-/* L = 1 << lsh lanes per head, N chunks of V elements per lane; a workgroup takes tokens
- * tpw * blockIdx.x .. and heads hpw * blockIdx.y .. of them (queries first, then keys). */
+/* 1 << lsh lanes per head, N chunks of V elements per lane; `split` waves per token */
 template <int TYPE, int V, int N>
-__global__ __launch_bounds__(HD_THREADS) void heads_kernel(K3kHeads a, int lsh, int tpw, int hpw)
+__global__ __launch_bounds__(64 * HD_WAVES) void heads_kernel(K3kHeads a, int lsh, int split)
 {
-    __shared__ float cs[HD_MAXANG], sn[HD_MAXANG];
-    const int h2 = a.rot / 2, H = a.v[0].heads + a.v[1].heads;
-    const int t0 = blockIdx.x * tpw, nt = min(tpw, a.T - t0);
-    const int g0 = blockIdx.y * hpw, nh = min(hpw, H - g0);
-    for (int i = threadIdx.x; i < nt * h2; i += HD_THREADS)
-        turn((double)a.pos[t0 + i / h2] * a.freq[i % h2], a.rot_scale, &cs[i], &sn[i]);
-    __syncthreads();
-
-    const int L = 1 << lsh, l = threadIdx.x & (L - 1);
+    extern __shared__ float turns[];
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = blockIdx.x * HD_WAVES + wv, t = wave / split, part = wave % split;
+    if (t >= a.T) return;
+    const double f0 = lane < a.rot / 2 ? a.freq[lane] : 0.0;
+    const int pos = a.pos ? a.pos[t] : 0;
+    if (pos < 0) return;
+    const int h2 = a.rot / 2, L = 1 << lsh, l = lane & (L - 1), HP = 64 >> lsh;
+    const int H = a.v[0].heads + a.v[1].heads, first = (int)((long)H * part / split), last = (int)((long)H * (part + 1) / split);
+    float *const cs = turns + (size_t)wv * a.rot, *const sn = cs + h2;
     const float rdim = 1.0f / (float)a.dim;
-    for (int it = threadIdx.x >> lsh; it < nt * nh; it += HD_THREADS >> lsh) {
-        const int tt = it / nh, t = t0 + tt, gh = g0 + it % nh;
-        if (a.pos && a.pos[t] < 0) continue;
-        const int side = gh >= a.v[0].heads, h = side ? gh - a.v[0].heads : gh;
-        const void *in = a.v[side].in;
-        const size_t ib = (size_t)t * a.v[side].ld + (size_t)h * a.v[side].hs;
-        const size_t ob = (size_t)t * a.v[side].ldo + (size_t)h * a.v[side].hso;
-        const float *w = a.v[side].w;
+    bool turned = false;
+
+    for (int side = 0; side < 2; side++) {
+        const int off = side ? a.v[0].heads : 0;
+        const int hb = max(first, off) - off, he = min(last, off + a.v[side].heads) - off;
+        if (hb >= he) continue;
+        const void *const in = a.v[side].in;
+        void *const out = a.v[side].out;
+        const size_t ib = (size_t)t * a.v[side].ld, ob = (size_t)t * a.v[side].ldo;
+        const float *const w = a.v[side].w;
         Chunk<TYPE, V> u[N], o[N];
-        float ss = 0.0f;
+        auto load = [&](int h) {
+            if (h >= he) h = he - 1;        /* (lanes without a head repeat the last one's reads) */
+            const size_t at = ib + (size_t)h * a.v[side].hs;
 #pragma unroll
-        for (int j = 0; j < N; j++) {
-            const int e = (l + j * L) * V;
-            if (e >= a.dim) continue;
-            u[j].load(in, ib + e);
-            const int r = e - a.rot_off;
-            if (r >= 0 && r < a.rot) {
-                if (a.pairs == K3D_ROT_HALVES) o[j].load(in, ib + (r < h2 ? e + h2 : e - h2));
-                else if (V == 1) o[j].load(in, ib + (r & 1 ? e - 1 : e + 1));
+            for (int j = 0; j < N; j++) {
+                const int e = (l + j * L) * V, r = e - a.rot_off;
+                u[j].zero();
+                o[j].zero();
+                if (e >= a.dim) continue;
+                u[j].load(in, at + e);
+                if (r < 0 || r >= a.rot) continue;
+                if (a.pairs == K3D_ROT_HALVES) o[j].load(in, at + (r < h2 ? e + h2 : e - h2));
+                else if (V == 1) o[j].load(in, at + (r & 1 ? e - 1 : e + 1));
             }
-#pragma unroll
-            for (int i = 0; i < V; i++) ss = fmaf(u[j].f[i], u[j].f[i], ss);
+        };
+        load(hb + (lane >> lsh));
+        if (!turned) {
+            for (int i = lane; i < h2; i += 64) turn((double)pos * (i < 64 ? f0 : a.freq[i]), a.rot_scale, &cs[i], &sn[i]);
+            __builtin_amdgcn_wave_barrier();
+            turned = true;
         }
-        for (int x = L >> 1; x; x >>= 1) ss += __shfl_xor(ss, x);
-        const float rs = 1.0f / sqrtf(fmaf(ss, rdim, a.eps));
+        float A[N][V], B[N][V];
 #pragma unroll
         for (int j = 0; j < N; j++) {
-            const int e = (l + j * L) * V;
+            const int e = (l + j * L) * V, r = e - a.rot_off;       /* (a chunk lies in or outside the range as a whole) */
+#pragma unroll
+            for (int i = 0; i < V; i++) A[j][i] = 1.0f, B[j][i] = 0.0f;
             if (e >= a.dim) continue;
-            const int r = e - a.rot_off;
-            if (w)
+            if (w) __builtin_memcpy(A[j], w + e, V * 4);
+            if (r < 0 || r >= a.rot) continue;
+            if (a.pairs == K3D_ROT_HALVES) {
+                const bool one = r < h2;
+                const int k = one ? r : r - h2;
+                float c[V], d[V];
+                if (w) __builtin_memcpy(B[j], w + (one ? e + h2 : e - h2), V * 4);
+                __builtin_memcpy(c, __builtin_assume_aligned(cs + k, V * 4), V * 4);
+                __builtin_memcpy(d, __builtin_assume_aligned(sn + k, V * 4), V * 4);
 #pragma unroll
-                for (int i = 0; i < V; i++) u[j].f[i] *= rs * w[e + i];
-            else
+                for (int i = 0; i < V; i++) {
+                    const float q = w ? B[j][i] * d[i] : d[i];
+                    A[j][i] *= c[i];
+                    B[j][i] = one ? -q : q;
+                }
+            } else {
 #pragma unroll
-                for (int i = 0; i < V; i++) u[j].f[i] *= rs;
-            if (r >= 0 && r < a.rot) {
-                const float *c = cs + tt * h2, *s = sn + tt * h2;
-                if (a.pairs == K3D_ROT_HALVES) {
-                    const bool first = r < h2;
-                    const int p = first ? e + h2 : e - h2, k = first ? r : r - h2;
-#pragma unroll
-                    for (int i = 0; i < V; i++) {
-                        const float x = o[j].f[i] * (w ? rs * w[p + i] : rs);
-                        u[j].f[i] = fmaf(u[j].f[i], c[k + i], first ? -x * s[k + i] : x * s[k + i]);
-                    }
-                } else if constexpr (V == 1) {
-                    const int p = r & 1 ? e - 1 : e + 1;
-                    const float x = o[j].f[0] * (w ? rs * w[p] : rs);
-                    u[j].f[0] = fmaf(u[j].f[0], c[r / 2], r & 1 ? x * s[r / 2] : -x * s[r / 2]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; i += 2) {
-                        const float x = u[j].f[i], y = u[j].f[i + 1], cc = c[(r + i) / 2], sc = s[(r + i) / 2];
-                        u[j].f[i] = fmaf(x, cc, -y * sc);
-                        u[j].f[i + 1] = fmaf(y, cc, x * sc);
-                    }
+                for (int i = 0; i < V; i++) {
+                    const bool one = !((r + i) & 1);
+                    const float p = V > 1 ? (w ? w[e + (i ^ (V > 1))] : 1.0f) : w ? w[one ? e + 1 : e - 1] : 1.0f;
+                    const float q = p * sn[(r + i) / 2];
+                    A[j][i] *= cs[(r + i) / 2];
+                    B[j][i] = one ? -q : q;
                 }
             }
         }
+        for (int h = hb + (lane >> lsh); h - (lane >> lsh) < he; h += HP) {
+            float x[N][V], y[N][V], ss = 0.0f;
 #pragma unroll
-        for (int j = 0; j < N; j++) {
-            const int e = (l + j * L) * V;
-            if (e < a.dim) u[j].store(a.v[side].out, ob + e);
+            for (int j = 0; j < N; j++)
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    x[j][i] = u[j].get(i);
+                    y[j][i] = V > 1 && a.pairs == K3D_ROT_INTERLEAVED ? u[j].get(i ^ (V > 1)) : o[j].get(i);
+                    ss = fmaf(x[j][i], x[j][i], ss);
+                }
+            if (h - (lane >> lsh) + HP < he) load(h + HP);
+            for (int q = L >> 1; q; q >>= 1) ss += __shfl_xor(ss, q);
+            const float rs = 1.0f / sqrtf(fmaf(ss, rdim, a.eps));
+            if (h < he) {
+                const size_t at = ob + (size_t)h * a.v[side].hso;
+#pragma unroll
+                for (int j = 0; j < N; j++) {
+                    const int e = (l + j * L) * V, r = e - a.rot_off;
+                    if (e >= a.dim) continue;
+                    float f[V];
+                    if (r >= 0 && r < a.rot) {
+#pragma unroll
+                        for (int i = 0; i < V; i++) f[i] = rs * fmaf(x[j][i], A[j][i], y[j][i] * B[j][i]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < V; i++) f[i] = rs * (x[j][i] * A[j][i]);
+                    }
+                    Chunk<TYPE, V>::store(out, at + e, f);
+                }
+            }
         }
     }
 }
@@ -201,35 +214,43 @@ bool fits(const K3kHeads *a, int v)
     return a->rot_off % v == 0 && (a->pairs == K3D_ROT_HALVES ? (a->rot / 2) % v == 0 : a->rot % v == 0);
 }
 
+/* A token's heads go over several waves while there are fewer waves than this per CU to keep the memory busy: 4 a SIMD
+ * (777 tokens of 13 heads of 192 in fp32 8.1 us, 8.6 with 2 and 9.5 with 8; 4096 of 72 of 128 27.4, with 8 29.7;
+ * 2000 of 72 of 256 27.3, 28.6 with 2 or 8). */
+constexpr long HD_WANT = 16;
+
 template <int TYPE, int V, int N>
 void launch(const K3kHeads *a, hipStream_t st)
 {
     const int chunks = (a->dim / V + N - 1) / N;
     int lsh = 0;
     while ((1 << lsh) < chunks) lsh++;
-    const int per = HD_THREADS >> lsh, H = a->v[0].heads + a->v[1].heads;   /* heads at a time */
-    int tpw = H < per ? per / H : 1;
-    if (tpw > a->T) tpw = a->T;
-    while (tpw > 1 && tpw * (a->rot / 2) > HD_MAXANG) tpw--;
-    const long cus = k3k_cu_count();
-    int hpw = H;
-    /* few tokens: their heads over more workgroups */
-    while (hpw > per && (long)((a->T + tpw - 1) / tpw) * ((H + hpw - 1) / hpw) < 2 * cus) hpw = (hpw + 1) / 2;
-    const dim3 grid((a->T + tpw - 1) / tpw, (H + hpw - 1) / hpw);
-    heads_kernel<TYPE, V, N><<<grid, HD_THREADS, 0, st>>>(*a, lsh, tpw, hpw);
+    const int HP = 64 >> lsh, H = a->v[0].heads + a->v[1].heads, passes = (H + HP - 1) / HP;
+    const long want = HD_WANT * k3k_cu_count();
+    int split = (int)((want + a->T - 1) / a->T);
+    if (split > passes) split = passes;
+    const long waves = (long)a->T * split;
+    heads_kernel<TYPE, V, N><<<(unsigned)((waves + HD_WAVES - 1) / HD_WAVES), 64 * HD_WAVES, (size_t)HD_WAVES * a->rot * 4, st>>>(*a, lsh, split);
 }
 
+/* a head of up to 1024 elements in at most 64 lanes */
 template <int TYPE, int V>
 void pick(const K3kHeads *a, hipStream_t st)
 {
-    const int c = a->dim / V;
-    if (c <= 64) launch<TYPE, V, 1>(a, st);
-    else if (c <= 128) launch<TYPE, V, 2>(a, st);
-    else if (c <= 256) launch<TYPE, V, 4>(a, st);
-    else if constexpr (V <= 2) {
-        if (c <= 512) launch<TYPE, V, 8>(a, st);
-        else if constexpr (V == 1) launch<TYPE, V, 16>(a, st);
-    }
+    const int c = a->dim / V, n = (c + 63) / 64;
+    /* Three times a power of two: three chunks a lane leave no lane idle (4096 tokens of 192 heads of 192 in bf16 164 -> 123 us),
+     * where they leave waves enough (777 of 13 in fp32 8.2 us with one chunk, 9.4 with three). */
+    if constexpr (V == (TYPE == K3D_F32 ? 4 : 8))
+        if (c % 3 == 0 && c <= 192 && ((c / 3) & (c / 3 - 1)) == 0 &&
+            (long)a->T * (a->v[0].heads + a->v[1].heads) * (c / 3) / 64 >= HD_WANT * k3k_cu_count())
+            return launch<TYPE, V, 3>(a, st);
+    if (n <= 1) return launch<TYPE, V, 1>(a, st);
+    if (n <= 2) return launch<TYPE, V, 2>(a, st);
+    if constexpr (V <= 4)
+        if (n <= 4) return launch<TYPE, V, 4>(a, st);
+    if constexpr (V <= 2)
+        if (n <= 8) return launch<TYPE, V, 8>(a, st);
+    if constexpr (V == 1) launch<TYPE, V, 16>(a, st);
 }
 
 }  // namespace
