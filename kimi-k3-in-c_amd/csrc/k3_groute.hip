@@ -10,12 +10,13 @@
  * exponential was rounded to 32; but few experts are close to a border. So lane l holds the choices of experts
  * l + 64 i in fp32, each within a bound E of its definition (the same E for the wave), and what fp32 leaves open is
  * settled in 64 bits:
- *  - groups: their values within 2 E; where the last kept group and the first one left out lie closer, the
- *    token is routed in 64 bits throughout (route_exact);
+ *  - groups: their values within 2 E; where the last kept group and the first one left out lie closer, every group's
+ *    value is formed again in 64 bits;
  *  - top-k: the k-th largest of the lanes' maxima is at most the k-th largest choice, so only choices of at least
  *    that less 2 E can be selected: about 1.3 topk of them. They are packed, a lane each, computed in 64 bits, and
- *    ranked by counting, equal ones by their order. More than 64 (rows of equal logits): route_exact.
- * 8192 tokens of 896 experts, top 16 in 4 of 8 groups: NEW_US us, 205 with every choice in 64 bits and topk rounds of
+ *    ranked by counting, equal ones by their order. More than 64 (rows of equal logits): every choice in 64 bits and
+ *    topk rounds of wave maxima (route_exact).
+ * 8192 tokens of 896 experts, top 16 in 4 of 8 groups: 23 us, 205 with every choice in 64 bits and topk rounds of
  * wave maxima; its bytes take 6 us at the rate of a copy. Bound by vector instructions, about 50 per expert row of
  * 64; one token by the latency of its chain.
  */
@@ -25,13 +26,6 @@
 #include "k3k.h"
 
 namespace {
-
-__device__ __forceinline__ double wave_sum_f64(double v)
-{
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
 
 /* order-preserving bits of a choice; 0 for one that cannot be taken (NaN, -inf) */
 __device__ __forceinline__ uint64_t choice_key(double c)
@@ -45,6 +39,15 @@ __device__ __forceinline__ double key_value(uint64_t k)
 {
     return __longlong_as_double((long long)((k >> 63) ? k & 0x7fffffffffffffffull : ~k));
 }
+
+/* order-preserving bits of an fp32 choice, 0 for one that cannot be taken */
+__device__ __forceinline__ uint32_t choice_key32(float c)
+{
+    const uint32_t b = __float_as_uint(c);
+    return c > -INFINITY ? ((b >> 31) ? ~b : b | 0x80000000u) : 0u;
+}
+
+__device__ __forceinline__ float key32_value(uint32_t k) { return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k); }
 
 template <int TYPE>
 __device__ __forceinline__ float load_logit(const void *p, size_t i)
@@ -100,22 +103,21 @@ __device__ __forceinline__ uint64_t key64(const K3kRoute &a, float l, int e, flo
     return l > -INFINITY ? k : 0ull;
 }
 
+template <int CTRL>
+__device__ __forceinline__ float dpp_f32(float v)
+{
+    return __uint_as_float(dpp_u32<CTRL, 0xf, 0u>(__float_as_uint(v)));
+}
+
 __device__ __forceinline__ uint64_t lane64(uint64_t v, int l)
 {
     return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32) |
            (uint32_t)__builtin_amdgcn_readlane((int)v, l);
 }
 
-/* order-preserving bits of an fp32 choice, 0 for one that cannot be taken */
-__device__ __forceinline__ uint32_t choice_key32(float c)
-{
-    const uint32_t b = __float_as_uint(c);
-    return c > -INFINITY ? ((b >> 31) ? ~b : b | 0x80000000u) : 0u;
-}
-
-/* The token's experts with every choice in 64 bits: lane j gets the j-th, or -1. keys: n of LDS. */
+/* The token's experts with every choice in 64 bits, of those with c > -inf: lane j gets the j-th, or -1. */
 template <int TYPE, int P, int SCORE>
-__device__ int route_exact(const K3kRoute &a, size_t row, float m, double sum, uint64_t *keys)
+__device__ int route_exact(const K3kRoute &a, size_t row, float m, double sum, const float (&c)[P])
 {
     const int lane = threadIdx.x & 63, n = a.n;
     /* (the compiler must not keep what the other path formed from these loads: it would be P doubles) */
@@ -123,39 +125,10 @@ __device__ int route_exact(const K3kRoute &a, size_t row, float m, double sum, u
     uint64_t key[P];
 #pragma unroll
     for (int i = 0; i < P; i++) {
-        const int e = lane + 64 * i, in = min(e, n - 1);
+        const int in = min(lane + 64 * i, n - 1);
         const uint64_t k = key64<SCORE>(a, load_logit<TYPE>(a.logits, row + in), in, m, sum);
-        key[i] = e < n ? k : 0ull;
+        key[i] = c[i] > -INFINITY ? k : 0ull;
         __builtin_amdgcn_sched_barrier(0);      /* (one after another: side by side they take ten registers each) */
-    }
-    if (a.top_groups < a.n_groups) {
-        /* a group per lane: its value; then every lane counts the groups above its own */
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int i = 0; i < P; i++)
-            if (lane + 64 * i < n) keys[lane + 64 * i] = key[i];
-        __builtin_amdgcn_wave_barrier();
-        const int gs = n / a.n_groups;
-        uint64_t v = 0ull;
-        if (lane < a.n_groups) {
-            uint64_t k1 = 0ull, k2 = 0ull;
-            for (int j = 0; j < gs; j++) {
-                const uint64_t k = keys[lane * gs + j];
-                k2 = k > k1 ? k1 : k > k2 ? k : k2;
-                k1 = k > k1 ? k : k1;
-            }
-            v = k1;
-            if (a.group_top == 2 && k2) v = choice_key(key_value(k1) + key_value(k2));
-        }
-        int rank = 0;
-        for (int g = 0; g < a.n_groups; g++) {
-            const uint64_t o = lane64(v, g);
-            rank += o > v || (o == v && g < lane);
-        }
-        const uint64_t keep = __ballot(lane < a.n_groups && v && rank < a.top_groups);
-#pragma unroll
-        for (int i = 0; i < P; i++)
-            if (!((keep >> ((lane + 64 * i) / gs & 63)) & 1)) key[i] = 0ull;
     }
     /* topk rounds: the wave's largest key, of equals the lowest expert */
     int mine = -1;
@@ -184,7 +157,7 @@ __device__ int route_exact(const K3kRoute &a, size_t row, float m, double sum, u
 
 /* P: experts per lane. LDS per wave: lds bytes (the wave's choices by expert where there are groups, 64 candidates) */
 template <int TYPE, int P, int SCORE>
-__global__ __launch_bounds__(256) void route_kernel(K3kRoute a, int lds)
+__global__ __launch_bounds__(256, P <= 14 ? 5 : 1) void route_kernel(K3kRoute a, int lds)
 {
     extern __shared__ uint64_t smem[];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -206,8 +179,8 @@ __global__ __launch_bounds__(256) void route_kernel(K3kRoute a, int lds)
     if constexpr (SCORE == K3D_SCORE_SOFTMAX) {
 #pragma unroll
         for (int i = 0; i < P; i++) m = fmaxf(m, c[i]);         /* (fmaxf passes over NaN) */
-#pragma unroll
-        for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        const uint32_t km = wave_reduce_u32<true>(choice_key32(m));
+        m = km ? key32_value(km) : -INFINITY;
         float s[P];
 #pragma unroll
         for (int i = 0; i < P; i++) {
@@ -216,7 +189,7 @@ __global__ __launch_bounds__(256) void route_kernel(K3kRoute a, int lds)
             s[i] = (float)q;
             if (i % 2) __builtin_amdgcn_sched_barrier(0);
         }
-        sum = wave_sum_f64(sum);
+        sum = wave_total_f64(sum);
         const float inv = (float)(1.0 / sum);
 #pragma unroll
         for (int i = 0; i < P; i++) c[i] = c[i] > -INFINITY ? s[i] * inv : -INFINITY;
@@ -227,9 +200,11 @@ __global__ __launch_bounds__(256) void route_kernel(K3kRoute a, int lds)
             c[i] = c[i] > -INFINITY ? s : -INFINITY;
         }
     }
-    /* The bound E. A sigmoid: the exponent's rounding moves e^-l by (|l| + 4) 2^-23 of itself; where |l| > 64 the score is within
-     * 2^-90 of 0 or 1. So 2^-16 of the score, and 2^-23 of the choice for the additions and the reciprocal.
-     * The softmax is closer. */
+    /* The bound E. A sigmoid: the exponent's rounding and the exponential move e^-l by (0.7 |l| + 1) 2^-23 of itself, the
+     * score s by s (1 - s) times that, which is at most 0.5 * 2^-23, and the sum's and the reciprocal's roundings by
+     * 1.5 * 2^-23 s: under 2^-22 for any l, and where all scores are small, (|l| + 4) 2^-23 of them for |l| up to 64 (past it they are
+     * within 2^-90 of 0 or 1). The softmax: three roundings of a score. Twice that, and 2^-22 of the largest choice for
+     * the additions of the bias and of a group's two choices. */
     float top_s = 0.0f, top_c = 0.0f;
 #pragma unroll
     for (int i = 0; i < P; i++) {
@@ -242,9 +217,9 @@ __global__ __launch_bounds__(256) void route_kernel(K3kRoute a, int lds)
     /* (positive floats compare as their bits) */
     top_s = __uint_as_float(wave_reduce_u32<true>(__float_as_uint(top_s)));
     top_c = __uint_as_float(wave_reduce_u32<true>(__float_as_uint(top_c)));
-    const float E = fmaf(0x1p-16f, top_s, fmaf(0x1p-22f, top_c, 0x1p-80f));
+    const float Es = SCORE == K3D_SCORE_SIGMOID ? fminf(0x1p-21f, 0x1p-15f * top_s) : 0x1p-21f * top_s;
+    const float E = fmaf(0x1p-22f, top_c, Es + 0x1p-80f);
 
-    bool sure = true;
     if (a.top_groups < a.n_groups) {
         /* 64 / n_groups lanes (a power of two of them) take a group: its two largest choices */
 #pragma unroll
@@ -255,74 +230,97 @@ __global__ __launch_bounds__(256) void route_kernel(K3kRoute a, int lds)
         const int g = lane >> lsh;
         float k1 = -INFINITY, k2 = -INFINITY;
         if (g < a.n_groups)
+#pragma unroll 4
             for (int j = lane & (LG - 1); j < gs; j += LG) {
                 const float v = ch[g * gs + j];
                 k2 = fmaxf(k2, fminf(k1, v));
                 k1 = fmaxf(k1, v);
             }
-        for (int o = LG >> 1; o; o >>= 1) {
-            const float o1 = __shfl_xor(k1, o), o2 = __shfl_xor(k2, o);
+        auto meet = [&](float o1, float o2) {
             k2 = fmaxf(fmaxf(k2, o2), fminf(k1, o1));
             k1 = fmaxf(k1, o1);
-        }
+        };
+        /* (neighbours, pairs, quads, eights by mirroring: every lane of a part holds the same) */
+        if (LG >= 2) meet(dpp_f32<0xB1>(k1), dpp_f32<0xB1>(k2));
+        if (LG >= 4) meet(dpp_f32<0x4E>(k1), dpp_f32<0x4E>(k2));
+        if (LG >= 8) meet(dpp_f32<0x141>(k1), dpp_f32<0x141>(k2));
+        if (LG >= 16) meet(dpp_f32<0x140>(k1), dpp_f32<0x140>(k2));
+        if (LG >= 32) meet(__shfl_xor(k1, 16), __shfl_xor(k2, 16));
         const float v = a.group_top == 2 && k2 > -INFINITY ? k1 + k2 : k1;
         int rank = 0;
         for (int q = 0; q < a.n_groups; q++) {
             const float o = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), q << lsh));
             rank += o > v || (o == v && q < g);
         }
-        const bool keep = g < a.n_groups && v > -INFINITY && rank < a.top_groups;
+        bool keep = g < a.n_groups && v > -INFINITY && rank < a.top_groups;
         /* the least kept and the largest left out (as order-preserving bits; no group: the far end) */
         const uint32_t kv = choice_key32(v);
         const uint32_t in = wave_reduce_u32<false>(keep ? kv : 0xffffffffu);
         const uint32_t out = wave_reduce_u32<true>(keep || g >= a.n_groups ? 0u : kv);
-        if (out) {
-            const float least = __uint_as_float((in >> 31) ? in & 0x7fffffffu : ~in), most = __uint_as_float((out >> 31) ? out & 0x7fffffffu : ~out);
-            sure = least - most > 4.0f * E;     /* (each within 2 E; false where both are infinite) */
+        /* (each within 2 E of its definition; not where both are infinite) */
+        if (out && !(key32_value(in) - key32_value(out) > 4.0f * E)) {
+            uint64_t x1 = 0ull, x2 = 0ull;
+            if (g < a.n_groups)
+                for (int j = lane & (LG - 1); j < gs; j += LG) {
+                    const int e = g * gs + j;
+                    const uint64_t k = key64<SCORE>(a, load_logit<TYPE>(a.logits, row + e), e, m, sum);
+                    x2 = k > x1 ? x1 : k > x2 ? k : x2;
+                    x1 = k > x1 ? k : x1;
+                }
+            for (int o = LG >> 1; o; o >>= 1) {
+                const uint64_t o1 = __shfl_xor(x1, o), o2 = __shfl_xor(x2, o), less = x1 < o1 ? x1 : o1;
+                x1 = x1 > o1 ? x1 : o1;
+                x2 = x2 > o2 ? x2 : o2;
+                x2 = x2 > less ? x2 : less;
+            }
+            const uint64_t x = a.group_top == 2 && x2 ? choice_key(key_value(x1) + key_value(x2)) : x1;
+            rank = 0;
+            for (int q = 0; q < a.n_groups; q++) {
+                const uint64_t o = lane64(x, q << lsh);
+                rank += o > x || (o == x && q < g);
+            }
+            keep = g < a.n_groups && x && rank < a.top_groups;
         }
-        if (sure) {
-            if (!keep && g < a.n_groups)
-                for (int j = lane & (LG - 1); j < gs; j += LG) ch[g * gs + j] = -INFINITY;
-            __builtin_amdgcn_wave_barrier();
+        if (!keep && g < a.n_groups)
+            for (int j = lane & (LG - 1); j < gs; j += LG) ch[g * gs + j] = -INFINITY;
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int i = 0; i < P; i++)
-                if (lane + 64 * i < n) c[i] = ch[lane + 64 * i];
-        }
+        for (int i = 0; i < P; i++)
+            if (lane + 64 * i < n) c[i] = ch[lane + 64 * i];
     }
 
     int ncand = 0;
-    if (sure) {
-        /* a bound that at least topk lanes' maxima reach (fewer lanes with any: all choices), by halving the keys' range */
-        float lm = c[0];
+    /* a bound that at least topk lanes' maxima reach (fewer lanes with any: all choices), by halving the keys' range */
+    float lm = c[0];
 #pragma unroll
-        for (int i = 1; i < P; i++) lm = fmaxf(lm, c[i]);
-        const uint32_t km = choice_key32(lm);
-        uint32_t lo = 0, hi = wave_reduce_u32<true>(km);
-        if (__popcll(__ballot(km != 0u)) >= a.topk) {
-            lo = wave_reduce_u32<false>(km ? km : 0xffffffffu);
-            if (a.topk == 1) lo = hi;
-            for (int q = 0; q < 14 && lo < hi; q++) {
-                const uint32_t mid = lo + ((hi - lo + 1) >> 1);
-                if (__popcll(__ballot(km >= mid)) >= a.topk) lo = mid;
-                else hi = mid - 1;
-            }
+    for (int i = 1; i < P; i++) lm = fmaxf(lm, c[i]);
+    const uint32_t km = choice_key32(lm);
+    uint32_t lo = 0, hi = wave_reduce_u32<true>(km);
+    if (__popcll(__ballot(km != 0u)) >= a.topk) {
+        lo = wave_reduce_u32<false>(km ? km : 0xffffffffu);
+        if (a.topk == 1) lo = hi;
+        for (int q = 0; q < 12 && lo < hi; q++) {
+            const uint32_t mid = lo + ((hi - lo + 1) >> 1);
+            const int above = __popcll(__ballot(km >= mid));
+            if (above >= a.topk) lo = mid;
+            else hi = mid - 1;
+            if (above == a.topk) break;
         }
-        const float thr = lo ? __uint_as_float((lo >> 31) ? lo & 0x7fffffffu : ~lo) : -INFINITY;
-        const float least = thr < INFINITY ? fmaf(-2.0f, E, thr) : thr;
-        /* the candidates, in the experts' order */
+    }
+    const float thr = lo ? key32_value(lo) : -INFINITY;
+    const float least = thr < INFINITY ? fmaf(-2.0f, E, thr) : thr;
+    /* the candidates, in the experts' order */
 #pragma unroll
-        for (int i = 0; i < P; i++) {
-            const bool in = c[i] >= least && c[i] > -INFINITY;
-            const uint64_t who = __ballot(in);
-            const int slot = ncand + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
-            if (in && slot < 64) cand[slot] = lane + 64 * i;
-            ncand += __popcll(who);
-        }
-        sure = ncand <= 64;
+    for (int i = 0; i < P; i++) {
+        const bool in = c[i] >= least && c[i] > -INFINITY;
+        const uint64_t who = __ballot(in);
+        const int slot = ncand + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+        if (in && slot < 64) cand[slot] = lane + 64 * i;
+        ncand += __popcll(who);
     }
     __builtin_amdgcn_wave_barrier();
     int mine = -1, at = lane;                   /* the lane's expert and its place */
-    if (sure) {
+    if (ncand <= 64) {
         uint64_t key = 0ull;
         if (lane < ncand) {
             mine = cand[lane];
@@ -338,12 +336,12 @@ __global__ __launch_bounds__(256) void route_kernel(K3kRoute a, int lds)
         /* places that no candidate takes */
         if (lane >= ncand && lane < a.topk) at = lane;
     } else {
-        mine = route_exact<TYPE, P, SCORE>(a, row, m, sum, reinterpret_cast<uint64_t *>(ch));
+        mine = route_exact<TYPE, P, SCORE>(a, row, m, sum, c);
     }
     double w = 0.0;
     if (mine >= 0) w = score64<SCORE>(load_logit<TYPE>(a.logits, row + mine), m, sum);
     if (a.renorm) {
-        const double s = wave_sum_f64(w);
+        const double s = wave_total_f64(w);
         w = s > 0.0 ? w / s : 0.0;
     }
     if (at < a.topk) {
@@ -356,7 +354,7 @@ template <int TYPE, int P, int SCORE>
 void launch(const K3kRoute *a, hipStream_t st)
 {
     const int waves = a->T < 1024 ? 1 : 4;
-    const int lds = 256 + (a->top_groups < a->n_groups ? (a->n * 8 + 255) / 256 * 256 : 0);
+    const int lds = 256 + (a->top_groups < a->n_groups ? (a->n * 4 + 255) / 256 * 256 : 0);
     route_kernel<TYPE, P, SCORE><<<(a->T + waves - 1) / waves, 64 * waves, (size_t)waves * lds, st>>>(*a, lds);
 }
 
