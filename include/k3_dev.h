@@ -197,10 +197,11 @@ enum { K3D_F32 = 0, K3D_BF16 = 1 };
  * their elements. fp32 x counts in full: cut into three bf16 terms that hold all 24 bits of it
  * (an infinite weight then gives NaN where it meets a finite x). Sums, bias, activation and
  * residual are formed in fp32 and rounded once to y_type. Which kernel runs, and with it the order
- * of a sum, goes by the shape, the types and the alignment; a call's bits repeat. in, ldx and ldw up to
- * K3D_LINEAR_MAX_LD. y must not overlap x, W, bias or ws. */
+ * of a sum, goes by the shape, the types and the alignment; a call's bits repeat. ldx and ldw up to
+ * K3D_LINEAR_MAX_LD, in up to K3D_LINEAR_MAX_IN. y must not overlap x, W, bias or ws. */
 enum { K3D_ACT_NONE = 0, K3D_ACT_RELU = 1, K3D_ACT_SILU = 2, K3D_ACT_GELU = 3 /* erf */, K3D_ACT_GELU_TANH = 4 };
 #define K3D_LINEAR_MAX_LD (1 << 22)
+#define K3D_LINEAR_MAX_IN (1 << 20)
 size_t k3d_linear_ws(int T, int in, int out, int x_type);
 int k3d_linear(void *y, int y_type, long ldy, const void *x, int x_type, long ldx, int T, const uint16_t *W,
                long ldw, int in, int out, const float *bias, int act, const void *res, long ldr, void *ws,

@@ -38,7 +38,8 @@ int k3d_linear(void *y, int y_type, long ldy, const void *x, int x_type, long ld
     if (T < 0 || out < 0 || in < 1) return k3dx_bad("k3d_linear: need T >= 0, out >= 0, in >= 1");
     if (T == 0 || out == 0) return 0;
     if (ldx < in || ldw < in || ldy < out || (res && ldr < out)) return k3dx_bad("k3d_linear: a stride is shorter than its row");
-    if (ldx > K3D_LINEAR_MAX_LD || ldw > K3D_LINEAR_MAX_LD) return k3dx_bad("k3d_linear: ldx and ldw up to K3D_LINEAR_MAX_LD");
+    if (ldx > K3D_LINEAR_MAX_LD || ldw > K3D_LINEAR_MAX_LD || in > K3D_LINEAR_MAX_IN)
+        return k3dx_bad("k3d_linear: ldx and ldw up to K3D_LINEAR_MAX_LD, in up to K3D_LINEAR_MAX_IN");
     if (!y || !x || !W) return k3dx_bad("k3d_linear: y, x and W must be given");
     if (res == y && ldr != ldy) return k3dx_bad("k3d_linear: res in y's place needs y's stride");
     if (!aligned(y, type_size(y_type)) || !aligned(res, type_size(y_type)) || !aligned(x, type_size(x_type)) ||

@@ -521,17 +521,16 @@ __device__ __forceinline__ void tile_of(const LinTile &p, int b, int &tt, int &t
     tt = q * GT + r % h;
 }
 
-template <int BT, int BO, int WT, int WO, int NST, bool WREG>
+template <int BT, int BO, int WT, int WO, int NST, bool WREG, int POL>
 __global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
 {
     constexpr int NW = WT * WO, FT = BT / WT / 16, FO = BO / WO / 16;
     constexpr int XD = BT / 8 / NW, WD = WREG ? 0 : BO / 8 / NW, DN = XD + WD;      /* DMAs of a wave per step */
     constexpr int WR = WREG ? BO * 8 / (64 * NW) : 1;                                /* 16-byte pieces of W per thread */
     constexpr int FG = FO % 4 == 0 ? 4 : FO % 2 == 0 ? 2 : 1;       /* fragments that share a run of outputs */
-    static_assert(XD >= 1 && (WREG || WD >= 1) && NST >= 2 && NST <= 8, "tile");
+    static_assert(XD >= 1 && (WREG || WD >= 1) && NST >= 2 && NST <= 4, "tile");
     constexpr int SZ = (BT + BO) * LIN_KS;
-    __shared__ __attribute__((aligned(1024))) uint16_t S0[SZ], S1[SZ], S2[NST > 2 ? SZ : 8], S3[NST > 3 ? SZ : 8], S4[NST > 4 ? SZ : 8],
-        S5[NST > 5 ? SZ : 8], S6[NST > 6 ? SZ : 8], S7[NST > 7 ? SZ : 8];
+    __shared__ __attribute__((aligned(1024))) uint16_t S0[SZ], S1[SZ], S2[NST > 2 ? SZ : 8], S3[NST > 3 ? SZ : 8];
 
     const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -569,11 +568,7 @@ __global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
         if constexpr (S == 0) return S0;
         else if constexpr (S == 1) return S1;
         else if constexpr (S == 2) return S2;
-        else if constexpr (S == 3) return S3;
-        else if constexpr (S == 4) return S4;
-        else if constexpr (S == 5) return S5;
-        else if constexpr (S == 6) return S6;
-        else return S7;
+        else return S3;
     };
     /* Stages are requested in order: step `xk` of x, which is column block `wk` of W (of a term), the last one
      * of a row from where its 64 columns end with the row. Past the slice: zeros, so that every step requests
@@ -587,29 +582,47 @@ __global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
 #pragma unroll
         for (int i = 0; i < XD; i++) k3_dma16(rx, b + (i * NW + wv) * 8 * LIN_KS, xo[i] | none, xs);
 #pragma unroll
-        for (int i = 0; i < WD; i++) k3_dma16(rw, b + (BT + (i * NW + wv) * 8) * LIN_KS, wo_[i] | none, ws);
+        for (int i = 0; i < WD; i++) k3_dma16<POL>(rw, b + (BT + (i * NW + wv) * 8) * LIN_KS, wo_[i] | none, ws);
         xk++;
         if (++wk == p.nks) wk = 0;
     };
-    /* weights at any alignment: through registers */
-    uint4 wr[WR];
-    int gk = k0 % p.nks;
-    auto wload = [&]() {
+    /* Weights at any alignment: through registers, requested NST steps before they are stored (the hardware loads 16
+     * bytes from any address). A piece that passes the end of its row is read from 8 elements before it and
+     * shifted when it is stored; past the slice the last block comes again. */
+    uint4 wr[WREG ? NST : 1][WR];
+    const uint16_t *wb[WR];
+    int gk = k0 % p.nks, gn = n, sk = gk;
+    if (WREG)
 #pragma unroll
-        for (int i = 0; i < WR; i++) {
-            const int c = tid + 64 * NW * i, r = c >> 3, k = gk * LIN_KS + (c & 7) * 8, left = p.a.in - k;
-            const uint16_t *q = p.a.W + (size_t)(o0 + min(r, on - 1)) * p.a.ldw + k;
-            wr[i] = left >= 8 ? load8_any(q) : load8_upto(q, left);
-        }
-        if (++gk == p.nks) gk = 0;
+        for (int i = 0; i < WR; i++) wb[i] = p.a.W + (size_t)(o0 + min((tid + 64 * NW * i) >> 3, on - 1)) * p.a.ldw;
+    auto wload = [&](auto slot) {
+        constexpr int S = WREG ? decltype(slot)::value : 0;
+        const int k = min(gk * LIN_KS + (tid & 7) * 8, p.a.in - 8);
+#pragma unroll
+        for (int i = 0; i < WR; i++) wr[S][i] = load8_any(wb[i] + k);
+        if (--gn > 0 && ++gk == p.nks) gk = 0;
     };
     auto wstore = [&](auto slot) {
+        constexpr int S = WREG ? decltype(slot)::value : 0;
         uint16_t *const b = buf_of(slot);
+        if (sk == p.nks - 1 && p.a.in % LIN_KS) {
+            const int k = sk * LIN_KS + (tid & 7) * 8, over = k - min(k, p.a.in - 8), sh = 16 * (over & 3);
+#pragma unroll
+            for (int i = 0; i < WR; i++) {
+                uint64_t lo = (uint64_t)wr[S][i].y << 32 | wr[S][i].x, hi = (uint64_t)wr[S][i].w << 32 | wr[S][i].z;
+                if (over & 4) lo = hi, hi = 0;
+                lo = sh ? lo >> sh | hi << (64 - sh) : lo;
+                hi >>= sh;
+                if (over >= 8) lo = hi = 0;
+                wr[S][i] = make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
+            }
+        }
 #pragma unroll
         for (int i = 0; i < WR; i++) {
             const int c = tid + 64 * NW * i, r = c >> 3;
-            *reinterpret_cast<uint4 *>(b + (BT + r) * LIN_KS + ((c & 7) ^ sww(r)) * 8) = wr[i];
+            *reinterpret_cast<uint4 *>(b + (BT + r) * LIN_KS + ((c & 7) ^ sww(r)) * 8) = wr[S][i];
         }
+        if (++sk == p.nks) sk = 0;
     };
 
     /* where the lane's fragments lie: x row 16 j + r16 of the wave's tokens, W row as above (their swizzles are
@@ -652,8 +665,9 @@ __global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
         });
         __builtin_amdgcn_sched_group_barrier(0x008, NMF, 0);
     };
-    /* all but the last NST - 2 stages' requests (with weights through registers: all) */
-    constexpr int WAITN = WREG ? 0 : DN * (NST - 2);
+    /* all but the last NST - 2 stages' requests (with weights through registers, whose loads follow a stage's
+     * requests: and those of the stage before) */
+    constexpr int WAITN = WREG ? WR + (XD + WR) * (NST - 2) : DN * (NST - 2);
     constexpr int WAIT_STAGE = (WAITN & 15) | (7 << 4) | (0 << 8) | ((WAITN >> 4) << 14);       /* and LDS: none */
     static_assert(WAITN < 64, "requests in flight");
     constexpr int WAIT_VM0 = (7 << 4) | (15 << 8);
@@ -676,22 +690,19 @@ __global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
         __builtin_amdgcn_sched_barrier(0);
         if (WREG) wstore(slot);
         issue(slot);
-        if (WREG) wload();
+        if (WREG) wload(slot);
         if (WREG) __builtin_amdgcn_sched_barrier(0);
         read(nb, 0, fx0, fw0);          /* (past the last step: what lies there, unused) */
         mma(fx1, fw1);
         pin(std::integral_constant<int, WREG ? 0 : DN>{});
         __builtin_amdgcn_sched_barrier(0);
     };
-    auto start = [&](auto slot) {
-        if (WREG) {
-            wload();
-            wstore(slot);
-        }
+    if (WREG) each_stage<0, NST>(wload);
+    each_stage<0, NST>([&](auto slot) {
+        if (WREG) wstore(slot);
         issue(slot);
-    };
-    each_stage<0, NST>(start);
-    if (WREG) wload();
+    });
+    if (WREG) each_stage<0, NST>(wload);
     __builtin_amdgcn_s_waitcnt(WAIT_VM0);
     __syncthreads();
     read(S0, 0, fx0, fw0);
@@ -881,10 +892,10 @@ float skinny_cost(int T, int in, int out, bool f32, int rw, long cus)
 }
 
 /* ---- many tokens ---- */
-template <int BT, int BO, int WT, int WO, int NST, bool WREG>
+template <int BT, int BO, int WT, int WO, int NST, bool WREG, int POL = K3_LD_DEFAULT>
 void tile_go(const LinTile *p, hipStream_t st)
 {
-    lin_tile_kernel<BT, BO, WT, WO, NST, WREG><<<p->nt * p->no * p->nsl, 64 * WT * WO, 0, st>>>(*p);
+    lin_tile_kernel<BT, BO, WT, WO, NST, WREG, POL><<<p->nt * p->no * p->nsl, 64 * WT * WO, 0, st>>>(*p);
 }
 
 /* Microseconds of a launch of lin_tile_kernel and, with slices, the join: rounds of as many workgroups as fit the chip, each
@@ -956,12 +967,12 @@ extern "C" int k3k_linear(const K3kLinear *a, void *stream)
             K3K_LAUNCH_CHECK("linear: few tokens");
             return 0;
         }
-        if (!dma) {
-            if (f32) stream_pick<true>(a, st);
-            else stream_pick<false>(a, st);
-            K3K_LAUNCH_CHECK("linear: any alignment");
-            return 0;
-        }
+    }
+    if (!dma && (a->T <= 64 || a->in < LIN_KS)) {
+        if (f32) stream_pick<true>(a, st);
+        else stream_pick<false>(a, st);
+        K3K_LAUNCH_CHECK("linear: any alignment");
+        return 0;
     }
 
     LinTile p;
@@ -993,11 +1004,15 @@ extern "C" int k3k_linear(const K3kLinear *a, void *stream)
         case 1: tile_go<256, 128, 4, 2, 3, false>(&p, st); break;
         case 2: tile_go<128, 128, 2, 2, 4, false>(&p, st); break;
         case 3: tile_go<128, 64, 2, 2, 3, false>(&p, st); break;
-        case 4: tile_go<64, 128, 1, 4, 3, false>(&p, st); break;
+        case 4:
+            /* (one tile of tokens: W is read once) */
+            if (p.nt == 1 && (size_t)a->in * a->out * 2 >= LIN_NT_BYTES) tile_go<64, 128, 1, 4, 3, false, K3_LD_NT>(&p, st);
+            else tile_go<64, 128, 1, 4, 3, false>(&p, st);
+            break;
         default: tile_go<64, 64, 2, 2, 4, false>(&p, st); break;
         }
     } else if (shape == 2) {
-        tile_go<128, 128, 2, 2, 2, true>(&p, st);
+        tile_go<128, 128, 2, 2, 3, true>(&p, st);
     } else {
         tile_go<64, 64, 2, 2, 4, true>(&p, st);
     }

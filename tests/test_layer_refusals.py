@@ -19,7 +19,7 @@ LINEAR = dict(y=A, y_type=1, ldy=64, x=A, x_type=1, ldx=32, T=4, W=A, ldw=32, in
     (dict(y_type=2), "x_type"), (dict(x_type=-1), "x_type"), (dict(act=5), "activation"), (dict(act=-1), "activation"),
     (dict(T=-1), "T >= 0"), (dict(inn=0), "in >= 1"), (dict(out=-3), "out >= 0"), (dict(ldx=31), "stride"),
     (dict(ldw=31), "stride"), (dict(ldy=63), "stride"), (dict(res=A, ldr=63), "stride"), (dict(ldx=(1 << 22) + 1), "MAX_LD"),
-    (dict(ldw=(1 << 22) + 1), "MAX_LD"), (dict(y=None), "must be given"), (dict(x=None), "must be given"),
+    (dict(ldw=(1 << 22) + 1), "MAX_LD"), (dict(inn=(1 << 20) + 1, ldx=1 << 21, ldw=1 << 21), "MAX_IN"), (dict(y=None), "must be given"), (dict(x=None), "must be given"),
     (dict(W=None), "must be given"), (dict(res=A, ldr=65), "y's stride"), (dict(y=A + 1), "aligned"),
     (dict(x=A + 1), "aligned"), (dict(W=A + 1), "aligned"), (dict(bias=A + 2), "aligned"), (dict(res=A + 1, ldr=64), "aligned"),
     (dict(y_type=0, y=A + 2), "aligned"), (dict(x_type=0, x=A + 2), "aligned")])
