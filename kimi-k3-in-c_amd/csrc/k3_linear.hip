@@ -2,6 +2,21 @@
 /*
  * k3_linear.hip -- dense products with bias, activation and residual (k3d_linear):
  *   y[t][o] = act(sum_k x[t][k] W[o][k] + bias[o]) + res[t][o],   W bf16, x bf16 or fp32.
+ *
+ * All products run on the matrix cores as bf16 with fp32 sums. An fp32 x is cut into three bf16 terms that hold its
+ * 24 bits, so its products are as exact as fp32 ones, for three times the matrix work.
+ *
+ * What bounds it, and the kernel for it:
+ *   - up to 64 tokens: reading W. lin_skinny_kernel, 16 to 64 rows of W to a workgroup, its waves sharing the columns, each
+ *     with a ring of LDS stages of its own filled by DMA (one token of 12288 -> 7168, 176 MB, 26.8 us = 6.6 TB/s);
+ *   - more: the matrix cores. lin_tile_kernel, tiles of 64 x 64 to 256 x 256, over slices of the columns where the tiles alone
+ *     leave CUs idle; the slices' sums are joined in slice order by lin_join_kernel (4096 tokens of 7168 -> 12288 with
+ *     gelu_tanh 573 us = 1.26 PFLOP/s, the library's product alone 545);
+ *   - weights that are not 16-byte aligned rows of whole 16 bytes: the same tiles, with W through registers instead of
+ *     DMA (which wants 16-byte addresses); small ones for a few tokens, and rows shorter than a step, by lin_stream_kernel;
+ *   - x that does not suit the DMA, rows that end inside a step, and fp32 x for many tiles of outputs: lin_pack_kernel lays it out
+ *     in the workspace first.
+ * Which of them, and the tile and slices, go by the costs estimated below.
  */
 #include "k3_common.h"
 #include "k3_dev.h"
@@ -122,18 +137,20 @@ __device__ __forceinline__ void bias4(const K3kLinear &a, int o, float (&b)[4])
 __device__ __forceinline__ void cut3(const float (&f)[8], uint32_t (&h)[4], uint32_t (&m)[4], uint32_t (&l)[4])
 {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const uint32_t u = __float_as_uint(f[i]);
-        const bool fin = (u & 0x7f800000u) != 0x7f800000u;
-        const uint32_t uh = (u & 0xffff0000u) | (f[i] != f[i] ? 0x00400000u : 0u);
-        const float r1 = fin ? f[i] - __uint_as_float(uh) : 0.0f;
-        const uint32_t um = __float_as_uint(r1) & 0xffff0000u;
-        const uint32_t ul = __float_as_uint(r1 - __uint_as_float(um));
-        if (i & 1) {
-            h[i / 2] |= uh, m[i / 2] |= um, l[i / 2] |= ul & 0xffff0000u;
-        } else {
-            h[i / 2] = uh >> 16, m[i / 2] = um >> 16, l[i / 2] = ul >> 16;
+    for (int i = 0; i < 4; i++) {
+        uint32_t u[3][2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const float v = f[2 * i + e];
+            u[0][e] = __float_as_uint(v);
+            const float r1 = __builtin_amdgcn_classf(v, 0x204) ? 0.0f : v - __uint_as_float(u[0][e] & 0xffff0000u);
+            u[1][e] = __float_as_uint(r1);
+            u[2][e] = __float_as_uint(r1 - __uint_as_float(u[1][e] & 0xffff0000u));
         }
+        /* the upper halves of a pair */
+        h[i] = __builtin_amdgcn_perm(u[0][1], u[0][0], 0x07060302u);
+        m[i] = __builtin_amdgcn_perm(u[1][1], u[1][0], 0x07060302u);
+        l[i] = __builtin_amdgcn_perm(u[2][1], u[2][0], 0x07060302u);
     }
 }
 
@@ -162,96 +179,62 @@ __device__ __forceinline__ uint4 load8_upto(const uint16_t *p, int n)
     return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
 }
 
-/* ---- few tokens: weights straight into registers ---------------------------------------- */
-/* A workgroup takes 16 RF rows of W and 16 NT tokens; its waves share the columns, each a run of
- * 32-column steps, and their sums meet in LDS. A lane's weights (row lane % 16, columns 8 (lane / 16)
- * ..+8 of a step) are an MFMA operand as loaded. Rows and tokens past the ends repeat the last one; only
- * the last step can pass the end of a row (guarded, zeros behind). */
-template <int RF, int NT, int U, int MAXW, bool XF32>
-__global__ __launch_bounds__(64 * MAXW) void lin_stream_kernel(K3kLinear a, int nw)
+/* ---- short rows at any alignment: operands straight into registers -------------------------- */
+/* A workgroup takes 16 rows of W and 16 tokens; its waves share the columns, each a run of 32-column steps, and
+ * their sums meet in LDS. A lane's weights (row lane % 16, columns 8 (lane / 16) ..+8 of a step) are an MFMA operand
+ * as loaded. Rows and tokens past the ends repeat the last one; only the last step can pass the end of
+ * a row (guarded, zeros behind). */
+template <int U, bool XF32>
+__global__ __launch_bounds__(512) void lin_stream_kernel(K3kLinear a, int nw)
 {
-    extern __shared__ float4 part[];
+    __shared__ float4 part[8 * 64];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, r16 = lane & 15, g = lane >> 4;
-    const int o0 = blockIdx.x * 16 * RF, t0 = blockIdx.y * 16 * NT;
+    const int og = (a.out + 15) / 16;
+    const int o0 = (int)(blockIdx.x % og) * 16, t0 = (int)(blockIdx.x / og) * 16;
     const int steps = (a.in + 31) / 32, per = (steps + nw - 1) / nw;
     const int s0 = wv * per, n = min(per, steps - s0);          /* (n < 1: nothing for this wave) */
-
-    const uint16_t *wp[RF];
-    const char *xp[NT];
-#pragma unroll
-    for (int i = 0; i < RF; i++) wp[i] = a.W + (size_t)min(o0 + 16 * i + r16, a.out - 1) * a.ldw + 8 * g;
-#pragma unroll
-    for (int j = 0; j < NT; j++)
-        xp[j] = (const char *)a.x + ((size_t)min(t0 + 16 * j + r16, a.T - 1) * a.ldx + 8 * g) * (XF32 ? 4 : 2);
-
-    k3_f32x4 acc[RF][NT];
-#pragma unroll
-    for (int i = 0; i < RF; i++)
-#pragma unroll
-        for (int j = 0; j < NT; j++) acc[i][j] = k3_f32x4{0.f, 0.f, 0.f, 0.f};
+    constexpr int XS = XF32 ? 4 : 2;
+    const uint16_t *const wp = a.W + (size_t)min(o0 + r16, a.out - 1) * a.ldw + 8 * g;
+    const char *const xp = (const char *)a.x + ((size_t)min(t0 + r16, a.T - 1) * a.ldx + 8 * g) * XS;
+    k3_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 
     struct Slot {
-        uint4 w[RF], x[NT][XF32 ? 2 : 1];
+        uint4 w, x[XF32 ? 2 : 1];
     };
     auto load = [&](Slot &s, int step) {
-        const int k = step * 32;
-#pragma unroll
-        for (int i = 0; i < RF; i++) s.w[i] = load8_any(wp[i] + k);
-#pragma unroll
-        for (int j = 0; j < NT; j++) {
-            const char *p = xp[j] + (size_t)k * (XF32 ? 4 : 2);
-            if (XF32) {
-                __builtin_memcpy(&s.x[j][0], p, 16);
-                __builtin_memcpy(&s.x[j][XF32 ? 1 : 0], p + 16, 16);
-            } else {
-                s.x[j][0] = load8_any((const uint16_t *)p);
-            }
-        }
+        s.w = load8_any(wp + step * 32);
+        const char *p = xp + (size_t)step * 32 * XS;
+        s.x[0] = load8_any((const uint16_t *)p);
+        if constexpr (XF32) s.x[1] = load8_any((const uint16_t *)(p + 16));
     };
     /* the step that passes the end of the rows */
     auto load_last = [&](Slot &s, int step) {
         const int k = step * 32, left = a.in - k - 8 * g;
+        s.w = load8_upto(wp + k, left);
+        const char *p = xp + (size_t)k * XS;
+        if constexpr (XF32) {
+            float f[8];
 #pragma unroll
-        for (int i = 0; i < RF; i++) s.w[i] = load8_upto(wp[i] + k, left);
-#pragma unroll
-        for (int j = 0; j < NT; j++) {
-            const char *p = xp[j] + (size_t)k * (XF32 ? 4 : 2);
-            if (XF32) {
-                float f[8];
-#pragma unroll
-                for (int i = 0; i < 8; i++) f[i] = i < left ? ((const float *)p)[i] : 0.0f;
-                __builtin_memcpy(&s.x[j][0], f, 16);
-                __builtin_memcpy(&s.x[j][XF32 ? 1 : 0], f + 4, 16);
-            } else {
-                s.x[j][0] = load8_upto((const uint16_t *)p, left);
-            }
+            for (int i = 0; i < 8; i++) f[i] = i < left ? ((const float *)p)[i] : 0.0f;
+            __builtin_memcpy(s.x, f, 32);
+        } else {
+            s.x[0] = load8_upto((const uint16_t *)p, left);
         }
     };
     auto use = [&](const Slot &s) {
-#pragma unroll
-        for (int j = 0; j < NT; j++) {
-            if (XF32) {
-                float f[8];
-                uint32_t h[4], m[4], l[4];
-                __builtin_memcpy(f, &s.x[j][0], 16);
-                __builtin_memcpy(f + 4, &s.x[j][XF32 ? 1 : 0], 16);
-                cut3(f, h, m, l);
-                const k3_bf16x8 xl = as_frag(l), xm = as_frag(m), xh = as_frag(h);
-#pragma unroll
-                for (int i = 0; i < RF; i++) {
-                    const k3_bf16x8 w = k3_as_bf16x8(s.w[i]);
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, xl, acc[i][j], 0, 0, 0);
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, xm, acc[i][j], 0, 0, 0);
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, xh, acc[i][j], 0, 0, 0);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < RF; i++)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k3_as_bf16x8(s.w[i]), k3_as_bf16x8(s.x[j][0]), acc[i][j], 0, 0, 0);
-            }
+        const k3_bf16x8 w = k3_as_bf16x8(s.w);
+        if constexpr (XF32) {
+            float f[8];
+            uint32_t h[4], m[4], l[4];
+            __builtin_memcpy(f, s.x, 32);
+            cut3(f, h, m, l);
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, as_frag(l), acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, as_frag(m), acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, as_frag(h), acc, 0, 0, 0);
+        } else {
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, k3_as_bf16x8(s.x[0]), acc, 0, 0, 0);
         }
     };
-
     /* whole steps through a ring of U slots (past the end the last one is requested again and goes unused) */
     const int whole = min(n, a.in / 32 - s0);
     if (whole > 0) {
@@ -274,23 +257,18 @@ __global__ __launch_bounds__(64 * MAXW) void lin_stream_kernel(K3kLinear a, int 
         load_last(s, s0 + n - 1);
         use(s);
     }
-
-#pragma unroll
-    for (int i = 0; i < RF; i++)
-#pragma unroll
-        for (int j = 0; j < NT; j++)
-            part[(wv * RF * NT + i * NT + j) * 64 + lane] = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+    part[wv * 64 + lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
     __syncthreads();
-    for (int q = wv; q < RF * NT; q += nw) {
-        const int o = o0 + 16 * (q / NT) + 4 * g;
+    if (wv == 0) {
+        const int o = o0 + 4 * g;
         float b[4];
         bias4(a, o, b);
-        float4 s = part[q * 64 + lane];
+        float4 s = part[lane];
         for (int w = 1; w < nw; w++) {
-            const float4 v = part[(w * RF * NT + q) * 64 + lane];
+            const float4 v = part[w * 64 + lane];
             s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
         }
-        put4(a, t0 + 16 * (q % NT) + r16, o, s, b);
+        put4(a, t0 + r16, o, s, b);
     }
 }
 
@@ -496,7 +474,7 @@ __global__ __launch_bounds__(256) void lin_pack_kernel(uint16_t *xs, const void 
 /* ---- many tokens: tiles through LDS -------------------------------------------------------- */
 typedef struct {
     K3kLinear a;
-    const uint16_t *x;      /* bf16 rows, 16-byte aligned, ldx % 8 == 0 */
+    const void *x;          /* bf16 rows (or fp32 ones, to be cut as they are read), 16-byte aligned with their stride */
     long ldx;
     int xcols;              /* columns of x: in, or all terms' padded ones */
     int nks, steps;         /* steps of one term, of all */
@@ -506,7 +484,8 @@ typedef struct {
 } LinTile;
 
 /* Which token and output tile workgroup b takes. The dispatcher deals workgroups to the XCDs in turn; each XCD
- * gets a run of tiles of its own, in blocks of 8 token tiles by all... */
+ * gets a run of tiles of its own, slice by slice, down 8 token tiles before the next outputs: what a run reads of W it reads
+ * once from its L2, and its x stays there. */
 __device__ __forceinline__ void tile_of(const LinTile &p, int b, int &tt, int &to, int &sl)
 {
     const int tiles = p.nt * p.no, all = tiles * p.nsl;
@@ -521,15 +500,16 @@ __device__ __forceinline__ void tile_of(const LinTile &p, int b, int &tt, int &t
     tt = q * GT + r % h;
 }
 
-template <int BT, int BO, int WT, int WO, int NST, bool WREG, int POL>
+template <int BT, int BO, int WT, int WO, int NST, bool WREG, int POL, bool XF32>
 __global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
 {
     constexpr int NW = WT * WO, FT = BT / WT / 16, FO = BO / WO / 16;
-    constexpr int XD = BT / 8 / NW, WD = WREG ? 0 : BO / 8 / NW, DN = XD + WD;      /* DMAs of a wave per step */
+    constexpr int XE = XF32 ? 2 * LIN_KS : LIN_KS, XR = 512 / XE;                     /* a row of x in 2-byte units; rows of a DMA */
+    constexpr int XD = BT / XR / NW, WD = WREG ? 0 : BO / 8 / NW, DN = XD + WD;      /* DMAs of a wave per step */
     constexpr int WR = WREG ? BO * 8 / (64 * NW) : 1;                                /* 16-byte pieces of W per thread */
     constexpr int FG = FO % 4 == 0 ? 4 : FO % 2 == 0 ? 2 : 1;       /* fragments that share a run of outputs */
     static_assert(XD >= 1 && (WREG || WD >= 1) && NST >= 2 && NST <= 4, "tile");
-    constexpr int SZ = (BT + BO) * LIN_KS;
+    constexpr int SZ = BT * XE + BO * LIN_KS;
     __shared__ __attribute__((aligned(1024))) uint16_t S0[SZ], S1[SZ], S2[NST > 2 ? SZ : 8], S3[NST > 3 ? SZ : 8];
 
     const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
@@ -544,19 +524,20 @@ __global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
      * fragment read (one column) fall on all 64 banks. x: fragment rows are consecutive. W: the
      * rows of fragment q of FG are 4 FG j + 4 q + e (j: lane group, e: register of the result), so that a
      * lane's results of FG fragments are 4 FG consecutive outputs. */
-    auto swx = [](int r) { return (r >> 1) & 7; };
+    auto swx = [](int r) { return XF32 ? r & 15 : (r >> 1) & 7; };
     auto sww = [](int r) { return FG == 1 ? (r >> 1) & 7 : (((r / (4 * FG)) & 3) << 1) | ((r >> 1) & 1); };
 
     const int tn = min(BT, p.a.T - t0), on = min(BO, p.a.out - o0);
-    const k3_rsrc rx = k3_make_rsrc(p.x + (size_t)t0 * p.ldx, (uint32_t)(((size_t)(tn - 1) * p.ldx + p.xcols) * 2));
+    constexpr int XS = XF32 ? 4 : 2;
+    const k3_rsrc rx = k3_make_rsrc((const char *)p.x + (size_t)t0 * p.ldx * XS, (uint32_t)(((size_t)(tn - 1) * p.ldx + p.xcols) * XS));
     const k3_rsrc rw = k3_make_rsrc(p.a.W + (size_t)o0 * p.a.ldw, (uint32_t)(((size_t)(on - 1) * p.a.ldw + p.a.in) * 2));
     /* DMA i of wave wv fills LDS rows 8 (NW i + wv) ..+8, a lane a 16-byte slot. Rows past the last one repeat
      * it (their sums go unused), so every read lies in its matrix. */
     uint32_t xo[XD], wo_[WD > 0 ? WD : 1];
 #pragma unroll
     for (int i = 0; i < XD; i++) {
-        const int r = (i * NW + wv) * 8 + lane / 8;
-        xo[i] = (uint32_t)min(r, tn - 1) * (uint32_t)(p.ldx * 2) + ((lane & 7) ^ swx(r)) * 16;
+        const int r = (i * NW + wv) * XR + lane / (64 / XR);
+        xo[i] = (uint32_t)min(r, tn - 1) * (uint32_t)(p.ldx * XS) + ((lane & (64 / XR - 1)) ^ swx(r)) * 16;
     }
 #pragma unroll
     for (int i = 0; i < WD; i++) {
@@ -578,11 +559,11 @@ __global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
     auto issue = [&](auto slot) {
         uint16_t *const b = buf_of(slot);
         const uint32_t none = xk < kend ? 0u : LIN_OOB;
-        const uint32_t xs = (uint32_t)xk * (LIN_KS * 2), ws = (uint32_t)(wk == p.nks - 1 ? p.a.in - LIN_KS : wk * LIN_KS) * 2;
+        const uint32_t xs = (uint32_t)xk * (LIN_KS * XS), ws = (uint32_t)(wk == p.nks - 1 ? p.a.in - LIN_KS : wk * LIN_KS) * 2;
 #pragma unroll
-        for (int i = 0; i < XD; i++) k3_dma16(rx, b + (i * NW + wv) * 8 * LIN_KS, xo[i] | none, xs);
+        for (int i = 0; i < XD; i++) k3_dma16(rx, b + (i * NW + wv) * 512, xo[i] | none, xs);
 #pragma unroll
-        for (int i = 0; i < WD; i++) k3_dma16<POL>(rw, b + (BT + (i * NW + wv) * 8) * LIN_KS, wo_[i] | none, ws);
+        for (int i = 0; i < WD; i++) k3_dma16<POL>(rw, b + BT * XE + (i * NW + wv) * 512, wo_[i] | none, ws);
         xk++;
         if (++wk == p.nks) wk = 0;
     };
@@ -620,7 +601,7 @@ __global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
 #pragma unroll
         for (int i = 0; i < WR; i++) {
             const int c = tid + 64 * NW * i, r = c >> 3;
-            *reinterpret_cast<uint4 *>(b + (BT + r) * LIN_KS + ((c & 7) ^ sww(r)) * 8) = wr[S][i];
+            *reinterpret_cast<uint4 *>(b + BT * XE + r * LIN_KS + ((c & 7) ^ sww(r)) * 8) = wr[S][i];
         }
         if (++sk == p.nks) sk = 0;
     };
@@ -628,34 +609,58 @@ __global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
     /* where the lane's fragments lie: x row 16 j + r16 of the wave's tokens, W row as above (their swizzles are
      * the same for every fragment); column 8 g of a half step */
     const int xr = wt * (BT / WT) + r16, wr0 = wo * (BO / WO) + (r16 >> 2) * 4 * FG + (r16 & 3);
-    int xa[2], wa[2];
+    int xa[2], xb[2], wa[2];
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        xa[h] = xr * LIN_KS + (((4 * h + g) ^ swx(xr)) * 8);
-        wa[h] = (BT + wr0) * LIN_KS + (((4 * h + g) ^ sww(wr0)) * 8);
+        const int c = XF32 ? 8 * h + 2 * g : 4 * h + g;         /* (8 floats: two 16-byte columns) */
+        xa[h] = xr * XE + ((c ^ swx(xr)) * 8);
+        xb[h] = xr * XE + (((c + 1) ^ swx(xr)) * 8);
+        wa[h] = BT * XE + wr0 * LIN_KS + (((4 * h + g) ^ sww(wr0)) * 8);
     }
-    auto read = [&](const uint16_t *b, int half, k3_bf16x8 (&xf)[FT], k3_bf16x8 (&wf)[FO]) {
+    struct XFrag {
+        u32x4 v[XF32 ? 2 : 1];
+    };
+    auto read = [&](const uint16_t *b, int half, XFrag (&xf)[FT], k3_bf16x8 (&wf)[FO]) {
 #pragma unroll
         for (int i = 0; i < FO; i++)
             wf[i] = k3_as_bf16x8(*reinterpret_cast<const uint4 *>(b + wa[half] + ((i / FG) * 16 * FG + (i % FG) * 4) * LIN_KS));
 #pragma unroll
-        for (int j = 0; j < FT; j++) xf[j] = k3_as_bf16x8(*reinterpret_cast<const uint4 *>(b + xa[half] + 16 * j * LIN_KS));
+        for (int j = 0; j < FT; j++) {
+            xf[j].v[0] = *reinterpret_cast<const u32x4 *>(b + xa[half] + 16 * j * XE);
+            if constexpr (XF32) xf[j].v[1] = *reinterpret_cast<const u32x4 *>(b + xb[half] + 16 * j * XE);
+        }
     };
     k3_f32x4 acc[FO][FT];
 #pragma unroll
     for (int i = 0; i < FO; i++)
 #pragma unroll
         for (int j = 0; j < FT; j++) acc[i][j] = k3_f32x4{0.f, 0.f, 0.f, 0.f};
-    auto mma = [&](const k3_bf16x8 (&xf)[FT], const k3_bf16x8 (&wf)[FO]) {
+    auto mma = [&](const XFrag (&xf)[FT], const k3_bf16x8 (&wf)[FO]) {
+        if constexpr (XF32) {
 #pragma unroll
-        for (int i = 0; i < FO; i++)
+            for (int j = 0; j < FT; j++) {
+                float f[8];
+                uint32_t c[3][4];
 #pragma unroll
-            for (int j = 0; j < FT; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[i], xf[j], acc[i][j], 0, 0, 0);
+                for (int e = 0; e < 8; e++) f[e] = __uint_as_float(xf[j].v[e / 4][e % 4]);
+                cut3(f, c[2], c[1], c[0]);
+#pragma unroll
+                for (int q = 0; q < 3; q++)
+#pragma unroll
+                    for (int i = 0; i < FO; i++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[i], as_frag(c[q]), acc[i][j], 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < FO; i++)
+#pragma unroll
+                for (int j = 0; j < FT; j++)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[i], __builtin_bit_cast(k3_bf16x8, xf[j].v[0]), acc[i][j], 0, 0, 0);
+        }
     };
     /* issue order of a half: a fragment read of the other half behind each of the first MFMAs, and, behind the
      * barrier, the next stage's requests between them too (in a burst they keep the SIMD from its MFMAs for
      * some hundred cycles) */
-    constexpr int NRD = FO + FT, NMF = FO * FT, GAP = NMF / NRD > 0 ? NMF / NRD : 1;
+    constexpr int NRD = FO + FT * (XF32 ? 2 : 1), NMF = FO * FT * (XF32 ? 3 : 1), GAP = NMF / NRD > 0 ? NMF / NRD : 1;
     auto pin = [&](auto dma) {
         each_stage<0, NRD>([&](auto at) {
             constexpr int I = decltype(at)::value, ND = decltype(dma)::value, Q = (I + 1) * ND / NRD - I * ND / NRD;
@@ -671,7 +676,8 @@ __global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
     constexpr int WAIT_STAGE = (WAITN & 15) | (7 << 4) | (0 << 8) | ((WAITN >> 4) << 14);       /* and LDS: none */
     static_assert(WAITN < 64, "requests in flight");
     constexpr int WAIT_VM0 = (7 << 4) | (15 << 8);
-    k3_bf16x8 fx0[FT], fw0[FO], fx1[FT], fw1[FO];
+    XFrag fx0[FT], fx1[FT];
+    k3_bf16x8 fw0[FO], fw1[FO];
 
     /* Step k: its second half is read while the first is multiplied; then every wave is past its reads of
      * buffer k % NST and stage k + 1 has landed (one barrier), so stage k + NST goes into that buffer and the
@@ -806,27 +812,15 @@ size_t part_bytes(int T, int out)
     return most < LIN_PART_CAP ? most : LIN_PART_CAP;
 }
 
-/* ---- at any alignment, or rows shorter than a stage ---- */
-template <int RF, int NT, int U, int MAXW, bool XF32>
-void stream_go(const K3kLinear *a, int nw, hipStream_t st)
+/* ---- short rows at any alignment ---- */
+void short_rows(const K3kLinear *a, hipStream_t st)
 {
-    const dim3 grid((a->out + 16 * RF - 1) / (16 * RF), (a->T + 16 * NT - 1) / (16 * NT));
-    lin_stream_kernel<RF, NT, U, MAXW, XF32><<<grid, 64 * nw, (size_t)nw * RF * NT * 1024, st>>>(*a, nw);
-}
-
-template <bool XF32>
-void stream_pick(const K3kLinear *a, hipStream_t st)
-{
-    const int nt = (a->T + 15) / 16, rf = nt == 1 ? 1 : 2;
-    const long wgs = (a->out + 16 * rf - 1) / (16 * rf);
-    const int steps = (a->in + 31) / 32, cus = k3k_cu_count();
+    const unsigned grid = (unsigned)((a->out + 15) / 16) * (unsigned)((a->T + 15) / 16);
     /* waves that share a workgroup's columns: enough for the chip, each with a few steps */
-    int nw = wgs < 2 * cus ? 8 : 4;
-    while (nw > 1 && steps < 2 * nw) nw /= 2;
-    if (nt == 1) stream_go<1, 1, XF32 ? 4 : 8, 8, XF32>(a, nw, st);
-    else if (nt == 2) stream_go<2, 2, 4, 8, XF32>(a, nw, st);
-    else if (nt == 3) stream_go<2, 3, XF32 ? 2 : 4, 8, XF32>(a, nw, st);
-    else stream_go<2, 4, XF32 ? 2 : 4, 8, XF32>(a, nw, st);
+    int nw = grid < 2 * k3k_cu_count() ? 8 : 4;
+    while (nw > 1 && (a->in + 31) / 32 < 2 * nw) nw /= 2;
+    if (a->x_type == K3D_F32) lin_stream_kernel<4, true><<<grid, 64 * nw, 0, st>>>(*a, nw);
+    else lin_stream_kernel<8, false><<<grid, 64 * nw, 0, st>>>(*a, nw);
 }
 
 /* ---- few tokens ---- */
@@ -892,10 +886,10 @@ float skinny_cost(int T, int in, int out, bool f32, int rw, long cus)
 }
 
 /* ---- many tokens ---- */
-template <int BT, int BO, int WT, int WO, int NST, bool WREG, int POL = K3_LD_DEFAULT>
+template <int BT, int BO, int WT, int WO, int NST, bool WREG, int POL = K3_LD_DEFAULT, bool XF32 = false>
 void tile_go(const LinTile *p, hipStream_t st)
 {
-    lin_tile_kernel<BT, BO, WT, WO, NST, WREG, POL><<<p->nt * p->no * p->nsl, 64 * WT * WO, 0, st>>>(*p);
+    lin_tile_kernel<BT, BO, WT, WO, NST, WREG, POL, XF32><<<p->nt * p->no * p->nsl, 64 * WT * WO, 0, st>>>(*p);
 }
 
 /* Microseconds of a launch of lin_tile_kernel and, with slices, the join: rounds of as many workgroups as fit the chip, each
@@ -922,6 +916,22 @@ float tile_cost(const Shape &s, int T, int in, int out, int steps, int nsl, long
     return t;
 }
 
+/* Microseconds with fp32 rows cut in the kernel, 64 tokens by 64 or 128 outputs, two workgroups to a CU: a step takes one
+ * 0.50 or 0.74 us alone and 0.72 or 1.01 beside another. (Cutting them once, in a launch before, costs a write and a read of
+ * three terms and a longer product: 300 tokens of 7168 -> 384 26.1 us that way, 18.5 this way; 4000 tokens 135 and 74; but
+ * 1024 of 7168 -> 7168 294 and 353, as each tile of outputs cuts its tokens again.) */
+float cut_cost(int bo, int T, int in, int out, int nsl, long cus)
+{
+    const int nks = in / LIN_KS, per = (nks + nsl - 1) / nsl;
+    const long wgs = (long)((T + 63) / 64) * ((out + bo - 1) / bo) * nsl, slots = 2 * cus;
+    const float one = bo == 64 ? 0.50f : 0.74f, two = bo == 64 ? 0.72f : 1.01f, kb = bo / 8.0f + 16.0f;
+    auto round = [&](long n) { return both(per * (n <= cus ? one : two), per * kb * n / 18400.0f); };
+    float t = (float)(wgs / slots) * round(slots) + (wgs % slots ? round(wgs % slots) : 0.0f);
+    t = 4.5f + both(t, ((float)out + 2.0f * T) * in * 2.0f / 4.2e6f);
+    if (nsl > 1) t += 1.5f + 0.39f * nsl + (nsl + 1.0f) * T * out * 4.0f / 3.2e6f;
+    return t;
+}
+
 }  // namespace
 
 extern "C" size_t k3k_linear_ws(int T, int in, int out, int x_type)
@@ -938,7 +948,8 @@ extern "C" int k3k_linear(const K3kLinear *a, void *stream)
     const bool x16 = ((uintptr_t)a->x & 15) == 0 && a->ldx % (f32 ? 4 : 8) == 0;
     /* weights by DMA, or, at other alignments and in rows shorter than a stage, through registers */
     const bool dma = w16 && a->in % 8 == 0 && a->in >= LIN_KS;
-    const int nks = (a->in + LIN_KS - 1) / LIN_KS, steps = nks * (f32 ? 3 : 1);
+    const int nks = (a->in + LIN_KS - 1) / LIN_KS;
+    int steps = nks * (f32 ? 3 : 1);
     const bool pack = f32 || !x16 || a->in % LIN_KS;
 
     /* the cheapest tile shape and number of slices */
@@ -954,6 +965,15 @@ extern "C" int k3k_linear(const K3kLinear *a, void *stream)
         }
     }
     if (pack) best += 2.5f + (float)a->T * kpad(a->in) * (f32 ? 10 : 4) / 4e6f;
+    /* or fp32 rows as they are */
+    int cut = 0;
+    if (f32 && dma && x16 && a->in % LIN_KS == 0)
+        for (int bo : {64, 128})
+            for (int n : {1, 2, 3, 4, 6, 8, 12, LIN_MAX_SLICES}) {
+                if (n > 1 && (n * one > room || nks < 4 * n)) break;
+                const float t = cut_cost(bo, a->T, a->in, a->out, n, cus);
+                if (t < best) best = t, cut = bo, nsl = n;
+            }
     if (a->T <= 64) {
         int rw = 0;
         if (dma && x16)
@@ -968,37 +988,43 @@ extern "C" int k3k_linear(const K3kLinear *a, void *stream)
             return 0;
         }
     }
-    if (!dma && (a->T <= 64 || a->in < LIN_KS)) {
-        if (f32) stream_pick<true>(a, st);
-        else stream_pick<false>(a, st);
-        K3K_LAUNCH_CHECK("linear: any alignment");
+    /* (16 tokens of 777 -> 999 9.6 us, as tiles 10.7, one 6.8 and 9.9; but 16 of 5001 -> 4097 47 us, as tiles 21) */
+    if (!dma && (a->in < LIN_KS || (a->T <= 16 && (long)a->in * a->out <= 1L << 21))) {
+        short_rows(a, st);
+        K3K_LAUNCH_CHECK("linear: short rows");
         return 0;
     }
 
     LinTile p;
     p.a = *a;
     p.nks = nks;
+    if (cut) steps = nks;
     p.steps = steps;
-    if (pack) {
+    if (pack && !cut) {
         const int kp = kpad(a->in), over = dma ? kp - a->in : 0;
         const size_t n = (size_t)a->T * (kp / 8);
         const unsigned grid = (unsigned)((n + 255) / 256);
         if (f32) lin_pack_kernel<true><<<grid, 256, 0, st>>>((uint16_t *)a->ws, a->x, a->ldx, a->T, a->in, kp, over);
         else lin_pack_kernel<false><<<grid, 256, 0, st>>>((uint16_t *)a->ws, a->x, a->ldx, a->T, a->in, kp, over);
         K3K_LAUNCH_CHECK("linear: pack");
-        p.x = (const uint16_t *)a->ws;
+        p.x = a->ws;
         p.ldx = p.xcols = p.steps * LIN_KS;
     } else {
-        p.x = (const uint16_t *)a->x;
+        p.x = a->x;
         p.ldx = a->ldx;
         p.xcols = a->in;
     }
     p.part = (float *)((char *)a->ws + pack_bytes(a->T, a->in, a->x_type));
-    p.nt = (a->T + SHAPES[shape].bt - 1) / SHAPES[shape].bt;
-    p.no = (a->out + SHAPES[shape].bo - 1) / SHAPES[shape].bo;
+    const int bt = cut ? 64 : SHAPES[shape].bt, bo = cut ? cut : SHAPES[shape].bo;
+    p.nt = (a->T + bt - 1) / bt;
+    p.no = (a->out + bo - 1) / bo;
     p.per = (steps + nsl - 1) / nsl;
     p.nsl = (steps + p.per - 1) / p.per;
-    if (dma) {
+    if (cut == 64) {
+        tile_go<64, 64, 4, 1, 3, false, K3_LD_DEFAULT, true>(&p, st);
+    } else if (cut) {
+        tile_go<64, 128, 4, 1, 2, false, K3_LD_DEFAULT, true>(&p, st);
+    } else if (dma) {
         switch (shape) {
         case 0: tile_go<256, 256, 2, 4, 2, false>(&p, st); break;
         case 1: tile_go<256, 128, 4, 2, 3, false>(&p, st); break;
