@@ -177,3 +177,26 @@ def test_far_rows(gpu, k3):
     y = torch.zeros(9, 1 << 28, device="cuda", dtype=BF16)[:, :out]
     x = torch.randn(9, 64, device="cuda", generator=lo.gen(12)).to(BF16)
     lo.within(lo.linear(k3, x, w, y=y), lo.linear64(x, w, None, "none", None, BF16))
+
+
+@pytest.mark.parametrize("T,inn,out", [
+    (1, 7168, 7168), (6, 4096, 4096), (14, 2048, 8192), (22, 7168, 896), (30, 2048, 2048), (38, 12288, 4100), (46, 512, 16384),
+    (60, 8192, 6400), (64, 7168, 7000), (96, 7168, 7168), (200, 7168, 2048), (1024, 2048, 2048), (1500, 1024, 3584),
+    (2048, 2048, 4096), (4096, 1024, 4096), (300, 7168, 384), (1000, 7168, 130)])
+@pytest.mark.parametrize("x_type", [F32, BF16])
+@pytest.mark.parametrize("off", [0, 1])
+def test_every_kernel(gpu, k3, T, inn, out, x_type, off):
+    """Large enough that each kernel, tile, slicing and way of reading W is some shape's choice, with W aligned and not. Operands
+    are integers whose sums stay below 2^24, so fp32 forms them exactly in any order and the result is one only."""
+    say(f"case: {T} x {inn} -> {out} {x_type} off {off}")
+    x, w, b, r = operands(T, inn, out, x_type, F32, T, offw=off)
+    big, one = (511, 1) if x_type == F32 else (3, 3)               # (of fp32 the two upper terms; 511 * 12288 < 2^23)
+    x.copy_(torch.randint(-big, big + 1, x.shape, device="cuda", generator=lo.gen(T)))
+    w.copy_(torch.randint(-one, one + 1, w.shape, device="cuda", generator=lo.gen(T + 1)))
+    for t in (b, r):
+        t.copy_((t * 100).round())
+    y = torch.full((T + 1, out + 3), 7.0, device="cuda", dtype=F32)
+    got = lo.linear(k3, x, w, b, "relu", r, y=y[:T, :out])
+    want = (x.double() @ w.double().T + b).clamp(min=0) + r
+    assert torch.equal(got.double(), want)
+    assert (y[T] == 7).all() and (y[:, out:] == 7).all()
