@@ -184,8 +184,9 @@ int k3d_moe_experts(float *out, const int *idx, const float *wt, const float *x,
 
 /* ---- the operators of the layer around the routed experts -------------------------------
  * No counterpart in the reference as single calls. Strides are in elements; nothing is allocated,
- * nothing synchronises, and the calls can be captured in a HIP graph. The stream belongs to the
- * current device. */
+ * nothing synchronises, and the calls can be captured in a HIP graph. The stream and the tensors
+ * belong to the current device. Up to K3D_MAX_TOKENS tokens in a call. */
+#define K3D_MAX_TOKENS (1 << 24)
 
 /* Element types of the tensors below. */
 enum { K3D_F32 = 0, K3D_BF16 = 1 };
@@ -198,7 +199,9 @@ enum { K3D_F32 = 0, K3D_BF16 = 1 };
  * (an infinite weight then gives NaN where it meets a finite x). Sums, bias, activation and
  * residual are formed in fp32 and rounded once to y_type. Which kernel runs, and with it the order
  * of a sum, goes by the shape, the types and the alignment; a call's bits repeat. ldx and ldw up to
- * K3D_LINEAR_MAX_LD, in up to K3D_LINEAR_MAX_IN. y must not overlap x, W, bias or ws. */
+ * K3D_LINEAR_MAX_LD, in up to K3D_LINEAR_MAX_IN. y must not overlap x, W, bias or ws, nor res unless it
+ * is y itself. ws (k3d_linear_ws bytes, which hold any fewer tokens too; 16-byte aligned) is scratch of
+ * one call: calls and graphs that may run at the same time need one each. */
 enum { K3D_ACT_NONE = 0, K3D_ACT_RELU = 1, K3D_ACT_SILU = 2, K3D_ACT_GELU = 3 /* erf */, K3D_ACT_GELU_TANH = 4 };
 #define K3D_LINEAR_MAX_LD (1 << 22)
 #define K3D_LINEAR_MAX_IN (1 << 20)
@@ -230,7 +233,8 @@ int k3d_route(int *idx, float *wt, const void *logits, int type, long ld, int T,
 
 /* RMSNorm of every query and key head, and the position rotation behind it. Head h of token t
  * is the `dim` elements at q + t * ldq + h * hsq (k likewise); it goes to qo / ko in the same form,
- * which may be the input itself (same pointer and strides), else must not overlap it.
+ * which may be the input itself (same pointer and strides), else must overlap neither q nor k. Outputs
+ * lie token by token (ldqo >= (hq - 1) * hsqo + dim) or head by head (hsqo >= (T - 1) * ldqo + dim).
  *   u = v / sqrt(mean(v^2) + eps) * w     (w: qw or kw, fp32 [dim], or NULL for ones)
  *   rotated over u[rot_off .. rot_off + rot): the pairs (i, i + rot/2) (K3D_ROT_HALVES) or
  *   (2i, 2i + 1) (K3D_ROT_INTERLEAVED) turn by the angle pos[t] * inv_freq[i], i < rot/2, and are

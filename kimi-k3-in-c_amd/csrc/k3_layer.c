@@ -37,6 +37,7 @@ int k3d_linear(void *y, int y_type, long ldy, const void *x, int x_type, long ld
     if (act < K3D_ACT_NONE || act > K3D_ACT_GELU_TANH) return k3dx_bad("k3d_linear: unknown activation");
     if (T < 0 || out < 0 || in < 1) return k3dx_bad("k3d_linear: need T >= 0, out >= 0, in >= 1");
     if (T == 0 || out == 0) return 0;
+    if (T > K3D_MAX_TOKENS) return k3dx_bad("k3d_linear: up to K3D_MAX_TOKENS tokens");
     if (ldx < in || ldw < in || ldy < out || (res && ldr < out)) return k3dx_bad("k3d_linear: a stride is shorter than its row");
     if (ldx > K3D_LINEAR_MAX_LD || ldw > K3D_LINEAR_MAX_LD || in > K3D_LINEAR_MAX_IN)
         return k3dx_bad("k3d_linear: ldx and ldw up to K3D_LINEAR_MAX_LD, in up to K3D_LINEAR_MAX_IN");
@@ -48,6 +49,7 @@ int k3d_linear(void *y, int y_type, long ldy, const void *x, int x_type, long ld
     const size_t need = k3k_linear_ws(T, in, out, x_type);
     if (need && (!ws || ws_bytes < need)) return k3dx_bad("k3d_linear: workspace too small");
     if (need && !aligned(ws, 16)) return k3dx_bad("k3d_linear: the workspace must be 16-byte aligned");
+    if (y == x || y == W || y == ws || (const void *)y == bias) return k3dx_bad("k3d_linear: y lies in an operand's place");
     K3kLinear a;
     a.y = y;
     a.x = x;
@@ -88,6 +90,7 @@ int k3d_route(int *idx, float *wt, const void *logits, int type, long ld, int T,
         return k3dx_bad("k3d_route: topk is 1 to 64 and at most the experts of top_groups groups");
     if (ld < n_experts) return k3dx_bad("k3d_route: ld is shorter than a row");
     if (T == 0) return 0;
+    if (T > K3D_MAX_TOKENS) return k3dx_bad("k3d_route: up to K3D_MAX_TOKENS tokens");
     if (!idx || !wt || !logits) return k3dx_bad("k3d_route: idx, wt and logits must be given");
     if (!aligned(idx, 4) || !aligned(wt, 4) || !aligned(bias, 4) || !aligned(logits, type_size(type)))
         return k3dx_bad("k3d_route: a pointer is not aligned to its elements");
@@ -127,6 +130,7 @@ int k3d_qk_norm_rope(void *qo, long ldqo, long hsqo, void *ko, long ldko, long h
         return k3dx_bad("k3d_qk_norm_rope: rot is even and lies within the head");
     if (!(eps >= 0.0f)) return k3dx_bad("k3d_qk_norm_rope: eps >= 0");
     if (T == 0 || hq + hk == 0) return 0;
+    if (T > K3D_MAX_TOKENS) return k3dx_bad("k3d_qk_norm_rope: up to K3D_MAX_TOKENS tokens");
     if (rot && (!pos || !inv_freq)) return k3dx_bad("k3d_qk_norm_rope: a rotation needs pos and inv_freq");
     if ((hq && (!q || !qo)) || (hk && (!k || !ko))) return k3dx_bad("k3d_qk_norm_rope: heads without their tensors");
     if (!aligned(pos, 4) || !aligned(inv_freq, 8) || !aligned(qw, 4) || !aligned(kw, 4)) return k3dx_bad("k3d_qk_norm_rope: a pointer is not aligned to its elements");
@@ -156,6 +160,11 @@ int k3d_qk_norm_rope(void *qo, long ldqo, long hsqo, void *ko, long ldko, long h
         if (T > 1 && (a.v[i].ld < dim || a.v[i].ldo < dim)) return k3dx_bad("k3d_qk_norm_rope: tokens overlap");
         if (a.v[i].in == a.v[i].out && ((T > 1 && a.v[i].ld != a.v[i].ldo) || (a.v[i].heads > 1 && a.v[i].hs != a.v[i].hso)))
             return k3dx_bad("k3d_qk_norm_rope: in place needs the same strides");
+        if (a.v[i].heads > 1 && T > 1) {                       /* of two writes to one place either could come last */
+            const unsigned __int128 ld = a.v[i].ldo, hs = a.v[i].hso;
+            if (ld < hs * (unsigned)(a.v[i].heads - 1) + (unsigned)dim && hs < ld * (unsigned)(T - 1) + (unsigned)dim)
+                return k3dx_bad("k3d_qk_norm_rope: the outputs of a token and of a head overlap");
+        }
     }
     a.type = type;
     a.T = T;
