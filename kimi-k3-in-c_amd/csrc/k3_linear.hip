@@ -924,11 +924,11 @@ float cut_cost(int bo, int T, int in, int out, int nsl, long cus)
 {
     const int nks = in / LIN_KS, per = (nks + nsl - 1) / nsl;
     const long wgs = (long)((T + 63) / 64) * ((out + bo - 1) / bo) * nsl, slots = 2 * cus;
-    const float one = bo == 64 ? 0.50f : 0.74f, two = bo == 64 ? 0.72f : 1.01f, kb = bo / 8.0f + 16.0f;
-    auto round = [&](long n) { return both(per * (n <= cus ? one : two), per * kb * n / 18400.0f); };
+    const float one = bo == 64 ? 0.49f : 0.73f, two = bo == 64 ? 0.70f : 1.00f, kb = bo / 8.0f + 16.0f;
+    auto round = [&](long n) { return both(per * (n <= cus ? one : two), per * kb * n / 25000.0f); };
     float t = (float)(wgs / slots) * round(slots) + (wgs % slots ? round(wgs % slots) : 0.0f);
-    t = 4.5f + both(t, ((float)out + 2.0f * T) * in * 2.0f / 4.2e6f);
-    if (nsl > 1) t += 1.5f + 0.39f * nsl + (nsl + 1.0f) * T * out * 4.0f / 3.2e6f;
+    t = 4.5f + both(t, ((float)out + 2.0f * T) * in * 2.0f / 5.3e6f);
+    t += nsl > 1 ? 1.3f + 0.38f * nsl + (nsl + 1.0f) * T * out * 4.0f / 3.2e6f : (float)T * out * 4.0f / 4.7e6f;
     return t;
 }
 

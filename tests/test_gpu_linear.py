@@ -200,3 +200,11 @@ def test_every_kernel(gpu, k3, T, inn, out, x_type, off):
     want = (x.double() @ w.double().T + b).clamp(min=0) + r
     assert torch.equal(got.double(), want)
     assert (y[T] == 7).all() and (y[:, out:] == 7).all()
+
+
+@pytest.mark.parametrize("inn,out", [(1024, 2000), (512, 5200), (1024, 8200), (8192, 6400), (4096, 12300), (16384, 3500)])
+@pytest.mark.parametrize("x_type", [F32, BF16])
+@pytest.mark.parametrize("T", [8, 13, 32, 48, 62])
+def test_every_few(gpu, k3, T, inn, out, x_type):
+    """Each group of tokens with each number of rows of W a workgroup takes, and with W past the caches."""
+    test_every_kernel(gpu, k3, T, inn, out, x_type, 0)
