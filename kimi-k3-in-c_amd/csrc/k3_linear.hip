@@ -435,8 +435,14 @@ template <bool XF32>
 __global__ __launch_bounds__(256) void lin_pack_kernel(uint16_t *xs, const void *x, long ldx, int T, int in, int kp, int over)
 {
     const int per = kp / 8;
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-    const int t = (int)(i / per), kb = (int)(i % per) * 8;
+    int t, kb;
+    if (gridDim.x <= 1u << 24) {                                        /* (a 64-bit division takes 0.2 us) */
+        const unsigned i = blockIdx.x * 256 + threadIdx.x;
+        t = (int)(i / (unsigned)per), kb = (int)(i - (unsigned)t * per) * 8;
+    } else {
+        const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+        t = (int)(i / per), kb = (int)(i % per) * 8;
+    }
     if (t >= T) return;
     const int last = kp - LIN_KS, k = kb >= last ? kb - over : kb;      /* the first of the eight columns */
     const bool whole = k >= (kb >= last ? last : 0) && k + 8 <= in;
@@ -766,29 +772,32 @@ __global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
     }
 }
 
-/* the slices' sums, in slice order, and the epilogue */
-__global__ __launch_bounds__(256) void lin_join_kernel(K3kLinear a, const float *part, int nsl)
+/* the slices' sums, in slice order, and the epilogue; four slices requested at once (300 tokens of 384 outputs in 8 slices
+ * 4.6 us one after another, 4.1 so). At most LIN_PART_CAP bytes of sums: their indexes fit 32 bits. */
+__global__ __launch_bounds__(64) void lin_join_kernel(K3kLinear a, const float *part, int nsl)
 {
-    const int per = (a.out + 3) / 4;
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-    const int t = (int)(i / per), o = (int)(i % per) * 4;
+    const unsigned per = (a.out + 3) / 4, i = blockIdx.x * 64 + threadIdx.x;
+    const int t = (int)(i / per), o = (int)(i - (unsigned)t * per) * 4;
     if (t >= a.T) return;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    const bool whole = a.out % 4 == 0;
-    for (int s = 0; s < nsl; s++) {
-        const float *q = part + ((size_t)s * a.T + t) * a.out + o;
-        if (whole) {
-            const float4 f = *reinterpret_cast<const float4 *>(q);
-            v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (o + e < a.out) v[e] += q[e];
-        }
-    }
     float b[4];
     bias4(a, o, b);
-    put4(a, t, o, make_float4(v[0], v[1], v[2], v[3]), b);
+    const float *const q = part + (size_t)t * a.out + o;
+    const size_t one = (size_t)a.T * a.out;
+    const int n = min(4, a.out - o);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < nsl; s += 4) {
+        float4 f[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float *p = q + one * min(s + j, nsl - 1);
+            if (n == 4) __builtin_memcpy(&f[j], p, 16);
+            else f[j] = make_float4(p[0], n > 1 ? p[1] : 0.f, n > 2 ? p[2] : 0.f, 0.f);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (s + j < nsl) v.x += f[j].x, v.y += f[j].y, v.z += f[j].z, v.w += f[j].w;
+    }
+    put4(a, t, o, v, b);
 }
 
 /* ---- launches -------------------------------------------------------------------------------- */
@@ -1045,7 +1054,7 @@ extern "C" int k3k_linear(const K3kLinear *a, void *stream)
     K3K_LAUNCH_CHECK("linear: tiles");
     if (p.nsl > 1) {
         const size_t n = (size_t)a->T * ((a->out + 3) / 4);
-        lin_join_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(*a, p.part, p.nsl);
+        lin_join_kernel<<<(unsigned)((n + 63) / 64), 64, 0, st>>>(*a, p.part, p.nsl);
         K3K_LAUNCH_CHECK("linear: join");
     }
     return 0;
