@@ -96,11 +96,17 @@ __device__ __forceinline__ double score64(float l, float m, double sum)
     else return soft_term(l, m) / sum;
 }
 
+/* the key of expert e's choice, from its score s */
+__device__ __forceinline__ uint64_t score_key(const K3kRoute &a, double s, float l, int e)
+{
+    const uint64_t k = choice_key(s + (a.bias ? (double)a.bias[e] : 0.0));
+    return l > -INFINITY ? k : 0ull;
+}
+
 template <int SCORE>
 __device__ __forceinline__ uint64_t key64(const K3kRoute &a, float l, int e, float m, double sum)
 {
-    const uint64_t k = choice_key(score64<SCORE>(l, m, sum) + (a.bias ? (double)a.bias[e] : 0.0));
-    return l > -INFINITY ? k : 0ull;
+    return score_key(a, score64<SCORE>(l, m, sum), l, e);
 }
 
 template <int CTRL>
@@ -320,11 +326,14 @@ __global__ __launch_bounds__(256, P <= 14 ? 5 : 1) void route_kernel(K3kRoute a,
     }
     __builtin_amdgcn_wave_barrier();
     int mine = -1, at = lane;                   /* the lane's expert and its place */
+    double w = 0.0;                             /* its score */
     if (ncand <= 64) {
         uint64_t key = 0ull;
         if (lane < ncand) {
             mine = cand[lane];
-            key = key64<SCORE>(a, load_logit<TYPE>(a.logits, row + mine), mine, m, sum);
+            const float l = load_logit<TYPE>(a.logits, row + mine);
+            w = score64<SCORE>(l, m, sum);
+            key = score_key(a, w, l, mine);
         }
         int rank = 0;
         for (int q = 0; q < ncand; q++) {
@@ -337,9 +346,9 @@ __global__ __launch_bounds__(256, P <= 14 ? 5 : 1) void route_kernel(K3kRoute a,
         if (lane >= ncand && lane < a.topk) at = lane;
     } else {
         mine = route_exact<TYPE, P, SCORE>(a, row, m, sum, c);
+        if (mine >= 0) w = score64<SCORE>(load_logit<TYPE>(a.logits, row + mine), m, sum);
     }
-    double w = 0.0;
-    if (mine >= 0) w = score64<SCORE>(load_logit<TYPE>(a.logits, row + mine), m, sum);
+    if (mine < 0) w = 0.0;
     if (a.renorm) {
         const double s = wave_total_f64(w);
         w = s > 0.0 ? w / s : 0.0;
