@@ -199,12 +199,13 @@ enum { K3D_F32 = 0, K3D_BF16 = 1 };
  * (an infinite weight then gives NaN where it meets a finite x). Sums, bias, activation and
  * residual are formed in fp32 and rounded once to y_type. Which kernel runs, and with it the order
  * of a sum, goes by the shape, the types and the alignment; a call's bits repeat. ldx and ldw up to
- * K3D_LINEAR_MAX_LD, in up to K3D_LINEAR_MAX_IN. y must not overlap x, W, bias or ws, nor res unless it
- * is y itself. ws (k3d_linear_ws bytes, which hold any fewer tokens too; 16-byte aligned) is scratch of
- * one call: calls and graphs that may run at the same time need one each. */
+ * K3D_LINEAR_MAX_LD, in up to K3D_LINEAR_MAX_IN, out up to K3D_LINEAR_MAX_OUT. y must not overlap x, W,
+ * bias or ws, nor res unless it is y itself. ws (k3d_linear_ws bytes, which hold any fewer tokens too;
+ * 16-byte aligned) is scratch of one call: calls and graphs that may run at the same time need one each. */
 enum { K3D_ACT_NONE = 0, K3D_ACT_RELU = 1, K3D_ACT_SILU = 2, K3D_ACT_GELU = 3 /* erf */, K3D_ACT_GELU_TANH = 4 };
 #define K3D_LINEAR_MAX_LD (1 << 22)
 #define K3D_LINEAR_MAX_IN (1 << 20)
+#define K3D_LINEAR_MAX_OUT (1 << 28)
 size_t k3d_linear_ws(int T, int in, int out, int x_type);
 int k3d_linear(void *y, int y_type, long ldy, const void *x, int x_type, long ldx, int T, const uint16_t *W,
                long ldw, int in, int out, const float *bias, int act, const void *res, long ldr, void *ws,
@@ -233,8 +234,8 @@ int k3d_route(int *idx, float *wt, const void *logits, int type, long ld, int T,
 
 /* RMSNorm of every query and key head, and the position rotation behind it. Head h of token t
  * is the `dim` elements at q + t * ldq + h * hsq (k likewise); it goes to qo / ko in the same form,
- * which may be the input itself (same pointer and strides), else must overlap neither q nor k. Outputs
- * lie token by token (ldqo >= (hq - 1) * hsqo + dim) or head by head (hsqo >= (T - 1) * ldqo + dim).
+ * which may be the input itself (same pointer and strides), else must overlap neither q nor k; qo and
+ * ko are apart. Outputs lie token by token (ldqo >= (hq - 1) * hsqo + dim) or head by head (hsqo >= (T - 1) * ldqo + dim).
  *   u = v / sqrt(mean(v^2) + eps) * w     (w: qw or kw, fp32 [dim], or NULL for ones)
  *   rotated over u[rot_off .. rot_off + rot): the pairs (i, i + rot/2) (K3D_ROT_HALVES) or
  *   (2i, 2i + 1) (K3D_ROT_INTERLEAVED) turn by the angle pos[t] * inv_freq[i], i < rot/2, and are

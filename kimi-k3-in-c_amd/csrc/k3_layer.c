@@ -41,6 +41,7 @@ int k3d_linear(void *y, int y_type, long ldy, const void *x, int x_type, long ld
     if (ldx < in || ldw < in || ldy < out || (res && ldr < out)) return k3dx_bad("k3d_linear: a stride is shorter than its row");
     if (ldx > K3D_LINEAR_MAX_LD || ldw > K3D_LINEAR_MAX_LD || in > K3D_LINEAR_MAX_IN)
         return k3dx_bad("k3d_linear: ldx and ldw up to K3D_LINEAR_MAX_LD, in up to K3D_LINEAR_MAX_IN");
+    if (out > K3D_LINEAR_MAX_OUT) return k3dx_bad("k3d_linear: out up to K3D_LINEAR_MAX_OUT");
     if (!y || !x || !W) return k3dx_bad("k3d_linear: y, x and W must be given");
     if (res == y && ldr != ldy) return k3dx_bad("k3d_linear: res in y's place needs y's stride");
     if (!aligned(y, type_size(y_type)) || !aligned(res, type_size(y_type)) || !aligned(x, type_size(x_type)) ||
@@ -166,6 +167,7 @@ int k3d_qk_norm_rope(void *qo, long ldqo, long hsqo, void *ko, long ldko, long h
                 return k3dx_bad("k3d_qk_norm_rope: the outputs of a token and of a head overlap");
         }
     }
+    if (hq && hk && qo == ko) return k3dx_bad("k3d_qk_norm_rope: qo and ko are one place");
     a.type = type;
     a.T = T;
     a.dim = dim;

@@ -355,7 +355,7 @@ typedef struct {
 } K3kRoute;
 int k3k_route(const K3kRoute *a, void *stream);
 
-/* The arguments of k3d_qk_norm_rope, checked; views[0]: queries, views[1]: keys. */
+/* The arguments of k3d_qk_norm_rope, checked; v[0]: queries, v[1]: keys. */
 typedef struct {
     struct {
         void *out;

@@ -208,3 +208,17 @@ def test_every_kernel(gpu, k3, T, inn, out, x_type, off):
 def test_every_few(gpu, k3, T, inn, out, x_type):
     """Each group of tokens with each number of rows of W a workgroup takes, and with W past the caches."""
     test_every_kernel(gpu, k3, T, inn, out, x_type, 0)
+
+
+@pytest.mark.parametrize("T,inn,out", [(2, 64, 20), (20, 128, 40), (90, 256, 140), (90, 200, 140), (3, 40, 20)])
+def test_nan_payloads(gpu, k3, T, inn, out):
+    """An fp32 NaN whose payload lies in any of its three parts makes its row NaN, an infinity infinite, and no other row either."""
+    say(f"case: {T} {inn} {out}")
+    bits = [0x7f800001, 0xff800100, 0x7f810000, 0x7fc00000, 0xffffffff]
+    for b in bits + [0x7f800000]:
+        x = torch.ones(T, inn, device="cuda")
+        x.view(torch.int32)[T - 1, inn - 1] = b - (1 << 32) if b >> 31 else b
+        w = torch.ones(out, inn, device="cuda", dtype=BF16)
+        y = lo.linear(k3, x, w)
+        assert (y[T - 1] == float("inf")).all() if b == 0x7f800000 else torch.isnan(y[T - 1]).all()
+        assert (y[:T - 1] == inn).all()

@@ -95,7 +95,7 @@ APART = dict(LINEAR, x=2 * A, W=3 * A, bias=4 * A, ws=5 * A)
 
 
 @pytest.mark.parametrize("change,word", [
-    (dict(T=(1 << 24) + 1), "MAX_TOKENS"), (dict(y=2 * A), "operand"), (dict(y=3 * A), "operand"), (dict(y=4 * A), "operand"),
+    (dict(T=(1 << 24) + 1), "MAX_TOKENS"), (dict(out=(1 << 28) + 1, ldy=1 << 30), "MAX_OUT"), (dict(y=2 * A), "operand"), (dict(y=3 * A), "operand"), (dict(y=4 * A), "operand"),
     (dict(y=5 * A), "operand")])
 def test_linear_places(k3, change, word):
     refused(k3, k3.lib().k3d_linear(*dict(APART, **change).values(), None), word)
@@ -107,7 +107,7 @@ def test_route_tokens(k3):
 
 @pytest.mark.parametrize("change,word", [
     (dict(T=(1 << 24) + 1), "MAX_TOKENS"),
-    (dict(ldqo=255), "token and of a head"), (dict(ldqo=64, hsqo=255), "token and of a head"),
+    (dict(qo=3 * A, ko=3 * A), "one place"), (dict(ldqo=255), "token and of a head"), (dict(ldqo=64, hsqo=255), "token and of a head"),
     (dict(ldko=64, hsko=64), "token and of a head"), (dict(ldqo=1 << 62, hsqo=1 << 62), "token and of a head")])
 def test_heads_places(k3, change, word):
     refused(k3, k3.lib().k3d_qk_norm_rope(*dict(HEADS, **change).values(), None), word)
