@@ -14,8 +14,10 @@
  *     gelu_tanh 573 us = 1.26 PFLOP/s, the library's product alone 545);
  *   - weights that are not 16-byte aligned rows of whole 16 bytes: the same tiles, with W through registers instead of
  *     DMA (which wants 16-byte addresses); small ones for a few tokens, and rows shorter than a step, by lin_stream_kernel;
- *   - x that does not suit the DMA, rows that end inside a step, and fp32 x for many tiles of outputs: lin_pack_kernel lays it out
- *     in the workspace first.
+ *   - x that does not suit the DMA, and fp32 x for many tiles of outputs: lin_pack_kernel lays it out in the
+ *     workspace first.
+ *   - rows that end inside a step: the last step takes their last 64 columns, with zeros for those that come twice (300
+ *     tokens of 4104 -> 2048 19.1 us; with x laid out first 21.9; 4096 of 4104 -> 4096, where that counts least, 136 and 130).
  * Which of them, and the tile and slices, go by the costs estimated below.
  */
 #include "k3_common.h"
@@ -317,19 +319,35 @@ __global__ __launch_bounds__(64 * NW) void lin_skinny_kernel(K3kLinear a)
         else b = S3;
         return b + wv * STG;
     };
-    /* the stage of column block xk; the last block of a row ends with it (columns of the block before come
-     * again, see `over`); past the wave's run: zeros, so that every stage requests as much */
+    /* the columns of the last block that the one before it holds, per parity of a DMA (the swizzle's period) */
+    const int over = nks * KS - a.in;
+    uint32_t again[XF32 ? 3 : 1][2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int c = (lane & (C - 1)) ^ swz(RD * i + lane / C);
+        again[0][i] = 8 * c < over ? LIN_OOB : 0u;
+        if constexpr (XF32) again[1][i] = 4 * c < over ? LIN_OOB : 0u, again[2][i] = 4 * (C + c) < over ? LIN_OOB : 0u;
+    }
+    /* the stage of column block xk; the last block of a row ends with it, with zeros (of W and of x: either may be
+     * infinite) for the columns that come twice; past the wave's run: zeros, so that every stage requests as much */
     int xk = k0;
     auto issue = [&](auto slot) {
         uint16_t *const b = buf_of(slot);
         const uint32_t none = xk < k1 ? 0u : LIN_OOB;
-        const uint32_t c = xk == nks - 1 ? a.in - KS : xk * KS;
+        const bool end = xk == nks - 1;
+        const uint32_t c = end ? a.in - KS : xk * KS;
+        uint32_t no[XF32 ? 3 : 1][2];
 #pragma unroll
-        for (int i = 0; i < WD; i++) k3_dma16<POL>(rw, b + i * 512, wo[i] | none, c * 2);
+        for (int q = 0; q < (XF32 ? 3 : 1); q++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) no[q][i] = none | (end ? again[q][i] : 0u);
+#pragma unroll
+        for (int i = 0; i < WD; i++) k3_dma16<POL>(rw, b + i * 512, wo[i] | no[0][i & 1], c * 2);
 #pragma unroll
         for (int h = 0; h < XB; h++)
 #pragma unroll
-            for (int i = 0; i < XD; i++) k3_dma16(rx, b + (WD + h * XD + i) * 512, xo[i] | none, c * (XF32 ? 4 : 2) + h * KS * 2);
+            for (int i = 0; i < XD; i++)
+                k3_dma16(rx, b + (WD + h * XD + i) * 512, xo[i] | no[XF32 ? 1 + h : 0][i & 1], c * (XF32 ? 4 : 2) + h * KS * 2);
         xk++;
     };
     k3_f32x4 acc[RW][NT];
@@ -337,12 +355,11 @@ __global__ __launch_bounds__(64 * NW) void lin_skinny_kernel(K3kLinear a)
     for (int i = 0; i < RW; i++)
 #pragma unroll
         for (int j = 0; j < NT; j++) acc[i][j] = k3_f32x4{0.f, 0.f, 0.f, 0.f};
-    const int sw = swz(r16), over = nks * KS - a.in;
+    const int sw = swz(r16);
     constexpr int WAITN = DN * (NST - 1);
     constexpr int WAIT_STAGE = (WAITN & 15) | (7 << 4) | (15 << 8) | ((WAITN >> 4) << 14);
     constexpr int WAIT_LGKM0 = 15 | (7 << 4) | (0 << 8) | (3 << 14);
     static_assert(WAITN < 64, "requests in flight");
-    int rk = k0;
     auto step = [&](auto slot) {
         const uint16_t *const b = buf_of(slot);
         __builtin_amdgcn_s_waitcnt(WAIT_STAGE);
@@ -369,17 +386,15 @@ __global__ __launch_bounds__(64 * NW) void lin_skinny_kernel(K3kLinear a)
         __builtin_amdgcn_sched_barrier(0);
         issue(slot);
         __builtin_amdgcn_sched_barrier(0);
-        const int skip = rk++ == nks - 1 ? over : 0;
 #pragma unroll
         for (int h = 0; h < KS / 32; h++)
 #pragma unroll
             for (int j = 0; j < NT; j++) {
-                const bool zero = 32 * h + 8 * g < skip;
                 if constexpr (XF32) {
                     float f[8];
                     uint32_t t[3][4];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) f[e] = zero ? 0.0f : __uint_as_float(xf[h][j][e / 4][e % 4]);
+                    for (int e = 0; e < 8; e++) f[e] = __uint_as_float(xf[h][j][e / 4][e % 4]);
                     cut3(f, t[2], t[1], t[0]);
 #pragma unroll
                     for (int q = 0; q < 3; q++)
@@ -387,9 +402,7 @@ __global__ __launch_bounds__(64 * NW) void lin_skinny_kernel(K3kLinear a)
                         for (int i = 0; i < RW; i++)
                             acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(k3_bf16x8, wf[h][i]), as_frag(t[q]), acc[i][j], 0, 0, 0);
                 } else {
-                    u32x4 v = xf[h][j][0];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) v[e] = zero ? 0u : v[e];
+                    const u32x4 v = xf[h][j][0];
 #pragma unroll
                     for (int i = 0; i < RW; i++)
                         acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(k3_bf16x8, wf[h][i]), __builtin_bit_cast(k3_bf16x8, v), acc[i][j], 0, 0, 0);
@@ -484,6 +497,7 @@ typedef struct {
     long ldx;
     int xcols;              /* columns of x: in, or all terms' padded ones */
     int nks, steps;         /* steps of one term, of all */
+    int xend;               /* the step that reads x's last 64 columns where they end (its first ones again as zeros), or -1 */
     int nt, no;             /* tiles over tokens and outputs */
     int nsl, per;           /* slices of the steps, steps of one */
     float *part;            /* [nsl][T][out] sums of the slices (nsl > 1) */
@@ -506,7 +520,8 @@ __device__ __forceinline__ void tile_of(const LinTile &p, int b, int &tt, int &t
     tt = q * GT + r % h;
 }
 
-template <int BT, int BO, int WT, int WO, int NST, bool WREG, int POL, bool XF32>
+/* TAIL: rows that end inside a step (without what that takes in each step 4096 tokens of 7168 -> 12288 562 us, with it 586) */
+template <int BT, int BO, int WT, int WO, int NST, bool WREG, int POL, bool XF32, bool TAIL>
 __global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
 {
     constexpr int NW = WT * WO, FT = BT / WT / 16, FO = BO / WO / 16;
@@ -550,6 +565,18 @@ __global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
         const int r = (i * NW + wv) * 8 + lane / 8;
         wo_[i] = (uint32_t)min(r, on - 1) * (uint32_t)(p.a.ldw * 2) + ((lane & 7) ^ sww(r)) * 16;
     }
+    /* The last block of a row: zeros, of x (step xend) and of W (either may be infinite), for the 16-byte columns that the block before it
+     * holds. A lane's column of x is the same in each of its DMAs, of W in every second one. */
+    static_assert(NW * XR % 16 == 0 && NW * 16 % 64 == 0, "swizzles repeat from DMA to DMA");
+    /* (one register: bit 2 - i W's DMAs of parity i, bit 0 x's) */
+    const int over = p.nks * LIN_KS - p.a.in;
+    auto twice = [&](int ln) -> uint32_t {
+        auto w = [&](int i) { return 8 * ((ln & 7) ^ sww((i * NW + wv) * 8 + ln / 8)) < over; };
+        return (16 * ((ln & (64 / XR - 1)) ^ swx(wv * XR + ln / (64 / XR))) < over * XS) | w(0) << 2 | w(1) << 1;
+    };
+    constexpr bool FULL = BT * BO >= 256 * 256;     /* (no register left: formed again in each step) */
+    const uint32_t twice0 = FULL || !TAIL ? 0u : twice(lane);
+    constexpr bool WSAME = NW * 8 % (FG == 4 ? 64 : FG == 2 ? 32 : 16) == 0;        /* one column in all of them */
     auto buf_of = [&](auto slot) -> uint16_t * {
         constexpr int S = decltype(slot)::value;
         if constexpr (S == 0) return S0;
@@ -558,18 +585,27 @@ __global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
         else return S3;
     };
     /* Stages are requested in order: step `xk` of x, which is column block `wk` of W (of a term), the last one
-     * of a row from where its 64 columns end with the row. Past the slice: zeros, so that every step requests
+     * of a row from where its 64 columns end with the row (x: zeros in the columns that come twice). Past the slice: zeros, so that every step requests
      * as much and none is under a branch. */
     int xk = k0, wk = k0 % p.nks;
     const int kend = k0 + n;
     auto issue = [&](auto slot) {
         uint16_t *const b = buf_of(slot);
         const uint32_t none = xk < kend ? 0u : LIN_OOB;
-        const uint32_t xs = (uint32_t)xk * (LIN_KS * XS), ws = (uint32_t)(wk == p.nks - 1 ? p.a.in - LIN_KS : wk * LIN_KS) * 2;
+        const bool end = TAIL && xk == p.xend, wend = TAIL && wk == p.nks - 1;
+        const uint32_t xs = (uint32_t)(end ? p.a.in - LIN_KS : xk * LIN_KS) * XS, ws = (uint32_t)(wend ? p.a.in - LIN_KS : wk * LIN_KS) * 2;
+        uint32_t again = twice0;
+        if (FULL && TAIL) {
+            uint32_t all = 0xffffffffu;
+            asm volatile("" : "+s"(all));
+            again = twice(__builtin_amdgcn_mbcnt_hi(all, __builtin_amdgcn_mbcnt_lo(all, 0)));
+        }
+        const uint32_t nx = none | (end ? again << 31 : 0u), w0 = none | (wend ? again << 29 & LIN_OOB : 0u);
+        const uint32_t w1 = WSAME ? w0 : none | (wend ? again << 30 & LIN_OOB : 0u);
 #pragma unroll
-        for (int i = 0; i < XD; i++) k3_dma16(rx, b + (i * NW + wv) * 512, xo[i] | none, xs);
+        for (int i = 0; i < XD; i++) k3_dma16(rx, b + (i * NW + wv) * 512, xo[i] | nx, xs);
 #pragma unroll
-        for (int i = 0; i < WD; i++) k3_dma16<POL>(rw, b + BT * XE + (i * NW + wv) * 512, wo_[i] | none, ws);
+        for (int i = 0; i < WD; i++) k3_dma16<POL>(rw, b + BT * XE + (i * NW + wv) * 512, wo_[i] | (i & 1 ? w1 : w0), ws);
         xk++;
         if (++wk == p.nks) wk = 0;
     };
@@ -898,7 +934,9 @@ float skinny_cost(int T, int in, int out, bool f32, int rw, long cus)
 template <int BT, int BO, int WT, int WO, int NST, bool WREG, int POL = K3_LD_DEFAULT, bool XF32 = false>
 void tile_go(const LinTile *p, hipStream_t st)
 {
-    lin_tile_kernel<BT, BO, WT, WO, NST, WREG, POL, XF32><<<p->nt * p->no * p->nsl, 64 * WT * WO, 0, st>>>(*p);
+    const int grid = p->nt * p->no * p->nsl;
+    if (WREG || p->a.in % LIN_KS) lin_tile_kernel<BT, BO, WT, WO, NST, WREG, POL, XF32, true><<<grid, 64 * WT * WO, 0, st>>>(*p);
+    else if constexpr (!WREG) lin_tile_kernel<BT, BO, WT, WO, NST, WREG, POL, XF32, false><<<grid, 64 * WT * WO, 0, st>>>(*p);
 }
 
 /* Microseconds of a launch of lin_tile_kernel and, with slices, the join: rounds of as many workgroups as fit the chip, each
@@ -931,7 +969,7 @@ float tile_cost(const Shape &s, int T, int in, int out, int steps, int nsl, long
  * 1024 of 7168 -> 7168 294 and 353, as each tile of outputs cuts its tokens again.) */
 float cut_cost(int bo, int T, int in, int out, int nsl, long cus)
 {
-    const int nks = in / LIN_KS, per = (nks + nsl - 1) / nsl;
+    const int nks = (in + LIN_KS - 1) / LIN_KS, per = (nks + nsl - 1) / nsl;
     const long wgs = (long)((T + 63) / 64) * ((out + bo - 1) / bo) * nsl, slots = 2 * cus;
     const float one = bo == 64 ? 0.49f : 0.73f, two = bo == 64 ? 0.70f : 1.00f, kb = bo / 8.0f + 16.0f;
     auto round = [&](long n) { return both(per * (n <= cus ? one : two), per * kb * n / 25000.0f); };
@@ -959,7 +997,7 @@ extern "C" int k3k_linear(const K3kLinear *a, void *stream)
     const bool dma = w16 && a->in % 8 == 0 && a->in >= LIN_KS;
     const int nks = (a->in + LIN_KS - 1) / LIN_KS;
     int steps = nks * (f32 ? 3 : 1);
-    const bool pack = f32 || !x16 || a->in % LIN_KS;
+    const bool pack = f32 || !x16 || !dma;
 
     /* the cheapest tile shape and number of slices */
     float best = 0.0f;
@@ -976,7 +1014,7 @@ extern "C" int k3k_linear(const K3kLinear *a, void *stream)
     if (pack) best += 2.5f + (float)a->T * kpad(a->in) * (f32 ? 10 : 4) / 4e6f;
     /* or fp32 rows as they are */
     int cut = 0;
-    if (f32 && dma && x16 && a->in % LIN_KS == 0)
+    if (f32 && dma && x16)
         for (int bo : {64, 128})
             for (int n : {1, 2, 3, 4, 6, 8, 12, LIN_MAX_SLICES}) {
                 if (n > 1 && (n * one > room || nks < 4 * n)) break;
@@ -1018,10 +1056,12 @@ extern "C" int k3k_linear(const K3kLinear *a, void *stream)
         K3K_LAUNCH_CHECK("linear: pack");
         p.x = a->ws;
         p.ldx = p.xcols = p.steps * LIN_KS;
+        p.xend = -1;
     } else {
         p.x = a->x;
         p.ldx = a->ldx;
         p.xcols = a->in;
+        p.xend = nks - 1;
     }
     p.part = (float *)((char *)a->ws + pack_bytes(a->T, a->in, a->x_type));
     const int bt = cut ? 64 : SHAPES[shape].bt, bo = cut ? cut : SHAPES[shape].bo;

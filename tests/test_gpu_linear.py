@@ -222,3 +222,32 @@ def test_nan_payloads(gpu, k3, T, inn, out):
         y = lo.linear(k3, x, w)
         assert (y[T - 1] == float("inf")).all() if b == 0x7f800000 else torch.isnan(y[T - 1]).all()
         assert (y[:T - 1] == inn).all()
+
+
+@pytest.mark.parametrize("T,inn,out", [(2, 72, 20), (9, 200, 40), (20, 520, 70), (48, 136, 33), (64, 1096, 64), (90, 200, 140), (300, 1160, 260),
+                                       (700, 328, 513), (90, 201, 140), (3, 40, 20), (3, 201, 20), (1500, 777, 999)])
+def test_infinite_weight(gpu, k3, T, inn, out):
+    """An infinite weight in any column, those at the end of a row among them, makes its own outputs infinite and no other; so does an
+    infinite activation, in bf16 and in fp32."""
+    say(f"case: {T} {inn} {out}")
+    for x_type in (BF16, F32):
+        x, w, b, r = operands(T, inn, out, x_type, F32, 3)
+        x.abs_().add_(0.5)
+        w.abs_().add_(0.125)
+        clean = lo.linear(k3, x, w, b, "none", r)
+        for k in sorted({0, 1, inn // 2, max(0, inn - 64), max(0, inn - 57), inn - inn % 64 - 1 if inn > 64 else 0, inn - 8, inn - 1}):
+            if x_type == BF16:                                     # (with fp32 x it meets the terms that are zero)
+                keep = w[7, k].clone()
+                w[7, k] = float("inf")
+                y = lo.linear(k3, x, w, b, "none", r)
+                w[7, k] = keep
+                assert (y[:, 7] == float("inf")).all(), k
+                on = torch.arange(out, device="cuda") != 7
+                assert torch.equal(y[:, on], clean[:, on])
+            keep = x[1, k].clone()
+            x[1, k] = float("-inf")
+            y = lo.linear(k3, x, w, b, "none", r)
+            x[1, k] = keep
+            assert (y[1] == float("-inf")).all(), k
+            on = torch.arange(T, device="cuda") != 1
+            assert torch.equal(y[on], clean[on])
