@@ -153,3 +153,41 @@ def test_graph(gpu, k3, T):
         if ex:
             L.k3d_graph_destroy(ex)
         L.k3d_stream_destroy(st)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("pairs", [0, 1])
+@pytest.mark.parametrize("dim", [4, 5, 7, 8, 9, 11, 15, 16, 17, 23, 31, 63, 65, 129, 255, 257, 519, 1021])
+def test_any_borders(gpu, k3, dim, pairs, dtype):
+    """Rotated ranges that begin, halve and end anywhere, at odd strides and starts, out of place and in place; what lies between the heads
+    stays as it is."""
+    for n, (rot, off) in enumerate([(dim // 2 * 2, dim % 2), (2, dim - 2), (dim // 4 * 2, 1), (dim // 6 * 2, dim // 3), (0, 0)]):
+        say(f"case: {dim} {rot} {off} {pairs} {dtype}")
+        T, hq, hk, hs = 6, 5, 2, dim + 1 + n
+        ld = (hq + hk) * hs + 3
+        g = lo.gen(dim + n)
+        buf = torch.randn(T * ld + 5, device="cuda", generator=g).to(dtype)
+        def views(b):
+            rows = b[1 + n % 2:1 + n % 2 + T * ld].view(T, ld)[:, :(hq + hk) * hs].unflatten(1, (hq + hk, hs))
+            return rows[:, :hq, :dim], rows[:, hq:, :dim]
+        q, k = views(buf)
+        qw = torch.rand(dim, device="cuda", generator=g) + 0.5
+        pos = torch.randint(0, 5000, (T,), device="cuda", generator=g).int()
+        pos[2] = -1
+        on = torch.arange(T, device="cuda") != 2
+        freq = freqs(rot) if rot else torch.ones(1, device="cuda", dtype=torch.float64)
+        want = [lo.heads64(v[on], w, pos[on], freq, rot, off, pairs, 1e-6, 1.0) for v, w in ((q, qw), (k, None))]
+        out = torch.full_like(buf, 7.0)
+        qo, ko = views(out)
+        was = buf.clone()
+        lo.heads(k3, q, k, qw, None, pos, freq, rot, off, pairs, qo=qo, ko=ko)
+        assert torch.equal(buf, was)
+        for v, w in zip((qo, ko), want):
+            lo.within(v[on], w)
+            v[on] = 7.0
+        assert (out == 7).all()                                    # the padding token and all between the heads
+        lo.heads(k3, q, k, qw, None, pos, freq, rot, off, pairs, qo=q, ko=k)
+        for v, u, w in zip((q, k), views(was), want):
+            lo.within(v[on], w)
+            v[on] = u[on]
+        assert torch.equal(buf, was)
