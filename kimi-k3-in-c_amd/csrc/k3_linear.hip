@@ -44,84 +44,99 @@ __device__ __forceinline__ void each_stage(F &&f)
 }
 
 /* ---- epilogue ------------------------------------------------------------------------ */
-/* v / (1 + e^-z). e^-z as 2^t (1 + r ln 2), t = -z log2 e rounded and r what the rounding left: within 3 units in the last
- * place, for a third of the instructions of expf and a division (silu of 4096 x 12288 outputs, bf16: 592 -> 580 us
- * with the product). */
+/* v / (1 + e^-z). e^-z as 2^t (1 + r ln 2), t = -z log2 e rounded and r what the rounding left, and a corrected reciprocal: within
+ * 3 units in the last place of fp32, for a third of the instructions of expf and a division. Not FINE, for a result that
+ * is rounded to bf16: without r and the correction, which leaves |t| 2^-24 and two units, under 2^-17 of the value, where the rounding
+ * takes up to 2^-9 (8192 tokens of 512 -> 2048 with silu 44.4 us, 35.7 so, 5.6 of it by
+ * the instruction that rounds to bf16). */
+template <bool FINE>
 __device__ __forceinline__ float over_1p_exp(float v, float z)
 {
     const float t = -1.44269504f * z;
-    const float r = fabsf(t) < 127.0f ? fmaf(z, -1.92596299e-8f, fmaf(z, -1.44269504f, -t)) : 0.0f;
     const float e = __builtin_amdgcn_exp2f(t);
-    const float d1 = fmaf(e, fmaf(r, 0.693147181f, 1.0f), 1.0f);
+    float d1 = 1.0f + e;
+    if (FINE) {
+        const float r = fabsf(t) < 127.0f ? fmaf(z, -1.92596299e-8f, fmaf(z, -1.44269504f, -t)) : 0.0f;
+        d1 = fmaf(e, fmaf(r, 0.693147181f, 1.0f), 1.0f);
+    }
     const float k = d1 > 0x1p64f ? 0x1p-64f : 1.0f, d = d1 * k;     /* (the reciprocal stays normal) */
-    const float q = __builtin_amdgcn_rcpf(d), w = v * k * q, c = fmaf(fmaf(-d, w, v * k), q, w);
+    const float q = __builtin_amdgcn_rcpf(d), w = v * k * q;
+    if (!FINE) return w;
+    const float c = fmaf(fmaf(-d, w, v * k), q, w);
     return c == c ? c : w;          /* (no correction where d or w is infinite) */
 }
 
+template <bool FINE>
 __device__ __forceinline__ float act_of(float v, int act)
 {
     switch (act) {
     case K3D_ACT_RELU: return v < 0.0f ? 0.0f : v;
-    case K3D_ACT_SILU: return over_1p_exp(v, v);
+    case K3D_ACT_SILU: return over_1p_exp<FINE>(v, v);
     case K3D_ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678f));
-    case K3D_ACT_GELU_TANH: return over_1p_exp(v, 1.59576912f * v * fmaf(0.044715f * v, v, 1.0f));
+    case K3D_ACT_GELU_TANH: return over_1p_exp<FINE>(v, 1.59576912f * v * fmaf(0.044715f * v, v, 1.0f));
     default: return v;
     }
 }
 
-/* outputs o .. o + 3 of token t (those below a.out), from their sums; b: their bias */
-__device__ __forceinline__ void put4(const K3kLinear &a, int t, int o, float4 acc, const float (&b)[4])
+/* the residual of outputs o ..+4 of token t as it lies in memory, requested apart from its use: an epilogue that waits for each row's
+ * costs more than the bytes (8192 tokens of 512 -> 2048 with silu and a residual 54 us, four rows requested ahead 48) */
+__device__ __forceinline__ uint4 res4(const K3kLinear &a, int t, int o)
+{
+    uint4 r = make_uint4(0, 0, 0, 0);
+    if (!a.res || t >= a.T || o >= a.out) return r;
+    const size_t at = (size_t)t * a.ldr + o;
+    const int n = a.out - o;
+    if (a.y_type == K3D_F32) {
+        const uint32_t *q = (const uint32_t *)a.res + at;
+        if (n >= 4) __builtin_memcpy(&r, q, 16);
+        else r.x = q[0], r.y = n > 1 ? q[1] : 0u, r.z = n > 2 ? q[2] : 0u;
+    } else {
+        const uint16_t *q = (const uint16_t *)a.res + at;
+        if (n >= 4) __builtin_memcpy(&r, q, 8);
+        else r.x = q[0] | (n > 1 ? (uint32_t)q[1] << 16 : 0u), r.y = n > 2 ? q[2] : 0u;
+    }
+    return r;
+}
+
+/* outputs o ..+4 of token t: acc + bias b through the activation, plus the residual r (any alignment: the hardware stores 16
+ * bytes to any address) */
+__device__ __forceinline__ void put4(const K3kLinear &a, int t, int o, float4 acc, const float (&b)[4], uint4 r)
 {
     if (t >= a.T || o >= a.out) return;
-    const size_t yi = (size_t)t * a.ldy + o, ri = (size_t)t * a.ldr + o;
+    const size_t yi = (size_t)t * a.ldy + o;
     const int n = min(4, a.out - o);
     float v[4] = {acc.x + b[0], acc.y + b[1], acc.z + b[2], acc.w + b[3]};
-    if (a.act)
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = act_of(v[i], a.act);
     if (a.y_type == K3D_F32) {
-        float *y = (float *)a.y + yi;
-        const float *r = (const float *)a.res + ri;
-        if (a.res) {
-            if (n == 4 && ((uintptr_t)r & 15) == 0) {
-                const float4 q = *reinterpret_cast<const float4 *>(r);
-                v[0] += q.x, v[1] += q.y, v[2] += q.z, v[3] += q.w;
-            } else {
+        if (a.act)
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (i < n) v[i] += r[i];
-            }
-        }
-        if (n == 4 && ((uintptr_t)y & 15) == 0) {
-            *reinterpret_cast<float4 *>(y) = make_float4(v[0], v[1], v[2], v[3]);
+            for (int i = 0; i < 4; i++) v[i] = act_of<true>(v[i], a.act);
+        float *y = (float *)a.y + yi;
+        if (a.res) v[0] += __uint_as_float(r.x), v[1] += __uint_as_float(r.y), v[2] += __uint_as_float(r.z), v[3] += __uint_as_float(r.w);
+        if (n == 4) {
+            __builtin_memcpy(y, v, 16);
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < 3; i++)
                 if (i < n) y[i] = v[i];
         }
     } else {
+        if (a.act)
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = act_of<false>(v[i], a.act);
         uint16_t *y = (uint16_t *)a.y + yi;
-        const uint16_t *r = (const uint16_t *)a.res + ri;
         if (a.res) {
-            if (n == 4 && ((uintptr_t)r & 7) == 0) {
-                const uint2 q = *reinterpret_cast<const uint2 *>(r);
-                v[0] += __uint_as_float(q.x << 16), v[1] += __uint_as_float(q.x & 0xffff0000u);
-                v[2] += __uint_as_float(q.y << 16), v[3] += __uint_as_float(q.y & 0xffff0000u);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (i < n) v[i] += k3_bf16_to_f32(r[i]);
-            }
+            v[0] += __uint_as_float(r.x << 16), v[1] += __uint_as_float(r.x & 0xffff0000u);
+            v[2] += __uint_as_float(r.y << 16), v[3] += __uint_as_float(r.y & 0xffff0000u);
         }
-        uint16_t h[4];
+        __bf16 h[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) h[i] = k3_bf16_rne(v[i]);
-        if (n == 4 && ((uintptr_t)y & 7) == 0) {
-            *reinterpret_cast<uint2 *>(y) = make_uint2((uint32_t)h[0] | (uint32_t)h[1] << 16, (uint32_t)h[2] | (uint32_t)h[3] << 16);
+        for (int i = 0; i < 4; i++) h[i] = (__bf16)v[i];
+        if (n == 4) {
+            __builtin_memcpy(y, h, 8);
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (i < n) y[i] = h[i];
+            for (int i = 0; i < 3; i++)
+                if (i < n) y[i] = __builtin_bit_cast(uint16_t, h[i]);
         }
     }
 }
@@ -265,12 +280,13 @@ __global__ __launch_bounds__(512) void lin_stream_kernel(K3kLinear a, int nw)
         const int o = o0 + 4 * g;
         float b[4];
         bias4(a, o, b);
+        const uint4 res = res4(a, t0 + r16, o);
         float4 s = part[lane];
         for (int w = 1; w < nw; w++) {
             const float4 v = part[w * 64 + lane];
             s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
         }
-        put4(a, t0 + r16, o, s, b);
+        put4(a, t0 + r16, o, s, b, res);
     }
 }
 
@@ -429,6 +445,7 @@ __global__ __launch_bounds__(64 * NW) void lin_skinny_kernel(K3kLinear a)
         const int o = o0 + 16 * (q / NT) + 4 * g, t = 16 * (q % NT) + r16;
         float b[4];
         bias4(a, o, b);
+        const uint4 res = res4(a, t, o);
         const float4 *p = reinterpret_cast<const float4 *>(S0) + q * 64 + lane;
         float4 s = p[0];
 #pragma unroll
@@ -436,7 +453,7 @@ __global__ __launch_bounds__(64 * NW) void lin_skinny_kernel(K3kLinear a)
             const float4 v = p[w * (STG / 8)];
             s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
         }
-        put4(a, t, o, s, b);
+        put4(a, t, o, s, b, res);
     }
 }
 
@@ -760,7 +777,6 @@ __global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
     each_stage<0, NST - 1>([&](auto slot) {
         if (decltype(slot)::value < left) step(slot);
     });
-    __builtin_amdgcn_s_waitcnt(WAIT_VM0);      /* the last requests land before LDS is used again */
 
     /* A lane holds token r16 of each token fragment and 4 FG consecutive outputs of FG fragments. The sums go
      * through LDS (the stage buffers, a region per wave, JR token fragments at a time; 16-byte column c of row r
@@ -773,8 +789,17 @@ __global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
     if (PER < NW) stage = wv / PER == 0 ? S0 : S1;
     float4 *const reg = reinterpret_cast<float4 *>(stage + (wv % PER) * (RB / 2));
     const int c = lane % C, o = o0 + wo * WOUT + 4 * c;
+    /* the residuals of the first PF iterations; each, once used, makes room for the one PF further */
+    constexpr int RI = 64 / C, IT = 16 * JR / RI, NIT = 16 * FT / RI, PF = IT < 4 ? IT : 4;
+    static_assert(IT % PF == 0, "residuals");
+    const int row0 = t0 + wt * (BT / WT) + lane / C;
+    uint4 res[PF];
+    if (p.nsl == 1)
+#pragma unroll
+        for (int k = 0; k < PF; k++) res[k] = res4(p.a, row0 + k * RI, o);
     float b[4];
     bias4(p.a, p.nsl > 1 ? p.a.out : o, b);
+    __builtin_amdgcn_s_waitcnt(WAIT_VM0);      /* the last requests land before LDS is used again */
     __syncthreads();
 #pragma unroll
     for (int j0 = 0; j0 < FT; j0 += JR) {
@@ -786,24 +811,28 @@ __global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
                 reg[r * C + (oc ^ (r16 & (C - 1)))] = make_float4(acc[i][j0 + j][0], acc[i][j0 + j][1], acc[i][j0 + j][2], acc[i][j0 + j][3]);
             }
         __builtin_amdgcn_wave_barrier();
-#pragma unroll 2
-        for (int r = lane / C; r < 16 * JR; r += 64 / C) {
-            const float4 v = reg[r * C + (c ^ (r & 15 & (C - 1)))];
-            const int t = t0 + wt * (BT / WT) + 16 * j0 + r;
-            if (p.nsl == 1) {
-                put4(p.a, t, o, v, b);
-            } else if (t < p.a.T && o < p.a.out) {
-                float *q = p.part + ((size_t)sl * p.a.T + t) * p.a.out + o;
-                if (o + 4 <= p.a.out && ((uintptr_t)q & 15) == 0) {
-                    *reinterpret_cast<float4 *>(q) = v;
-                } else {
-                    const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll 1
+        for (int i = 0; i < IT; i += PF)
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (o + i < p.a.out) q[i] = e[i];
+            for (int k = 0; k < PF; k++) {
+                const int r = lane / C + (i + k) * RI, t = row0 + 16 * j0 + (i + k) * RI;
+                const float4 v = reg[r * C + (c ^ (r & 15 & (C - 1)))];
+                if (p.nsl == 1) {
+                    const uint4 q = res[k];
+                    if (j0 * 16 / RI + i + k + PF < NIT) res[k] = res4(p.a, t + PF * RI, o);
+                    put4(p.a, t, o, v, b, q);
+                } else if (t < p.a.T && o < p.a.out) {
+                    float *q = p.part + ((size_t)sl * p.a.T + t) * p.a.out + o;
+                    if (o + 4 <= p.a.out) {
+                        __builtin_memcpy(q, &v, 16);
+                    } else {
+                        const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int n = 0; n < 3; n++)
+                            if (o + n < p.a.out) q[n] = e[n];
+                    }
                 }
             }
-        }
         __builtin_amdgcn_wave_barrier();
     }
 }
@@ -817,6 +846,7 @@ __global__ __launch_bounds__(64) void lin_join_kernel(K3kLinear a, const float *
     if (t >= a.T) return;
     float b[4];
     bias4(a, o, b);
+    const uint4 res = res4(a, t, o);
     const float *const q = part + (size_t)t * a.out + o;
     const size_t one = (size_t)a.T * a.out;
     const int n = min(4, a.out - o);
@@ -833,7 +863,7 @@ __global__ __launch_bounds__(64) void lin_join_kernel(K3kLinear a, const float *
         for (int j = 0; j < 4; j++)
             if (s + j < nsl) v.x += f[j].x, v.y += f[j].y, v.z += f[j].z, v.w += f[j].w;
     }
-    put4(a, t, o, v, b);
+    put4(a, t, o, v, b, res);
 }
 
 /* ---- launches -------------------------------------------------------------------------------- */
