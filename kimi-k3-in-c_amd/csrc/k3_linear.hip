@@ -11,7 +11,7 @@
  *     with a ring of LDS stages of its own filled by DMA (one token of 12288 -> 7168, 176 MB, 26.8 us = 6.6 TB/s);
  *   - more: the matrix cores. lin_tile_kernel, tiles of 64 x 64 to 256 x 256, over slices of the columns where the tiles alone
  *     leave CUs idle; the slices' sums are joined in slice order by lin_join_kernel (4096 tokens of 7168 -> 12288 with
- *     gelu_tanh 573 us = 1.26 PFLOP/s, the library's product alone 545);
+ *     silu 566 us = 1.27 PFLOP/s, the library's product alone 543);
  *   - weights that are not 16-byte aligned rows of whole 16 bytes: the same tiles, with W through registers instead of
  *     DMA (which wants 16-byte addresses); small ones for a few tokens, and rows shorter than a step, by lin_stream_kernel;
  *   - x that does not suit the DMA, and fp32 x for many tiles of outputs: lin_pack_kernel lays it out in the
@@ -66,13 +66,32 @@ __device__ __forceinline__ float over_1p_exp(float v, float z)
     return c == c ? c : w;          /* (no correction where d or w is infinite) */
 }
 
+/* v (1 + erf(v / sqrt 2)) / 2 through erfc(z) = t P(t) e^-z^2, z = |v| / sqrt 2, t = 1 / (1 + 0.38 z): P of degree 8 interpolates
+ * erfc(z) e^z^2 / t at the Chebyshev nodes of 0 <= z <= 10, within 2.5e-8 of itself (past it e^-z^2 is 0 in fp32). Off by at most 3 * 2^-24 |v|
+ * and, where v < 0, by z^2 2^-24 of the value, where 1 + erf cancels (4096 tokens of 1024 -> 4096 with erff 57.6 us, 52.0 so). */
+__device__ __forceinline__ float gelu(float v)
+{
+    const float z = fabsf(v) * 0.707106781f, t = __builtin_amdgcn_rcpf(fmaf(0.38f, z, 1.0f));
+    float p = 2.981513138e-02f;
+    p = fmaf(p, t, -1.327961542e-01f);
+    p = fmaf(p, t, 1.854386980e-01f);
+    p = fmaf(p, t, -8.483748560e-02f);
+    p = fmaf(p, t, 1.179101926e-01f);
+    p = fmaf(p, t, 6.806875096e-02f);
+    p = fmaf(p, t, 1.022790763e-01f);
+    p = fmaf(p, t, 1.069136054e-01f);
+    p = fmaf(p, t, 1.072081952e-01f);
+    const float h = t * p * __builtin_amdgcn_exp2f(-1.44269504f * z * z);        /* erfc(z) / 2 */
+    return v * (v > 0.0f ? 1.0f - h : h);
+}
+
 template <bool FINE>
 __device__ __forceinline__ float act_of(float v, int act)
 {
     switch (act) {
     case K3D_ACT_RELU: return v < 0.0f ? 0.0f : v;
     case K3D_ACT_SILU: return over_1p_exp<FINE>(v, v);
-    case K3D_ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678f));
+    case K3D_ACT_GELU: return gelu(v);
     case K3D_ACT_GELU_TANH: return over_1p_exp<FINE>(v, 1.59576912f * v * fmaf(0.044715f * v, v, 1.0f));
     default: return v;
     }
