@@ -251,3 +251,28 @@ def test_infinite_weight(gpu, k3, T, inn, out):
             assert (y[1] == float("-inf")).all(), k
             on = torch.arange(T, device="cuda") != 1
             assert torch.equal(y[on], clean[on])
+
+
+@pytest.mark.parametrize("T,inn,out", [
+    (8, 1032, 8200), (13, 4104, 12300), (30, 2056, 5200), (60, 8200, 6400), (46, 136, 130), (4100, 520, 2050), (1030, 1096, 12304), (1030, 1032, 4096),
+    (700, 7176, 896), (200, 7176, 896), (300, 1032, 4096), (300, 264, 1160), (2000, 1024, 2051), (2001, 800, 4099), (513, 960, 1021)])
+@pytest.mark.parametrize("x_type", [F32, BF16])
+@pytest.mark.parametrize("y_type", [F32, BF16])
+def test_every_tail(gpu, k3, T, inn, out, x_type, y_type):
+    """Rows that end inside a step, and edges of the outputs with residuals, on the kernels for few tokens and on every tile. Integers again: the
+    fp32 result is exact, a bf16 one its one rounding."""
+    say(f"case: {T} x {inn} -> {out} {x_type} {y_type}")
+    x, w, b, r = operands(T, inn, out, x_type, y_type, T, padx=8, padw=16)
+    big, one = (511, 1) if x_type == F32 else (3, 3)
+    x.copy_(torch.randint(-big, big + 1, x.shape, device="cuda", generator=lo.gen(T)))
+    w.copy_(torch.randint(-one, one + 1, w.shape, device="cuda", generator=lo.gen(T + 1)))
+    b.copy_((b * 100).round())
+    r.copy_((r.float() * 10).round())
+    y = torch.full((T + 1, out + 3), 7.0, device="cuda", dtype=y_type)
+    got = lo.linear(k3, x, w, b, "relu", r, y=y[:T, :out])
+    want = (x.double() @ w.double().T + b).clamp(min=0) + r.double()
+    assert torch.equal(got, want.float().to(y_type))
+    assert (y[T] == 7).all() and (y[:, out:] == 7).all()
+    y[:T, :out] = r                                                # the residual in the result's place
+    assert torch.equal(lo.linear(k3, x, w, b, "relu", y[:T, :out], y=y[:T, :out]), want.float().to(y_type))
+    assert (y[T] == 7).all() and (y[:, out:] == 7).all()
