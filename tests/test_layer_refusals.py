@@ -95,7 +95,8 @@ APART = dict(LINEAR, x=2 * A, W=3 * A, bias=4 * A, ws=5 * A)
 
 
 @pytest.mark.parametrize("change,word", [
-    (dict(T=(1 << 24) + 1), "MAX_TOKENS"), (dict(out=(1 << 28) + 1, ldy=1 << 30), "MAX_OUT"), (dict(y=2 * A), "operand"), (dict(y=3 * A), "operand"), (dict(y=4 * A), "operand"),
+    (dict(T=(1 << 24) + 1), "MAX_TOKENS"), (dict(out=(1 << 28) + 1, ldy=1 << 30), "MAX_OUT"),
+    (dict(T=1 << 20, out=(1 << 13) + 1, ldy=1 << 14), "2^33"), (dict(y=2 * A), "operand"), (dict(y=3 * A), "operand"), (dict(y=4 * A), "operand"),
     (dict(y=5 * A), "operand")])
 def test_linear_places(k3, change, word):
     refused(k3, k3.lib().k3d_linear(*dict(APART, **change).values(), None), word)
