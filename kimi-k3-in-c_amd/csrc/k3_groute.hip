@@ -252,7 +252,10 @@ __global__ __launch_bounds__(256, P <= 14 ? 5 : 1) void route_kernel(K3kRoute a,
         if (LG >= 8) meet(dpp_f32<0x141>(k1), dpp_f32<0x141>(k2));
         if (LG >= 16) meet(dpp_f32<0x140>(k1), dpp_f32<0x140>(k2));
         if (LG >= 32) meet(__shfl_xor(k1, 16), __shfl_xor(k2, 16));
-        const float v = a.group_top == 2 && k2 > -INFINITY ? k1 + k2 : k1;
+        /* (the sum of two finite choices stays finite: two at the lowest value are past fp32, not past 64 bits, and such groups may
+         * be taken. Held at the end of the range they compare as equal, which 64 bits then settle.) */
+        const float sum2 = __builtin_amdgcn_fmed3f(k1 + k2, -0x1.fffffep127f, 0x1.fffffep127f);
+        const float v = a.group_top == 2 && k2 > -INFINITY && k1 < INFINITY ? sum2 : k1;
         int rank = 0;
         for (int q = 0; q < a.n_groups; q++) {
             const float o = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), q << lsh));
