@@ -749,19 +749,22 @@ __global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
         __builtin_amdgcn_sched_group_barrier(0x008, NMF, 0);
     };
     /* all but the last NST - 2 stages' requests (with weights through registers, whose loads follow a stage's
-     * requests: and those of the stage before) */
+     * requests: and those of the stage before). A count holds only where each counted load is there: the weights' are while a later step
+     * stores them, which those of the last steps are not (the compiler drops them), so these request nothing and wait for all. */
     constexpr int WAITN = WREG ? WR + (XD + WR) * (NST - 2) : DN * (NST - 2);
     constexpr int WAIT_STAGE = (WAITN & 15) | (7 << 4) | (0 << 8) | ((WAITN >> 4) << 14);       /* and LDS: none */
     static_assert(WAITN < 64, "requests in flight");
-    constexpr int WAIT_VM0 = (7 << 4) | (15 << 8);
+    constexpr int WAIT_VM0 = (7 << 4) | (15 << 8), WAIT_ALL = 7 << 4;
     XFrag fx0[FT], fx1[FT];
     k3_bf16x8 fw0[FO], fw1[FO];
 
     /* Step k: its second half is read while the first is multiplied; then every wave is past its reads of
      * buffer k % NST and stage k + 1 has landed (one barrier), so stage k + NST goes into that buffer and the
-     * next step's first half is read while the second is multiplied. */
-    auto step = [&](auto slot) {
+     * next step's first half is read while the second is multiplied. `last`: of the steps behind the loop, past which
+     * no stage is wanted. */
+    auto step = [&](auto slot, auto last) {
         constexpr int S = decltype(slot)::value;
+        constexpr bool DRAIN = WREG && decltype(last)::value;
         uint16_t *const b = buf_of(slot);
         uint16_t *const nb = buf_of(std::integral_constant<int, (S + 1) % NST>{});
         read(b, 1, fx1, fw1);
@@ -769,13 +772,18 @@ __global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
         pin(std::integral_constant<int, 0>{});
         __builtin_amdgcn_sched_barrier(0);
         /* (__syncthreads would wait for every request) */
-        __builtin_amdgcn_s_waitcnt(WAIT_STAGE);
+        __builtin_amdgcn_s_waitcnt(DRAIN ? WAIT_ALL : WAIT_STAGE);
         asm volatile("s_barrier" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
-        if (WREG) wstore(slot);
-        issue(slot);
-        if (WREG) wload(slot);
-        if (WREG) __builtin_amdgcn_sched_barrier(0);
+        if (!DRAIN) {
+            if (WREG) wstore(slot);
+            issue(slot);
+            if (WREG) {
+                __builtin_amdgcn_sched_barrier(0);      /* (in this order: WAITN) */
+                wload(slot);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
         read(nb, 0, fx0, fw0);          /* (past the last step: what lies there, unused) */
         mma(fx1, fw1);
         pin(std::integral_constant<int, WREG ? 0 : DN>{});
@@ -792,9 +800,9 @@ __global__ __launch_bounds__(64 * WT * WO) void lin_tile_kernel(LinTile p)
     read(S0, 0, fx0, fw0);
     /* (whole rounds in the loop: a way out of its middle costs copies of the accumulators) */
     int left = n;
-    for (; left >= NST; left -= NST) each_stage<0, NST>(step);
+    for (; left >= NST; left -= NST) each_stage<0, NST>([&](auto slot) { step(slot, std::false_type{}); });
     each_stage<0, NST - 1>([&](auto slot) {
-        if (decltype(slot)::value < left) step(slot);
+        if (decltype(slot)::value < left) step(slot, std::true_type{});
     });
 
     /* A lane holds token r16 of each token fragment and 4 FG consecutive outputs of FG fragments. The sums go
