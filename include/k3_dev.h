@@ -198,7 +198,8 @@ enum { K3D_F32 = 0, K3D_BF16 = 1 };
  * their elements. fp32 x counts in full: cut into three bf16 terms that hold all 24 bits of it
  * (an infinite weight then gives NaN where it meets a finite x). Sums, bias, activation and
  * residual are formed in fp32 and rounded once to y_type; silu is within 8 * 2^-24 of its value under either type, gelu_tanh
- * within 6 |z| 2^-24 more, z = 1.6 v (1 + .045 v^2), which z's own roundings cost. Which kernel runs, and with it the order
+ * within 6 |z| 2^-24 more, z = 1.6 v (1 + .045 v^2), which z's own roundings cost; gelu within 18 * 2^-24 of its value
+ * (for bf16 10 * 2^-24 |v|, and where v < 0 (18 + 1.5 v^2) 2^-24 of its value, before that rounding). Which kernel runs, and with it the order
  * of a sum, goes by the shape, the types and the alignment; a call's bits repeat. ldx and ldw up to
  * K3D_LINEAR_MAX_LD, in up to K3D_LINEAR_MAX_IN, out up to K3D_LINEAR_MAX_OUT, T * out up to
  * 2^33 where in is under 64. y must not overlap x, W, bias or ws, nor res unless it is y itself. ws

@@ -74,3 +74,34 @@ def test_gate_of_fp32_results(gpu, k3, act, span):
     tol = units_of_gate(v.astype(np.float64), act) * UNIT * np.abs(a) + 2.0 ** -148      # (two roundings of a subnormal result)
     got = apply(k3, v, act)
     assert (np.abs(got - a) <= tol).all(), (np.abs(got - a) / np.abs(a) / UNIT).max()
+
+
+def off_of_gelu(v, a, y_type):
+    """How far v (1 - h) or v h may be off, h = erfc(|v| / sqrt 2) / 2, a the value.
+    fp32 results, past |v| = 1: t 2 units and its correction's 1, with at most 2.5 times their weight in h, the polynomial 4, its products 2, the
+    exponential 2 with its correction 1: 16.5, and v's product 1, of v h; of 1 - h, h < 0.16, 3.2 and 2. Up to 1: the series 3, under .342 of
+    a sum of at least .158 (v < 0) or .5, and 2.
+    bf16 results before their rounding: t 3 with up to 3 times its weight, the polynomial 4, products 2, the exponential 2 and 1.5 v^2 for its
+    argument's roundings: 17 + 1.5 v^2 of h, and v's product. Of 1 - h: at most 8.5 |v| (where h is a half) and 1 |v|."""
+    if y_type == F32:
+        return UNIT * np.abs(a) * np.where(np.abs(v) <= 1, np.where(v > 0, 5.0, 9.0), np.where(v > 0, 6.0, 17.5))
+    return UNIT * np.where(v > 0, 10 * np.abs(v), (18 + 1.5 * v * v) * np.abs(a))
+
+
+@pytest.mark.parametrize("y_type", [F32, BF16])
+@pytest.mark.parametrize("span", [(-13, -5), (-5, -1), (-1, 0), (0, 1), (1, 3), (3, 20)])
+def test_gelu(gpu, k3, span, y_type):
+    say(f"case: {span} {y_type}")
+    v = arguments(*span, 100000 if y_type == F32 else 400000, 3)
+    a = lo.act64(v.astype(np.float64), "gelu")
+    if y_type == F32:
+        got, want, r = apply(k3, v, "gelu"), a, None
+    else:
+        r = torch.from_numpy(a).cuda().to(BF16)
+        near = np.abs(a - lo.f64(r)) <= 2.0 ** -17 * np.abs(a)
+        v, a, r = v[near], a[near], -r[torch.from_numpy(near).cuda()].unsqueeze(1)
+        assert len(v) > 1000
+        got, want = apply(k3, v, "gelu", r, BF16), a + lo.f64(r)[:, 0]
+    tol = off_of_gelu(v.astype(np.float64), a, y_type) + 2.0 ** -145        # (h may be a subnormal: v 2^-149)
+    half = 0 if r is None else np.maximum((np.abs(want) + tol) * lo.HALF[BF16], 2.0 ** -134)
+    assert (np.abs(got - want) <= tol + half).all(), (np.abs(got - want) / np.abs(a) / UNIT).max()
