@@ -33,3 +33,50 @@ def test_any_number_of_steps(gpu, k3, T, out, x_type, steps):
         w.copy_(torch.randint(-3, 4, w.shape, device="cuda", generator=lo.gen(steps + 100)))
         for _ in range(2):
             assert torch.equal(lo.linear(k3, x, w).double(), x.double() @ w.double().T)
+
+
+def terms(x):
+    """fp32 as the sum of three of 8 significant bits each, by truncation."""
+    cut = lambda v: (v.contiguous().view(torch.int32) & -65536).view(F32)
+    h = cut(x)
+    m = cut(x - h)
+    return h, m, x - h - m
+
+
+KERNELS = [(1, 7168, 7168), (6, 4096, 4096), (14, 2048, 8192), (22, 7168, 896), (30, 2048, 2048), (38, 12288, 4100), (46, 512, 16384),
+           (60, 8192, 6400), (64, 7168, 7000), (96, 7168, 7168), (200, 7168, 2048), (1024, 2048, 2048), (1500, 1024, 3584),
+           (2048, 2048, 4096), (4096, 1024, 4096), (300, 7168, 384), (1000, 7168, 130)]
+FEW = [(T, inn, out) for T in (8, 13, 32, 48, 62) for inn, out in ((1024, 2000), (512, 5200), (1024, 8200), (8192, 6400), (4096, 12300), (16384, 3500))]
+TAILS = [(8, 1032, 8200), (13, 4104, 12300), (30, 2056, 5200), (60, 8200, 6400), (46, 136, 130), (4100, 520, 2050), (1030, 1096, 12304),
+         (1030, 1032, 4096), (700, 7176, 896), (200, 7176, 896), (300, 1032, 4096), (300, 264, 1160), (2000, 1024, 2051),
+         (2001, 800, 4099), (513, 960, 1021)]
+SMALL = [(1, 1, 1), (2, 31, 17), (9, 40, 48), (16, 48, 20), (100, 7, 9), (20, 128, 40), (1, 64, 64), (300, 1001, 77), (128, 72, 256)]
+
+
+@pytest.mark.parametrize("T,inn,out,pad,off", [s + (0, 0) for s in KERNELS + FEW + TAILS + SMALL] + [s + (1, 1) for s in KERNELS[::2] + TAILS[::3] + SMALL] +
+                         [s + (4, 0) for s in TAILS + SMALL])
+def test_all_of_fp32(gpu, k3, T, inn, out, pad, off):
+    """fp32 activations that need all 24 bits (or 21): integers of three parts, none of them zero, one for each term, and weights that are zero but for
+    a few of a row, so that every sum is exact. Without the third term no result would be right, which is checked of the operands."""
+    say(f"case: {T} x {inn} -> {out} pad {pad} off {off}")
+    g = lo.gen(T + inn + out)
+    x, w = rows(T, inn, F32, pad=pad), rows(out, inn, BF16, pad=8 * pad, off=off)
+    o = torch.arange(out, device="cuda")
+    part = lambda least, end: torch.randint(least, end, x.shape, device="cuda", generator=g)
+    for low, count in ((8, 1), (5, 4)):                           # under 2^24, and 4 * 2^21 + residuals < 2^24
+        v = (part(128, 256) << (low + 8)) + (part(128, 256) << low) + part(0, 1 << (low - 1)) * 2 + 1
+        x.copy_(v * (torch.randint(0, 2, x.shape, device="cuda", generator=g) * 2 - 1))
+        third = terms(x)[2]
+        assert (third != 0).all()
+        w.zero_()
+        for i in range(count):
+            at = torch.randint(0, inn, (out,), device="cuda", generator=g)
+            if i % 2 == 0:                                        # (every other output out of the last columns of a row)
+                at[1::2] = inn - 1 - at[1::2] % min(inn, 64)
+            w[o, at] = (torch.randint(0, 2, (out,), device="cuda", generator=g) * 2 - 1).to(BF16)
+        r = torch.randint(-1000, 1001, (T, out), device="cuda", generator=g).float() if count > 1 else None
+        want = x.double() @ w.double().T
+        lost = third.double() @ w.double().T
+        assert (lost != 0).all() if count == 1 else (lost != 0).float().mean() > 0.5
+        got = lo.linear(k3, x, w, res=r)
+        assert torch.equal(got.double(), want if r is None else want + r)
