@@ -202,13 +202,14 @@ enum { K3D_F32 = 0, K3D_BF16 = 1 };
  * (for bf16 10 * 2^-24 |v|, and where v < 0 (18 + 1.5 v^2) 2^-24 of its value, before that rounding). Which kernel runs, and with it the order
  * of a sum, goes by the shape, the types and the alignment; a call's bits repeat. ldx and ldw up to
  * K3D_LINEAR_MAX_LD, in up to K3D_LINEAR_MAX_IN, out up to K3D_LINEAR_MAX_OUT, T * out up to
- * 2^33 where in is under 64. y must not overlap x, W, bias or ws, nor res unless it is y itself. ws
+ * K3D_LINEAR_MAX_RESULTS, 2^33 where in is under 64. y must not overlap x, W, bias or ws, nor res unless it is y itself. ws
  * (k3d_linear_ws bytes, which hold any fewer tokens too; 16-byte aligned) is scratch of one call: calls
  * and graphs that may run at the same time need one each. */
 enum { K3D_ACT_NONE = 0, K3D_ACT_RELU = 1, K3D_ACT_SILU = 2, K3D_ACT_GELU = 3 /* erf */, K3D_ACT_GELU_TANH = 4 };
 #define K3D_LINEAR_MAX_LD (1 << 22)
 #define K3D_LINEAR_MAX_IN (1 << 20)
 #define K3D_LINEAR_MAX_OUT (1 << 28)
+#define K3D_LINEAR_MAX_RESULTS (1L << 37)
 size_t k3d_linear_ws(int T, int in, int out, int x_type);
 int k3d_linear(void *y, int y_type, long ldy, const void *x, int x_type, long ldx, int T, const uint16_t *W,
                long ldw, int in, int out, const float *bias, int act, const void *res, long ldr, void *ws,

@@ -42,6 +42,7 @@ int k3d_linear(void *y, int y_type, long ldy, const void *x, int x_type, long ld
     if (ldx > K3D_LINEAR_MAX_LD || ldw > K3D_LINEAR_MAX_LD || in > K3D_LINEAR_MAX_IN)
         return k3dx_bad("k3d_linear: ldx and ldw up to K3D_LINEAR_MAX_LD, in up to K3D_LINEAR_MAX_IN");
     if (out > K3D_LINEAR_MAX_OUT) return k3dx_bad("k3d_linear: out up to K3D_LINEAR_MAX_OUT");
+    if ((long)T * out > K3D_LINEAR_MAX_RESULTS) return k3dx_bad("k3d_linear: T * out up to K3D_LINEAR_MAX_RESULTS");
     if (in < 64 && (long)T * out > 1L << 33) return k3dx_bad("k3d_linear: up to 2^33 results of rows under 64 columns");
     if (!y || !x || !W) return k3dx_bad("k3d_linear: y, x and W must be given");
     if (res == y && ldr != ldy) return k3dx_bad("k3d_linear: res in y's place needs y's stride");

@@ -501,19 +501,14 @@ __global__ __launch_bounds__(64 * NW) void lin_skinny_kernel(K3kLinear a)
 /* ---- x for the tile kernel: terms and padding ------------------------------------------- */
 /* xs[t][terms][kp] bf16, kp a multiple of 64: fp32 x as l, m, h; bf16 x as it is. Where the rows' length is
  * no multiple of 64, the last block of 64 columns holds the rest with zeros behind it (over 0), or columns
- * in - 64 .. in with zeros in place of those that the block before it holds (over 64 - in % 64). */
+ * in - 64 .. in with zeros in place of those that the block before it holds (over 64 - in % 64). Under 2^31 pieces of eight
+ * columns in a launch (a 64-bit division takes 0.2 us). */
 template <bool XF32>
 __global__ __launch_bounds__(256) void lin_pack_kernel(uint16_t *xs, const void *x, long ldx, int T, int in, int kp, int over)
 {
     const int per = kp / 8;
-    int t, kb;
-    if (gridDim.x <= 1u << 24) {                                        /* (a 64-bit division takes 0.2 us) */
-        const unsigned i = blockIdx.x * 256 + threadIdx.x;
-        t = (int)(i / (unsigned)per), kb = (int)(i - (unsigned)t * per) * 8;
-    } else {
-        const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-        t = (int)(i / per), kb = (int)(i % per) * 8;
-    }
+    const unsigned i = blockIdx.x * 256 + threadIdx.x;
+    const int t = (int)(i / (unsigned)per), kb = (int)(i - (unsigned)t * per) * 8;
     if (t >= T) return;
     const int last = kp - LIN_KS, k = kb >= last ? kb - over : kb;      /* the first of the eight columns */
     const bool whole = k >= (kb >= last ? last : 0) && k + 8 <= in;
@@ -916,6 +911,9 @@ __global__ __launch_bounds__(64) void lin_join_kernel(K3kLinear a, const float *
 }
 
 /* ---- launches -------------------------------------------------------------------------------- */
+/* A launch takes under 2^32 work-items: no kernel is chosen where its grid holds more. */
+bool fits_launch(long workgroups, int threads) { return workgroups * threads < 1L << 32; }
+
 constexpr int LIN_MAX_SLICES = 16;
 constexpr size_t LIN_PART_CAP = (size_t)64 << 20;
 /* weights that no cache keeps from one call to the next, from here on read past the caches (102 MB times 64
@@ -997,12 +995,12 @@ float both(float a, float b) { return sqrtf(a * a + b * b); }
  * rows of W and all of x for them), the weights come at 5.9 GB/ms, fp32 x costs a wave 0.26 us to cut 8 tokens of a
  * stage. The constants of this and of tile_cost are fitted to 40 shapes of 1 to 4096 tokens, each on every kernel: they are off by
  * 10 % on average, and what they choose is 2.5 % slower than the best of them (16 % at 64 tokens of 7168 -> 576, 23 %
- * at 1024 of 7168 -> 384 at the worst). 0: does not fit the LDS. */
+ * at 1024 of 7168 -> 384 at the worst). 0: does not fit the LDS, or a launch. */
 float skinny_cost(int T, int in, int out, bool f32, int rw, long cus)
 {
     const int xr = sk_group(T);
-    if (sk_nst(rw, xr, f32) == 0) return 0.0f;
     const long wgs = (out + 16 * rw - 1) / (16 * rw), rounds = (wgs + cus - 1) / cus;
+    if (sk_nst(rw, xr, f32) == 0 || !fits_launch(wgs, 64 * SK_NW)) return 0.0f;
     const float kb = (float)in * 2.0f / 1024.0f * (16 * rw + 8 * xr * (f32 ? 2 : 1));
     const float rate = fminf(82.0f, 17800.0f / (float)(wgs < cus ? wgs : cus));
     const float cut = f32 ? (float)((in + LIN_KS - 1) / LIN_KS) / SK_NW * xr * 0.26f : 0.0f;
@@ -1020,16 +1018,17 @@ void tile_go(const LinTile *p, hipStream_t st)
 
 /* Microseconds of a launch of lin_tile_kernel and, with slices, the join: rounds of as many workgroups as fit the chip, each
  * of `per` steps; a step takes what a CU takes in at 74 KB/us and the chip at 35 GB/ms, or the matrix cores at
- * 1.66 PFLOP/s of the chip; W and x come at 6.7 GB/ms. */
+ * 1.66 PFLOP/s of the chip; W and x come at 6.7 GB/ms. 0: does not fit a launch. */
 struct Shape {
-    int bt, bo, per_cu;
+    int bt, bo, per_cu, threads;
 };
-constexpr Shape SHAPES[] = {{256, 256, 1}, {256, 128, 1}, {128, 128, 1}, {128, 64, 2}, {64, 128, 2}, {64, 64, 2}};
+constexpr Shape SHAPES[] = {{256, 256, 1, 512}, {256, 128, 1, 512}, {128, 128, 1, 256}, {128, 64, 2, 256}, {64, 128, 2, 256}, {64, 64, 2, 256}};
 constexpr int N_SHAPES = sizeof SHAPES / sizeof SHAPES[0];
 
 float tile_cost(const Shape &s, int T, int in, int out, int steps, int nsl, long cus)
 {
     const long wgs = (long)((T + s.bt - 1) / s.bt) * ((out + s.bo - 1) / s.bo) * nsl, slots = cus * s.per_cu;
+    if (!fits_launch(wgs, s.threads)) return 0.0f;
     const int per = (steps + nsl - 1) / nsl;
     const float kb = (s.bt + s.bo) * LIN_KS * 2.0f / 1024.0f, mfma = 2.0f * s.bt * s.bo * LIN_KS / 6.5e6f;
     auto round = [&](long n) {
@@ -1045,11 +1044,12 @@ float tile_cost(const Shape &s, int T, int in, int out, int steps, int nsl, long
 /* Microseconds with fp32 rows cut in the kernel, 64 tokens by 64 or 128 outputs, two workgroups to a CU: a step takes one
  * 0.50 or 0.74 us alone and 0.72 or 1.01 beside another. (Cutting them once, in a launch before, costs a write and a read of
  * three terms and a longer product: 300 tokens of 7168 -> 384 26.1 us that way, 18.5 this way; 4000 tokens 135 and 74; but
- * 1024 of 7168 -> 7168 294 and 353, as each tile of outputs cuts its tokens again.) */
+ * 1024 of 7168 -> 7168 294 and 353, as each tile of outputs cuts its tokens again.) 0: does not fit a launch. */
 float cut_cost(int bo, int T, int in, int out, int nsl, long cus)
 {
     const int nks = (in + LIN_KS - 1) / LIN_KS, per = (nks + nsl - 1) / nsl;
     const long wgs = (long)((T + 63) / 64) * ((out + bo - 1) / bo) * nsl, slots = 2 * cus;
+    if (!fits_launch(wgs, 256)) return 0.0f;
     const float one = bo == 64 ? 0.49f : 0.73f, two = bo == 64 ? 0.70f : 1.00f, kb = bo / 8.0f + 16.0f;
     auto round = [&](long n) { return both(per * (n <= cus ? one : two), per * kb * n / 25000.0f); };
     float t = (float)(wgs / slots) * round(slots) + (wgs % slots ? round(wgs % slots) : 0.0f);
@@ -1087,7 +1087,7 @@ extern "C" int k3k_linear(const K3kLinear *a, void *stream)
         for (int n : {1, 2, 3, 4, 6, 8, 12, LIN_MAX_SLICES}) {
             if (n > 1 && (n * one > room || steps < 4 * n)) break;
             const float t = tile_cost(SHAPES[i], a->T, a->in, a->out, steps, n, cus);
-            if (best == 0.0f || t < best) best = t, shape = i, nsl = n;
+            if (t > 0.0f && (best == 0.0f || t < best)) best = t, shape = i, nsl = n;
         }
     }
     if (pack) best += 2.5f + (float)a->T * kpad(a->in) * (f32 ? 10 : 4) / 4e6f;
@@ -1098,7 +1098,7 @@ extern "C" int k3k_linear(const K3kLinear *a, void *stream)
             for (int n : {1, 2, 3, 4, 6, 8, 12, LIN_MAX_SLICES}) {
                 if (n > 1 && (n * one > room || nks < 4 * n)) break;
                 const float t = cut_cost(bo, a->T, a->in, a->out, n, cus);
-                if (t < best) best = t, cut = bo, nsl = n;
+                if (t > 0.0f && t < best) best = t, cut = bo, nsl = n;
             }
     if (a->T <= 64) {
         int rw = 0;
@@ -1128,11 +1128,16 @@ extern "C" int k3k_linear(const K3kLinear *a, void *stream)
     p.steps = steps;
     if (pack && !cut) {
         const int kp = kpad(a->in), over = dma ? kp - a->in : 0;
-        const size_t n = (size_t)a->T * (kp / 8);
-        const unsigned grid = (unsigned)((n + 255) / 256);
-        if (f32) lin_pack_kernel<true><<<grid, 256, 0, st>>>((uint16_t *)a->ws, a->x, a->ldx, a->T, a->in, kp, over);
-        else lin_pack_kernel<false><<<grid, 256, 0, st>>>((uint16_t *)a->ws, a->x, a->ldx, a->T, a->in, kp, over);
-        K3K_LAUNCH_CHECK("linear: pack");
+        const int most = (int)((1u << 31) / (unsigned)(kp / 8)), terms = f32 ? 3 : 1;       /* tokens of a launch */
+        for (int t = 0; t < a->T; t += most) {
+            const int n = a->T - t < most ? a->T - t : most;
+            uint16_t *const xs = (uint16_t *)a->ws + (size_t)t * terms * kp;
+            const char *const x = (const char *)a->x + (size_t)t * a->ldx * (f32 ? 4 : 2);
+            const unsigned grid = (unsigned)(((size_t)n * (kp / 8) + 255) / 256);
+            if (f32) lin_pack_kernel<true><<<grid, 256, 0, st>>>(xs, x, a->ldx, n, a->in, kp, over);
+            else lin_pack_kernel<false><<<grid, 256, 0, st>>>(xs, x, a->ldx, n, a->in, kp, over);
+            K3K_LAUNCH_CHECK("linear: pack");
+        }
         p.x = a->ws;
         p.ldx = p.xcols = p.steps * LIN_KS;
         p.xend = -1;
