@@ -195,8 +195,8 @@ enum { K3D_F32 = 0, K3D_BF16 = 1 };
  *   y[t][o] = act(sum_k x[t][k] W[o][k] + bias[o]) + res[t][o],   t < T, o < out, k < in.
  * W bf16 [out][ldw], x [T][ldx] of x_type, bias fp32 [out] or NULL, res [T][ldr] of y_type or NULL
  * (it may be y itself, with its stride), y [T][ldy] of y_type; rows and pointers at any alignment of
- * their elements. fp32 x counts in full: cut into three bf16 terms that hold all 24 bits of it
- * (an infinite weight then gives NaN where it meets a finite x). Sums, bias, activation and
+ * their elements. fp32 x counts in full: cut into three bf16 terms that hold all 24 bits of it,
+ * down to bf16's least step of 2^-133 (an infinite weight then gives NaN where it meets a finite x). Sums, bias, activation and
  * residual are formed in fp32 and rounded once to y_type; silu is within 8 * 2^-24 of its value under either type, gelu_tanh
  * within 6 |z| 2^-24 more, z = 1.6 v (1 + .045 v^2), which z's own roundings cost; gelu within 18 * 2^-24 of its value
  * (for bf16 10 * 2^-24 |v|, and where v < 0 (18 + 1.5 v^2) 2^-24 of its value, before that rounding). Which kernel runs, and with it the order
@@ -228,7 +228,8 @@ int k3d_linear(void *y, int y_type, long ldy, const void *x, int x_type, long ld
  * NaN, is an expert that cannot be taken (a masked one; a NaN logit is left out of the softmax too); a
  * group has the value of those it can give, and one without any is never taken; where fewer than topk
  * are left, the last slots get idx -1 and wt 0 (k3d_moe_experts skips them), and weights
- * that sum to 0 are 0. Logits of +inf share a softmax among themselves.
+ * that sum to 0 are 0. (-inf masks an expert at no cost; a large finite bias is as right, but every choice of a token that has one is
+ * formed in 64 bits, which takes three times as long.) Logits of +inf share a softmax among themselves.
  * 1 <= n_experts <= 2048, n_groups <= 64 and a divisor of it, topk <= 64 and at most the experts of
  * top_groups groups. */
 enum { K3D_SCORE_SIGMOID = 0, K3D_SCORE_SOFTMAX = 1 };
@@ -245,7 +246,7 @@ int k3d_route(int *idx, float *wt, const void *logits, int type, long ld, int T,
  *   (2i, 2i + 1) (K3D_ROT_INTERLEAVED) turn by the angle pos[t] * inv_freq[i], i < rot/2, and are
  *   multiplied by rot_scale; the rest of u stays as it is.
  * Angles are formed and reduced in 64 bits (inv_freq fp64), so far positions lose nothing; the rest is fp32,
- * rounded once. A token of negative position is padding: its rows of qo and ko are left as they were.
+ * rounded once (the squares too: a head whose sum of them passes fp32's range, values of 10^18 and more, becomes 0). A token of negative position is padding: its rows of qo and ko are left as they were.
  * hq or hk may be 0. 1 <= dim <= 1024; rot even (0: no rotation, pos may then be NULL: no padding);
  * eps >= 0. */
 enum { K3D_ROT_HALVES = 0, K3D_ROT_INTERLEAVED = 1 };

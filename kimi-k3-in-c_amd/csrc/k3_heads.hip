@@ -12,7 +12,8 @@
  * An element's other one (half the rotated range away) is read a second time, out of the L1, rather than
  * fetched from the lane that holds it; where lengths, strides or borders do not fit 16 bytes, it comes through LDS
  * (heads_any_kernel). The next heads' rows are requested before these are worked on; the
- * reads of a head all come before its writes, so a head may be written over itself.
+ * reads of a head all come before its writes, so a head may be written over itself. 4096 tokens of 72 heads of 128 in bf16: 36.6 us
+ * = 4.1 TB/s out of memory (two times beside each other, below, are measured alike, with heads that the last cache holds).
  */
 #include "k3_common.h"
 #include "k3_dev.h"
@@ -219,7 +220,8 @@ __global__ __launch_bounds__(64 * HD_WAVES) void heads_kernel(K3kHeads a, int ls
 /* Heads of any length from V, at any alignment, with the rotated range and its halves anywhere: a lane's chunk may lie on
  * both sides of a border, and the last one of a head, read where it ends with the head, holds elements of the one before it too
  * (computed twice, counted once, written twice alike). An element's other one comes out of LDS, where the wave lays its heads
- * as they are read. 4096 tokens of 72 heads of 128 in bf16, 74 of them rotated: 36.3 us; an element a lane and load, which such
+ * as they are read. Out of memory 4096 tokens of 13 heads of 154 take 23 us (bytes: 6.6), bound by instructions: 1934 a wave, 341 of them for its angles,
+ * most of the rest to set up two factors an element on either side. 4096 tokens of 72 heads of 128 in bf16, 74 of them rotated: 36.3 us; an element a lane and load, which such
  * borders otherwise allow, 81.7 (one token 4.8 and 3.6); 32 + 4 heads of 256 with 100 rotated 34.5, two elements a load 42.7. */
 template <int TYPE, int V, int N>
 __global__ __launch_bounds__(64 * HD_WAVES) void heads_any_kernel(K3kHeads a, int lsh, int split, int pitch)

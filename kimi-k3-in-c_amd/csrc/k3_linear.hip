@@ -8,17 +8,18 @@
  *
  * What bounds it, and the kernel for it:
  *   - up to 64 tokens: reading W. lin_skinny_kernel, 16 to 64 rows of W to a workgroup, its waves sharing the columns, each
- *     with a ring of LDS stages of its own filled by DMA (one token of 12288 -> 7168, 176 MB, 26.8 us = 6.6 TB/s);
+ *     with a ring of LDS stages of its own filled by DMA (one token of 7168 -> 12288, 176 MB, 28.6 us = 6.2 TB/s);
  *   - more: the matrix cores. lin_tile_kernel, tiles of 64 x 64 to 256 x 256, over slices of the columns where the tiles alone
  *     leave CUs idle; the slices' sums are joined in slice order by lin_join_kernel (4096 tokens of 7168 -> 12288 with
- *     silu 566 us = 1.27 PFLOP/s, the library's product alone 543);
+ *     silu 567 us = 1.27 PFLOP/s, the library's product alone 543);
  *   - weights that are not 16-byte aligned rows of whole 16 bytes: the same tiles, with W through registers instead of
  *     DMA (which wants 16-byte addresses); small ones for a few tokens, and rows shorter than a step, by lin_stream_kernel;
  *   - x that does not suit the DMA, and fp32 x for many tiles of outputs: lin_pack_kernel lays it out in the
  *     workspace first.
  *   - rows that end inside a step: the last step takes their last 64 columns, with zeros for those that come twice (300
  *     tokens of 4104 -> 2048 19.1 us; with x laid out first 21.9; 4096 of 4104 -> 4096, where that counts least, 136 and 130).
- * Which of them, and the tile and slices, go by the costs estimated below.
+ * Which of them, and the tile and slices, go by the costs estimated below. Two times beside each other, here and below, are measured alike,
+ * most with operands that the last cache holds from the call before; out of memory both are up to a quarter longer.
  */
 #include "k3_common.h"
 #include "k3_dev.h"

@@ -80,3 +80,19 @@ def test_all_of_fp32(gpu, k3, T, inn, out, pad, off):
         assert (lost != 0).all() if count == 1 else (lost != 0).float().mean() > 0.5
         got = lo.linear(k3, x, w, res=r)
         assert torch.equal(got.double(), want if r is None else want + r)
+
+
+@pytest.mark.parametrize("T,inn,out", [(1, 64, 16), (100, 64, 128), (300, 64, 256), (3, 40, 16), (90, 201, 70)])
+@pytest.mark.parametrize("x_type", [F32, BF16])
+def test_smallest_values(gpu, k3, T, inn, out, x_type):
+    """Subnormal operands count in full, and of an fp32 one all bits down to bf16's least step of 2^-133."""
+    say(f"case: {T} x {inn} -> {out} {x_type}")
+    x, w = torch.zeros(T, inn, device="cuda", dtype=x_type), torch.zeros(out, inn, device="cuda", dtype=BF16)
+    for e in (-133, -130, -127, -126, -110):
+        x[:, inn - 1], w[:, inn - 1] = 2.0 ** e, 2.0 ** 100
+        assert (lo.linear(k3, x, w) == 2.0 ** (e + 100)).all(), e
+        x[:, inn - 1], w[:, inn - 1] = 2.0 ** 100, 2.0 ** e
+        assert (lo.linear(k3, x, w) == 2.0 ** (e + 100)).all(), e
+    if x_type == F32:
+        x[:, inn - 1], w[:, inn - 1] = (1 + 2.0 ** -23) * 2.0 ** -110, 2.0 ** 100
+        assert (lo.linear(k3, x, w) == (1 + 2.0 ** -23) * 2.0 ** -10).all()
