@@ -255,6 +255,83 @@ int k3d_qk_norm_rope(void *qo, long ldqo, long hsqo, void *ko, long ldko, long h
                      const float *kw, float eps, const int *pos, const double *inv_freq, int rot, int rot_off,
                      int pairs, float rot_scale, void *stream);
 
+/* ---- a layer's path in 8 bits -------------------------------------------------------------
+ * No counterpart in the reference. Activations: rows of OCP e4m3 codes, one fp32 scale for each 128 columns of a row; a
+ * value is code * scale. A row holds whole blocks: ceil(n / 128) * 128 codes, those behind column n the code of 0 (the entry
+ * points that write rows write them so); rows and pointers of codes 16-byte aligned. Weights: e4m3 codes laid out once by k3d_f8_tile, one fp32
+ * scale for each block of 128 rows x 128 columns. Strides are in elements; nothing is allocated, nothing synchronises, the calls can be captured
+ * in a HIP graph. The stream and the tensors belong to the current device. */
+#define K3D_NORM_MAX_N (1 << 16)
+#define K3D_F8_MAX_IN (1 << 20)
+#define K3D_F8_MAX_OUT (1 << 18)
+#define K3D_F8_MAX_LD (1 << 22)
+#define K3D_F8_MAX_RESULTS (1L << 37)
+#define K3D_F8_MAX_SLOTS (1 << 24)
+#define K3D_F8_MAX_X (1L << 31)
+
+/* The gated activations act(gate) * up: K3D_GLU_SILU silu(gate) * up; K3D_GLU_SITU b1 tanh(gate / b1) sigmoid(gate) * b2 tanh(up / b2), as
+ * K3_ACT_SITU of k3.h. */
+enum { K3D_GLU_NONE = -1, K3D_GLU_SITU = 0, K3D_GLU_SILU = 1 };
+
+/* Residual and RMSNorm, into 8 bits and / or y, t < T, i < n <= K3D_NORM_MAX_N:
+ *   v = x[t][i] + res[t][i] (res may be NULL);  sum = v, rounded to r_type (sum may be NULL);
+ *   u = v / sqrt(mean_i(v^2) + eps) * w[i]  (w fp32 or NULL for ones);  y = u, rounded to y_type (y may be NULL);
+ *   q, qs (may be NULL): scale = max(max |u| over 128 columns, 2^-100) / 448, code = u / scale to nearest, ties to even.
+ * All in fp32, v unrounded (the squares too: a row whose sum of them passes fp32's range becomes 0). x is of x_type, res and sum of r_type; res, sum and y at any alignment of
+ * their elements. sum may be res or x itself, y too (same type and stride). A NaN in a block of u makes its scale and codes NaN; an infinity the scale infinite. */
+int k3d_add_norm(void *y, int y_type, long ldy, uint8_t *q, long ldq, float *qs, long ldqs, void *sum, long ldsum,
+                 const void *x, int x_type, long ldx, const void *res, int r_type, long ldr, int T, int n, const float *w,
+                 float eps, void *stream);
+
+/* The rows of x in 8 bits (act K3D_GLU_NONE), or of act(gate) * up: row t of x is gate [n], then up [n]. Scales and codes as above;
+ * the activation in fp32. b1, b2 > 0 for K3D_GLU_SITU. */
+int k3d_quant_f8(uint8_t *q, long ldq, float *qs, long ldqs, const void *x, int x_type, long ldx, int T, int n, int act,
+                 float b1, float b2, void *stream);
+
+/* The layout of weights: mats matrices of e4m3 codes [rows][ldw] one after another (rows * ldw apart) into k3d_f8_tiled_bytes(rows, in) bytes
+ * each, one after another; t 16-byte aligned, W at any alignment. Tiles of 16 rows x 128 columns in the order the
+ * kernels read them; rows up to a multiple of 128 and columns up to whole blocks are there as zeros. */
+size_t k3d_f8_tiled_bytes(int rows, int in);
+int k3d_f8_tile(uint8_t *t, const uint8_t *W, long ldw, int rows, int in, int mats, void *stream);
+
+/* Dense product, t < T, o < out:
+ *   y[t][o] = act(sum_b xs[t][b] Ws[o / 128][b] p[t][o][b] + bias[o]) + res[t][o],
+ * p the sum over block b's 128 columns of the codes' products, in fp32 on the matrix cores. x [T][ldx] codes with scales xs [T][ldxs];
+ * W from k3d_f8_tile, Ws [ceil(out / 128)][ldws]; bias, act, res and y as k3d_linear has them. The two scales' product is formed
+ * in fp32, as are the sum over blocks, bias, activation and residual; one rounding to y_type. Which kernel runs, and with it the order of the
+ * sum over blocks, goes by the shape; a call's bits repeat. ws (k3d_linear_f8_ws bytes, which hold any fewer tokens too; 16-byte aligned) is
+ * scratch of one call: calls and graphs that may run at the same time need one each. y must not overlap an operand, nor res unless
+ * it is y itself. */
+size_t k3d_linear_f8_ws(int T, int in, int out);
+int k3d_linear_f8(void *y, int y_type, long ldy, const uint8_t *x, long ldx, const float *xs, long ldxs, int T,
+                  const uint8_t *W, const float *Ws, long ldws, int in, int out, const float *bias, int act,
+                  const void *res, long ldr, void *ws, size_t ws_bytes, void *stream);
+
+/* A routing's slots by expert: offsets [n_experts + 1], perm [T * topk]: perm[offsets[e] .. offsets[e + 1]) are the slots t * topk + j with
+ * idx[t][j] == e, ascending. Slots whose idx lies outside [0, n_experts) are in none, and perm behind offsets[n_experts] is left
+ * as it was. n_experts up to 2048, topk up to 64, T * topk up to K3D_F8_MAX_SLOTS. ws (k3d_group_ws bytes, none up to 4096 slots) is scratch of one call. */
+size_t k3d_group_ws(int T, int topk, int n_experts);
+int k3d_group(int *offsets, int *perm, const int *idx, int T, int topk, int n_experts, void *ws, size_t ws_bytes, void *stream);
+
+/* Products by expert: rows offsets[e] <= r < offsets[e + 1] (device; `rows` is what offsets[n_experts] is at most) with expert e's weights,
+ *   y[Y(r)][o] = sum_b xs[X(r)][b] Ws[e][o / 128][b] p[..],  X(r) = x_rows ? x_rows[r] / x_div : r,  Y(r) = y_rows ? y_rows[r] : r.
+ * W: n_experts matrices [out][in] from k3d_f8_tile, Ws [n_experts][ceil(out / 128)][ceil(in / 128)]. With k3d_group's perm as x_rows and x_div = topk a
+ * row takes its token of x; as y_rows it returns to its slot. x has x_cap rows, y y_cap; a row with X(r) or Y(r) outside them is left as it was,
+ * and so is every row of y that no r has. No Y(r) may come twice. Experts without rows cost nothing; offsets that fall or leave [0, rows] count as no rows there. */
+int k3d_grouped_f8(void *y, int y_type, long ldy, const int *y_rows, int y_cap, const uint8_t *x, long ldx, const float *xs,
+                   long ldxs, const int *x_rows, int x_div, int x_cap, const int *offsets, int rows, int n_experts,
+                   const uint8_t *W, const float *Ws, int in, int out, void *stream);
+
+/* The experts' layer for a routing in idx/wt [T][topk] (k3d_route's), weights in 8 bits: out[t] = sum_j wt[t][j] W2_e (act(W1_e x[t]) * (W3_e x[t])),
+ * e = idx[t][j], act and b1, b2 as in k3d_quant_f8. The gated activation goes through 8 bits as k3d_quant_f8 rounds it; everything else is
+ * fp32, out rounded once to out_type. Slots whose idx lies outside [0, n_experts) contribute nothing; a token without any becomes 0. w1, w3 [n_experts] matrices [inter][hidden], w2
+ * [hidden][inter] from k3d_f8_tile, s1, s3, s2 their scales as in k3d_grouped_f8. ws (k3d_moe_f8_ws bytes; 16-byte aligned) is scratch of one call. */
+size_t k3d_moe_f8_ws(int T, int hidden, int inter, int n_experts, int topk);
+int k3d_moe_f8(void *out, int out_type, long ldo, const int *idx, const float *wt, const uint8_t *x, long ldx, const float *xs,
+               long ldxs, int T, const uint8_t *w1, const float *s1, const uint8_t *w3, const float *s3, const uint8_t *w2,
+               const float *s2, int hidden, int inter, int n_experts, int topk, int act, float b1, float b2, void *ws,
+               size_t ws_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

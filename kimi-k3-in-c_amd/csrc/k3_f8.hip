@@ -1,0 +1,742 @@
+/* SPDX-License-Identifier: Apache-2.0 */
+/*
+ * k3_f8.hip -- products of e4m3 codes with a scale for each 128 columns of a row of x and for each 128 x 128 block of W
+ * (k3d_linear_f8, k3d_grouped_f8 and the products of k3d_moe_f8):
+ *   y[t][o] = act(sum_b xs[t][b] ws[o / 128][b] (sum over block b of x[t][k] W[o][k]) + bias[o]) + res[t][o]
+ *
+ * A block's 128 columns are one 8-bit matrix instruction (16 x 16 x 128), so each instruction starts from zero and its sums enter the
+ * fp32 accumulators through one multiplication by the two scales' product: four vector FMAs to 32 cycles of the matrix cores. The
+ * 8-bit instructions (all shapes of them alike, as measured) add each 8 neighbouring products after aligning them to the largest's exponent, and what is more
+ * than 13 bits below that is cut off: 1.5 * 2^-16 of a sum of random products. That is far under the rounding of a bf16 result or of the next 8-bit
+ * row, but not of an fp32 one; those products (WIDE) are formed by the bf16 instruction out of the codes widened to bf16 (exactly),
+ * at half the rate.
+ *
+ * W is laid out once, by k3d_f8_tile: tiles of 16 rows x 128 columns in the operand's own order, 2 KB, F8_G row tiles side by side,
+ * column block after column block, zeros where rows or columns end. So every load of W is contiguous at any size.
+ */
+#include "k3_common.h"
+#include "k3_dev.h"
+#include "k3_f8.h"
+#include "k3k.h"
+
+#include <type_traits>
+
+namespace {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));     /* (a load of uint4 loses what tells LDS arrays apart) */
+constexpr uint32_t F8_OOB = 0x80000000u;        /* a buffer offset past any descriptor used here */
+
+/* f(0), f(1) .. f(N - 1), the numbers as constants */
+template <int S, int N, class F>
+__device__ __forceinline__ void each_of(F &&f)
+{
+    if constexpr (S < N) {
+        f(std::integral_constant<int, S>{});
+        each_of<S + 1, N>(f);
+    }
+}
+
+/* sum over a block's 128 columns: a lane holds 32 bytes of row lane % 16 of either operand, 16-byte pieces g and 4 + g of the
+ * block (g = lane / 16); it gets token lane % 16, outputs 4 g ..+4 */
+__device__ __forceinline__ k3_f32x4 f8_mfma(u32x4 w0, u32x4 w1, u32x4 x0, u32x4 x1)
+{
+    const i32x8 w = {(int)w0.x, (int)w0.y, (int)w0.z, (int)w0.w, (int)w1.x, (int)w1.y, (int)w1.z, (int)w1.w};
+    const i32x8 x = {(int)x0.x, (int)x0.y, (int)x0.z, (int)x0.w, (int)x1.x, (int)x1.y, (int)x1.z, (int)x1.w};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, k3_f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+}
+
+/* 32 codes as bf16: exact */
+struct Wide {
+    k3_bf16x8 v[4];
+};
+__device__ __forceinline__ k3_bf16x8 widen8(uint32_t a, uint32_t b)
+{
+    const k3_bf16x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false), p1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true);
+    const k3_bf16x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false), p3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true);
+    return k3_bf16x8{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
+}
+__device__ __forceinline__ Wide widen(u32x4 a, u32x4 b)
+{
+    return Wide{{widen8(a.x, a.y), widen8(a.z, a.w), widen8(b.x, b.y), widen8(b.z, b.w)}};
+}
+
+/* f8_mfma's sum with products and additions in fp32 */
+__device__ __forceinline__ k3_f32x4 wide_mfma(const Wide &w, const Wide &x)
+{
+    k3_f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int q = 0; q < 4; q++) v = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v[q], x.v[q], v, 0, 0, 0);
+    return v;
+}
+
+/* 4 bytes per lane from a buffer straight into LDS: lane L writes lds + 4 L */
+__device__ __forceinline__ void dma4(k3_rsrc r, void *lds, uint32_t voff, uint32_t soff)
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)lds, 4, voff, soff, 0, 0);
+#else
+    (void)r; (void)lds; (void)voff; (void)soff;
+#endif
+}
+
+template <int POL>
+__device__ __forceinline__ u32x4 bload16(k3_rsrc r, uint32_t off)
+{
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, POL));
+}
+
+/* ---- layout ---------------------------------------------------------------------------- */
+constexpr int F8_TILE = 2048;                   /* bytes of 16 rows x 128 columns */
+constexpr int F8_G = 8;                         /* row tiles side by side: the 128 rows of a scale */
+constexpr uint32_t F8_KSTEP = F8_G * F8_TILE;   /* from one column block to the next */
+
+__host__ __device__ __forceinline__ int blocks(int n) { return (n + 127) / 128; }
+__host__ __device__ __forceinline__ size_t tiled_bytes(int rows, int in) { return (size_t)blocks(rows) * blocks(in) * F8_KSTEP; }
+
+/* 16 bytes of tile (128-row block, column block, row tile) to a thread; loads by the row's alignment */
+__global__ __launch_bounds__(128) void tile_kernel(uint8_t *t, const uint8_t *W, size_t ldw, int rows, int in, int nkb, unsigned first)
+{
+    /* a workgroup: 2 KB, one row tile of one column block of one matrix */
+    const size_t i = (size_t)first + blockIdx.x;
+    const size_t per = (size_t)blocks(rows) * nkb * F8_G, m = i / per;
+    const unsigned j = (unsigned)(i - m * per), rt = j % F8_G, kb = j / F8_G % nkb, rb = j / F8_G / nkb;
+    const int h = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int row = (int)(rb * F8_G + rt) * 16 + (lane & 15), col = (int)kb * 128 + (4 * h + (lane >> 4)) * 16;
+    uint32_t v[4] = {0, 0, 0, 0};
+    if (row < rows && col < in) {
+        const uint8_t *p = W + m * rows * ldw + (size_t)row * ldw + col;
+        if (col + 16 <= in) __builtin_memcpy(v, p, 16);
+        else
+            for (int b = 0; b < in - col; b++) v[b / 4] |= (uint32_t)p[b] << (8 * (b % 4));
+    }
+    *reinterpret_cast<uint4 *>(t + i * F8_TILE + threadIdx.x * 16) = make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+/* ---- which rows ------------------------------------------------------------------------ */
+struct Job {
+    int e, r0, n;       /* expert, its first row here, rows (0: nothing to do) */
+};
+
+/* Of the experts' rows, cut into passes of `most`: how many passes there are, and (find_job) the j-th. Each lane holds a run of
+ * experts. Offsets out of order or range count as no rows. */
+struct Jobs {
+    int total, before, mine, per;       /* passes; of the lanes before; of this lane; experts a lane */
+};
+
+__device__ __forceinline__ int rows_of(const K3kF8 &a, int e, int &r0)
+{
+    if (e >= a.n_experts) return 0;
+    const int p = a.offsets[e], q = min(a.offsets[e + 1], a.rows);
+    r0 = p;
+    return p < 0 || q <= p ? 0 : q - p;
+}
+
+__device__ __forceinline__ Jobs count_jobs(const K3kF8 &a, int most)
+{
+    const int lane = threadIdx.x & 63;
+    Jobs s;
+    s.per = (a.n_experts + 63) / 64;
+    s.mine = 0;
+    for (int i = 0; i < s.per; i += 4) {
+        int n[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            int r0 = 0;
+            n[u] = i + u < s.per ? rows_of(a, lane * s.per + i + u, r0) : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) s.mine += (n[u] + most - 1) / most;
+    }
+    int sum = s.mine;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int o = __shfl_up(sum, d);
+        sum += lane >= d ? o : 0;
+    }
+    s.before = sum - s.mine;
+    s.total = __builtin_amdgcn_readlane(sum, 63);
+    return s;
+}
+
+__device__ __forceinline__ Job find_job(const K3kF8 &a, const Jobs &s, int j, int most)
+{
+    const int lane = threadIdx.x & 63;
+    Job job = {0, 0, 0};
+    const uint64_t who = __ballot(j >= s.before && j < s.before + s.mine);
+    if (!who) return job;
+    const int l = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)who) - 1);
+    int left = j - __builtin_amdgcn_readlane(s.before, l);
+    /* the lane's experts, one to a lane now */
+    int r0 = 0, n = lane < s.per ? rows_of(a, l * s.per + lane, r0) : 0;
+    const int p = (n + most - 1) / most;
+    int sum = p;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int o = __shfl_up(sum, d);
+        sum += lane >= d ? o : 0;
+    }
+    const int f = __builtin_amdgcn_readfirstlane(__ffsll(__ballot(left >= sum - p && left < sum)) - 1);
+    left -= __builtin_amdgcn_readlane(sum - p, f);
+    job.e = l * s.per + f;
+    job.r0 = __builtin_amdgcn_readlane(r0, f) + left * most;
+    job.n = min(most, __builtin_amdgcn_readlane(n, f) - left * most);
+    return job;
+}
+
+/* the row of x of a job's i-th row, -1 for none */
+__device__ __forceinline__ int x_row(const K3kF8 &a, int r)
+{
+    if (!a.offsets) return r;
+    int t = r;
+    if (a.x_rows) {
+        t = a.x_rows[r];
+        t = t < 0 ? -1 : t / a.x_div;
+    }
+    return t < a.x_cap ? t : -1;
+}
+
+/* the row of y, past every row for one that is left as it was */
+__device__ __forceinline__ int y_row(const K3kF8 &a, int r)
+{
+    if (!a.offsets) return r;
+    int t = a.y_rows ? a.y_rows[r] : r;
+    if (a.x_rows && x_row(a, r) < 0) t = -1;
+    return (unsigned)t < (unsigned)a.T ? t : a.T;
+}
+
+/* ---- few rows: W straight into operands ------------------------------------------------- */
+/* A workgroup takes 16 RW rows of W and up to 8 NP rows of x; its waves share the column blocks, each with a ring of U blocks
+ * in registers. W's tiles are operands as loaded, 1 KB a load; rows of x are loaded 8 lanes to a row's 128 bytes and turned into
+ * operands through the wave's own LDS (16-byte column c of row r in slot c ^ (r / 2 % 8): the 16 rows of a fragment fall on all
+ * banks). Past the wave's run and behind the last row requests return zeros without reading. */
+/* LDS bytes of a wave: 8 NP rows of a block, or its sums */
+constexpr int stream_lds(int rw, int np) { return (np + 1) / 2 * (rw > 2 ? rw * 1024 : 2048); }
+
+template <int RW, int NP, int U, int NW, int POL, bool WIDE>
+__device__ __forceinline__ void stream_rows(const K3kF8 &a, const Job &job, int rt0, uint32_t *lds)
+{
+    constexpr int NT = (NP + 1) / 2, WAVE = stream_lds(RW, NP) / 4;
+    const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int nkb = blocks(a.in), k0 = nkb * wv / NW, k1 = nkb * (wv + 1) / NW, n = k1 - k0;
+    uint32_t *const mine = lds + wv * WAVE;
+
+    const uint8_t *const W = a.W + (size_t)job.e * a.w_step + (size_t)(rt0 / F8_G) * nkb * F8_KSTEP;
+    const k3_rsrc rw = k3_make_rsrc(W, (uint32_t)nkb * F8_KSTEP);
+    const uint32_t wo = (uint32_t)(rt0 % F8_G) * F8_TILE + lane * 16;
+    const k3_rsrc rx = k3_make_rsrc(a.x, F8_OOB), rs = k3_make_rsrc(a.xs, F8_OOB);
+    uint32_t xo[NP], so[NT];
+#pragma unroll
+    for (int p = 0; p < NP; p++) {
+        const int r = 8 * p + lane / 8, t = r < job.n ? x_row(a, job.r0 + r) : -1;
+        xo[p] = t < 0 ? F8_OOB : (uint32_t)t * (uint32_t)a.ldx + (lane & 7) * 16;
+    }
+#pragma unroll
+    for (int j = 0; j < NT; j++) {
+        const int r = 16 * j + r16, t = r < job.n ? x_row(a, job.r0 + r) : -1;
+        so[j] = t < 0 ? F8_OOB : (uint32_t)t * (uint32_t)a.ldxs * 4;
+    }
+    /* W's scales: a lane each, 64 column blocks at a time */
+    const float *const Ws = a.Ws + (size_t)job.e * a.ws_step + (size_t)(rt0 / F8_G) * a.ldws;
+    float wsc = n > 0 ? Ws[min(k0 + lane, nkb - 1)] : 0.0f;
+
+    struct Slot {
+        u32x4 w[RW][2], x[NP];
+        float s[NT];
+    };
+    Slot ring[U];
+    auto load = [&](Slot &s, int i) {
+        const uint32_t none = i < n ? 0u : F8_OOB, kb = k0 + i;
+#pragma unroll
+        for (int q = 0; q < RW; q++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) s.w[q][h] = bload16<POL>(rw, (wo + kb * F8_KSTEP + q * F8_TILE + h * 1024) | none);
+#pragma unroll
+        for (int p = 0; p < NP; p++) s.x[p] = bload16<0>(rx, (xo[p] + kb * 128) | none);
+#pragma unroll
+        for (int j = 0; j < NT; j++) s.s[j] = __uint_as_float(k3_bload4(rs, (so[j] + kb * 4) | none));
+    };
+    k3_f32x4 acc[RW][NT];
+#pragma unroll
+    for (int q = 0; q < RW; q++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) acc[q][j] = k3_f32x4{0.f, 0.f, 0.f, 0.f};
+    auto slot = [](int r, int c) { return r * 32 + ((c ^ (r >> 1)) & 7) * 4; };
+    auto use = [&](const Slot &s, int i) {
+        const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wsc), i & 63));
+#pragma unroll
+        for (int p = 0; p < NP; p++) *reinterpret_cast<u32x4 *>(mine + slot(8 * p + lane / 8, lane & 7)) = s.x[p];
+        __builtin_amdgcn_wave_barrier();
+        Wide ww[WIDE ? RW : 1];
+        if constexpr (WIDE)
+#pragma unroll
+            for (int q = 0; q < RW; q++) ww[q] = widen(s.w[q][0], s.w[q][1]);
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            const int r = 16 * j + (NP == 1 ? r16 & 7 : r16);
+            const u32x4 x0 = *reinterpret_cast<const u32x4 *>(mine + slot(r, g)), x1 = *reinterpret_cast<const u32x4 *>(mine + slot(r, 4 + g));
+            const float f = s.s[j] * w;
+            Wide xw;
+            if constexpr (WIDE) xw = widen(x0, x1);
+#pragma unroll
+            for (int q = 0; q < RW; q++) {
+                k3_f32x4 v;
+                if constexpr (WIDE) v = wide_mfma(ww[q], xw);
+                else v = f8_mfma(s.w[q][0], s.w[q][1], x0, x1);
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[q][j][e] = fmaf(f, v[e], acc[q][j][e]);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    };
+#pragma unroll
+    for (int u = 0; u < U; u++) load(ring[u], u);
+    int i = 0;
+    for (; i + U <= n; i += U) {
+        if (i && i % 64 == 0) wsc = Ws[min(k0 + i / 64 * 64 + lane, nkb - 1)];       /* (U divides 64) */
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            use(ring[u], i + u);
+            load(ring[u], i + u + U);
+        }
+    }
+    if (i < n && i && i % 64 == 0) wsc = Ws[min(k0 + i / 64 * 64 + lane, nkb - 1)];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+        if (i + u < n) use(ring[u], i + u);
+    static_assert(64 % U == 0, "scales are fetched between rounds");
+
+    /* the waves' sums, in their order */
+    float4 *const part = reinterpret_cast<float4 *>(mine);
+#pragma unroll
+    for (int q = 0; q < RW; q++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) part[(q * NT + j) * 64 + lane] = make_float4(acc[q][j][0], acc[q][j][1], acc[q][j][2], acc[q][j][3]);
+    __syncthreads();
+    for (int f = wv; f < RW * NT; f += NW) {
+        const int o = (rt0 + f / NT) * 16 + 4 * g, r = 16 * (f % NT) + r16;
+        const int t = r < job.n ? y_row(a, job.r0 + r) : a.T;
+        float b[4];
+        bias4(a, o, b);
+        const uint4 res = res4(a, t, o);
+        const float4 *p = reinterpret_cast<const float4 *>(lds) + f * 64 + lane;
+        float4 s = p[0];
+#pragma unroll
+        for (int w = 1; w < NW; w++) {
+            const float4 v = p[w * (WAVE / 4)];
+            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+        }
+        put4(a, t, o, s, b, res);
+    }
+}
+
+template <int RW, int NP, int U, int NW, int POL, bool WIDE>
+__global__ __launch_bounds__(64 * NW) void f8_stream_kernel(K3kF8 a, int o0, int og)
+{
+    __shared__ __attribute__((aligned(16))) uint32_t lds[NW * stream_lds(RW, NP) / 4];
+    Job job = {0, 0, a.T};
+    int o = blockIdx.x;
+    if (a.offsets) {
+        const int j = blockIdx.x / (unsigned)og;
+        o -= j * og;
+        job = find_job(a, count_jobs(a, 8 * NP), j, 8 * NP);
+        if (job.n == 0) return;
+    }
+    stream_rows<RW, NP, U, NW, POL, WIDE>(a, job, (o0 + o) * RW, lds);
+}
+
+/* ---- many rows: LDS tiles ---------------------------------------------------------------- */
+typedef struct {
+    K3kF8 a;
+    int nt, no;             /* tiles over rows (dense) and outputs */
+    int nsl, per;           /* slices of the column blocks, blocks of one */
+    float *part;            /* [nsl][T][out] sums of the slices (nsl > 1) */
+} F8Tile;
+
+/* Which row and output tile workgroup b of nt * no * nsl takes: each XCD gets a run of tiles of its own, slice by
+ * slice, down 8 row tiles before the next outputs (what a run reads of W it reads once from its L2, and its x stays there). */
+__device__ __forceinline__ bool tile_of(int nt, int no, int nsl, int b, int &tt, int &to, int &sl)
+{
+    const int tiles = nt * no, all = tiles * nsl;
+    if (b >= all) return false;
+    const int full = all / K3_NXCD * K3_NXCD;
+    int i = b;
+    if (b < full) i = (b % K3_NXCD) * (all / K3_NXCD) + b / K3_NXCD;
+    sl = i / tiles;
+    i -= sl * tiles;
+    constexpr int GT = 8;
+    const int blk = GT * no, q = i / blk, h = min(GT, nt - q * GT), r = i - q * blk;
+    to = r / h;
+    tt = q * GT + r % h;
+    return true;
+}
+
+template <int BT, int BO, int WT, int WO, int NST, bool WIDE>
+__global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
+{
+    constexpr int NW = WT * WO, FT = BT / WT / 16, FO = BO / WO / 16;
+    constexpr int XD = BT / 8 / NW, WD = BO / 8 / NW, SD = (BT / 64 + NW - 1) / NW, DN = XD + WD + SD;      /* requests of a wave per step */
+    constexpr int SZ = (BT + BO) * 32 + SD * NW * 64;           /* a stage, in 4-byte units */
+    static_assert(XD >= 1 && WD >= 1 && NST >= 2 && NST <= 4 && BO / WO <= 128 && (BO <= 128 || BO % 128 == 0), "tile");
+    __shared__ __attribute__((aligned(1024))) uint32_t S0[SZ], S1[SZ], S2[NST > 2 ? SZ : 4], S3[NST > 3 ? SZ : 4];
+
+    const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wt = wv % WT, wo = wv / WT;
+    const K3kF8 &a = p.a;
+    int tt, to, sl;
+    Job job;
+    if (a.offsets) {
+        const Jobs s = count_jobs(a, BT);
+        if (!tile_of(s.total, p.no, 1, blockIdx.x, tt, to, sl)) return;
+        job = find_job(a, s, tt, BT);
+    } else {
+        if (!tile_of(p.nt, p.no, p.nsl, blockIdx.x, tt, to, sl)) return;
+        job = Job{0, tt * BT, min(BT, a.T - tt * BT)};
+    }
+    const int o0 = to * BO, nkb = blocks(a.in);
+    const int k0 = sl * p.per, n = min(p.per, nkb - k0);
+
+    /* Row r's 16-byte column c lies in slot c ^ (r / 2 % 8): the 16 rows of a fragment read fall on all 64 banks. */
+    auto sw = [](int r) { return (r >> 1) & 7; };
+    const size_t xbase = a.offsets ? 0 : (size_t)job.r0;        /* (dense: offsets from the tile's own rows) */
+    const k3_rsrc rx = k3_make_rsrc(a.x + xbase * a.ldx, F8_OOB), rs = k3_make_rsrc(a.xs + xbase * a.ldxs, F8_OOB);
+    const int rb = o0 / 128;
+    const k3_rsrc rw = k3_make_rsrc(a.W + (size_t)job.e * a.w_step + (size_t)rb * nkb * F8_KSTEP, (uint32_t)min((size_t)F8_OOB, (size_t)(blocks(a.out) - rb) * nkb * F8_KSTEP));
+    /* DMA i of wave wv fills rows 8 (NW i + wv) ..+8 of x, a lane a 16-byte slot; rows past the job's come as zeros */
+    uint32_t xo[XD], wof[WD], so[SD];
+    auto row_at = [&](int r) -> int { return r < job.n ? (a.offsets ? x_row(a, job.r0 + r) : r) : -1; };
+#pragma unroll
+    for (int i = 0; i < XD; i++) {
+        const int r = (i * NW + wv) * 8 + lane / 8, t = row_at(r);
+        xo[i] = t < 0 ? F8_OOB : (uint32_t)t * (uint32_t)a.ldx + ((lane & 7) ^ sw(r)) * 16;
+    }
+#pragma unroll
+    for (int i = 0; i < SD; i++) {
+        const int r = (i * NW + wv) * 64 + lane, t = r < BT ? row_at(r) : -1;
+        so[i] = t < 0 ? F8_OOB : (uint32_t)t * (uint32_t)a.ldxs * 4;
+    }
+    /* W: the stage holds row tiles in their order, DMA i half tile NW i + wv */
+#pragma unroll
+    for (int i = 0; i < WD; i++) {
+        const int h = i * NW + wv, rt = o0 / 16 + h / 2, b = rt / F8_G - rb;
+        wof[i] = (uint32_t)b * (uint32_t)nkb * F8_KSTEP + (uint32_t)(rt % F8_G) * F8_TILE + (h & 1) * 1024 + lane * 16;
+    }
+    auto buf_of = [&](auto slot) -> uint32_t * {
+        constexpr int S = decltype(slot)::value;
+        if constexpr (S == 0) return S0;
+        else if constexpr (S == 1) return S1;
+        else if constexpr (S == 2) return S2;
+        else return S3;
+    };
+    int kx = k0;
+    const int kend = k0 + n;
+    auto issue = [&](auto slot) {
+        uint32_t *const b = buf_of(slot);
+        const uint32_t none = kx < kend ? 0u : F8_OOB;
+#pragma unroll
+        for (int i = 0; i < XD; i++) k3_dma16(rx, b + (i * NW + wv) * 256, xo[i] | none, kx * 128);
+#pragma unroll
+        for (int i = 0; i < WD; i++) k3_dma16(rw, b + BT * 32 + (i * NW + wv) * 256, wof[i] | none, kx * F8_KSTEP);
+#pragma unroll
+        for (int i = 0; i < SD; i++) dma4(rs, b + (BT + BO) * 32 + (i * NW + wv) * 64, so[i] | none, kx * 4);
+        kx++;
+    };
+    /* W's scales of the wave's outputs: a lane each, 64 column blocks at a time */
+    const float *const Ws = a.Ws + (size_t)job.e * a.ws_step + (size_t)min((o0 + wo * (BO / WO)) / 128, blocks(a.out) - 1) * a.ldws;
+    float wsc = Ws[min(k0 + lane, nkb - 1)];
+
+    k3_f32x4 acc[FO][FT];
+#pragma unroll
+    for (int i = 0; i < FO; i++)
+#pragma unroll
+        for (int j = 0; j < FT; j++) acc[i][j] = k3_f32x4{0.f, 0.f, 0.f, 0.f};
+    const int xr = wt * (BT / WT) + r16;
+    const int xa0 = xr * 32 + ((g ^ sw(xr)) & 7) * 4, xa1 = xr * 32 + (((4 + g) ^ sw(xr)) & 7) * 4;
+    const int wa = BT * 32 + wo * (BO / WO) * 32 + lane * 4, sa = (BT + BO) * 32 + wt * (BT / WT) + r16;
+    constexpr int WAITN = DN * (NST - 2);
+    constexpr int WAIT_STAGE = (WAITN & 15) | (7 << 4) | (0 << 8) | ((WAITN >> 4) << 14);       /* and LDS: none */
+    constexpr int WAIT_VM0 = (7 << 4) | (15 << 8);
+    static_assert(WAITN < 64, "requests in flight");
+    /* Step k: fragments of rows one after another, each read while the one before is multiplied. Once the last one's read
+     * has returned, every wave is past its reads of buffer k % NST and stage k + 1 has landed (one barrier), so stage k + NST goes into that
+     * buffer, and the next step's fragments of W and first rows are read under the last rows' products. */
+    u32x4 wf[2][FO][2], xf[2][2];
+    Wide ww[WIDE ? FO : 1];
+    float sf[2];
+    auto read_w = [&](const uint32_t *b, u32x4 (&f)[FO][2]) {
+#pragma unroll
+        for (int i = 0; i < FO; i++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) f[i][h] = *reinterpret_cast<const u32x4 *>(b + wa + i * 512 + h * 256);
+    };
+    auto read_x = [&](const uint32_t *b, int j, u32x4 (&f)[2], float &s) {
+        f[0] = *reinterpret_cast<const u32x4 *>(b + xa0 + j * 512);
+        f[1] = *reinterpret_cast<const u32x4 *>(b + xa1 + j * 512);
+        s = __uint_as_float(b[sa + 16 * j]);
+    };
+    static_assert(NST % 2 == 0 && FT % 2 == 0, "fragment rings");
+    int at = 0;
+    auto step = [&](auto slot) {
+        constexpr int S = decltype(slot)::value;
+        const uint32_t *const b = buf_of(slot);
+        const uint32_t *const nb = buf_of(std::integral_constant<int, (S + 1) % NST>{});
+        const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wsc), at & 63));
+#pragma unroll
+        for (int j = 0; j < FT; j++) {
+            if (j + 1 < FT) {
+                read_x(b, j + 1, xf[(j + 1) % 2], sf[(j + 1) % 2]);
+            } else {
+                /* (__syncthreads would wait for every request) */
+                __builtin_amdgcn_s_waitcnt(WAIT_STAGE);
+                asm volatile("s_barrier" ::: "memory");
+                __builtin_amdgcn_sched_barrier(0);
+                issue(slot);
+                read_w(nb, wf[(S + 1) % 2]);            /* (past the last step: what lies there, unused) */
+                read_x(nb, 0, xf[0], sf[0]);
+            }
+            const float f = sf[j % 2] * w;
+            k3_f32x4 v[FO];
+            if constexpr (WIDE) {
+                if (j == 0)
+#pragma unroll
+                    for (int i = 0; i < FO; i++) ww[i] = widen(wf[S % 2][i][0], wf[S % 2][i][1]);
+                const Wide xw = widen(xf[j % 2][0], xf[j % 2][1]);
+#pragma unroll
+                for (int i = 0; i < FO; i++) v[i] = wide_mfma(ww[i], xw);
+            } else
+#pragma unroll
+            for (int i = 0; i < FO; i++) v[i] = f8_mfma(wf[S % 2][i][0], wf[S % 2][i][1], xf[j % 2][0], xf[j % 2][1]);
+#pragma unroll
+            for (int i = 0; i < FO; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[i][j][e] = fmaf(f, v[i][e], acc[i][j][e]);
+            /* (the sums are formed here: the compiler would put all of them off, and hold the products) */
+#pragma unroll
+            for (int i = 0; i < FO; i++) asm volatile("" : "+v"(acc[i][j]));
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if ((++at & 63) == 0) wsc = Ws[min(k0 + at + lane, nkb - 1)];
+    };
+    each_of<0, NST>(issue);
+    __builtin_amdgcn_s_waitcnt(WAIT_VM0);
+    __syncthreads();
+    read_w(S0, wf[0]);
+    read_x(S0, 0, xf[0], sf[0]);
+    int left = n;
+    for (; left >= NST; left -= NST) each_of<0, NST>(step);
+    each_of<0, NST - 1>([&](auto slot) {
+        if (decltype(slot)::value < left) step(slot);
+    });
+
+    /* The sums go through LDS (the stage buffers, a region per wave, JR fragments of rows at a time; 16-byte column c of row r in
+     * c ^ (r % 16)), so that a wave writes whole rows of its outputs, and the epilogue's code is there once. */
+    constexpr int WOUT = BO / WO, C = WOUT / 4;
+    constexpr int RB1 = 16 * WOUT;              /* 4-byte units of one fragment of rows */
+    constexpr int JR = SZ / (FT * RB1) * NST >= NW ? FT : SZ / (FT / 2 * RB1) * NST >= NW ? FT / 2 : FT / 4;
+    constexpr int RB = JR * RB1, PER = SZ / RB;
+    static_assert(JR >= 1 && FT % JR == 0 && PER >= 1 && PER * NST >= NW && 64 % C == 0, "epilogue regions");
+    uint32_t *stage = S0;
+    if (PER < NW) stage = wv / PER == 0 ? S0 : wv / PER == 1 ? S1 : wv / PER == 2 ? S2 : S3;
+    float4 *const reg = reinterpret_cast<float4 *>(stage + (wv % PER) * RB);
+    const int c = lane % C, o = o0 + wo * WOUT + 4 * c;
+    constexpr int RI = 64 / C, IT = 16 * JR / RI;
+    const int row0 = wt * (BT / WT) + lane / C;
+    float bs[4];
+    bias4(a, p.nsl > 1 ? a.out : o, bs);
+    __builtin_amdgcn_s_waitcnt(WAIT_VM0);      /* the last requests land before LDS is used again */
+    __syncthreads();
+#pragma unroll
+    for (int j0 = 0; j0 < FT; j0 += JR) {
+#pragma unroll
+        for (int j = 0; j < JR; j++)
+#pragma unroll
+            for (int i = 0; i < FO; i++) {
+                const int r = 16 * j + r16, oc = 4 * i + g;
+                reg[r * C + (oc ^ (r16 & (C - 1)))] = make_float4(acc[i][j0 + j][0], acc[i][j0 + j][1], acc[i][j0 + j][2], acc[i][j0 + j][3]);
+            }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 2
+        for (int i = 0; i < IT; i++) {
+            const int r = lane / C + i * RI, at = row0 + 16 * j0 + i * RI;
+            const float4 v = reg[r * C + (c ^ (r & 15 & (C - 1)))];
+            const int t = at < job.n ? y_row(a, job.r0 + at) : a.T;
+            if (p.nsl == 1) {
+                put4(a, t, o, v, bs, res4(a, t, o));
+            } else if (t < a.T && o < a.out) {
+                float *q = p.part + ((size_t)sl * a.T + t) * a.out + o;
+                if (o + 4 <= a.out) {
+                    __builtin_memcpy(q, &v, 16);
+                } else {
+                    const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int m = 0; m < 3; m++)
+                        if (o + m < a.out) q[m] = e[m];
+                }
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+/* the slices' sums, in slice order, and the epilogue; four slices requested at once */
+__global__ __launch_bounds__(64) void f8_join_kernel(K3kF8 a, const float *part, int nsl)
+{
+    const unsigned per = (a.out + 3) / 4, i = blockIdx.x * 64 + threadIdx.x;
+    const int t = (int)(i / per), o = (int)(i - (unsigned)t * per) * 4;
+    if (t >= a.T) return;
+    float b[4];
+    bias4(a, o, b);
+    const uint4 res = res4(a, t, o);
+    const float *const q = part + (size_t)t * a.out + o;
+    const size_t one = (size_t)a.T * a.out;
+    const int n = min(4, a.out - o);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < nsl; s += 4) {
+        float4 f[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float *p = q + one * min(s + j, nsl - 1);
+            if (n == 4) __builtin_memcpy(&f[j], p, 16);
+            else f[j] = make_float4(p[0], n > 1 ? p[1] : 0.f, n > 2 ? p[2] : 0.f, 0.f);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (s + j < nsl) v.x += f[j].x, v.y += f[j].y, v.z += f[j].z, v.w += f[j].w;
+    }
+    put4(a, t, o, v, b, res);
+}
+
+/* ---- launches -------------------------------------------------------------------------------- */
+constexpr int F8_MAX_SLICES = 16;
+constexpr size_t F8_PART_CAP = (size_t)64 << 20;
+
+/* the slices' sums of any batch up to T: a call takes slices only as far as they fit this */
+size_t part_bytes(int T, int out)
+{
+    const size_t most = (size_t)F8_MAX_SLICES * T * out * 4;
+    return most < F8_PART_CAP ? most : F8_PART_CAP;
+}
+
+/* passes of up to `most` rows that the experts can need */
+long most_jobs(const K3kF8 *a, int most)
+{
+    return (long)a->rows / most + (a->rows < a->n_experts ? a->rows : a->n_experts);
+}
+
+template <int RW, int NP, int U, int NW>
+void stream_launch(const K3kF8 *a, long jobs, hipStream_t st)
+{
+    /* (a launch takes under 2^32 work-items) */
+    const long og = ((a->out + 15) / 16 + RW - 1) / RW, most = ((1L << 32) - 1) / (64 * NW) / jobs;
+    for (long o = 0; o < og; o += most) {
+        const int n = (int)(og - o < most ? og - o : most);
+        if (a->y_type == K3D_F32) f8_stream_kernel<RW, NP, U, NW, K3_LD_NT, true><<<(unsigned)(jobs * n), 64 * NW, 0, st>>>(*a, (int)o, n);
+        else f8_stream_kernel<RW, NP, U, NW, K3_LD_NT, false><<<(unsigned)(jobs * n), 64 * NW, 0, st>>>(*a, (int)o, n);
+    }
+}
+
+template <int RW, int NP, int U>
+void stream_go(const K3kF8 *a, hipStream_t st)
+{
+    /* waves that share a workgroup's columns: enough for the chip, each with a few blocks */
+    const long jobs = a->offsets ? most_jobs(a, 8 * NP) : 1, wgs = jobs * (((a->out + 15) / 16 + RW - 1) / RW);
+    const int nkb = blocks(a->in);
+    if (wgs * 4 < k3k_cu_count() * 8 && nkb >= 16) stream_launch<RW, NP, U, 8>(a, jobs, st);
+    else if (nkb >= 8) stream_launch<RW, NP, U, 4>(a, jobs, st);
+    else stream_launch<RW, NP, U, 2>(a, jobs, st);
+}
+
+void stream(const K3kF8 *a, int rows, hipStream_t st)
+{
+    if (rows <= 8) stream_go<1, 1, 8>(a, st);
+    else if (rows <= 16) stream_go<1, 2, 4>(a, st);
+    else if (rows <= 32) stream_go<2, 4, 2>(a, st);
+    else stream_go<2, 8, 2>(a, st);
+}
+
+template <int BT, int BO, int WT, int WO, int NST, bool WIDE = false>
+void tile_go(F8Tile *p, int nsl, hipStream_t st)
+{
+    const int nkb = blocks(p->a.in);
+    p->nt = (p->a.T + BT - 1) / BT;
+    p->no = (p->a.out + BO - 1) / BO;
+    p->per = (nkb + nsl - 1) / nsl;
+    p->nsl = (nkb + p->per - 1) / p->per;
+    const long grid = (p->a.offsets ? most_jobs(&p->a, BT) : (long)p->nt) * p->no * p->nsl;
+    f8_tile_kernel<BT, BO, WT, WO, NST, WIDE><<<(unsigned)grid, 64 * WT * WO, 0, st>>>(*p);
+}
+
+}  // namespace
+
+extern "C" size_t k3k_f8_tiled_bytes(int rows, int in) { return tiled_bytes(rows, in); }
+
+extern "C" int k3k_f8_tile(uint8_t *t, const uint8_t *W, long ldw, int rows, int in, int mats, void *stream)
+{
+    const int nkb = blocks(in);
+    const size_t all = (size_t)mats * blocks(rows) * nkb * F8_G, most = (size_t)1 << 24;
+    for (size_t i = 0; i < all; i += most) {
+        /* (a launch counts its workgroups from the first one's number, which fits 32 bits: see k3d_f8_tile) */
+        tile_kernel<<<(unsigned)(all - i < most ? all - i : most), 128, 0, (hipStream_t)stream>>>(t, W, (size_t)ldw, rows, in, nkb, (unsigned)i);
+        K3K_LAUNCH_CHECK("f8_tile");
+    }
+    return 0;
+}
+
+extern "C" size_t k3k_linear_f8_ws(int T, int in, int out)
+{
+    (void)in;
+    return part_bytes(T, out);
+}
+
+extern "C" int k3k_linear_f8(const K3kF8 *a, void *stream_)
+{
+    hipStream_t st = (hipStream_t)stream_;
+    if (a->T <= 64) {
+        stream(a, a->T, st);
+        K3K_LAUNCH_CHECK("linear_f8: few rows");
+        return 0;
+    }
+    F8Tile p;
+    p.a = *a;
+    p.part = (float *)a->ws;
+    const long cus = k3k_cu_count();
+    const int nkb = blocks(a->in);
+    const long tiles = (long)((a->T + 255) / 256) * ((a->out + 255) / 256);
+    if (tiles >= cus && a->y_type == K3D_BF16) {
+        tile_go<256, 256, 2, 4, 2>(&p, 1, st);
+    } else {
+        const long small = (long)((a->T + 127) / 128) * ((a->out + 127) / 128);
+        int nsl = 1;
+        while (nsl < F8_MAX_SLICES && small * nsl * 2 <= cus && nkb >= 4 * nsl && (size_t)2 * nsl * a->T * a->out * 4 <= part_bytes(a->T, a->out)) nsl *= 2;
+        if (a->y_type == K3D_F32) tile_go<128, 128, 2, 2, 4, true>(&p, nsl, st);
+        else tile_go<128, 128, 2, 2, 4>(&p, nsl, st);
+    }
+    K3K_LAUNCH_CHECK("linear_f8: tiles");
+    if (p.nsl > 1) {
+        const size_t n = (size_t)a->T * ((a->out + 3) / 4);
+        f8_join_kernel<<<(unsigned)((n + 63) / 64), 64, 0, st>>>(*a, p.part, p.nsl);
+        K3K_LAUNCH_CHECK("linear_f8: join");
+    }
+    return 0;
+}
+
+extern "C" int k3k_grouped_f8(const K3kF8 *a, void *stream_)
+{
+    hipStream_t st = (hipStream_t)stream_;
+    const int each = (a->rows + a->n_experts - 1) / a->n_experts;       /* rows of an expert, on average */
+    if (each <= 48) {
+        stream(a, each <= 4 ? 8 : each <= 12 ? 16 : each <= 24 ? 32 : 64, st);
+        K3K_LAUNCH_CHECK("grouped_f8: few rows");
+        return 0;
+    }
+    F8Tile p;
+    p.a = *a;
+    p.part = NULL;
+    if (a->y_type == K3D_F32) tile_go<128, 128, 2, 2, 4, true>(&p, 1, st);
+    else if (each <= 128) tile_go<128, 128, 2, 2, 4>(&p, 1, st);
+    else tile_go<256, 256, 2, 4, 2>(&p, 1, st);
+    K3K_LAUNCH_CHECK("grouped_f8: tiles");
+    return 0;
+}

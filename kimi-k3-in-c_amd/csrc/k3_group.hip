@@ -1,0 +1,169 @@
+/* SPDX-License-Identifier: Apache-2.0 */
+/*
+ * k3_group.hip -- a routing's slots by expert (k3d_group): offsets[e] .. offsets[e + 1] of perm are the slots t * topk + j
+ * whose expert is e, ascending; slots without an expert are in none.
+ *
+ * A counting sort, the same order every time: a wave ranks its slots among equal experts by ballots, its workgroup's waves
+ * add their counts to the experts' one after another. Up to 4096 slots in one workgroup; more in chunks of 1024, whose
+ * counts are summed by chunk before the slots take their places. Bound by latency: barriers and launches.
+ */
+#include "k3_common.h"
+#include "k3k.h"
+
+namespace {
+
+constexpr int GR_C = 1024, GR_ONE = 4, GR_MAXE = 2048;
+
+/* this slot's place among the wave's slots of its expert, their number, and whether it is the first of them */
+__device__ __forceinline__ void rank_wave(int e, bool valid, int &rank, int &count, bool &first)
+{
+    const int lane = threadIdx.x & 63;
+    rank = count = 0;
+    first = false;
+    for (uint64_t todo = __ballot(valid); todo;) {
+        const int l = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)todo) - 1);
+        const uint64_t same = __ballot(valid && e == __builtin_amdgcn_readlane(e, l));
+        if (same >> lane & 1) {
+            rank = __popcll(same & ((1ull << lane) - 1));
+            count = __popcll(same);
+            first = lane == l;
+        }
+        todo &= ~same;
+    }
+}
+
+/* the slot's place among its expert's slots up to here: cnt counts them, wave after wave */
+__device__ __forceinline__ int rank_chunk(int *cnt, int e, bool valid)
+{
+    int rank, count;
+    bool first;
+    rank_wave(e, valid, rank, count, first);
+    const int wv = threadIdx.x >> 6;
+    for (int w = 0; w < GR_C / 64; w++) {
+        if (w == wv && valid) {
+            const int base = cnt[e];
+            __builtin_amdgcn_wave_barrier();
+            if (first) cnt[e] = base + count;
+            rank += base;
+        }
+        __syncthreads();
+    }
+    return rank;
+}
+
+/* off[e]: the sum of n[0 .. e) of GR_MAXE entries, two a thread; the whole sum returned */
+__device__ __forceinline__ int scan_experts(const int *n, int *off, int *waves)
+{
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const int a = n[2 * tid], b = n[2 * tid + 1];
+    int sum = a + b;
+    for (int d = 1; d < 64; d *= 2) {
+        const int o = __shfl_up(sum, d);
+        sum += lane >= d ? o : 0;
+    }
+    if (lane == 63) waves[wv] = sum;
+    __syncthreads();
+    int before = 0, total = 0;
+    for (int w = 0; w < GR_C / 64; w++) {
+        if (w < wv) before += waves[w];
+        total += waves[w];
+    }
+    off[2 * tid] = before + sum - a - b;
+    off[2 * tid + 1] = before + sum - b;
+    __syncthreads();
+    return total;
+}
+
+__global__ __launch_bounds__(GR_C) void group_one_kernel(int *offsets, int *perm, const int *idx, int N, int E)
+{
+    __shared__ int cnt[GR_MAXE], off[GR_MAXE], waves[GR_C / 64];
+    const int tid = threadIdx.x;
+    int e[GR_ONE], rank[GR_ONE];
+    for (int u = 0; u < GR_ONE; u++) e[u] = u * GR_C + tid < N ? idx[u * GR_C + tid] : -1;
+    cnt[tid] = cnt[GR_C + tid] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < GR_ONE; u++)
+        if (u * GR_C < N) rank[u] = rank_chunk(cnt, e[u], (unsigned)e[u] < (unsigned)E);
+    const int total = scan_experts(cnt, off, waves);
+    for (int i = tid; i <= E; i += GR_C) offsets[i] = i < E ? off[i] : total;
+#pragma unroll
+    for (int u = 0; u < GR_ONE; u++)
+        if ((unsigned)e[u] < (unsigned)E) perm[off[e[u]] + rank[u]] = u * GR_C + tid;
+}
+
+/* hist[c][e]: slots of expert e in chunk c */
+__global__ __launch_bounds__(GR_C) void group_count_kernel(int *hist, const int *idx, int N, int E)
+{
+    __shared__ int cnt[GR_MAXE];
+    const int tid = threadIdx.x, i = blockIdx.x * GR_C + tid;
+    const int e = i < N ? idx[i] : -1;
+    cnt[tid] = cnt[GR_C + tid] = 0;
+    __syncthreads();
+    if ((unsigned)e < (unsigned)E) atomicAdd(&cnt[e], 1);
+    __syncthreads();
+    for (int k = tid; k < E; k += GR_C) hist[(size_t)blockIdx.x * E + k] = cnt[k];
+}
+
+/* hist[c][e] becomes the place of the chunk's first slot of expert e */
+__global__ __launch_bounds__(GR_C) void group_scan_kernel(int *offsets, int *hist, int E, int chunks)
+{
+    __shared__ int cnt[GR_MAXE], off[GR_MAXE], waves[GR_C / 64];
+    const int tid = threadIdx.x;
+    cnt[tid] = cnt[GR_C + tid] = 0;
+    for (int e = tid; e < E; e += GR_C) {
+        int s = 0;
+#pragma unroll 8
+        for (int c = 0; c < chunks; c++) s += hist[(size_t)c * E + e];
+        cnt[e] = s;
+    }
+    __syncthreads();
+    const int total = scan_experts(cnt, off, waves);
+    for (int e = tid; e <= E; e += GR_C) offsets[e] = e < E ? off[e] : total;
+    for (int e = tid; e < E; e += GR_C) {
+        int s = off[e];
+#pragma unroll 8
+        for (int c = 0; c < chunks; c++) {
+            int *const h = hist + (size_t)c * E + e;
+            const int v = *h;
+            *h = s;
+            s += v;
+        }
+    }
+}
+
+__global__ __launch_bounds__(GR_C) void group_place_kernel(int *perm, const int *hist, const int *idx, int N, int E)
+{
+    __shared__ int cnt[GR_MAXE];
+    const int tid = threadIdx.x, i = blockIdx.x * GR_C + tid;
+    const int e = i < N ? idx[i] : -1;
+    for (int k = tid; k < E; k += GR_C) cnt[k] = hist[(size_t)blockIdx.x * E + k];
+    __syncthreads();
+    const bool valid = (unsigned)e < (unsigned)E;
+    const int at = rank_chunk(cnt, e, valid);
+    if (valid) perm[at] = i;
+}
+
+}  // namespace
+
+extern "C" size_t k3k_group_ws(int N, int n_experts)
+{
+    return N <= GR_ONE * GR_C ? 0 : (size_t)((N + GR_C - 1) / GR_C) * n_experts * 4;
+}
+
+extern "C" int k3k_group(int *offsets, int *perm, const int *idx, int N, int n_experts, int *hist, void *stream)
+{
+    hipStream_t st = (hipStream_t)stream;
+    if (N <= GR_ONE * GR_C) {
+        group_one_kernel<<<1, GR_C, 0, st>>>(offsets, perm, idx, N, n_experts);
+    } else {
+        const int chunks = (N + GR_C - 1) / GR_C;
+        group_count_kernel<<<chunks, GR_C, 0, st>>>(hist, idx, N, n_experts);
+        K3K_LAUNCH_CHECK("group: count");
+        group_scan_kernel<<<1, GR_C, 0, st>>>(offsets, hist, n_experts, chunks);
+        K3K_LAUNCH_CHECK("group: scan");
+        group_place_kernel<<<chunks, GR_C, 0, st>>>(perm, hist, idx, N, n_experts);
+    }
+    K3K_LAUNCH_CHECK("group");
+    return 0;
+}

@@ -31,6 +31,24 @@ __device__ __forceinline__ uint32_t wave_reduce_u32(uint32_t v)
     return __builtin_amdgcn_readlane(v, 63);
 }
 
+/* Sum of the wave's floats, the same in every lane, in a fixed order. */
+template <int CTRL, int RM>
+__device__ __forceinline__ float dpp_add_f32(float v)
+{
+    return v + __uint_as_float(dpp_u32<CTRL, RM, 0u>(__float_as_uint(v)));
+}
+
+__device__ __forceinline__ float wave_total_f32(float v)
+{
+    v = dpp_add_f32<0xB1, 0xf>(v);
+    v = dpp_add_f32<0x4E, 0xf>(v);
+    v = dpp_add_f32<0x141, 0xf>(v);
+    v = dpp_add_f32<0x140, 0xf>(v);
+    v = dpp_add_f32<0x142, 0xa>(v);
+    v = dpp_add_f32<0x143, 0xc>(v);
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 63));
+}
+
 /* Sum of the wave's doubles, the same in every lane, in a fixed order (the steps of wave_reduce_u32; 18 instructions, where
  * shuffles through the LDS take 12 round trips). */
 template <int CTRL, int RM>

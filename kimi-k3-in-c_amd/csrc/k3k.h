@@ -371,6 +371,65 @@ typedef struct {
 } K3kHeads;
 int k3k_heads(const K3kHeads *a, void *stream);
 
+/* ---- the 8-bit path of a layer (k3_rows.hip, k3_f8.hip) ------------------------------ */
+/* The arguments of k3d_add_norm, checked. */
+typedef struct {
+    void *y, *sum;
+    uint8_t *q;
+    float *qs;
+    const void *x, *res;
+    const float *w;
+    long ldy, ldsum, ldq, ldqs, ldx, ldr;
+    int y_type, x_type, r_type, T, n;
+    float eps;
+} K3kNorm;
+int k3k_add_norm(const K3kNorm *a, void *stream);
+
+/* The arguments of k3d_quant_f8, checked. */
+typedef struct {
+    uint8_t *q;
+    float *qs;
+    const void *x;
+    long ldq, ldqs, ldx;
+    int x_type, T, n, act;
+    float b1, b2;
+} K3kQuant;
+int k3k_quant_f8(const K3kQuant *a, void *stream);
+
+/* Products with 8-bit operands: W in k3k_f8_tile's layout, Ws [out blocks][ldws]. With offsets (k3d_grouped_f8): the experts'
+ * matrices w_step bytes and ws_step scales apart, rows [offsets[e], offsets[e + 1]) of `rows` for expert e; row r is row x_rows[r] / x_div (r
+ * itself without x_rows) of x, below x_cap, and row y_rows[r] (r) of y, below T. */
+typedef struct {
+    void *y;
+    const uint8_t *x, *W;
+    const float *xs, *Ws, *bias;
+    const void *res;
+    const int *offsets, *x_rows, *y_rows;
+    long ldy, ldx, ldxs, ldws, ldr;
+    size_t w_step, ws_step;
+    int y_type, T, in, out, act, rows, x_div, x_cap, n_experts;
+    void *ws;
+} K3kF8;
+size_t k3k_f8_tiled_bytes(int rows, int in);
+int k3k_f8_tile(uint8_t *t, const uint8_t *W, long ldw, int rows, int in, int mats, void *stream);
+size_t k3k_linear_f8_ws(int T, int in, int out);
+int k3k_linear_f8(const K3kF8 *a, void *stream);
+int k3k_grouped_f8(const K3kF8 *a, void *stream);
+
+/* The slots of idx [N] by expert (k3_group.hip; up to 2048 experts); hist: k3k_group_ws bytes. */
+size_t k3k_group_ws(int N, int n_experts);
+int k3k_group(int *offsets, int *perm, const int *idx, int N, int n_experts, int *hist, void *stream);
+
+/* out[t] = sum_j wt[t][j] y[t * topk + j], j ascending, over slots with 0 <= idx < n_experts; out of out_type. */
+typedef struct {
+    void *out;
+    const float *y, *wt;
+    const int *idx;
+    long ldo;
+    int out_type, T, topk, n, n_experts;
+} K3kSum;
+int k3k_sum_slots(const K3kSum *a, void *stream);
+
 /* ---- the allocation-free workspace (k3_static.hip) --------------------------------- */
 /* Looks up, once per device, the device address of the library's static workspace for the
  * current device (called by k3d_init). */

@@ -26,6 +26,7 @@ K3D_F32, K3D_BF16 = 0, 1
 K3D_ACT_NONE, K3D_ACT_RELU, K3D_ACT_SILU, K3D_ACT_GELU, K3D_ACT_GELU_TANH = 0, 1, 2, 3, 4
 K3D_SCORE_SIGMOID, K3D_SCORE_SOFTMAX = 0, 1
 K3D_ROT_HALVES, K3D_ROT_INTERLEAVED = 0, 1
+K3D_GLU_NONE, K3D_GLU_SITU, K3D_GLU_SILU = -1, 0, 1
 STAGES = ("begin", "router", "gather", "gateup", "down", "combine", "gemv", "shared")
 
 _lib = None
@@ -156,6 +157,17 @@ def _declare(L):
     d("k3d_linear", I, P, I, LG, P, I, LG, I, P, LG, I, I, P, I, P, LG, P, SZ, P)
     d("k3d_route", I, P, P, P, I, LG, I, I, P, I, I, I, I, I, I, F, P)
     d("k3d_qk_norm_rope", I, P, LG, LG, P, LG, LG, P, LG, LG, P, LG, LG, I, I, I, I, I, P, P, F, P, P, I, I, I, F, P)
+    d("k3d_add_norm", I, P, I, LG, P, LG, P, LG, P, LG, P, I, LG, P, I, LG, I, I, P, F, P)
+    d("k3d_quant_f8", I, P, LG, P, LG, P, I, LG, I, I, I, F, F, P)
+    d("k3d_f8_tiled_bytes", SZ, I, I)
+    d("k3d_f8_tile", I, P, P, LG, I, I, I, P)
+    d("k3d_linear_f8_ws", SZ, I, I, I)
+    d("k3d_linear_f8", I, P, I, LG, P, LG, P, LG, I, P, P, LG, I, I, P, I, P, LG, P, SZ, P)
+    d("k3d_group_ws", SZ, I, I, I)
+    d("k3d_group", I, P, P, P, I, I, I, P, SZ, P)
+    d("k3d_grouped_f8", I, P, I, LG, P, I, P, LG, P, LG, P, I, I, P, I, I, P, P, I, I, P)
+    d("k3d_moe_f8_ws", SZ, I, I, I, I, I)
+    d("k3d_moe_f8", I, P, I, LG, P, P, P, LG, P, LG, I, P, P, P, P, P, P, I, I, I, I, I, F, F, P, SZ, P)
     # generator
     d("k3g_u64", C.c_uint64, C.c_uint64, C.c_uint64)
     d("k3g_bytes", None, P, SZ, C.c_uint64)
