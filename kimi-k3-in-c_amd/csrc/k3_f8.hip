@@ -376,7 +376,7 @@ template <int BT, int BO, int WT, int WO, int NST, bool WIDE>
 __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
 {
     constexpr int NW = WT * WO, FT = BT / WT / 16, FO = BO / WO / 16;
-    constexpr int XD = BT / 8 / NW, WD = BO / 8 / NW, SD = (BT / 64 + NW - 1) / NW, DN = XD + WD + SD;      /* requests of a wave per step */
+    constexpr int XD = BT / 8 / NW, WD = BO / 8 / NW, SD = ((BT + 63) / 64 + NW - 1) / NW, DN = XD + WD + SD;      /* requests of a wave per step */
     constexpr int SZ = (BT + BO) * 32 + SD * NW * 64;           /* a stage, in 4-byte units */
     static_assert(XD >= 1 && WD >= 1 && NST >= 2 && NST <= 4 && BO / WO <= 128 && (BO <= 128 || BO % 128 == 0), "tile");
     __shared__ __attribute__((aligned(1024))) uint32_t S0[SZ], S1[SZ], S2[NST > 2 ? SZ : 4], S3[NST > 3 ? SZ : 4];
@@ -477,6 +477,29 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
         s = __uint_as_float(b[sa + 16 * j]);
     };
     static_assert(NST % 2 == 0 && FT % 2 == 0, "fragment rings");
+    /* The sums of a fragment of rows join the accumulators while the next one's products run: behind their own they would wait for
+     * the last of them. */
+    k3_f32x4 v[2][FO];
+    float f[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < FO; i++) v[1][i] = k3_f32x4{0.f, 0.f, 0.f, 0.f};
+    auto add = [&](auto pin, int j, int h) {
+#pragma unroll
+        for (int i = 0; i < FO; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[i][j][e] = fmaf(f[h], v[h][i][e], acc[i][j][e]);
+        /* (formed here: the compiler would put all of them off, and hold the products) */
+#pragma unroll
+        for (int i = 0; i < FO; i++) asm volatile("" : "+v"(acc[i][j]));
+        if constexpr (decltype(pin)::value && !WIDE) {
+#pragma unroll
+            for (int i = 0; i < FO; i++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
+            }
+        }
+    };
     int at = 0;
     auto step = [&](auto slot) {
         constexpr int S = decltype(slot)::value;
@@ -496,25 +519,19 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
                 read_w(nb, wf[(S + 1) % 2]);            /* (past the last step: what lies there, unused) */
                 read_x(nb, 0, xf[0], sf[0]);
             }
-            const float f = sf[j % 2] * w;
-            k3_f32x4 v[FO];
+            f[j % 2] = sf[j % 2] * w;
             if constexpr (WIDE) {
                 if (j == 0)
 #pragma unroll
                     for (int i = 0; i < FO; i++) ww[i] = widen(wf[S % 2][i][0], wf[S % 2][i][1]);
                 const Wide xw = widen(xf[j % 2][0], xf[j % 2][1]);
 #pragma unroll
-                for (int i = 0; i < FO; i++) v[i] = wide_mfma(ww[i], xw);
-            } else
+                for (int i = 0; i < FO; i++) v[j % 2][i] = wide_mfma(ww[i], xw);
+            } else {
 #pragma unroll
-            for (int i = 0; i < FO; i++) v[i] = f8_mfma(wf[S % 2][i][0], wf[S % 2][i][1], xf[j % 2][0], xf[j % 2][1]);
-#pragma unroll
-            for (int i = 0; i < FO; i++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) acc[i][j][e] = fmaf(f, v[i][e], acc[i][j][e]);
-            /* (the sums are formed here: the compiler would put all of them off, and hold the products) */
-#pragma unroll
-            for (int i = 0; i < FO; i++) asm volatile("" : "+v"(acc[i][j]));
+                for (int i = 0; i < FO; i++) v[j % 2][i] = f8_mfma(wf[S % 2][i][0], wf[S % 2][i][1], xf[j % 2][0], xf[j % 2][1]);
+            }
+            add(std::integral_constant<int, 1>{}, (j + FT - 1) % FT, (j + 1) % 2);
             __builtin_amdgcn_sched_barrier(0);
         }
         if ((++at & 63) == 0) wsc = Ws[min(k0 + at + lane, nkb - 1)];
@@ -529,6 +546,7 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
     each_of<0, NST - 1>([&](auto slot) {
         if (decltype(slot)::value < left) step(slot);
     });
+    add(std::integral_constant<int, 0>{}, FT - 1, 1);
 
     /* The sums go through LDS (the stage buffers, a region per wave, JR fragments of rows at a time; 16-byte column c of row r in
      * c ^ (r % 16)), so that a wave writes whole rows of its outputs, and the epilogue's code is there once. */
