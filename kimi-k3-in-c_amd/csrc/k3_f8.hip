@@ -239,7 +239,12 @@ __device__ __forceinline__ void stream_rows(const K3kF8 &a, const Job &job, int 
     }
     /* W's scales: a lane each, 64 column blocks at a time */
     const float *const Ws = a.Ws + (size_t)job.e * a.ws_step + (size_t)(rt0 / F8_G) * a.ldws;
-    float wsc = n > 0 ? Ws[min(k0 + lane, nkb - 1)] : 0.0f;
+    auto scales = [&](int i) {
+        float v = Ws[min(k0 + i + lane, nkb - 1)];
+        asm volatile("" : "+v"(v));             /* (arrived when it returns: a wait at its use would be one for every request since) */
+        return v;
+    };
+    float wsc = scales(0);
 
     struct Slot {
         u32x4 w[RW][2], x[NP];
@@ -294,14 +299,14 @@ __device__ __forceinline__ void stream_rows(const K3kF8 &a, const Job &job, int 
     for (int u = 0; u < U; u++) load(ring[u], u);
     int i = 0;
     for (; i + U <= n; i += U) {
-        if (i && i % 64 == 0) wsc = Ws[min(k0 + i / 64 * 64 + lane, nkb - 1)];       /* (U divides 64) */
+        if (i && i % 64 == 0) wsc = scales(i);       /* (U divides 64) */
 #pragma unroll
         for (int u = 0; u < U; u++) {
             use(ring[u], i + u);
             load(ring[u], i + u + U);
         }
     }
-    if (i < n && i && i % 64 == 0) wsc = Ws[min(k0 + i / 64 * 64 + lane, nkb - 1)];
+    if (i < n && i && i % 64 == 0) wsc = scales(i);
 #pragma unroll
     for (int u = 0; u < U; u++)
         if (i + u < n) use(ring[u], i + u);
@@ -376,10 +381,10 @@ template <int BT, int BO, int WT, int WO, int NST, bool WIDE>
 __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
 {
     constexpr int NW = WT * WO, FT = BT / WT / 16, FO = BO / WO / 16;
-    constexpr int XD = BT / 8 / NW, WD = BO / 8 / NW, SD = ((BT + 63) / 64 + NW - 1) / NW, DN = XD + WD + SD;      /* requests of a wave per step */
-    constexpr int SZ = (BT + BO) * 32 + SD * NW * 64;           /* a stage, in 4-byte units */
+    constexpr int XD = BT / 8 / NW, WD = BO / 8 / NW, SD = (BT / 8 + NW - 1) / NW, DN = XD + WD;       /* requests of a wave: a step's, scales' */
+    constexpr int SZ = (BT + BO) * 32, SC = SD * NW * 64;       /* a stage, the scales of 8 column blocks, in 4-byte units */
     static_assert(XD >= 1 && WD >= 1 && NST >= 2 && NST <= 4 && BO / WO <= 128 && (BO <= 128 || BO % 128 == 0), "tile");
-    __shared__ __attribute__((aligned(1024))) uint32_t S0[SZ], S1[SZ], S2[NST > 2 ? SZ : 4], S3[NST > 3 ? SZ : 4];
+    __shared__ __attribute__((aligned(1024))) uint32_t S0[SZ], S1[SZ], S2[NST > 2 ? SZ : 4], S3[NST > 3 ? SZ : 4], SX[2 * SC];
 
     const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -412,9 +417,11 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
         const int r = (i * NW + wv) * 8 + lane / 8, t = row_at(r);
         xo[i] = t < 0 ? F8_OOB : (uint32_t)t * (uint32_t)a.ldx + ((lane & 7) ^ sw(r)) * 16;
     }
+    /* Scales of x: 8 column blocks at a time, 8 lanes to a row's 32 bytes (a step's alone would be a line of memory for each row and
+     * step); block c of row r in slot c ^ (r / 8 % 2 * 4), so that 16 rows' fall on 64 banks */
 #pragma unroll
     for (int i = 0; i < SD; i++) {
-        const int r = (i * NW + wv) * 64 + lane, t = r < BT ? row_at(r) : -1;
+        const int r = (i * NW + wv) * 8 + lane / 8, t = r < BT ? row_at(r) : -1;
         so[i] = t < 0 ? F8_OOB : (uint32_t)t * (uint32_t)a.ldxs * 4;
     }
     /* W: the stage holds row tiles in their order, DMA i half tile NW i + wv */
@@ -432,20 +439,32 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
     };
     int kx = k0;
     const int kend = k0 + n;
-    auto issue = [&](auto slot) {
-        uint32_t *const b = buf_of(slot);
+    auto issue_x = [&](auto slot) {
         const uint32_t none = kx < kend ? 0u : F8_OOB;
 #pragma unroll
-        for (int i = 0; i < XD; i++) k3_dma16(rx, b + (i * NW + wv) * 256, xo[i] | none, kx * 128);
+        for (int i = 0; i < XD; i++) k3_dma16(rx, buf_of(slot) + (i * NW + wv) * 256, xo[i] | none, kx * 128);
+    };
+    auto issue_w = [&](auto slot) {
+        const uint32_t none = kx < kend ? 0u : F8_OOB;
 #pragma unroll
-        for (int i = 0; i < WD; i++) k3_dma16(rw, b + BT * 32 + (i * NW + wv) * 256, wof[i] | none, kx * F8_KSTEP);
-#pragma unroll
-        for (int i = 0; i < SD; i++) dma4(rs, b + (BT + BO) * 32 + (i * NW + wv) * 64, so[i] | none, kx * 4);
+        for (int i = 0; i < WD; i++) k3_dma16(rw, buf_of(slot) + BT * 32 + (i * NW + wv) * 256, wof[i] | none, kx * F8_KSTEP);
         kx++;
+    };
+    auto issue_scales = [&](int c) {            /* of blocks k0 + 8 c ..+8 */
+        const int kb = k0 + 8 * c + ((lane & 7) ^ (wv & 1) * 4);
+        static_assert(NW % 2 == 0, "a request's rows are 8 i + wv, their parity the wave's");
+#pragma unroll
+        for (int i = 0; i < SD; i++) dma4(rs, SX + (c & 1) * SC + (i * NW + wv) * 64, (so[i] + kb * 4) | (kb < nkb ? 0u : F8_OOB), 0);
     };
     /* W's scales of the wave's outputs: a lane each, 64 column blocks at a time */
     const float *const Ws = a.Ws + (size_t)job.e * a.ws_step + (size_t)min((o0 + wo * (BO / WO)) / 128, blocks(a.out) - 1) * a.ldws;
-    float wsc = Ws[min(k0 + lane, nkb - 1)];
+    /* (arrived when it returns: a wait at its use would be one for every request since) */
+    auto scales = [&](int i) {
+        float v = Ws[min(k0 + i + lane, nkb - 1)];
+        asm volatile("" : "+v"(v));
+        return v;
+    };
+    float wsc = scales(0);
 
     k3_f32x4 acc[FO][FT];
 #pragma unroll
@@ -454,51 +473,36 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
         for (int j = 0; j < FT; j++) acc[i][j] = k3_f32x4{0.f, 0.f, 0.f, 0.f};
     const int xr = wt * (BT / WT) + r16;
     const int xa0 = xr * 32 + ((g ^ sw(xr)) & 7) * 4, xa1 = xr * 32 + (((4 + g) ^ sw(xr)) & 7) * 4;
-    const int wa = BT * 32 + wo * (BO / WO) * 32 + lane * 4, sa = (BT + BO) * 32 + wt * (BT / WT) + r16;
+    const int wa = BT * 32 + wo * (BO / WO) * 32 + lane * 4, sa = xr * 8 + ((r16 >> 3 & 1) * 4);
     constexpr int WAITN = DN * (NST - 2);
     constexpr int WAIT_STAGE = (WAITN & 15) | (7 << 4) | (0 << 8) | ((WAITN >> 4) << 14);       /* and LDS: none */
     constexpr int WAIT_VM0 = (7 << 4) | (15 << 8);
     static_assert(WAITN < 64, "requests in flight");
-    /* Step k: fragments of rows one after another, each read while the one before is multiplied. Once the last one's read
-     * has returned, every wave is past its reads of buffer k % NST and stage k + 1 has landed (one barrier), so stage k + NST goes into that
-     * buffer, and the next step's fragments of W and first rows are read under the last rows' products. */
-    u32x4 wf[2][FO][2], xf[2][2];
-    Wide ww[WIDE ? FO : 1];
-    float sf[2];
-    auto read_w = [&](const uint32_t *b, u32x4 (&f)[FO][2]) {
+    /* Step k: fragments of rows one after another, read three ahead. Once the last one's read has returned, every wave is past its
+     * reads of buffer k % NST and stage k + 1 has landed (one barrier, three fragments before the end), so stage k + NST goes into that
+     * buffer, and the next step's first rows and, behind their last use, fragments of W are read under the last rows' products. The scaled sums join the accumulators
+     * three products later: behind their own they would wait for it. */
+    constexpr int XR = 4, LA = 3, VR = 4, LAG = 3, NM = FT * FO;
+    static_assert(NST % 2 == 0 && FT % XR == 0 && NM % VR == 0, "fragment rings");
+    u32x4 wf[FO][2], xf[XR][2];
+    Wide ww[WIDE ? FO : 1], xw;
+    float sf[XR], f[XR];
+    k3_f32x4 v[VR];
+    auto read_w = [&](const uint32_t *b, int i) {
 #pragma unroll
-        for (int i = 0; i < FO; i++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) f[i][h] = *reinterpret_cast<const u32x4 *>(b + wa + i * 512 + h * 256);
+        for (int h = 0; h < 2; h++) wf[i][h] = *reinterpret_cast<const u32x4 *>(b + wa + i * 512 + h * 256);
     };
-    auto read_x = [&](const uint32_t *b, int j, u32x4 (&f)[2], float &s) {
-        f[0] = *reinterpret_cast<const u32x4 *>(b + xa0 + j * 512);
-        f[1] = *reinterpret_cast<const u32x4 *>(b + xa1 + j * 512);
-        s = __uint_as_float(b[sa + 16 * j]);
+    auto read_x = [&](const uint32_t *b, int j, int k) {        /* of the k-th block */
+        xf[j % XR][0] = *reinterpret_cast<const u32x4 *>(b + xa0 + j * 512);
+        xf[j % XR][1] = *reinterpret_cast<const u32x4 *>(b + xa1 + j * 512);
+        sf[j % XR] = __uint_as_float(SX[(k >> 3 & 1) * SC + (sa ^ (k & 7)) + 128 * j]);
     };
-    static_assert(NST % 2 == 0 && FT % 2 == 0, "fragment rings");
-    /* The sums of a fragment of rows join the accumulators while the next one's products run: behind their own they would wait for
-     * the last of them. */
-    k3_f32x4 v[2][FO];
-    float f[2] = {0.f, 0.f};
+    auto add = [&](int m) {
+        const int i = m % FO, j = m / FO;
 #pragma unroll
-    for (int i = 0; i < FO; i++) v[1][i] = k3_f32x4{0.f, 0.f, 0.f, 0.f};
-    auto add = [&](auto pin, int j, int h) {
-#pragma unroll
-        for (int i = 0; i < FO; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) acc[i][j][e] = fmaf(f[h], v[h][i][e], acc[i][j][e]);
+        for (int e = 0; e < 4; e++) acc[i][j][e] = fmaf(f[j % XR], v[m % VR][e], acc[i][j][e]);
         /* (formed here: the compiler would put all of them off, and hold the products) */
-#pragma unroll
-        for (int i = 0; i < FO; i++) asm volatile("" : "+v"(acc[i][j]));
-        if constexpr (decltype(pin)::value && !WIDE) {
-#pragma unroll
-            for (int i = 0; i < FO; i++) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
-            }
-        }
+        asm volatile("" : "+v"(acc[i][j]));
     };
     int at = 0;
     auto step = [&](auto slot) {
@@ -506,47 +510,69 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
         const uint32_t *const b = buf_of(slot);
         const uint32_t *const nb = buf_of(std::integral_constant<int, (S + 1) % NST>{});
         const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wsc), at & 63));
-#pragma unroll
-        for (int j = 0; j < FT; j++) {
-            if (j + 1 < FT) {
-                read_x(b, j + 1, xf[(j + 1) % 2], sf[(j + 1) % 2]);
-            } else {
+        each_of<0, FT>([&](auto jj) {
+            constexpr int j = decltype(jj)::value, past = j - (FT - LA);        /* fragments past the barrier (from 0 on) */
+            if constexpr (past == 0) {
                 /* (__syncthreads would wait for every request) */
                 __builtin_amdgcn_s_waitcnt(WAIT_STAGE);
                 asm volatile("s_barrier" ::: "memory");
                 __builtin_amdgcn_sched_barrier(0);
-                issue(slot);
-                read_w(nb, wf[(S + 1) % 2]);            /* (past the last step: what lies there, unused) */
-                read_x(nb, 0, xf[0], sf[0]);
             }
-            f[j % 2] = sf[j % 2] * w;
+            if constexpr (past == 0) issue_x(slot);
+            if constexpr (past == 1) issue_w(slot);
+            if constexpr (past == 2)
+                if ((at & 7) == 0) issue_scales(at / 8 + 1);
+            if constexpr (past < 0) {
+                read_x(b, j + LA, at);
+            } else {                            /* (past the last step: what lies there, unused) */
+                read_x(nb, past, at + 1);
+            }
             if constexpr (WIDE) {
-                if (j == 0)
+                if constexpr (j == 0)
 #pragma unroll
-                    for (int i = 0; i < FO; i++) ww[i] = widen(wf[S % 2][i][0], wf[S % 2][i][1]);
-                const Wide xw = widen(xf[j % 2][0], xf[j % 2][1]);
-#pragma unroll
-                for (int i = 0; i < FO; i++) v[j % 2][i] = wide_mfma(ww[i], xw);
-            } else {
-#pragma unroll
-                for (int i = 0; i < FO; i++) v[j % 2][i] = f8_mfma(wf[S % 2][i][0], wf[S % 2][i][1], xf[j % 2][0], xf[j % 2][1]);
+                    for (int i = 0; i < FO; i++) ww[i] = widen(wf[i][0], wf[i][1]);
+                xw = widen(xf[j % XR][0], xf[j % XR][1]);
             }
-            add(std::integral_constant<int, 1>{}, (j + FT - 1) % FT, (j + 1) % 2);
+            f[j % XR] = sf[j % XR] * w;
+            each_of<0, FO>([&](auto ii) {
+                constexpr int i = decltype(ii)::value, m = j * FO + i;
+                if constexpr (WIDE) v[m % VR] = wide_mfma(ww[i], xw);
+                else v[m % VR] = f8_mfma(wf[i][0], wf[i][1], xf[j % XR][0], xf[j % XR][1]);
+                add((m + NM - LAG) % NM);
+                if constexpr (j == FT - 1) read_w(nb, i);
+            });
+            if constexpr (!WIDE) {
+#pragma unroll
+                for (int i = 0; i < FO; i++) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, j < FT - 1 ? 1 : 3, 0);
+                    if (past >= 0) __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
+                }
+            }
             __builtin_amdgcn_sched_barrier(0);
-        }
-        if ((++at & 63) == 0) wsc = Ws[min(k0 + at + lane, nkb - 1)];
+        });
+        if ((++at & 63) == 0) wsc = scales(at);
     };
-    each_of<0, NST>(issue);
+#pragma unroll
+    for (int m = 0; m < VR; m++) v[m] = k3_f32x4{0.f, 0.f, 0.f, 0.f}, f[m] = 0.0f;
+    issue_scales(0);
+    each_of<0, NST>([&](auto slot) {
+        issue_x(slot);
+        issue_w(slot);
+    });
     __builtin_amdgcn_s_waitcnt(WAIT_VM0);
     __syncthreads();
-    read_w(S0, wf[0]);
-    read_x(S0, 0, xf[0], sf[0]);
+#pragma unroll
+    for (int i = 0; i < FO; i++) read_w(S0, i);
+#pragma unroll
+    for (int j = 0; j < LA; j++) read_x(S0, j, 0);
     int left = n;
     for (; left >= NST; left -= NST) each_of<0, NST>(step);
     each_of<0, NST - 1>([&](auto slot) {
         if (decltype(slot)::value < left) step(slot);
     });
-    add(std::integral_constant<int, 0>{}, FT - 1, 1);
+    each_of<NM - LAG, NM>([&](auto m) { add(decltype(m)::value); });
 
     /* The sums go through LDS (the stage buffers, a region per wave, JR fragments of rows at a time; 16-byte column c of row r in
      * c ^ (r % 16)), so that a wave writes whole rows of its outputs, and the epilogue's code is there once. */
