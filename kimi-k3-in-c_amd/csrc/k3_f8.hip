@@ -23,6 +23,7 @@
 
 namespace {
 
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));     /* (a load of uint4 loses what tells LDS arrays apart) */
 constexpr uint32_t F8_OOB = 0x80000000u;        /* a buffer offset past any descriptor used here */
@@ -70,13 +71,26 @@ __device__ __forceinline__ k3_f32x4 wide_mfma(const Wide &w, const Wide &x)
     return v;
 }
 
-/* 4 bytes per lane from a buffer straight into LDS: lane L writes lds + 4 L */
-__device__ __forceinline__ void dma4(k3_rsrc r, void *lds, uint32_t voff, uint32_t soff)
+/* Requests from a buffer straight into LDS, 4 or 16 bytes a lane: lane L writes lds + 4 L or 16 L. As instructions of their own that the compiler does
+ * not count: it would have reads of the same array wait for all of them, also where they read what arrived long before. The caller
+ * waits, by count, before a barrier. (Raw buffer: what lies past `bytes` comes as zeros.) */
+__device__ __forceinline__ i32x4 f8_rsrc(const void *base, uint32_t bytes)
+{
+    const uint64_t b = (uint64_t)(uintptr_t)base;
+    return i32x4{__builtin_amdgcn_readfirstlane((int)b), __builtin_amdgcn_readfirstlane((int)(b >> 32)), __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000};
+}
+
+/* where an array lies in LDS (of the array itself: an address computed from it would be checked for null) */
+__device__ __forceinline__ uint32_t lds_at(uint32_t *lds) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint32_t *)lds; }
+
+template <int BYTES>
+__device__ __forceinline__ void f8_dma(i32x4 r, uint32_t at, uint32_t voff, uint32_t soff)
 {
 #if defined(__HIP_DEVICE_COMPILE__)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)lds, 4, voff, soff, 0, 0);
+    if constexpr (BYTES == 16) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(at), "v"(voff), "s"(r), "s"(soff) : "memory", "m0");
+    else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(at), "v"(voff), "s"(r), "s"(soff) : "memory", "m0");
 #else
-    (void)r; (void)lds; (void)voff; (void)soff;
+    (void)r; (void)at; (void)voff; (void)soff;
 #endif
 }
 
@@ -377,14 +391,88 @@ __device__ __forceinline__ bool tile_of(int nt, int no, int nsl, int b, int &tt,
     return true;
 }
 
+/* up to n of eight sums of a slice */
+__device__ __forceinline__ void part8(float *q, const float (&v)[8], int n)
+{
+    if (n >= 8) {
+        __builtin_memcpy(q, v, 32);
+    } else {
+#pragma unroll
+        for (int m = 0; m < 7; m++)
+            if (m < n) q[m] = v[m];
+    }
+}
+
+/* (one choice for the eight: the activation is the same for all) */
+template <bool F32>
+__device__ __forceinline__ void act8(float (&v)[8], int act)
+{
+    each_of<K3D_ACT_RELU, K3D_ACT_GELU_TANH + 1>([&](auto which) {
+        if (act == decltype(which)::value)
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = act_of<F32>(v[i], decltype(which)::value);
+    });
+}
+
+/* outputs o ..+8 of row t: v + bias b through the activation, plus the residual */
+__device__ __forceinline__ void put8(const K3kF8 &a, int t, int o, float (&v)[8], const float (&b)[8])
+{
+    if (t >= a.T || o >= a.out) return;
+    const bool bf = a.y_type == K3D_BF16;
+    if (o + 8 > a.out) {                /* (the end of a row) */
+        put4(a, t, o, make_float4(v[0], v[1], v[2], v[3]), *(const float(*)[4])b, res4(a, t, o));
+        put4(a, t, o + 4, make_float4(v[4], v[5], v[6], v[7]), *(const float(*)[4])(b + 4), res4(a, t, o + 4));
+        return;
+    }
+    uint4 r0, r1;
+    if (a.res) {
+        const char *q = (const char *)a.res + ((size_t)t * a.ldr + o) * (bf ? 2 : 4);
+        __builtin_memcpy(&r0, q, 16);
+        if (!bf) __builtin_memcpy(&r1, q + 16, 16);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] += b[i];
+    if (bf) act8<false>(v, a.act);
+    else act8<true>(v, a.act);
+    const size_t at = (size_t)t * a.ldy + o;
+    if (bf) {
+        if (a.res) {
+            const uint32_t w[4] = {r0.x, r0.y, r0.z, r0.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[2 * i] += __uint_as_float(w[i] << 16), v[2 * i + 1] += __uint_as_float(w[i] & 0xffff0000u);
+        }
+        __bf16 h[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) h[i] = (__bf16)v[i];
+        __builtin_memcpy((uint16_t *)a.y + at, h, 16);
+    } else {
+        if (a.res) {
+            const uint32_t w[8] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] += __uint_as_float(w[i]);
+        }
+        __builtin_memcpy((float *)a.y + at, v, 32);
+    }
+}
+
+/* the third and fourth stage, for kernels that have them (an array of their own each: that tells their accesses apart) */
+template <int S, int SZ>
+__device__ __forceinline__ uint32_t *stage_of()
+{
+    __shared__ __attribute__((aligned(1024))) uint32_t b[SZ];
+    return b;
+}
+
 template <int BT, int BO, int WT, int WO, int NST, bool WIDE>
 __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
 {
     constexpr int NW = WT * WO, FT = BT / WT / 16, FO = BO / WO / 16;
     constexpr int XD = BT / 8 / NW, WD = BO / 8 / NW, SD = (BT / 8 + NW - 1) / NW, DN = XD + WD;       /* requests of a wave: a step's, scales' */
     constexpr int SZ = (BT + BO) * 32, SC = SD * NW * 64;       /* a stage, the scales of 8 column blocks, in 4-byte units */
+    /* two barriers a step, which release half a stage each: where a DMA of the workgroup fills half of a wave's rows */
+    constexpr bool EARLY = NST == 2 && BT / WT == 2 * NW * 8 && FT == 8;
     static_assert(XD >= 1 && WD >= 1 && NST >= 2 && NST <= 4 && BO / WO <= 128 && (BO <= 128 || BO % 128 == 0), "tile");
-    __shared__ __attribute__((aligned(1024))) uint32_t S0[SZ], S1[SZ], S2[NST > 2 ? SZ : 4], S3[NST > 3 ? SZ : 4], SX[2 * SC];
+    __shared__ __attribute__((aligned(1024))) uint32_t S0[SZ], S1[SZ], SX[2 * SC], SO[SC];
 
     const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -406,11 +494,12 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
     /* Row r's 16-byte column c lies in slot c ^ (r / 2 % 8): the 16 rows of a fragment read fall on all 64 banks. */
     auto sw = [](int r) { return (r >> 1) & 7; };
     const size_t xbase = a.offsets ? 0 : (size_t)job.r0;        /* (dense: offsets from the tile's own rows) */
-    const k3_rsrc rx = k3_make_rsrc(a.x + xbase * a.ldx, F8_OOB), rs = k3_make_rsrc(a.xs + xbase * a.ldxs, F8_OOB);
+    const i32x4 rx = f8_rsrc(a.x + xbase * a.ldx, F8_OOB), rs = f8_rsrc(a.xs + xbase * a.ldxs, F8_OOB);
     const int rb = o0 / 128;
-    const k3_rsrc rw = k3_make_rsrc(a.W + (size_t)job.e * a.w_step + (size_t)rb * nkb * F8_KSTEP, (uint32_t)min((size_t)F8_OOB, (size_t)(blocks(a.out) - rb) * nkb * F8_KSTEP));
+    const uint32_t wbytes = (uint32_t)min(blocks(a.out) - rb, (BO + 127) / 128) * (uint32_t)nkb * F8_KSTEP;     /* of the tile's row blocks */
+    const i32x4 rw = f8_rsrc(a.W + (size_t)job.e * a.w_step + (size_t)rb * nkb * F8_KSTEP, wbytes);
     /* DMA i of wave wv fills rows 8 (NW i + wv) ..+8 of x, a lane a 16-byte slot; rows past the job's come as zeros */
-    uint32_t xo[XD], wof[WD], so[SD];
+    uint32_t xo[XD];
     auto row_at = [&](int r) -> int { return r < job.n ? (a.offsets ? x_row(a, job.r0 + r) : r) : -1; };
 #pragma unroll
     for (int i = 0; i < XD; i++) {
@@ -422,39 +511,32 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
 #pragma unroll
     for (int i = 0; i < SD; i++) {
         const int r = (i * NW + wv) * 8 + lane / 8, t = r < BT ? row_at(r) : -1;
-        so[i] = t < 0 ? F8_OOB : (uint32_t)t * (uint32_t)a.ldxs * 4;
+        SO[i * NW * 64 + tid] = t < 0 ? F8_OOB : (uint32_t)t * (uint32_t)a.ldxs * 4;     /* (read by the thread that wrote it) */
     }
-    /* W: the stage holds row tiles in their order, DMA i half tile NW i + wv */
-#pragma unroll
-    for (int i = 0; i < WD; i++) {
-        const int h = i * NW + wv, rt = o0 / 16 + h / 2, b = rt / F8_G - rb;
-        wof[i] = (uint32_t)b * (uint32_t)nkb * F8_KSTEP + (uint32_t)(rt % F8_G) * F8_TILE + (h & 1) * 1024 + lane * 16;
-    }
+    /* W: the stage holds row tiles in their order, DMA i half tile NW i + wv: where it lies, from the first tile's row block */
+    auto w_at = [&](int i) -> uint32_t {
+        const int h = i * NW + wv, rt = o0 / 16 + h / 2;
+        return (uint32_t)(rt / F8_G - rb) * (uint32_t)nkb * F8_KSTEP + (uint32_t)(rt % F8_G) * F8_TILE + (h & 1) * 1024;
+    };
     auto buf_of = [&](auto slot) -> uint32_t * {
         constexpr int S = decltype(slot)::value;
         if constexpr (S == 0) return S0;
         else if constexpr (S == 1) return S1;
-        else if constexpr (S == 2) return S2;
-        else return S3;
+        else return stage_of<S, SZ>();
     };
-    int kx = k0;
     const int kend = k0 + n;
-    auto issue_x = [&](auto slot) {
-        const uint32_t none = kx < kend ? 0u : F8_OOB;
-#pragma unroll
-        for (int i = 0; i < XD; i++) k3_dma16(rx, buf_of(slot) + (i * NW + wv) * 256, xo[i] | none, kx * 128);
+    auto issue_x = [&](auto slot, int i, int k) {
+        f8_dma<16>(rx, lds_at(buf_of(slot)) + (i * NW + wv) * 1024, xo[i] | (k < kend ? 0u : F8_OOB), k * 128);
     };
-    auto issue_w = [&](auto slot) {
-        const uint32_t none = kx < kend ? 0u : F8_OOB;
-#pragma unroll
-        for (int i = 0; i < WD; i++) k3_dma16(rw, buf_of(slot) + BT * 32 + (i * NW + wv) * 256, wof[i] | none, kx * F8_KSTEP);
-        kx++;
+    auto issue_w = [&](auto slot, int i, int k) {
+        const uint32_t at = w_at(i), none = k < kend && at < wbytes ? 0u : F8_OOB;
+        f8_dma<16>(rw, lds_at(buf_of(slot)) + (BT * 128 + (i * NW + wv) * 1024), (lane * 16) | none, none ? 0 : at + k * F8_KSTEP);
     };
     auto issue_scales = [&](int c) {            /* of blocks k0 + 8 c ..+8 */
         const int kb = k0 + 8 * c + ((lane & 7) ^ (wv & 1) * 4);
         static_assert(NW % 2 == 0, "a request's rows are 8 i + wv, their parity the wave's");
 #pragma unroll
-        for (int i = 0; i < SD; i++) dma4(rs, SX + (c & 1) * SC + (i * NW + wv) * 64, (so[i] + kb * 4) | (kb < nkb ? 0u : F8_OOB), 0);
+        for (int i = 0; i < SD; i++) f8_dma<4>(rs, lds_at(SX) + ((c & 1) * SC + (i * NW + wv) * 64) * 4, (SO[i * NW * 64 + tid] + kb * 4) | (kb < nkb ? 0u : F8_OOB), 0);
     };
     /* W's scales of the wave's outputs: a lane each, 64 column blocks at a time */
     const float *const Ws = a.Ws + (size_t)job.e * a.ws_step + (size_t)min((o0 + wo * (BO / WO)) / 128, blocks(a.out) - 1) * a.ldws;
@@ -474,16 +556,19 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
     const int xr = wt * (BT / WT) + r16;
     const int xa0 = xr * 32 + ((g ^ sw(xr)) & 7) * 4, xa1 = xr * 32 + (((4 + g) ^ sw(xr)) & 7) * 4;
     const int wa = BT * 32 + wo * (BO / WO) * 32 + lane * 4, sa = xr * 8 + ((r16 >> 3 & 1) * 4);
-    constexpr int WAITN = DN * (NST - 2);
-    constexpr int WAIT_STAGE = (WAITN & 15) | (7 << 4) | (0 << 8) | ((WAITN >> 4) << 14);       /* and LDS: none */
+    /* all but the youngest N requests, and LDS: none */
+    constexpr int WAITN = EARLY ? XD + WD : DN * (NST - 2);
+    constexpr int WAIT_STAGE = (WAITN & 15) | (7 << 4) | (0 << 8) | ((WAITN >> 4) << 14);
     constexpr int WAIT_VM0 = (7 << 4) | (15 << 8);
     static_assert(WAITN < 64, "requests in flight");
-    /* Step k: fragments of rows one after another, read three ahead. Once the last one's read has returned, every wave is past its
-     * reads of buffer k % NST and stage k + 1 has landed (one barrier, three fragments before the end), so stage k + NST goes into that
-     * buffer, and the next step's first rows and, behind their last use, fragments of W are read under the last rows' products. The scaled sums join the accumulators
+    /* Step k: fragments of rows one after another, read three ahead. Three fragments before the end the last one's read has returned: behind
+     * a barrier every wave is past its reads of buffer k % NST, and stage k + 1 has landed. So stage k + NST goes into that
+     * buffer, and the next step's first rows and, behind their last use, fragments of W are read under the last rows' products. With two stages a
+     * request would have a step's time to arrive (256 x 256: 550 of its 3110 cycles were waits for them); so there (EARLY) W's part and half the rows', which are in registers
+     * by fragment 1, go behind a barrier of their own then, and what the last fragments read is waited for at the next step's. The scaled sums join the accumulators
      * three products later: behind their own they would wait for it. */
     constexpr int XR = 4, LA = 3, VR = 4, LAG = 3, NM = FT * FO;
-    static_assert(NST % 2 == 0 && FT % XR == 0 && NM % VR == 0, "fragment rings");
+    static_assert(FT % XR == 0 && NM % VR == 0, "fragment rings");
     u32x4 wf[FO][2], xf[XR][2];
     Wide ww[WIDE ? FO : 1], xw;
     float sf[XR], f[XR];
@@ -512,14 +597,12 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
         const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wsc), at & 63));
         each_of<0, FT>([&](auto jj) {
             constexpr int j = decltype(jj)::value, past = j - (FT - LA);        /* fragments past the barrier (from 0 on) */
-            if constexpr (past == 0) {
+            if constexpr (past == 0 || (EARLY && j == 1)) {
                 /* (__syncthreads would wait for every request) */
                 __builtin_amdgcn_s_waitcnt(WAIT_STAGE);
                 asm volatile("s_barrier" ::: "memory");
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if constexpr (past == 0) issue_x(slot);
-            if constexpr (past == 1) issue_w(slot);
             if constexpr (past == 2)
                 if ((at & 7) == 0) issue_scales(at / 8 + 1);
             if constexpr (past < 0) {
@@ -540,16 +623,18 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
                 else v[m % VR] = f8_mfma(wf[i][0], wf[i][1], xf[j % XR][0], xf[j % XR][1]);
                 add((m + NM - LAG) % NM);
                 if constexpr (j == FT - 1) read_w(nb, i);
-            });
-            if constexpr (!WIDE) {
-#pragma unroll
-                for (int i = 0; i < FO; i++) {
-                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x100, j < FT - 1 ? 1 : 3, 0);
-                    if (past >= 0) __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
+                /* a request behind each product */
+                constexpr int q = EARLY ? (past >= 0 ? past * FO + i : (j - 1) * FO + i) : past * FO + i;
+                if constexpr (EARLY && past < 0 && q >= 0) {
+                    if constexpr (q < WD) issue_w(slot, q, k0 + at + NST);
+                    else if constexpr (q - WD < XD / 2) issue_x(slot, 2 * (q - WD), k0 + at + NST);
                 }
-            }
+                if constexpr (EARLY && past >= 0 && q < XD / 2) issue_x(slot, 2 * q + 1, k0 + at + NST);
+                if constexpr (!EARLY && q >= 0 && q < XD) issue_x(slot, q, k0 + at + NST);
+                if constexpr (!EARLY && q >= XD && q - XD < WD) issue_w(slot, q - XD, k0 + at + NST);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            static_assert(XD + WD <= LA * FO, "requests behind the products");
             __builtin_amdgcn_sched_barrier(0);
         });
         if ((++at & 63) == 0) wsc = scales(at);
@@ -558,8 +643,11 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
     for (int m = 0; m < VR; m++) v[m] = k3_f32x4{0.f, 0.f, 0.f, 0.f}, f[m] = 0.0f;
     issue_scales(0);
     each_of<0, NST>([&](auto slot) {
-        issue_x(slot);
-        issue_w(slot);
+        constexpr int S = decltype(slot)::value;
+#pragma unroll
+        for (int i = 0; i < XD; i++) issue_x(slot, i, k0 + S);
+#pragma unroll
+        for (int i = 0; i < WD; i++) issue_w(slot, i, k0 + S);
     });
     __builtin_amdgcn_s_waitcnt(WAIT_VM0);
     __syncthreads();
@@ -575,20 +663,20 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
     each_of<NM - LAG, NM>([&](auto m) { add(decltype(m)::value); });
 
     /* The sums go through LDS (the stage buffers, a region per wave, JR fragments of rows at a time; 16-byte column c of row r in
-     * c ^ (r % 16)), so that a wave writes whole rows of its outputs, and the epilogue's code is there once. */
+     * c ^ (r % 16)), so that a wave writes whole rows of its outputs, eight to a lane, and the epilogue's code is there once. */
     constexpr int WOUT = BO / WO, C = WOUT / 4;
     constexpr int RB1 = 16 * WOUT;              /* 4-byte units of one fragment of rows */
-    constexpr int JR = SZ / (FT * RB1) * NST >= NW ? FT : SZ / (FT / 2 * RB1) * NST >= NW ? FT / 2 : FT / 4;
+    constexpr int JR = SZ / (FT * RB1) * 2 >= NW ? FT : SZ / (FT / 2 * RB1) * 2 >= NW ? FT / 2 : FT / 4;
     constexpr int RB = JR * RB1, PER = SZ / RB;
-    static_assert(JR >= 1 && FT % JR == 0 && PER >= 1 && PER * NST >= NW && 64 % C == 0, "epilogue regions");
+    static_assert(JR >= 1 && FT % JR == 0 && PER >= 1 && PER * 2 >= NW && 128 % C == 0, "epilogue regions");
     uint32_t *stage = S0;
-    if (PER < NW) stage = wv / PER == 0 ? S0 : wv / PER == 1 ? S1 : wv / PER == 2 ? S2 : S3;
+    if (PER < NW) stage = wv / PER == 0 ? S0 : S1;
     float4 *const reg = reinterpret_cast<float4 *>(stage + (wv % PER) * RB);
-    const int c = lane % C, o = o0 + wo * WOUT + 4 * c;
-    constexpr int RI = 64 / C, IT = 16 * JR / RI;
-    const int row0 = wt * (BT / WT) + lane / C;
-    float bs[4];
-    bias4(a, p.nsl > 1 ? a.out : o, bs);
+    constexpr int RI = 128 / C, IT = 16 * JR / RI;              /* rows of a round of the wave, rounds */
+    const int c = lane % (C / 2), o = o0 + wo * WOUT + 8 * c, row0 = wt * (BT / WT) + lane / (C / 2);
+    float bs[8];
+    bias4(a, p.nsl > 1 ? a.out : o, *(float(*)[4])bs);
+    bias4(a, p.nsl > 1 ? a.out : o + 4, *(float(*)[4])(bs + 4));
     __builtin_amdgcn_s_waitcnt(WAIT_VM0);      /* the last requests land before LDS is used again */
     __syncthreads();
 #pragma unroll
@@ -603,22 +691,12 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
         __builtin_amdgcn_wave_barrier();
 #pragma unroll 2
         for (int i = 0; i < IT; i++) {
-            const int r = lane / C + i * RI, at = row0 + 16 * j0 + i * RI;
-            const float4 v = reg[r * C + (c ^ (r & 15 & (C - 1)))];
+            const int r = lane / (C / 2) + i * RI, at = row0 + 16 * j0 + i * RI, x = r & 15 & (C - 1);
+            const float4 v0 = reg[r * C + (2 * c ^ x)], v1 = reg[r * C + ((2 * c + 1) ^ x)];
+            float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
             const int t = at < job.n ? y_row(a, job.r0 + at) : a.T;
-            if (p.nsl == 1) {
-                put4(a, t, o, v, bs, res4(a, t, o));
-            } else if (t < a.T && o < a.out) {
-                float *q = p.part + ((size_t)sl * a.T + t) * a.out + o;
-                if (o + 4 <= a.out) {
-                    __builtin_memcpy(q, &v, 16);
-                } else {
-                    const float e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int m = 0; m < 3; m++)
-                        if (o + m < a.out) q[m] = e[m];
-                }
-            }
+            if (p.nsl == 1) put8(a, t, o, v, bs);
+            else if (t < a.T && o < a.out) part8(p.part + ((size_t)sl * a.T + t) * a.out + o, v, a.out - o);
         }
         __builtin_amdgcn_wave_barrier();
     }
