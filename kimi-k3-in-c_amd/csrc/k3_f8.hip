@@ -359,6 +359,12 @@ __global__ __launch_bounds__(64 * NW) void f8_stream_kernel(K3kF8 a, int o0, int
     if (a.offsets) {
         const int j = blockIdx.x / (unsigned)og;
         o -= j * og;
+        if (a.W2 && 2 * o >= og) {              /* the second matrix, its outputs behind the first's */
+            o -= og / 2;
+            a.W = a.W2;
+            a.Ws = a.Ws2;
+            a.y = (float *)a.y + a.out;
+        }
         job = find_job(a, count_jobs(a, 8 * NP), j, 8 * NP);
         if (job.n == 0) return;
     }
@@ -463,7 +469,9 @@ __device__ __forceinline__ uint32_t *stage_of()
     return b;
 }
 
-template <int BT, int BO, int WT, int WO, int NST, bool WIDE>
+/* PAIR: the tile is 128 rows of W (gate) and the same of W2 (up), a wave has 32 of both, and what leaves is act(gate) up in 8 bits: a
+ * row's 128 columns are one block of it, so its scale is the workgroup's own business. */
+template <int BT, int BO, int WT, int WO, int NST, bool WIDE, bool PAIR>
 __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
 {
     constexpr int NW = WT * WO, FT = BT / WT / 16, FO = BO / WO / 16;
@@ -471,6 +479,7 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
     constexpr int SZ = (BT + BO) * 32, SC = SD * NW * 64;       /* a stage, the scales of 8 column blocks, in 4-byte units */
     /* two barriers a step, which release half a stage each: where a DMA of the workgroup fills half of a wave's rows */
     constexpr bool EARLY = NST == 2 && BT / WT == 2 * NW * 8 && FT == 8;
+    static_assert(!PAIR || (BO == 256 && WO == 4 && WD % 2 == 0 && !WIDE), "a block of gate and one of up");
     static_assert(XD >= 1 && WD >= 1 && NST >= 2 && NST <= 4 && BO / WO <= 128 && (BO <= 128 || BO % 128 == 0), "tile");
     __shared__ __attribute__((aligned(1024))) uint32_t S0[SZ], S1[SZ], SX[2 * SC], SO[SC];
 
@@ -488,7 +497,7 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
         if (!tile_of(p.nt, p.no, p.nsl, blockIdx.x, tt, to, sl)) return;
         job = Job{0, tt * BT, min(BT, a.T - tt * BT)};
     }
-    const int o0 = to * BO, nkb = blocks(a.in);
+    const int o0 = to * (PAIR ? BO / 2 : BO), nkb = blocks(a.in);
     const int k0 = sl * p.per, n = min(p.per, nkb - k0);
 
     /* Row r's 16-byte column c lies in slot c ^ (r / 2 % 8): the 16 rows of a fragment read fall on all 64 banks. */
@@ -496,8 +505,9 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
     const size_t xbase = a.offsets ? 0 : (size_t)job.r0;        /* (dense: offsets from the tile's own rows) */
     const i32x4 rx = f8_rsrc(a.x + xbase * a.ldx, F8_OOB), rs = f8_rsrc(a.xs + xbase * a.ldxs, F8_OOB);
     const int rb = o0 / 128;
-    const uint32_t wbytes = (uint32_t)min(blocks(a.out) - rb, (BO + 127) / 128) * (uint32_t)nkb * F8_KSTEP;     /* of the tile's row blocks */
-    const i32x4 rw = f8_rsrc(a.W + (size_t)job.e * a.w_step + (size_t)rb * nkb * F8_KSTEP, wbytes);
+    const uint32_t wbytes = (uint32_t)min(blocks(a.out) - rb, PAIR ? 1 : (BO + 127) / 128) * (uint32_t)nkb * F8_KSTEP;     /* of the tile's row blocks */
+    const size_t wfrom = (size_t)job.e * a.w_step + (size_t)rb * nkb * F8_KSTEP;
+    const i32x4 rw = f8_rsrc(a.W + wfrom, wbytes), rw2 = PAIR ? f8_rsrc(a.W2 + wfrom, wbytes) : rw;
     /* DMA i of wave wv fills rows 8 (NW i + wv) ..+8 of x, a lane a 16-byte slot; rows past the job's come as zeros */
     uint32_t xo[XD];
     auto row_at = [&](int r) -> int { return r < job.n ? (a.offsets ? x_row(a, job.r0 + r) : r) : -1; };
@@ -515,7 +525,7 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
     }
     /* W: the stage holds row tiles in their order, DMA i half tile NW i + wv: where it lies, from the first tile's row block */
     auto w_at = [&](int i) -> uint32_t {
-        const int h = i * NW + wv, rt = o0 / 16 + h / 2;
+        const int h = i * NW + wv, rt = o0 / 16 + (PAIR ? h / 2 % F8_G : h / 2);
         return (uint32_t)(rt / F8_G - rb) * (uint32_t)nkb * F8_KSTEP + (uint32_t)(rt % F8_G) * F8_TILE + (h & 1) * 1024;
     };
     auto buf_of = [&](auto slot) -> uint32_t * {
@@ -530,7 +540,7 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
     };
     auto issue_w = [&](auto slot, int i, int k) {
         const uint32_t at = w_at(i), none = k < kend && at < wbytes ? 0u : F8_OOB;
-        f8_dma<16>(rw, lds_at(buf_of(slot)) + (BT * 128 + (i * NW + wv) * 1024), (lane * 16) | none, none ? 0 : at + k * F8_KSTEP);
+        f8_dma<16>(PAIR && i >= WD / 2 ? rw2 : rw, lds_at(buf_of(slot)) + (BT * 128 + (i * NW + wv) * 1024), (lane * 16) | none, none ? 0 : at + k * F8_KSTEP);
     };
     auto issue_scales = [&](int c) {            /* of blocks k0 + 8 c ..+8 */
         const int kb = k0 + 8 * c + ((lane & 7) ^ (wv & 1) * 4);
@@ -539,14 +549,14 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
         for (int i = 0; i < SD; i++) f8_dma<4>(rs, lds_at(SX) + ((c & 1) * SC + (i * NW + wv) * 64) * 4, (SO[i * NW * 64 + tid] + kb * 4) | (kb < nkb ? 0u : F8_OOB), 0);
     };
     /* W's scales of the wave's outputs: a lane each, 64 column blocks at a time */
-    const float *const Ws = a.Ws + (size_t)job.e * a.ws_step + (size_t)min((o0 + wo * (BO / WO)) / 128, blocks(a.out) - 1) * a.ldws;
+    const size_t sfrom = (size_t)job.e * a.ws_step + (size_t)(PAIR ? rb : min((o0 + wo * (BO / WO)) / 128, blocks(a.out) - 1)) * a.ldws;
     /* (arrived when it returns: a wait at its use would be one for every request since) */
-    auto scales = [&](int i) {
-        float v = Ws[min(k0 + i + lane, nkb - 1)];
+    auto scales = [&](const float *Ws, int i) {
+        float v = Ws[sfrom + min(k0 + i + lane, nkb - 1)];
         asm volatile("" : "+v"(v));
         return v;
     };
-    float wsc = scales(0);
+    float wsc = scales(a.Ws, 0), wsc2 = PAIR ? scales(a.Ws2, 0) : 0.0f;
 
     k3_f32x4 acc[FO][FT];
 #pragma unroll
@@ -555,7 +565,7 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
         for (int j = 0; j < FT; j++) acc[i][j] = k3_f32x4{0.f, 0.f, 0.f, 0.f};
     const int xr = wt * (BT / WT) + r16;
     const int xa0 = xr * 32 + ((g ^ sw(xr)) & 7) * 4, xa1 = xr * 32 + (((4 + g) ^ sw(xr)) & 7) * 4;
-    const int wa = BT * 32 + wo * (BO / WO) * 32 + lane * 4, sa = xr * 8 + ((r16 >> 3 & 1) * 4);
+    const int wa = BT * 32 + wo * (BO / WO) * (PAIR ? 16 : 32) + lane * 4, sa = xr * 8 + ((r16 >> 3 & 1) * 4);
     /* all but the youngest N requests, and LDS: none */
     constexpr int WAITN = EARLY ? XD + WD : DN * (NST - 2);
     constexpr int WAIT_STAGE = (WAITN & 15) | (7 << 4) | (0 << 8) | ((WAITN >> 4) << 14);
@@ -567,15 +577,16 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
      * request would have a step's time to arrive (256 x 256: 550 of its 3110 cycles were waits for them); so there (EARLY) W's part and half the rows', which are in registers
      * by fragment 1, go behind a barrier of their own then, and what the last fragments read is waited for at the next step's. The scaled sums join the accumulators
      * three products later: behind their own they would wait for it. */
-    constexpr int XR = 4, LA = 3, VR = 4, LAG = 3, NM = FT * FO;
+    constexpr int XR = 4, LA = 3, VR = 4, LAG = 3, NM = FT * FO, FR = 2;
+    static_assert(FO > LAG, "scales of two fragments");
     static_assert(FT % XR == 0 && NM % VR == 0, "fragment rings");
     u32x4 wf[FO][2], xf[XR][2];
     Wide ww[WIDE ? FO : 1], xw;
-    float sf[XR], f[XR];
+    float sf[XR], f[FR], f2[FR];
     k3_f32x4 v[VR];
     auto read_w = [&](const uint32_t *b, int i) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) wf[i][h] = *reinterpret_cast<const u32x4 *>(b + wa + i * 512 + h * 256);
+        for (int h = 0; h < 2; h++) wf[i][h] = *reinterpret_cast<const u32x4 *>(b + wa + (PAIR ? i / 2 * F8_G * 512 + i % 2 * 512 : i * 512) + h * 256);
     };
     auto read_x = [&](const uint32_t *b, int j, int k) {        /* of the k-th block */
         xf[j % XR][0] = *reinterpret_cast<const u32x4 *>(b + xa0 + j * 512);
@@ -585,7 +596,7 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
     auto add = [&](int m) {
         const int i = m % FO, j = m / FO;
 #pragma unroll
-        for (int e = 0; e < 4; e++) acc[i][j][e] = fmaf(f[j % XR], v[m % VR][e], acc[i][j][e]);
+        for (int e = 0; e < 4; e++) acc[i][j][e] = fmaf(PAIR && i >= FO / 2 ? f2[j % FR] : f[j % FR], v[m % VR][e], acc[i][j][e]);
         /* (formed here: the compiler would put all of them off, and hold the products) */
         asm volatile("" : "+v"(acc[i][j]));
     };
@@ -595,6 +606,7 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
         const uint32_t *const b = buf_of(slot);
         const uint32_t *const nb = buf_of(std::integral_constant<int, (S + 1) % NST>{});
         const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wsc), at & 63));
+        const float w2 = PAIR ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wsc2), at & 63)) : 0.0f;
         each_of<0, FT>([&](auto jj) {
             constexpr int j = decltype(jj)::value, past = j - (FT - LA);        /* fragments past the barrier (from 0 on) */
             if constexpr (past == 0 || (EARLY && j == 1)) {
@@ -616,7 +628,8 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
                     for (int i = 0; i < FO; i++) ww[i] = widen(wf[i][0], wf[i][1]);
                 xw = widen(xf[j % XR][0], xf[j % XR][1]);
             }
-            f[j % XR] = sf[j % XR] * w;
+            f[j % FR] = sf[j % XR] * w;
+            if (PAIR) f2[j % FR] = sf[j % XR] * w2;
             each_of<0, FO>([&](auto ii) {
                 constexpr int i = decltype(ii)::value, m = j * FO + i;
                 if constexpr (WIDE) v[m % VR] = wide_mfma(ww[i], xw);
@@ -637,10 +650,13 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
             static_assert(XD + WD <= LA * FO, "requests behind the products");
             __builtin_amdgcn_sched_barrier(0);
         });
-        if ((++at & 63) == 0) wsc = scales(at);
+        if ((++at & 63) == 0) {
+            wsc = scales(a.Ws, at);
+            if (PAIR) wsc2 = scales(a.Ws2, at);
+        }
     };
 #pragma unroll
-    for (int m = 0; m < VR; m++) v[m] = k3_f32x4{0.f, 0.f, 0.f, 0.f}, f[m] = 0.0f;
+    for (int m = 0; m < VR; m++) v[m] = k3_f32x4{0.f, 0.f, 0.f, 0.f}, f[m % FR] = f2[m % FR] = 0.0f;
     issue_scales(0);
     each_of<0, NST>([&](auto slot) {
         constexpr int S = decltype(slot)::value;
@@ -662,6 +678,53 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
     });
     each_of<NM - LAG, NM>([&](auto m) { add(decltype(m)::value); });
 
+    if constexpr (PAIR) {
+        const float r1 = 1.0f / a.b1, r2 = 1.0f / a.b2;
+        auto glu = [&](auto act) {              /* in the gate's place */
+#pragma unroll
+            for (int j = 0; j < FT; j++)
+#pragma unroll
+                for (int i = 0; i < FO / 2; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[i][j][e] = glu_of(acc[i][j][e], acc[i + FO / 2][j][e], decltype(act)::value, a.b1, a.b2, r1, r2);
+        };
+        if (a.glu == K3D_GLU_SILU) glu(std::integral_constant<int, K3D_GLU_SILU>{});
+        else glu(std::integral_constant<int, K3D_GLU_SITU>{});
+        __builtin_amdgcn_s_waitcnt(WAIT_VM0);  /* the last requests land before LDS is used again */
+        __syncthreads();
+        /* a row's largest magnitude: of the lane's eight columns, the wave's 32, the four waves' */
+        static_assert(2 * SC >= 4 * BT, "largest magnitudes");
+#pragma unroll
+        for (int j = 0; j < FT; j++) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < FO / 2; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) m = max(m, abs_bits(acc[i][j][e]));
+            m = max(m, (uint32_t)__shfl_xor((int)m, 16));
+            m = max(m, (uint32_t)__shfl_xor((int)m, 32));
+            if (g == 0) SX[(xr + 16 * j) * 4 + wo] = m;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < FT; j++) {
+            const int r = xr + 16 * j;
+            const uint4 m = *reinterpret_cast<const uint4 *>(SX + r * 4);
+            const float sc = f8_scale(max(max(m.x, m.y), max(m.z, m.w))), inv = 1.0f / sc;
+            if (wo == 0 && g == 0 && r < job.n) a.hs[(size_t)(job.r0 + r) * blocks(a.out) + to] = sc;
+            /* codes 32 wo + 16 i + 4 g ..+4: 16-byte column 2 wo + i of the row, swizzled as x's */
+#pragma unroll
+            for (int i = 0; i < FO / 2; i++)
+                S0[r * 32 + ((2 * wo + i) ^ sw(r)) * 4 + g] = f8_codes(acc[i][j][0] * inv, acc[i][j][1] * inv, acc[i][j][2] * inv, acc[i][j][3] * inv);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < BT / 8 / NW; i++) {
+            const int r = (i * NW + wv) * 8 + lane / 8, c = lane & 7;
+            if (r < job.n) *reinterpret_cast<u32x4 *>(a.hq + (size_t)(job.r0 + r) * blocks(a.out) * 128 + to * 128 + c * 16) = *reinterpret_cast<const u32x4 *>(S0 + r * 32 + (c ^ sw(r)) * 4);
+        }
+        return;
+    }
     /* The sums go through LDS (the stage buffers, a region per wave, JR fragments of rows at a time; 16-byte column c of row r in
      * c ^ (r % 16)), so that a wave writes whole rows of its outputs, eight to a lane, and the epilogue's code is there once. */
     constexpr int WOUT = BO / WO, C = WOUT / 4;
@@ -751,10 +814,10 @@ template <int RW, int NP, int U, int NW>
 void stream_launch(const K3kF8 *a, long jobs, hipStream_t st)
 {
     /* (a launch takes under 2^32 work-items) */
-    const long og = ((a->out + 15) / 16 + RW - 1) / RW, most = ((1L << 32) - 1) / (64 * NW) / jobs;
+    const long og = ((a->out + 15) / 16 + RW - 1) / RW, mats = a->W2 ? 2 : 1, most = ((1L << 32) - 1) / (64 * NW) / (jobs * mats);
     for (long o = 0; o < og; o += most) {
-        const int n = (int)(og - o < most ? og - o : most);
-        if (a->y_type == K3D_F32) f8_stream_kernel<RW, NP, U, NW, K3_LD_NT, true><<<(unsigned)(jobs * n), 64 * NW, 0, st>>>(*a, (int)o, n);
+        const int n = (int)(og - o < most ? og - o : most) * mats;
+        if (a->wide) f8_stream_kernel<RW, NP, U, NW, K3_LD_NT, true><<<(unsigned)(jobs * n), 64 * NW, 0, st>>>(*a, (int)o, n);
         else f8_stream_kernel<RW, NP, U, NW, K3_LD_NT, false><<<(unsigned)(jobs * n), 64 * NW, 0, st>>>(*a, (int)o, n);
     }
 }
@@ -778,16 +841,16 @@ void stream(const K3kF8 *a, int rows, hipStream_t st)
     else stream_go<2, 8, 2>(a, st);
 }
 
-template <int BT, int BO, int WT, int WO, int NST, bool WIDE = false>
+template <int BT, int BO, int WT, int WO, int NST, bool WIDE = false, bool PAIR = false>
 void tile_go(F8Tile *p, int nsl, hipStream_t st)
 {
     const int nkb = blocks(p->a.in);
     p->nt = (p->a.T + BT - 1) / BT;
-    p->no = (p->a.out + BO - 1) / BO;
+    p->no = PAIR ? blocks(p->a.out) : (p->a.out + BO - 1) / BO;
     p->per = (nkb + nsl - 1) / nsl;
     p->nsl = (nkb + p->per - 1) / p->per;
     const long grid = (p->a.offsets ? most_jobs(&p->a, BT) : (long)p->nt) * p->no * p->nsl;
-    f8_tile_kernel<BT, BO, WT, WO, NST, WIDE><<<(unsigned)grid, 64 * WT * WO, 0, st>>>(*p);
+    f8_tile_kernel<BT, BO, WT, WO, NST, WIDE, PAIR><<<(unsigned)grid, 64 * WT * WO, 0, st>>>(*p);
 }
 
 }  // namespace
@@ -826,13 +889,13 @@ extern "C" int k3k_linear_f8(const K3kF8 *a, void *stream_)
     const long cus = k3k_cu_count();
     const int nkb = blocks(a->in);
     const long tiles = (long)((a->T + 255) / 256) * ((a->out + 255) / 256);
-    if (tiles >= cus && a->y_type == K3D_BF16) {
+    if (tiles >= cus && !a->wide) {
         tile_go<256, 256, 2, 4, 2>(&p, 1, st);
     } else {
         const long small = (long)((a->T + 127) / 128) * ((a->out + 127) / 128);
         int nsl = 1;
         while (nsl < F8_MAX_SLICES && small * nsl * 2 <= cus && nkb >= 4 * nsl && (size_t)2 * nsl * a->T * a->out * 4 <= part_bytes(a->T, a->out)) nsl *= 2;
-        if (a->y_type == K3D_F32) tile_go<128, 128, 2, 2, 4, true>(&p, nsl, st);
+        if (a->wide) tile_go<128, 128, 2, 2, 4, true>(&p, nsl, st);
         else tile_go<128, 128, 2, 2, 4>(&p, nsl, st);
     }
     K3K_LAUNCH_CHECK("linear_f8: tiles");
@@ -856,9 +919,31 @@ extern "C" int k3k_grouped_f8(const K3kF8 *a, void *stream_)
     F8Tile p;
     p.a = *a;
     p.part = NULL;
-    if (a->y_type == K3D_F32) tile_go<128, 128, 2, 2, 4, true>(&p, 1, st);
+    if (a->wide) tile_go<128, 128, 2, 2, 4, true>(&p, 1, st);
     else if (each <= 128) tile_go<128, 128, 2, 2, 4>(&p, 1, st);
     else tile_go<256, 256, 2, 4, 2>(&p, 1, st);
     K3K_LAUNCH_CHECK("grouped_f8: tiles");
     return 0;
+}
+
+/* gate and up: W, W2 [experts], into hq / hs; gu: room for their sums, where few rows make them a launch of their own */
+extern "C" int k3k_gateup_f8(const K3kF8 *a, float *gu, void *stream_)
+{
+    hipStream_t st = (hipStream_t)stream_;
+    const int each = (a->rows + a->n_experts - 1) / a->n_experts;
+    if (each > 48) {
+        F8Tile p;
+        p.a = *a;
+        p.part = NULL;
+        tile_go<256, 256, 2, 4, 2, false, true>(&p, 1, st);
+        K3K_LAUNCH_CHECK("gateup_f8");
+        return 0;
+    }
+    K3kF8 s = *a;
+    s.y = gu;
+    s.ldy = 2L * a->out;
+    s.T = a->rows;
+    if (k3k_grouped_f8(&s, stream_)) return -1;
+    K3kQuant q = {a->hq, a->hs, gu, blocks(a->out) * 128L, blocks(a->out), 2L * a->out, K3D_F32, a->rows, a->out, a->glu, a->b1, a->b2};
+    return k3k_quant_f8(&q, stream_);
 }

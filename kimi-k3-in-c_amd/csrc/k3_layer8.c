@@ -212,6 +212,7 @@ int k3d_linear_f8(void *y, int y_type, long ldy, const uint8_t *x, long ldx, con
     a.out = out;
     a.act = act;
     a.ws = ws;
+    a.wide = y_type == K3D_F32;
     k3k_prof_mark(stream, K3D_STAGE_BEGIN);
     if (k3k_linear_f8(&a, stream)) return fail(fn);
     k3k_prof_mark(stream, K3D_STAGE_GEMV);
@@ -298,6 +299,7 @@ int k3d_grouped_f8(void *y, int y_type, long ldy, const int *y_rows, int y_cap, 
     a.x_div = x_div;
     a.x_cap = x_cap;
     a.n_experts = n_experts;
+    a.wide = y_type == K3D_F32;
     k3k_prof_mark(stream, K3D_STAGE_BEGIN);
     if (k3k_grouped_f8(&a, stream)) return fail(fn);
     k3k_prof_mark(stream, K3D_STAGE_GATEUP);
@@ -373,14 +375,14 @@ int k3d_moe_f8(void *out, int out_type, long ldo, const int *idx, const float *w
     k3k_prof_mark(stream, K3D_STAGE_GATHER);
     K3kF8 a;
     memset(&a, 0, sizeof a);
-    a.y = w.gu;
     a.x = x;
     a.W = w1;
+    a.W2 = w3;
     a.xs = xs;
     a.Ws = s1;
+    a.Ws2 = s3;
     a.offsets = w.offsets;
     a.x_rows = w.perm;
-    a.ldy = 2L * inter;
     a.ldx = ldx;
     a.ldxs = ldxs;
     a.ldws = blocks(hidden);
@@ -394,36 +396,25 @@ int k3d_moe_f8(void *out, int out_type, long ldo, const int *idx, const float *w
     a.x_div = topk;
     a.x_cap = T;
     a.n_experts = n_experts;
-    if (k3k_grouped_f8(&a, stream)) return fail(fn);
-    a.y = w.gu + inter;
-    a.W = w3;
-    a.Ws = s3;
-    if (k3k_grouped_f8(&a, stream)) return fail(fn);
-    K3kQuant h;
-    h.q = w.hq;
-    h.qs = w.hs;
-    h.x = w.gu;
-    h.ldq = blocks(inter) * 128L;
-    h.ldqs = blocks(inter);
-    h.ldx = 2L * inter;
-    h.x_type = K3D_F32;
-    h.T = N;
-    h.n = inter;
-    h.act = act;
-    h.b1 = b1;
-    h.b2 = b2;
-    if (k3k_quant_f8(&h, stream)) return fail(fn);
+    a.hq = w.hq;
+    a.hs = w.hs;
+    a.glu = act;
+    a.b1 = b1;
+    a.b2 = b2;
+    if (k3k_gateup_f8(&a, w.gu, stream)) return fail(fn);
     k3k_prof_mark(stream, K3D_STAGE_GATEUP);
     a.y = w.y;
     a.x = w.hq;
     a.W = w2;
+    a.W2 = NULL;
+    a.wide = out_type == K3D_F32;       /* (a result of bf16 has no use for more than 8-bit instructions give) */
     a.xs = w.hs;
     a.Ws = s2;
     a.x_rows = NULL;
     a.y_rows = w.perm;
     a.ldy = hidden;
-    a.ldx = h.ldq;
-    a.ldxs = h.ldqs;
+    a.ldx = blocks(inter) * 128L;
+    a.ldxs = blocks(inter);
     a.ldws = blocks(inter);
     a.w_step = k3k_f8_tiled_bytes(hidden, inter);
     a.ws_step = (size_t)blocks(hidden) * blocks(inter);

@@ -409,12 +409,22 @@ typedef struct {
     size_t w_step, ws_step;
     int y_type, T, in, out, act, rows, x_div, x_cap, n_experts;
     void *ws;
+    int wide;                   /* products as exact as fp32 (else 8-bit instructions) */
+    /* k3k_gateup_f8 */
+    const uint8_t *W2;
+    const float *Ws2;
+    uint8_t *hq;                /* [rows][whole blocks], scales [rows][blocks] */
+    float *hs;
+    int glu;
+    float b1, b2;
 } K3kF8;
 size_t k3k_f8_tiled_bytes(int rows, int in);
 int k3k_f8_tile(uint8_t *t, const uint8_t *W, long ldw, int rows, int in, int mats, void *stream);
 size_t k3k_linear_f8_ws(int T, int in, int out);
 int k3k_linear_f8(const K3kF8 *a, void *stream);
 int k3k_grouped_f8(const K3kF8 *a, void *stream);
+/* act(W x) (W2 x) of sorted rows in 8 bits; gu: [rows][2 out] of scratch. */
+int k3k_gateup_f8(const K3kF8 *a, float *gu, void *stream);
 
 /* The slots of idx [N] by expert (k3_group.hip; up to 2048 experts); hist: k3k_group_ws bytes. */
 size_t k3k_group_ws(int N, int n_experts);
