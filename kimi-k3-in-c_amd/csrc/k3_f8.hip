@@ -461,18 +461,13 @@ __device__ __forceinline__ void put8(const K3kF8 &a, int t, int o, float (&v)[8]
     }
 }
 
-/* the third and fourth stage, for kernels that have them (an array of their own each: that tells their accesses apart) */
-template <int S, int SZ>
-__device__ __forceinline__ uint32_t *stage_of()
-{
-    __shared__ __attribute__((aligned(1024))) uint32_t b[SZ];
-    return b;
-}
+/* bytes of LDS: the stages, the scales of x for 16 column blocks, and where each row's lie */
+constexpr int tile_lds(int bt, int bo, int nw, int nst) { return nst * (bt + bo) * 128 + 3 * ((bt / 8 + nw - 1) / nw * nw) * 256; }
 
 /* PAIR: the tile is 128 rows of W (gate) and the same of W2 (up), a wave has 32 of both, and what leaves is act(gate) up in 8 bits: a
  * row's 128 columns are one block of it, so its scale is the workgroup's own business. */
 template <int BT, int BO, int WT, int WO, int NST, bool WIDE, bool PAIR>
-__global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
+__device__ __forceinline__ void tile_run(const F8Tile &p, const Job &job, int to, int sl, uint32_t *lds)
 {
     constexpr int NW = WT * WO, FT = BT / WT / 16, FO = BO / WO / 16;
     constexpr int XD = BT / 8 / NW, WD = BO / 8 / NW, SD = (BT / 8 + NW - 1) / NW, DN = XD + WD;       /* requests of a wave: a step's, scales' */
@@ -481,22 +476,13 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
     constexpr bool EARLY = NST == 2 && BT / WT == 2 * NW * 8 && FT == 8;
     static_assert(!PAIR || (BO == 256 && WO == 4 && WD % 2 == 0 && !WIDE), "a block of gate and one of up");
     static_assert(XD >= 1 && WD >= 1 && NST >= 2 && NST <= 4 && BO / WO <= 128 && (BO <= 128 || BO % 128 == 0), "tile");
-    __shared__ __attribute__((aligned(1024))) uint32_t S0[SZ], S1[SZ], SX[2 * SC], SO[SC];
+    static_assert((NST * SZ + 3 * SC) * 4 <= tile_lds(BT, BO, NW, NST), "LDS");
+    uint32_t *const SX = lds + NST * SZ, *const SO = SX + 2 * SC;
 
     const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wt = wv % WT, wo = wv / WT;
     const K3kF8 &a = p.a;
-    int tt, to, sl;
-    Job job;
-    if (a.offsets) {
-        const Jobs s = count_jobs(a, BT);
-        if (!tile_of(s.total, p.no, 1, blockIdx.x, tt, to, sl)) return;
-        job = find_job(a, s, tt, BT);
-    } else {
-        if (!tile_of(p.nt, p.no, p.nsl, blockIdx.x, tt, to, sl)) return;
-        job = Job{0, tt * BT, min(BT, a.T - tt * BT)};
-    }
     const int o0 = to * (PAIR ? BO / 2 : BO), nkb = blocks(a.in);
     const int k0 = sl * p.per, n = min(p.per, nkb - k0);
 
@@ -528,25 +514,21 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
         const int h = i * NW + wv, rt = o0 / 16 + (PAIR ? h / 2 % F8_G : h / 2);
         return (uint32_t)(rt / F8_G - rb) * (uint32_t)nkb * F8_KSTEP + (uint32_t)(rt % F8_G) * F8_TILE + (h & 1) * 1024;
     };
-    auto buf_of = [&](auto slot) -> uint32_t * {
-        constexpr int S = decltype(slot)::value;
-        if constexpr (S == 0) return S0;
-        else if constexpr (S == 1) return S1;
-        else return stage_of<S, SZ>();
-    };
+    auto buf_of = [&](auto slot) -> uint32_t * { return lds + decltype(slot)::value * SZ; };
+    const uint32_t base = lds_at(lds);
     const int kend = k0 + n;
     auto issue_x = [&](auto slot, int i, int k) {
-        f8_dma<16>(rx, lds_at(buf_of(slot)) + (i * NW + wv) * 1024, xo[i] | (k < kend ? 0u : F8_OOB), k * 128);
+        f8_dma<16>(rx, base + decltype(slot)::value * SZ * 4 + (i * NW + wv) * 1024, xo[i] | (k < kend ? 0u : F8_OOB), k * 128);
     };
     auto issue_w = [&](auto slot, int i, int k) {
         const uint32_t at = w_at(i), none = k < kend && at < wbytes ? 0u : F8_OOB;
-        f8_dma<16>(PAIR && i >= WD / 2 ? rw2 : rw, lds_at(buf_of(slot)) + (BT * 128 + (i * NW + wv) * 1024), (lane * 16) | none, none ? 0 : at + k * F8_KSTEP);
+        f8_dma<16>(PAIR && i >= WD / 2 ? rw2 : rw, base + decltype(slot)::value * SZ * 4 + BT * 128 + (i * NW + wv) * 1024, (lane * 16) | none, none ? 0 : at + k * F8_KSTEP);
     };
     auto issue_scales = [&](int c) {            /* of blocks k0 + 8 c ..+8 */
         const int kb = k0 + 8 * c + ((lane & 7) ^ (wv & 1) * 4);
         static_assert(NW % 2 == 0, "a request's rows are 8 i + wv, their parity the wave's");
 #pragma unroll
-        for (int i = 0; i < SD; i++) f8_dma<4>(rs, lds_at(SX) + ((c & 1) * SC + (i * NW + wv) * 64) * 4, (SO[i * NW * 64 + tid] + kb * 4) | (kb < nkb ? 0u : F8_OOB), 0);
+        for (int i = 0; i < SD; i++) f8_dma<4>(rs, base + (NST * SZ + (c & 1) * SC + (i * NW + wv) * 64) * 4, (SO[i * NW * 64 + tid] + kb * 4) | (kb < nkb ? 0u : F8_OOB), 0);
     };
     /* W's scales of the wave's outputs: a lane each, 64 column blocks at a time */
     const size_t sfrom = (size_t)job.e * a.ws_step + (size_t)(PAIR ? rb : min((o0 + wo * (BO / WO)) / 128, blocks(a.out) - 1)) * a.ldws;
@@ -668,9 +650,9 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
     __builtin_amdgcn_s_waitcnt(WAIT_VM0);
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < FO; i++) read_w(S0, i);
+    for (int i = 0; i < FO; i++) read_w(lds, i);
 #pragma unroll
-    for (int j = 0; j < LA; j++) read_x(S0, j, 0);
+    for (int j = 0; j < LA; j++) read_x(lds, j, 0);
     int left = n;
     for (; left >= NST; left -= NST) each_of<0, NST>(step);
     each_of<0, NST - 1>([&](auto slot) {
@@ -715,13 +697,13 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
             /* codes 32 wo + 16 i + 4 g ..+4: 16-byte column 2 wo + i of the row, swizzled as x's */
 #pragma unroll
             for (int i = 0; i < FO / 2; i++)
-                S0[r * 32 + ((2 * wo + i) ^ sw(r)) * 4 + g] = f8_codes(acc[i][j][0] * inv, acc[i][j][1] * inv, acc[i][j][2] * inv, acc[i][j][3] * inv);
+                lds[r * 32 + ((2 * wo + i) ^ sw(r)) * 4 + g] = f8_codes(acc[i][j][0] * inv, acc[i][j][1] * inv, acc[i][j][2] * inv, acc[i][j][3] * inv);
         }
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < BT / 8 / NW; i++) {
             const int r = (i * NW + wv) * 8 + lane / 8, c = lane & 7;
-            if (r < job.n) *reinterpret_cast<u32x4 *>(a.hq + (size_t)(job.r0 + r) * blocks(a.out) * 128 + to * 128 + c * 16) = *reinterpret_cast<const u32x4 *>(S0 + r * 32 + (c ^ sw(r)) * 4);
+            if (r < job.n) *reinterpret_cast<u32x4 *>(a.hq + (size_t)(job.r0 + r) * blocks(a.out) * 128 + to * 128 + c * 16) = *reinterpret_cast<const u32x4 *>(lds + r * 32 + (c ^ sw(r)) * 4);
         }
         return;
     }
@@ -729,12 +711,10 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
      * c ^ (r % 16)), so that a wave writes whole rows of its outputs, eight to a lane, and the epilogue's code is there once. */
     constexpr int WOUT = BO / WO, C = WOUT / 4;
     constexpr int RB1 = 16 * WOUT;              /* 4-byte units of one fragment of rows */
-    constexpr int JR = SZ / (FT * RB1) * 2 >= NW ? FT : SZ / (FT / 2 * RB1) * 2 >= NW ? FT / 2 : FT / 4;
-    constexpr int RB = JR * RB1, PER = SZ / RB;
-    static_assert(JR >= 1 && FT % JR == 0 && PER >= 1 && PER * 2 >= NW && 128 % C == 0, "epilogue regions");
-    uint32_t *stage = S0;
-    if (PER < NW) stage = wv / PER == 0 ? S0 : S1;
-    float4 *const reg = reinterpret_cast<float4 *>(stage + (wv % PER) * RB);
+    constexpr int LR = NST * SZ / NW;           /* of a wave's region */
+    constexpr int JR = LR >= FT * RB1 ? FT : LR >= FT / 2 * RB1 ? FT / 2 : FT / 4, RB = JR * RB1;
+    static_assert(JR >= 1 && FT % JR == 0 && RB <= LR && 128 % C == 0, "epilogue regions");
+    float4 *const reg = reinterpret_cast<float4 *>(lds + wv * RB);
     constexpr int RI = 128 / C, IT = 16 * JR / RI;              /* rows of a round of the wave, rounds */
     const int c = lane % (C / 2), o = o0 + wo * WOUT + 8 * c, row0 = wt * (BT / WT) + lane / (C / 2);
     float bs[8];
@@ -763,6 +743,29 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
         }
         __builtin_amdgcn_wave_barrier();
     }
+}
+
+/* DUAL: passes of at most half the rows by a kernel of half the rows and three stages, which takes little over half the time (2048 tokens, eight of 64
+ * experts each: half of the experts have a pass of some 16 rows behind one of 256) */
+template <int BT, int BO, int WT, int WO, int NST, bool WIDE, bool PAIR, bool DUAL>
+__global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
+{
+    constexpr int NW = WT * WO, A = tile_lds(BT, BO, NW, NST), B = DUAL ? tile_lds(BT / 2, BO, NW, 3) : 0;
+    __shared__ __attribute__((aligned(1024))) uint32_t lds[(A > B ? A : B) / 4];
+    const K3kF8 &a = p.a;
+    int tt, to, sl;
+    Job job;
+    if (a.offsets) {
+        const Jobs s = count_jobs(a, BT);
+        if (!tile_of(s.total, p.no, 1, blockIdx.x, tt, to, sl)) return;
+        job = find_job(a, s, tt, BT);
+    } else {
+        if (!tile_of(p.nt, p.no, p.nsl, blockIdx.x, tt, to, sl)) return;
+        job = Job{0, tt * BT, min(BT, a.T - tt * BT)};
+    }
+    if constexpr (DUAL)
+        if (job.n <= BT / 2) return tile_run<BT / 2, BO, WT, WO, 3, WIDE, PAIR>(p, job, to, sl, lds);
+    tile_run<BT, BO, WT, WO, NST, WIDE, PAIR>(p, job, to, sl, lds);
 }
 
 /* the slices' sums, in slice order, and the epilogue; four slices requested at once */
@@ -841,7 +844,7 @@ void stream(const K3kF8 *a, int rows, hipStream_t st)
     else stream_go<2, 8, 2>(a, st);
 }
 
-template <int BT, int BO, int WT, int WO, int NST, bool WIDE = false, bool PAIR = false>
+template <int BT, int BO, int WT, int WO, int NST, bool WIDE = false, bool PAIR = false, bool DUAL = false>
 void tile_go(F8Tile *p, int nsl, hipStream_t st)
 {
     const int nkb = blocks(p->a.in);
@@ -850,7 +853,7 @@ void tile_go(F8Tile *p, int nsl, hipStream_t st)
     p->per = (nkb + nsl - 1) / nsl;
     p->nsl = (nkb + p->per - 1) / p->per;
     const long grid = (p->a.offsets ? most_jobs(&p->a, BT) : (long)p->nt) * p->no * p->nsl;
-    f8_tile_kernel<BT, BO, WT, WO, NST, WIDE, PAIR><<<(unsigned)grid, 64 * WT * WO, 0, st>>>(*p);
+    f8_tile_kernel<BT, BO, WT, WO, NST, WIDE, PAIR, DUAL><<<(unsigned)grid, 64 * WT * WO, 0, st>>>(*p);
 }
 
 }  // namespace
@@ -921,7 +924,7 @@ extern "C" int k3k_grouped_f8(const K3kF8 *a, void *stream_)
     p.part = NULL;
     if (a->wide) tile_go<128, 128, 2, 2, 4, true>(&p, 1, st);
     else if (each <= 128) tile_go<128, 128, 2, 2, 4>(&p, 1, st);
-    else tile_go<256, 256, 2, 4, 2>(&p, 1, st);
+    else tile_go<256, 256, 2, 4, 2, false, false, true>(&p, 1, st);
     K3K_LAUNCH_CHECK("grouped_f8: tiles");
     return 0;
 }
@@ -935,7 +938,7 @@ extern "C" int k3k_gateup_f8(const K3kF8 *a, float *gu, void *stream_)
         F8Tile p;
         p.a = *a;
         p.part = NULL;
-        tile_go<256, 256, 2, 4, 2, false, true>(&p, 1, st);
+        tile_go<256, 256, 2, 4, 2, false, true, true>(&p, 1, st);
         K3K_LAUNCH_CHECK("gateup_f8");
         return 0;
     }
