@@ -19,6 +19,7 @@
 #include "k3_f8.h"
 #include "k3k.h"
 
+#include <math.h>
 #include <type_traits>
 
 namespace {
@@ -219,141 +220,30 @@ __device__ __forceinline__ int y_row(const K3kF8 &a, int r)
     return (unsigned)t < (unsigned)a.T ? t : a.T;
 }
 
-/* ---- few rows: W straight into operands ------------------------------------------------- */
-/* A workgroup takes 16 RW rows of W and up to 8 NP rows of x; its waves share the column blocks, each with a ring of U blocks
- * in registers. W's tiles are operands as loaded, 1 KB a load; rows of x are loaded 8 lanes to a row's 128 bytes and turned into
- * operands through the wave's own LDS (16-byte column c of row r in slot c ^ (r / 2 % 8): the 16 rows of a fragment fall on all
- * banks). Past the wave's run and behind the last row requests return zeros without reading. */
-/* LDS bytes of a wave: 8 NP rows of a block, or its sums */
-constexpr int stream_lds(int rw, int np) { return (np + 1) / 2 * (rw > 2 ? rw * 1024 : 2048); }
+/* ---- up to 64 rows: W straight into operands ---------------------------------------------- */
+constexpr int SK_NW = 4;                        /* waves */
 
-template <int RW, int NP, int U, int NW, int POL, bool WIDE>
-__device__ __forceinline__ void stream_rows(const K3kF8 &a, const Job &job, int rt0, uint32_t *lds)
+/* a stage, an array of its own: that tells the accesses of one from those of another */
+template <int S, int SZ>
+__device__ __forceinline__ uint32_t *stage_of()
 {
-    constexpr int NT = (NP + 1) / 2, WAVE = stream_lds(RW, NP) / 4;
-    const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
-    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int nkb = blocks(a.in), k0 = nkb * wv / NW, k1 = nkb * (wv + 1) / NW, n = k1 - k0;
-    uint32_t *const mine = lds + wv * WAVE;
-
-    const uint8_t *const W = a.W + (size_t)job.e * a.w_step + (size_t)(rt0 / F8_G) * nkb * F8_KSTEP;
-    const k3_rsrc rw = k3_make_rsrc(W, (uint32_t)nkb * F8_KSTEP);
-    const uint32_t wo = (uint32_t)(rt0 % F8_G) * F8_TILE + lane * 16;
-    const k3_rsrc rx = k3_make_rsrc(a.x, F8_OOB), rs = k3_make_rsrc(a.xs, F8_OOB);
-    uint32_t xo[NP], so[NT];
-#pragma unroll
-    for (int p = 0; p < NP; p++) {
-        const int r = 8 * p + lane / 8, t = r < job.n ? x_row(a, job.r0 + r) : -1;
-        xo[p] = t < 0 ? F8_OOB : (uint32_t)t * (uint32_t)a.ldx + (lane & 7) * 16;
-    }
-#pragma unroll
-    for (int j = 0; j < NT; j++) {
-        const int r = 16 * j + r16, t = r < job.n ? x_row(a, job.r0 + r) : -1;
-        so[j] = t < 0 ? F8_OOB : (uint32_t)t * (uint32_t)a.ldxs * 4;
-    }
-    /* W's scales: a lane each, 64 column blocks at a time */
-    const float *const Ws = a.Ws + (size_t)job.e * a.ws_step + (size_t)(rt0 / F8_G) * a.ldws;
-    auto scales = [&](int i) {
-        float v = Ws[min(k0 + i + lane, nkb - 1)];
-        asm volatile("" : "+v"(v));             /* (arrived when it returns: a wait at its use would be one for every request since) */
-        return v;
-    };
-    float wsc = scales(0);
-
-    struct Slot {
-        u32x4 w[RW][2], x[NP];
-        float s[NT];
-    };
-    Slot ring[U];
-    auto load = [&](Slot &s, int i) {
-        const uint32_t none = i < n ? 0u : F8_OOB, kb = k0 + i;
-#pragma unroll
-        for (int q = 0; q < RW; q++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) s.w[q][h] = bload16<POL>(rw, (wo + kb * F8_KSTEP + q * F8_TILE + h * 1024) | none);
-#pragma unroll
-        for (int p = 0; p < NP; p++) s.x[p] = bload16<0>(rx, (xo[p] + kb * 128) | none);
-#pragma unroll
-        for (int j = 0; j < NT; j++) s.s[j] = __uint_as_float(k3_bload4(rs, (so[j] + kb * 4) | none));
-    };
-    k3_f32x4 acc[RW][NT];
-#pragma unroll
-    for (int q = 0; q < RW; q++)
-#pragma unroll
-        for (int j = 0; j < NT; j++) acc[q][j] = k3_f32x4{0.f, 0.f, 0.f, 0.f};
-    auto slot = [](int r, int c) { return r * 32 + ((c ^ (r >> 1)) & 7) * 4; };
-    auto use = [&](const Slot &s, int i) {
-        const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wsc), i & 63));
-#pragma unroll
-        for (int p = 0; p < NP; p++) *reinterpret_cast<u32x4 *>(mine + slot(8 * p + lane / 8, lane & 7)) = s.x[p];
-        __builtin_amdgcn_wave_barrier();
-        Wide ww[WIDE ? RW : 1];
-        if constexpr (WIDE)
-#pragma unroll
-            for (int q = 0; q < RW; q++) ww[q] = widen(s.w[q][0], s.w[q][1]);
-#pragma unroll
-        for (int j = 0; j < NT; j++) {
-            const int r = 16 * j + (NP == 1 ? r16 & 7 : r16);
-            const u32x4 x0 = *reinterpret_cast<const u32x4 *>(mine + slot(r, g)), x1 = *reinterpret_cast<const u32x4 *>(mine + slot(r, 4 + g));
-            const float f = s.s[j] * w;
-            Wide xw;
-            if constexpr (WIDE) xw = widen(x0, x1);
-#pragma unroll
-            for (int q = 0; q < RW; q++) {
-                k3_f32x4 v;
-                if constexpr (WIDE) v = wide_mfma(ww[q], xw);
-                else v = f8_mfma(s.w[q][0], s.w[q][1], x0, x1);
-#pragma unroll
-                for (int e = 0; e < 4; e++) acc[q][j][e] = fmaf(f, v[e], acc[q][j][e]);
-            }
-        }
-        __builtin_amdgcn_wave_barrier();
-    };
-#pragma unroll
-    for (int u = 0; u < U; u++) load(ring[u], u);
-    int i = 0;
-    for (; i + U <= n; i += U) {
-        if (i && i % 64 == 0) wsc = scales(i);       /* (U divides 64) */
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            use(ring[u], i + u);
-            load(ring[u], i + u + U);
-        }
-    }
-    if (i < n && i && i % 64 == 0) wsc = scales(i);
-#pragma unroll
-    for (int u = 0; u < U; u++)
-        if (i + u < n) use(ring[u], i + u);
-    static_assert(64 % U == 0, "scales are fetched between rounds");
-
-    /* the waves' sums, in their order */
-    float4 *const part = reinterpret_cast<float4 *>(mine);
-#pragma unroll
-    for (int q = 0; q < RW; q++)
-#pragma unroll
-        for (int j = 0; j < NT; j++) part[(q * NT + j) * 64 + lane] = make_float4(acc[q][j][0], acc[q][j][1], acc[q][j][2], acc[q][j][3]);
-    __syncthreads();
-    for (int f = wv; f < RW * NT; f += NW) {
-        const int o = (rt0 + f / NT) * 16 + 4 * g, r = 16 * (f % NT) + r16;
-        const int t = r < job.n ? y_row(a, job.r0 + r) : a.T;
-        float b[4];
-        bias4(a, o, b);
-        const uint4 res = res4(a, t, o);
-        const float4 *p = reinterpret_cast<const float4 *>(lds) + f * 64 + lane;
-        float4 s = p[0];
-#pragma unroll
-        for (int w = 1; w < NW; w++) {
-            const float4 v = p[w * (WAVE / 4)];
-            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
-        }
-        put4(a, t, o, s, b, res);
-    }
+    __shared__ __attribute__((aligned(1024))) uint32_t b[SZ];
+    return b;
 }
 
-template <int RW, int NP, int U, int NW, int POL, bool WIDE>
-__global__ __launch_bounds__(64 * NW) void f8_stream_kernel(K3kF8 a, int o0, int og)
+/* A workgroup takes 16 RW rows of W and up to 8 NP rows of x; its four waves share the column blocks, each with a ring of R blocks: W's tiles
+ * are operands as loaded, 1 KB a load, into registers; rows of x come by DMA, 8 lanes to a row's 128 bytes, into LDS of the wave's own
+ * (16-byte column c of row r in slot c ^ (r / 2 % 8): the 16 rows of a fragment fall on all banks). So there is no barrier until the waves'
+ * sums meet. Past the wave's run and behind the last row requests return zeros without reading.
+ * Bound by reading W (one token of 7168 -> 12288, 88 MB, 16.3 us; 64 tokens on 384 experts of 7168 -> 2048, 4.1 GB, 603 us = 6.8 TB/s) and, for many
+ * rows, by what a CU takes in: x comes again for each 16 RW rows of W (64 tokens of 7168 -> 12288 24.5 us). Deeper rings change nothing. */
+template <int RW, int NP, int R, int POL, bool WIDE>
+__global__ __launch_bounds__(64 * SK_NW) void f8_skinny_kernel(K3kF8 a, int o0, int og)
 {
-    __shared__ __attribute__((aligned(16))) uint32_t lds[NW * stream_lds(RW, NP) / 4];
+    constexpr int NW = SK_NW;
+    constexpr int NT = (NP + 1) / 2, XW = NP * 256;              /* a wave's stage of x, in 4-byte units */
+    static_assert(NP % 2 == 0, "whole fragments");
+    __shared__ uint32_t SC[NW * NT * 256];
     Job job = {0, 0, a.T};
     int o = blockIdx.x;
     if (a.offsets) {
@@ -368,7 +258,154 @@ __global__ __launch_bounds__(64 * NW) void f8_stream_kernel(K3kF8 a, int o0, int
         job = find_job(a, count_jobs(a, 8 * NP), j, 8 * NP);
         if (job.n == 0) return;
     }
-    stream_rows<RW, NP, U, NW, POL, WIDE>(a, job, (o0 + o) * RW, lds);
+    const int rt0 = (o0 + o) * RW;
+    const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int nkb = blocks(a.in), k0 = nkb * wv / NW, k1 = nkb * (wv + 1) / NW, n = k1 - k0;
+
+    /* (three tiles can lie in two groups, with scales of their own) */
+    constexpr bool TWO = F8_G % RW != 0;
+    const int rb = rt0 / F8_G, left_rb = blocks(a.out) - rb;
+    const k3_rsrc rw = k3_make_rsrc(a.W + (size_t)job.e * a.w_step + (size_t)rb * nkb * F8_KSTEP, (uint32_t)min(left_rb, TWO ? 2 : 1) * (uint32_t)nkb * F8_KSTEP);
+    auto w_at = [&](int q) -> uint32_t {
+        const int rt = rt0 + q;
+        return (uint32_t)(rt / F8_G - rb) * (uint32_t)nkb * F8_KSTEP + (uint32_t)(rt % F8_G) * F8_TILE;
+    };
+    const k3_rsrc rx = k3_make_rsrc(a.x, F8_OOB), rs = k3_make_rsrc(a.xs, F8_OOB);
+    auto sw = [](int r) { return (r >> 1) & 7; };
+    uint32_t xo[NP], so[NT];
+#pragma unroll
+    for (int p = 0; p < NP; p++) {
+        const int r = 8 * p + lane / 8, t = r < job.n ? x_row(a, job.r0 + r) : -1;
+        xo[p] = t < 0 ? F8_OOB : (uint32_t)t * (uint32_t)a.ldx + ((lane & 7) ^ sw(r)) * 16;
+    }
+#pragma unroll
+    for (int j = 0; j < NT; j++) {
+        const int r = 16 * j + r16, t = r < job.n ? x_row(a, job.r0 + r) : -1;
+        so[j] = t < 0 ? F8_OOB : (uint32_t)t * (uint32_t)a.ldxs * 4;
+    }
+    const float *const Ws = a.Ws + (size_t)job.e * a.ws_step;
+    auto scales = [&](int b, int i) {
+        float v = Ws[(size_t)min(b, blocks(a.out) - 1) * a.ldws + min(k0 + i + lane, nkb - 1)];
+        asm volatile("" : "+v"(v));
+        return v;
+    };
+    float wsc = scales(rb, 0), wsc2 = TWO ? scales(rb + 1, 0) : 0.0f;
+    /* scales of x: 16 blocks at a time through LDS, [block][row] (one block's alone would be a line of memory for each row and block) */
+    uint32_t *const sc = SC + wv * NT * 256;
+    auto x_scales = [&](int c) {                /* of blocks k0 + c ..+16 */
+        float v[NT][4];
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int kb = k0 + c + 4 * g + e;
+                v[j][e] = __uint_as_float(k3_bload4(rs, (so[j] + kb * 4) | (kb < nkb ? 0u : F8_OOB)));
+            }
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) sc[(4 * g + e) * NT * 16 + 16 * j + r16] = __float_as_uint(v[j][e]);
+        __builtin_amdgcn_wave_barrier();
+    };
+    x_scales(0);
+    auto buf_of = [&](auto slot) -> uint32_t * { return stage_of<decltype(slot)::value, NW * XW>() + wv * XW; };
+    u32x4 wr[R][RW][2];
+    int at = 0;                                 /* the block requested next */
+    auto load = [&](auto slot) {
+        constexpr int S = decltype(slot)::value;
+        const uint32_t none = at < n ? 0u : F8_OOB, kb = k0 + at;
+#pragma unroll
+        for (int p = 0; p < NP; p++) k3_dma16(rx, buf_of(slot) + p * 256, xo[p] | none, kb * 128);
+#pragma unroll
+        for (int q = 0; q < RW; q++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) wr[S][q][h] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rw, (w_at(q) + lane * 16 + h * 1024) | none, kb * F8_KSTEP, POL));
+        at++;
+    };
+    k3_f32x4 acc[RW][NT];
+#pragma unroll
+    for (int q = 0; q < RW; q++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) acc[q][j] = k3_f32x4{0.f, 0.f, 0.f, 0.f};
+    int i = 0;
+    auto use = [&](auto slot) {
+        constexpr int S = decltype(slot)::value;
+        const uint32_t *const b = buf_of(slot);
+        const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wsc), i & 63));
+        const float w2 = TWO ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wsc2), i & 63)) : w;
+        /* W's last request of this block is younger than its rows of x: with it all have arrived */
+#pragma unroll
+        for (int q = 0; q < RW; q++) asm volatile("" : "+v"(wr[S][q][0]), "+v"(wr[S][q][1]));
+        __builtin_amdgcn_sched_barrier(0);
+        u32x4 xf[NT][2];
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) xf[j][h] = *reinterpret_cast<const u32x4 *>(b + (16 * j + r16) * 32 + (((4 * h + g) ^ sw(r16)) & 7) * 4);
+        Wide ww[WIDE ? RW : 1];
+        if constexpr (WIDE) each_of<0, RW>([&](auto q) { ww[decltype(q)::value] = widen(wr[S][decltype(q)::value][0], wr[S][decltype(q)::value][1]); });
+        each_of<0, NT>([&](auto jj) {
+            constexpr int j = decltype(jj)::value;
+            const float xs = __uint_as_float(sc[(i & 15) * NT * 16 + 16 * j + r16]);
+            Wide xw;
+            if constexpr (WIDE) xw = widen(xf[j][0], xf[j][1]);
+            each_of<0, RW>([&](auto qq) {
+                constexpr int q = decltype(qq)::value;
+                const float f = xs * (TWO && (rt0 + q) / F8_G != rb ? w2 : w);
+                k3_f32x4 v;
+                if constexpr (WIDE) v = wide_mfma(ww[q], xw);
+                else v = f8_mfma(wr[S][q][0], wr[S][q][1], xf[j][0], xf[j][1]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[q][j][e] = fmaf(f, v[e], acc[q][j][e]);
+                asm volatile("" : "+v"(acc[q][j]));
+            });
+        });
+        __builtin_amdgcn_sched_barrier(0);
+        if ((++i & 15) == 0 && i < n) {
+            x_scales(i);
+            if ((i & 63) == 0) {
+                wsc = scales(rb, i);
+                if (TWO) wsc2 = scales(rb + 1, i);
+            }
+        }
+    };
+    each_of<0, R - 1>(load);
+    int left = n;
+    /* block k is used while block k + R - 1 is requested, into the stage that block k - 1 left */
+    for (; left >= R; left -= R)
+        each_of<0, R>([&](auto slot) {
+            load(std::integral_constant<int, (decltype(slot)::value + R - 1) % R>{});
+            use(slot);
+        });
+    each_of<0, R - 1>([&](auto slot) {
+        if (decltype(slot)::value < left) use(slot);
+    });
+
+    /* the waves' sums, in their order, 16 rows of W at a time */
+    float4 *const part = reinterpret_cast<float4 *>(buf_of(std::integral_constant<int, 0>{}));
+    each_of<0, RW>([&](auto qq) {
+        constexpr int q = decltype(qq)::value;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < NT; j++) part[j * 64 + lane] = make_float4(acc[q][j][0], acc[q][j][1], acc[q][j][2], acc[q][j][3]);
+        __syncthreads();
+        for (int j = wv; j < NT; j += NW) {
+            const int out = (rt0 + q) * 16 + 4 * g, r = 16 * j + r16;
+            const int t = r < job.n ? y_row(a, job.r0 + r) : a.T;
+            float b[4];
+            bias4(a, out, b);
+            const uint4 res = res4(a, t, out);
+            const float4 *p = reinterpret_cast<const float4 *>(stage_of<0, NW * XW>()) + j * 64 + lane;
+            float4 s = p[0];
+#pragma unroll
+            for (int w = 1; w < NW; w++) {
+                const float4 v = p[w * (XW / 4)];
+                s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+            }
+            put4(a, t, out, s, b, res);
+        }
+    });
 }
 
 /* ---- many rows: LDS tiles ---------------------------------------------------------------- */
@@ -420,43 +457,49 @@ __device__ __forceinline__ void act8(float (&v)[8], int act)
     });
 }
 
+/* the residual of outputs o ..+8 of row t as it lies in memory */
+struct Res8 {
+    uint4 a, b;
+};
+__device__ __forceinline__ Res8 res8(const K3kF8 &a, int t, int o)
+{
+    Res8 r = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    if (!a.res || t >= a.T || o + 8 > a.out) return r;
+    const bool bf = a.y_type == K3D_BF16;
+    const char *q = (const char *)a.res + ((size_t)t * a.ldr + o) * (bf ? 2 : 4);
+    __builtin_memcpy(&r.a, q, 16);
+    if (!bf) __builtin_memcpy(&r.b, q + 16, 16);
+    return r;
+}
+
 /* outputs o ..+8 of row t: v + bias b through the activation, plus the residual */
-__device__ __forceinline__ void put8(const K3kF8 &a, int t, int o, float (&v)[8], const float (&b)[8])
+__device__ __forceinline__ void put8(const K3kF8 &a, int t, int o, float (&v)[8], const float (&b)[8], const Res8 &r)
 {
     if (t >= a.T || o >= a.out) return;
-    const bool bf = a.y_type == K3D_BF16;
     if (o + 8 > a.out) {                /* (the end of a row) */
         put4(a, t, o, make_float4(v[0], v[1], v[2], v[3]), *(const float(*)[4])b, res4(a, t, o));
         put4(a, t, o + 4, make_float4(v[4], v[5], v[6], v[7]), *(const float(*)[4])(b + 4), res4(a, t, o + 4));
         return;
     }
-    uint4 r0, r1;
-    if (a.res) {
-        const char *q = (const char *)a.res + ((size_t)t * a.ldr + o) * (bf ? 2 : 4);
-        __builtin_memcpy(&r0, q, 16);
-        if (!bf) __builtin_memcpy(&r1, q + 16, 16);
-    }
+    const bool bf = a.y_type == K3D_BF16;
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] += b[i];
     if (bf) act8<false>(v, a.act);
     else act8<true>(v, a.act);
     const size_t at = (size_t)t * a.ldy + o;
+    const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
     if (bf) {
-        if (a.res) {
-            const uint32_t w[4] = {r0.x, r0.y, r0.z, r0.w};
+        if (a.res)
 #pragma unroll
             for (int i = 0; i < 4; i++) v[2 * i] += __uint_as_float(w[i] << 16), v[2 * i + 1] += __uint_as_float(w[i] & 0xffff0000u);
-        }
         __bf16 h[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) h[i] = (__bf16)v[i];
         __builtin_memcpy((uint16_t *)a.y + at, h, 16);
     } else {
-        if (a.res) {
-            const uint32_t w[8] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
+        if (a.res)
 #pragma unroll
             for (int i = 0; i < 8; i++) v[i] += __uint_as_float(w[i]);
-        }
         __builtin_memcpy((float *)a.y + at, v, 32);
     }
 }
@@ -722,8 +765,8 @@ __device__ __forceinline__ void tile_run(const F8Tile &p, const Job &job, int to
     bias4(a, p.nsl > 1 ? a.out : o + 4, *(float(*)[4])(bs + 4));
     __builtin_amdgcn_s_waitcnt(WAIT_VM0);      /* the last requests land before LDS is used again */
     __syncthreads();
-#pragma unroll
-    for (int j0 = 0; j0 < FT; j0 += JR) {
+    each_of<0, FT / JR>([&](auto part) {
+        constexpr int j0 = decltype(part)::value * JR;
 #pragma unroll
         for (int j = 0; j < JR; j++)
 #pragma unroll
@@ -732,17 +775,30 @@ __device__ __forceinline__ void tile_run(const F8Tile &p, const Job &job, int to
                 reg[r * C + (oc ^ (r16 & (C - 1)))] = make_float4(acc[i][j0 + j][0], acc[i][j0 + j][1], acc[i][j0 + j][2], acc[i][j0 + j][3]);
             }
         __builtin_amdgcn_wave_barrier();
-#pragma unroll 2
-        for (int i = 0; i < IT; i++) {
-            const int r = lane / (C / 2) + i * RI, at = row0 + 16 * j0 + i * RI, x = r & 15 & (C - 1);
-            const float4 v0 = reg[r * C + (2 * c ^ x)], v1 = reg[r * C + ((2 * c + 1) ^ x)];
-            float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-            const int t = at < job.n ? y_row(a, job.r0 + at) : a.T;
-            if (p.nsl == 1) put8(a, t, o, v, bs);
-            else if (t < a.T && o < a.out) part8(p.part + ((size_t)sl * a.T + t) * a.out + o, v, a.out - o);
+        /* (residuals of four rounds requested ahead: one after another each round would wait for its own) */
+        constexpr int PF = IT < 4 ? IT : 4;
+        static_assert(IT % PF == 0, "rounds");
+#pragma unroll 1
+        for (int i0 = 0; i0 < IT; i0 += PF) {
+            int t[PF];
+            Res8 res[PF];
+#pragma unroll
+            for (int i = 0; i < PF; i++) {
+                const int at = row0 + 16 * j0 + (i0 + i) * RI;
+                t[i] = at < job.n ? y_row(a, job.r0 + at) : a.T;
+                if (p.nsl == 1) res[i] = res8(a, t[i], o);
+            }
+#pragma unroll
+            for (int i = 0; i < PF; i++) {
+                const int r = lane / (C / 2) + (i0 + i) * RI, x = r & 15 & (C - 1);
+                const float4 v0 = reg[r * C + (2 * c ^ x)], v1 = reg[r * C + ((2 * c + 1) ^ x)];
+                float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+                if (p.nsl == 1) put8(a, t[i], o, v, bs, res[i]);
+                else if (t[i] < a.T && o < a.out) part8(p.part + ((size_t)sl * a.T + t[i]) * a.out + o, v, a.out - o);
+            }
         }
         __builtin_amdgcn_wave_barrier();
-    }
+    });
 }
 
 /* DUAL: passes of at most half the rows by a kernel of half the rows and three stages, which takes little over half the time (2048 tokens, eight of 64
@@ -813,35 +869,50 @@ long most_jobs(const K3kF8 *a, int most)
     return (long)a->rows / most + (a->rows < a->n_experts ? a->rows : a->n_experts);
 }
 
-template <int RW, int NP, int U, int NW>
-void stream_launch(const K3kF8 *a, long jobs, hipStream_t st)
+/* weights that no cache keeps from one call to the next, from here on read past the caches (88 MB times one token 16.3 us, 18.2 otherwise; but
+ * 15 MB 6.1 and 5.9) */
+constexpr size_t F8_NT_BYTES = (size_t)48 << 20;
+
+template <int RW, int NP, int R>
+void skinny_go(const K3kF8 *a, long jobs, hipStream_t st)
 {
     /* (a launch takes under 2^32 work-items) */
-    const long og = ((a->out + 15) / 16 + RW - 1) / RW, mats = a->W2 ? 2 : 1, most = ((1L << 32) - 1) / (64 * NW) / (jobs * mats);
+    const long og = ((a->out + 15) / 16 + RW - 1) / RW, mats = a->W2 ? 2 : 1, most = ((1L << 32) - 1) / (64 * SK_NW) / (jobs * mats);
+    const bool nt = tiled_bytes(a->out, a->in) * (a->offsets ? a->n_experts * mats : 1) >= F8_NT_BYTES;
     for (long o = 0; o < og; o += most) {
         const int n = (int)(og - o < most ? og - o : most) * mats;
-        if (a->wide) f8_stream_kernel<RW, NP, U, NW, K3_LD_NT, true><<<(unsigned)(jobs * n), 64 * NW, 0, st>>>(*a, (int)o, n);
-        else f8_stream_kernel<RW, NP, U, NW, K3_LD_NT, false><<<(unsigned)(jobs * n), 64 * NW, 0, st>>>(*a, (int)o, n);
+        const unsigned grid = (unsigned)(jobs * n);
+        if (a->wide && nt) f8_skinny_kernel<RW, NP, R, K3_LD_NT, true><<<grid, 64 * SK_NW, 0, st>>>(*a, (int)o, n);
+        else if (a->wide) f8_skinny_kernel<RW, NP, R, K3_LD_DEFAULT, true><<<grid, 64 * SK_NW, 0, st>>>(*a, (int)o, n);
+        else if (nt) f8_skinny_kernel<RW, NP, R, K3_LD_NT, false><<<grid, 64 * SK_NW, 0, st>>>(*a, (int)o, n);
+        else f8_skinny_kernel<RW, NP, R, K3_LD_DEFAULT, false><<<grid, 64 * SK_NW, 0, st>>>(*a, (int)o, n);
     }
 }
 
-template <int RW, int NP, int U>
-void stream_go(const K3kF8 *a, hipStream_t st)
+template <int NP>
+void skinny_rows(const K3kF8 *a, hipStream_t st)
 {
-    /* waves that share a workgroup's columns: enough for the chip, each with a few blocks */
-    const long jobs = a->offsets ? most_jobs(a, 8 * NP) : 1, wgs = jobs * (((a->out + 15) / 16 + RW - 1) / RW);
-    const int nkb = blocks(a->in);
-    if (wgs * 4 < k3k_cu_count() * 8 && nkb >= 16) stream_launch<RW, NP, U, 8>(a, jobs, st);
-    else if (nkb >= 8) stream_launch<RW, NP, U, 4>(a, jobs, st);
-    else stream_launch<RW, NP, U, 2>(a, jobs, st);
+    /* The rows of W of a workgroup: a CU takes in 46 KB/us, W and x for each of its workgroups (64 tokens of 7168 -> 12288: 256 workgroups of 48 rows
+     * 24.5 us, 384 of 32 33, 192 of 64 26.7). By expert: as if each expert had one pass. */
+    const long jobs = a->offsets ? most_jobs(a, 8 * NP) : 1, about = a->offsets ? (a->rows < a->n_experts ? a->rows : a->n_experts) * (a->W2 ? 2 : 1) : 1;
+    const long tiles = (a->out + 15) / 16, cus = k3k_cu_count();
+    int rw = 1;
+    long best = 0;
+    for (int r = 1; r <= 3; r++) {
+        const long cost = ((about * ((tiles + r - 1) / r) + cus - 1) / cus) * (2 * r + NP);
+        if (r == 1 || cost < best) best = cost, rw = r;
+    }
+    if (rw == 1) skinny_go<1, NP, NP < 8 ? 4 : 3>(a, jobs, st);
+    else if (rw == 2) skinny_go<2, NP, NP < 8 ? 4 : 2>(a, jobs, st);
+    else skinny_go<3, NP, NP < 8 ? 4 : 3>(a, jobs, st);
 }
 
-void stream(const K3kF8 *a, int rows, hipStream_t st)
+void skinny(const K3kF8 *a, int rows, hipStream_t st)
 {
-    if (rows <= 8) stream_go<1, 1, 8>(a, st);
-    else if (rows <= 16) stream_go<1, 2, 4>(a, st);
-    else if (rows <= 32) stream_go<2, 4, 2>(a, st);
-    else stream_go<2, 8, 2>(a, st);
+    if (rows <= 16) skinny_rows<2>(a, st);
+    else if (rows <= 32) skinny_rows<4>(a, st);
+    else if (rows <= 48) skinny_rows<6>(a, st);
+    else skinny_rows<8>(a, st);
 }
 
 template <int BT, int BO, int WT, int WO, int NST, bool WIDE = false, bool PAIR = false, bool DUAL = false>
@@ -854,6 +925,24 @@ void tile_go(F8Tile *p, int nsl, hipStream_t st)
     p->nsl = (nkb + p->per - 1) / p->per;
     const long grid = (p->a.offsets ? most_jobs(&p->a, BT) : (long)p->nt) * p->no * p->nsl;
     f8_tile_kernel<BT, BO, WT, WO, NST, WIDE, PAIR, DUAL><<<(unsigned)grid, 64 * WT * WO, 0, st>>>(*p);
+}
+
+/* Microseconds of a launch of f8_tile_kernel and, with slices, the join: rounds of as many workgroups as fit the chip, each of `per` steps, its first
+ * requests and its epilogue (activations and residuals cost a tile more than the join); W comes at 5 GB/ms at the most. What it chooses is within 8 % of the best of all shapes and slices for 12 shapes of 100 to 4096
+ * tokens (1000 tokens of 2048 -> 12288 39 us as 256 x 256, 49 as 128 x 256, 57 as 128 x 128; 2048 of 7168 -> 4096 89, 60 and 77). */
+struct Shape {
+    int bt, bo, per_cu, wide;
+    float alone, full, over;    /* of a step, on a CU alone or with as many as fit; of the rest */
+};
+constexpr Shape SHAPES[] = {{256, 256, 1, 0, 1.62f, 1.62f, 13.0f}, {128, 256, 1, 0, 0.91f, 0.91f, 9.0f}, {128, 128, 1, 0, 0.64f, 0.64f, 7.0f}, {128, 128, 2, 1, 1.0f, 1.65f, 8.0f}};
+constexpr int N_SHAPES = sizeof SHAPES / sizeof SHAPES[0];
+
+float tile_cost(const Shape &s, int T, int in, int out, int nsl, float epilogue, long cus)
+{
+    const long wgs = (long)((T + s.bt - 1) / s.bt) * ((out + s.bo - 1) / s.bo) * nsl, slots = cus * s.per_cu;
+    const int per = (blocks(in) + nsl - 1) / nsl;
+    const float t = 3.0f + (float)((wgs + slots - 1) / slots) * (per * (wgs <= cus ? s.alone : s.full) + s.over + (nsl > 1 ? 0.0f : epilogue));
+    return fmaxf(t, 5.0f + (float)in * out / 5e6f) + (nsl > 1 ? 2.5f + (nsl + 1.0f) * T * out * 4.0f / 4.7e6f : 0.0f);
 }
 
 }  // namespace
@@ -882,24 +971,30 @@ extern "C" int k3k_linear_f8(const K3kF8 *a, void *stream_)
 {
     hipStream_t st = (hipStream_t)stream_;
     if (a->T <= 64) {
-        stream(a, a->T, st);
+        skinny(a, a->T, st);
         K3K_LAUNCH_CHECK("linear_f8: few rows");
         return 0;
     }
     F8Tile p;
     p.a = *a;
     p.part = (float *)a->ws;
-    const long cus = k3k_cu_count();
-    const int nkb = blocks(a->in);
-    const long tiles = (long)((a->T + 255) / 256) * ((a->out + 255) / 256);
-    if (tiles >= cus && !a->wide) {
-        tile_go<256, 256, 2, 4, 2>(&p, 1, st);
-    } else {
-        const long small = (long)((a->T + 127) / 128) * ((a->out + 127) / 128);
-        int nsl = 1;
-        while (nsl < F8_MAX_SLICES && small * nsl * 2 <= cus && nkb >= 4 * nsl && (size_t)2 * nsl * a->T * a->out * 4 <= part_bytes(a->T, a->out)) nsl *= 2;
-        if (a->wide) tile_go<128, 128, 2, 2, 4, true>(&p, nsl, st);
-        else tile_go<128, 128, 2, 2, 4>(&p, nsl, st);
+    /* the cheapest tile shape and number of slices */
+    float best = 0.0f;
+    int shape = 0, nsl = 1;
+    const size_t one = (size_t)a->T * a->out * 4, room = part_bytes(a->T, a->out);
+    for (int i = 0; i < N_SHAPES; i++) {
+        if (SHAPES[i].wide != a->wide) continue;
+        for (int n = 1; n <= F8_MAX_SLICES; n *= 2) {
+            if (n > 1 && (n * one > room || blocks(a->in) < 2 * n)) break;
+            const float t = tile_cost(SHAPES[i], a->T, a->in, a->out, n, (a->act ? 5.0f : 0.0f) + (a->res ? 4.0f : 0.0f), k3k_cu_count());
+            if (best == 0.0f || t < best) best = t, shape = i, nsl = n;
+        }
+    }
+    switch (shape) {
+    case 0: tile_go<256, 256, 2, 4, 2>(&p, nsl, st); break;
+    case 1: tile_go<128, 256, 2, 4, 3>(&p, nsl, st); break;
+    case 2: tile_go<128, 128, 2, 2, 4>(&p, nsl, st); break;
+    default: tile_go<128, 128, 2, 2, 2, true>(&p, nsl, st); break;
     }
     K3K_LAUNCH_CHECK("linear_f8: tiles");
     if (p.nsl > 1) {
@@ -910,20 +1005,27 @@ extern "C" int k3k_linear_f8(const K3kF8 *a, void *stream_)
     return 0;
 }
 
+/* Experts' rows without tiles: up to 10 on average in passes of 16 (64 experts of 7168 -> 2048: 8 each 145 us, as tiles 167), up to 16 of long rows
+ * in passes of 32 (162 us, as tiles 170; but of 2048 -> 7168 236 and 199). */
+static bool few_rows(const K3kF8 *a)
+{
+    const int each = (a->rows + a->n_experts - 1) / a->n_experts;
+    return each <= 10 || (each <= 16 && a->in >= 4096);
+}
+
 extern "C" int k3k_grouped_f8(const K3kF8 *a, void *stream_)
 {
     hipStream_t st = (hipStream_t)stream_;
     const int each = (a->rows + a->n_experts - 1) / a->n_experts;       /* rows of an expert, on average */
-    if (each <= 48) {
-        stream(a, each <= 4 ? 8 : each <= 12 ? 16 : each <= 24 ? 32 : 64, st);
+    if (few_rows(a)) {
+        skinny(a, each <= 10 ? 16 : 32, st);
         K3K_LAUNCH_CHECK("grouped_f8: few rows");
         return 0;
     }
     F8Tile p;
     p.a = *a;
     p.part = NULL;
-    if (a->wide) tile_go<128, 128, 2, 2, 4, true>(&p, 1, st);
-    else if (each <= 128) tile_go<128, 128, 2, 2, 4>(&p, 1, st);
+    if (a->wide) tile_go<128, 128, 2, 2, 2, true>(&p, 1, st);
     else tile_go<256, 256, 2, 4, 2, false, false, true>(&p, 1, st);
     K3K_LAUNCH_CHECK("grouped_f8: tiles");
     return 0;
@@ -933,8 +1035,7 @@ extern "C" int k3k_grouped_f8(const K3kF8 *a, void *stream_)
 extern "C" int k3k_gateup_f8(const K3kF8 *a, float *gu, void *stream_)
 {
     hipStream_t st = (hipStream_t)stream_;
-    const int each = (a->rows + a->n_experts - 1) / a->n_experts;
-    if (each > 48) {
+    if (!few_rows(a)) {
         F8Tile p;
         p.a = *a;
         p.part = NULL;
