@@ -433,10 +433,11 @@ int k3k_group(int *offsets, int *perm, const int *idx, int N, int n_experts, int
 /* out[t] = sum_j wt[t][j] y[t * topk + j], j ascending, over slots with 0 <= idx < n_experts; out of out_type. */
 typedef struct {
     void *out;
-    const float *y, *wt;
+    const void *y;              /* [T * topk][n] of y_type */
+    const float *wt;
     const int *idx;
     long ldo;
-    int out_type, T, topk, n, n_experts;
+    int out_type, y_type, T, topk, n, n_experts;
 } K3kSum;
 int k3k_sum_slots(const K3kSum *a, void *stream);
 

@@ -245,5 +245,6 @@ def moe64(X, idx, wt, W1, W3, W2, act, b1, b2, out_type):
             v, vt = product64(h, W2[e], out_type == BF16)
             vt = vt * 1.1 + ht @ np.abs(W2[e]).T
             y[t] += wt[t, j] * v[0]
-            tol[t] += abs(wt[t, j]) * (vt[0] + np.abs(v[0]) * k * 2.0 ** -22)
+            # (bf16: each slot's row is rounded, by half a step, before it is weighted)
+            tol[t] += abs(wt[t, j]) * (vt[0] + np.abs(v[0]) * k * 2.0 ** -22 + (HALF[BF16] * (np.abs(v[0]) + vt[0]) if out_type == BF16 else 0.0))
     return y, tol
