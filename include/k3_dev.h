@@ -284,7 +284,7 @@ int k3d_add_norm(void *y, int y_type, long ldy, uint8_t *q, long ldq, float *qs,
                  float eps, void *stream);
 
 /* The rows of x in 8 bits (act K3D_GLU_NONE), or of act(gate) * up: row t of x is gate [n], then up [n]. Scales and codes as above;
- * the activation in fp32. b1, b2 > 0 for K3D_GLU_SITU. */
+ * the activation in fp32. b1, b2 from 2^-64 to 2^64 for K3D_GLU_SITU. */
 int k3d_quant_f8(uint8_t *q, long ldq, float *qs, long ldqs, const void *x, int x_type, long ldx, int T, int n, int act,
                  float b1, float b2, void *stream);
 

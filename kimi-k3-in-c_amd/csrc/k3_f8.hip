@@ -216,7 +216,7 @@ __device__ __forceinline__ int y_row(const K3kF8 &a, int r)
 {
     if (!a.offsets) return r;
     int t = a.y_rows ? a.y_rows[r] : r;
-    if (a.x_rows && x_row(a, r) < 0) t = -1;
+    if (x_row(a, r) < 0) t = -1;
     return (unsigned)t < (unsigned)a.T ? t : a.T;
 }
 
@@ -382,7 +382,8 @@ __global__ __launch_bounds__(64 * SK_NW) void f8_skinny_kernel(K3kF8 a, int o0, 
         if (decltype(slot)::value < left) use(slot);
     });
 
-    /* the waves' sums, in their order, 16 rows of W at a time */
+    /* the waves' sums, in their order, 16 rows of W at a time, where the last requests (of zeros) have landed */
+    __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));
     float4 *const part = reinterpret_cast<float4 *>(buf_of(std::integral_constant<int, 0>{}));
     each_of<0, RW>([&](auto qq) {
         constexpr int q = decltype(qq)::value;

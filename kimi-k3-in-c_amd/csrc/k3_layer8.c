@@ -40,7 +40,8 @@ static const char *rows_bad(const void *q, long ldq, const void *s, long lds, in
 static const char *act_bad(int act, float b1, float b2)
 {
     if (act != K3D_GLU_SITU && act != K3D_GLU_SILU) return "unknown activation";
-    if (act == K3D_GLU_SITU && !(b1 > 0.0f && b2 > 0.0f)) return "situ needs limits above 0";
+    /* (within these a limit's reciprocal, and what the kernels multiply with them, stay in fp32) */
+    if (act == K3D_GLU_SITU && !(b1 >= 0x1p-64f && b1 <= 0x1p64f && b2 >= 0x1p-64f && b2 <= 0x1p64f)) return "situ needs limits from 2^-64 to 2^64";
     return NULL;
 }
 

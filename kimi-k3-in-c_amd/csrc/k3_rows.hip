@@ -14,6 +14,8 @@
 #include "k3_f8.h"
 #include "k3k.h"
 
+#include <math.h>
+
 namespace {
 
 /* (16 bytes at any alignment of their elements: as one vector, where a copy of eight elements became smaller stores, 51 against 47 us at
@@ -75,16 +77,30 @@ __device__ __forceinline__ void store8_of(void *p, int type, size_t row, int i, 
     }
 }
 
-/* the lane's eight columns (zeros behind the row's end) as codes, the first lane of a block its scale; every lane of the block takes part */
+/* u / s from r = 1 / s, with the remainder's share: u r alone is up to 1.5 units in the last place off, and a code is a choice that such a step
+ * can turn. s of infinity gives 0 as u r does. */
+__device__ __forceinline__ float quotient(float u, float s, float r)
+{
+    const float q = u * r;
+    return fmaf(fmaf(-q, s < INFINITY ? s : 0.0f, u), r, q);
+}
+
+/* the lane's eight columns (zeros behind the row's end) as codes, the first lane of a block its scale; every lane of the block takes part.
+ * EXACT: of quotients rounded once. Behind a gated activation, itself some 7 units off, they change no more than it does (32768 rows of 2048: 67.7
+ * against 65.1 us). */
+template <bool EXACT>
 __device__ __forceinline__ void put_codes(uint8_t *q, float *qs, size_t qrow, size_t srow, int i, const float (&u)[8], bool there)
 {
     uint32_t m = 0;
 #pragma unroll
     for (int j = 0; j < 8; j++) m = max(m, abs_bits(u[j]));
     const float s = f8_scale(row_max_bits(m)), r = 1.0f / s;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = EXACT ? quotient(u[j], s, r) : u[j] * r;
     uint2 c;
-    c.x = f8_codes(u[0] * r, u[1] * r, u[2] * r, u[3] * r);
-    c.y = f8_codes(u[4] * r, u[5] * r, u[6] * r, u[7] * r);
+    c.x = f8_codes(v[0], v[1], v[2], v[3]);
+    c.y = f8_codes(v[4], v[5], v[6], v[7]);
     if (!there) return;
     *reinterpret_cast<uint2 *>(q + qrow + i) = c;
     if ((threadIdx.x & 15) == 0) qs[srow + i / 128] = s;
@@ -125,7 +141,7 @@ __global__ __launch_bounds__(64 * NW) void add_norm_kernel(K3kNorm a, unsigned t
 #pragma unroll
         for (int w = 0; w < NW; w++) ss += part[w];
     }
-    const float rstd = 1.0f / sqrtf(ss / (float)a.n + a.eps);
+    const float rms = sqrtf(ss / (float)a.n + a.eps), rstd = 1.0f / rms;
 #pragma unroll
     for (int p = 0; p < P; p++) {
         const int i = (p * 64 * NW + tid) * 8;
@@ -135,9 +151,9 @@ __global__ __launch_bounds__(64 * NW) void add_norm_kernel(K3kNorm a, unsigned t
         for (int j = 0; j < 8; j++) w[j] = 1.0f;
         if (a.w) load8<K3D_F32>(w, a.w, i, a.n);
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[p][j] = i + j < a.n ? v[p][j] * rstd * w[j] : 0.0f;
+        for (int j = 0; j < 8; j++) v[p][j] = i + j < a.n ? quotient(v[p][j], rms, rstd) * w[j] : 0.0f;
         if (a.y && i < a.n) store8_of(a.y, a.y_type, t * a.ldy, i, a.n, v[p]);
-        if (a.q) put_codes(a.q, a.qs, t * a.ldq, t * a.ldqs, i, v[p], i < (a.n + 127) / 128 * 128);
+        if (a.q) put_codes<true>(a.q, a.qs, t * a.ldq, t * a.ldqs, i, v[p], i < (a.n + 127) / 128 * 128);
     }
 }
 
@@ -160,7 +176,7 @@ __global__ __launch_bounds__(256) void quant_kernel(K3kQuant a, unsigned t0, int
 #pragma unroll
             for (int j = 0; j < 8; j++) u[j] = i + j < a.n ? u[j] : 0.0f;
     }
-    put_codes(a.q, a.qs, t * a.ldq, t * a.ldqs, i, u, kb < nb);
+    put_codes<!GATED>(a.q, a.qs, t * a.ldq, t * a.ldqs, i, u, kb < nb);
 }
 
 /* Eight columns of one token to a thread; the slots' rows are requested four at a time. */

@@ -35,7 +35,8 @@ QUANT = dict(q=A, ldq=256, qs=2 * A, ldqs=2, x=3 * A, x_type=0, ldx=400, T=4, n=
 
 @pytest.mark.parametrize("change,word", [
     (dict(x_type=3), "x_type"), (dict(act=2), "activation"), (dict(act=-2), "activation"), (dict(act=0, b1=0.0), "limits"),
-    (dict(act=0, b2=-1.0), "limits"), (dict(act=0, b2=float("nan")), "limits"), (dict(T=-1), "T >= 0"), (dict(n=0), "n <="),
+    (dict(act=0, b2=-1.0), "limits"), (dict(act=0, b2=float("nan")), "limits"),
+    (dict(act=0, b1=float("inf")), "limits"), (dict(act=0, b2=1e30), "limits"), (dict(act=0, b1=1e-30), "limits"), (dict(T=-1), "T >= 0"), (dict(n=0), "n <="),
     (dict(n=65537, ldx=1 << 20), "NORM_MAX_N"), (dict(T=(1 << 24) + 1), "MAX_TOKENS"), (dict(x=None), "must be given"),
     (dict(ldx=399), "stride"), (dict(act=-1, ldx=199), "stride"), (dict(x=3 * A + 1), "aligned"), (dict(q=None), "must be given"),
     (dict(qs=None), "must be given"), (dict(q=A + 4), "aligned"), (dict(ldq=248), "aligned"), (dict(ldq=128), "whole blocks"),

@@ -27,7 +27,7 @@ def test_tile(gpu, out, inn):
 
 LIN = [(1, 128, 16), (1, 1, 1), (2, 130, 17), (3, 7168, 300), (8, 256, 128), (9, 1000, 100), (16, 4096, 512), (17, 1001, 300),
        (31, 7168, 40), (33, 640, 129), (48, 2304, 777), (64, 8320, 256), (64, 128, 64), (65, 128, 64), (100, 1001, 300), (128, 2048, 128),
-       (129, 512, 4096), (200, 7168, 384), (300, 129, 2047), (513, 1280, 257), (1000, 640, 1000), (2048, 512, 8192), (4097, 256, 4095)]
+       (129, 512, 4096), (200, 7168, 384), (300, 129, 2047), (513, 1280, 257), (1000, 640, 1000), (2048, 512, 8192), (4097, 256, 4095), (7, 33000, 130), (70, 9000, 300)]
 
 
 @pytest.mark.parametrize("T,inn,out", LIN)
@@ -61,6 +61,23 @@ def test_linear(gpu, T, inn, out, y_type):
     # the residual in y's place, and the same bits again
     place = res.clone()
     assert torch.equal(linear8(gpu, x, xs, wt, ws, inn, out, bias, ACTS[i], place, y=place), got)
+
+
+@pytest.mark.parametrize("y_type", [F32, BF16])
+@pytest.mark.parametrize("out", [4090, 8187, 12281])
+def test_linear_few_rows_wide(gpu, out, y_type):
+    """One to three tiles of W a workgroup, each number of pieces of x: exact integers (a bf16 result is their rounding)."""
+    g = gen(out)
+    inn = 700
+    w, ws = weights(g, 1, out, inn, True)
+    wt = tile(gpu, w)
+    W = torch.from_numpy(weights64(w[0], ws[0])).cuda()
+    for T in (1, 16, 17, 32, 33, 48, 49, 64):
+        x, xs = acts(g, T, inn, True)
+        want = torch.from_numpy(rows64(x, xs, inn)).cuda() @ W.T
+        y = torch.full((T + 1, out), 7.0, device="cuda", dtype=y_type)
+        linear8(gpu, x, xs, wt, ws, inn, out, y=y[:T])
+        assert torch.equal(y[:T], want.to(y_type)) and (y[T:] == 7).all(), T
 
 
 def test_linear_values(gpu):
@@ -109,7 +126,7 @@ def counts_to_offsets(n):
 
 GROUPED = [([0, 1, 0], 128, 16), ([3], 130, 17), ([1, 0, 2, 7, 8, 9, 0, 0, 15], 256, 130), ([16, 17, 31, 0, 33, 1], 1001, 300),
            ([64, 65, 0, 1, 30], 640, 128), ([100, 0, 127, 128, 129, 5, 300], 384, 257), ([256, 257, 600, 0, 1], 512, 520),
-           ([0] * 70 + [4] + [0] * 60 + [2, 3], 200, 40), ([1] * 384, 128, 33), ([2000, 0, 0, 1], 256, 128), ([0, 0], 128, 128)]
+           ([0] * 70 + [4] + [0] * 60 + [2, 3], 200, 40), ([1] * 384, 128, 33), ([2000, 0, 0, 1], 256, 128), ([0, 0], 128, 128), ([2] * 64, 128, 2040), ([12, 30, 1, 0, 17], 4200, 2040)]
 
 
 @pytest.mark.parametrize("case", range(len(GROUPED)))
@@ -173,6 +190,13 @@ def test_grouped_bounds(gpu):
         off = torch.tensor([-4, n + 7, 2, 1], device="cuda", dtype=torch.int32)
         grouped(gpu, y, x, xs, off, n, wt, ws, 128, 64)
         assert (y == 7).all()
+        # rows in their own order of which x has only the first ten
+        off = torch.tensor([0, n // 3, n // 2, n], device="cuda", dtype=torch.int32)
+        grouped(gpu, y, x, xs, off, n, wt, ws, 128, 64)
+        want = np.full((n, 64), 7.0)
+        for r in range(min(n, 10)):
+            want[r] = X[r] @ weights64(w[(r >= n // 3) + (r >= n // 2)], ws[(r >= n // 3) + (r >= n // 2)]).T
+        assert np.array_equal(f64(y), want)
 
 
 @pytest.mark.parametrize("y_type", [F32, BF16])
