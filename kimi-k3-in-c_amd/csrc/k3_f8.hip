@@ -505,12 +505,39 @@ __device__ __forceinline__ void put8(const K3kF8 &a, int t, int o, float (&v)[8]
     }
 }
 
+/* The largest magnitude among 8 neighbouring lanes. */
+__device__ __forceinline__ uint32_t max8_bits(uint32_t v)
+{
+    v = max(v, dpp_u32<0xB1, 0xf, 0u>(v));      /* quad_perm [1,0,3,2] */
+    v = max(v, dpp_u32<0x4E, 0xf, 0u>(v));      /* quad_perm [2,3,0,1] */
+    return max(v, dpp_u32<0x141, 0xf, 0u>(v));  /* row_half_mirror */
+}
+
+/* outputs o ..+8 of row t as 16-bit integers, 8 lanes to a group of 64 columns and its scale, max(largest magnitude, 2^-100) / 32767 (NaN or
+ * infinite as that is); every lane of the 8 takes part. Within 2^-15 of the group's largest: halves the bytes of fp32, where rows of bf16 would
+ * double the error of a bf16 result. */
+__device__ __forceinline__ void put8_ints(const K3kF8 &a, int t, int o, const float (&v)[8])
+{
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) m = max(m, abs_bits(v[i]));
+    const float most = __uint_as_float(max(max8_bits(m), __float_as_uint(0x1p-100f))), r = 1.0f / most;
+    if (t >= a.T || o >= a.ldy) return;
+    uint4 q;
+    q.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_i16(v[0] * r, v[1] * r));
+    q.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_i16(v[2] * r, v[3] * r));
+    q.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_i16(v[4] * r, v[5] * r));
+    q.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_i16(v[6] * r, v[7] * r));
+    *reinterpret_cast<uint4 *>((int16_t *)a.y + (size_t)t * a.ldy + o) = q;
+    if (o % 64 == 0) a.ys[(size_t)t * (a.ldy / 64) + o / 64] = most / 32767.0f;
+}
+
 /* bytes of LDS: the stages, the scales of x for 16 column blocks, and where each row's lie */
 constexpr int tile_lds(int bt, int bo, int nw, int nst) { return nst * (bt + bo) * 128 + 3 * ((bt / 8 + nw - 1) / nw * nw) * 256; }
 
 /* PAIR: the tile is 128 rows of W (gate) and the same of W2 (up), a wave has 32 of both, and what leaves is act(gate) up in 8 bits: a
- * row's 128 columns are one block of it, so its scale is the workgroup's own business. */
-template <int BT, int BO, int WT, int WO, int NST, bool WIDE, bool PAIR>
+ * row's 128 columns are one block of it, so its scale is the workgroup's own business. INTS: a.ys may ask for 16-bit integers. */
+template <int BT, int BO, int WT, int WO, int NST, bool WIDE, bool PAIR, bool INTS>
 __device__ __forceinline__ void tile_run(const F8Tile &p, const Job &job, int to, int sl, uint32_t *lds)
 {
     constexpr int NW = WT * WO, FT = BT / WT / 16, FO = BO / WO / 16;
@@ -757,6 +784,7 @@ __device__ __forceinline__ void tile_run(const F8Tile &p, const Job &job, int to
     constexpr int RB1 = 16 * WOUT;              /* 4-byte units of one fragment of rows */
     constexpr int LR = NST * SZ / NW;           /* of a wave's region */
     constexpr int JR = LR >= FT * RB1 ? FT : LR >= FT / 2 * RB1 ? FT / 2 : FT / 4, RB = JR * RB1;
+    static_assert(!INTS || WOUT == 64, "a group of 64 columns");
     static_assert(JR >= 1 && FT % JR == 0 && RB <= LR && 128 % C == 0, "epilogue regions");
     float4 *const reg = reinterpret_cast<float4 *>(lds + wv * RB);
     constexpr int RI = 128 / C, IT = 16 * JR / RI;              /* rows of a round of the wave, rounds */
@@ -794,7 +822,8 @@ __device__ __forceinline__ void tile_run(const F8Tile &p, const Job &job, int to
                 const int r = lane / (C / 2) + (i0 + i) * RI, x = r & 15 & (C - 1);
                 const float4 v0 = reg[r * C + (2 * c ^ x)], v1 = reg[r * C + ((2 * c + 1) ^ x)];
                 float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-                if (p.nsl == 1) put8(a, t[i], o, v, bs, res[i]);
+                if (INTS && a.ys) put8_ints(a, t[i], o, v);
+                else if (p.nsl == 1) put8(a, t[i], o, v, bs, res[i]);
                 else if (t[i] < a.T && o < a.out) part8(p.part + ((size_t)sl * a.T + t[i]) * a.out + o, v, a.out - o);
             }
         }
@@ -821,8 +850,8 @@ __global__ __launch_bounds__(64 * WT * WO) void f8_tile_kernel(F8Tile p)
         job = Job{0, tt * BT, min(BT, a.T - tt * BT)};
     }
     if constexpr (DUAL)
-        if (job.n <= BT / 2) return tile_run<BT / 2, BO, WT, WO, 3, WIDE, PAIR>(p, job, to, sl, lds);
-    tile_run<BT, BO, WT, WO, NST, WIDE, PAIR>(p, job, to, sl, lds);
+        if (job.n <= BT / 2) return tile_run<BT / 2, BO, WT, WO, 3, WIDE, PAIR, !PAIR>(p, job, to, sl, lds);
+    tile_run<BT, BO, WT, WO, NST, WIDE, PAIR, DUAL && !PAIR>(p, job, to, sl, lds);
 }
 
 /* the slices' sums, in slice order, and the epilogue; four slices requested at once */
@@ -1030,6 +1059,14 @@ extern "C" int k3k_grouped_f8(const K3kF8 *a, void *stream_)
     else tile_go<256, 256, 2, 4, 2, false, false, true>(&p, 1, st);
     K3K_LAUNCH_CHECK("grouped_f8: tiles");
     return 0;
+}
+
+extern "C" int k3k_slots_f8(const K3kF8 *a, float **ys, void *stream)
+{
+    K3kF8 s = *a;
+    s.y_type = K3D_F32;
+    *ys = s.ys = a->wide || few_rows(a) ? NULL : (float *)((int16_t *)a->y + (size_t)a->T * a->ldy);
+    return k3k_grouped_f8(&s, stream);
 }
 
 /* gate and up: W, W2 [experts], into hq / hs; gu: room for their sums, where few rows make them a launch of their own */

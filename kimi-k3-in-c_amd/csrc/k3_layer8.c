@@ -318,9 +318,9 @@ typedef struct {
 /* where each part lies in ws; the bytes of all (256-byte aligned parts) */
 static size_t moe_layout(MoeF8Ws *w, void *ws, int T, int hidden, int inter, int n_experts, int topk)
 {
-    const size_t N = (size_t)T * topk, nb = blocks(inter);
+    const size_t N = (size_t)T * topk, nb = blocks(inter), wide = ((size_t)hidden + 63) / 64 * 64;
     const size_t sizes[7] = {((size_t)n_experts + 1) * 4, N * 4, k3k_group_ws((int)N, n_experts), N * nb * 128, N * nb * 4,
-                             N * 2 * inter * 4, N * hidden * 4};
+                             N * 2 * inter * 4, N * wide * 4};
     size_t off = 0, at[7];
     for (int i = 0; i < 7; i++) {
         at[i] = off;
@@ -409,15 +409,13 @@ int k3d_moe_f8(void *out, int out_type, long ldo, const int *idx, const float *w
     a.x = w.hq;
     a.W = w2;
     a.W2 = NULL;
-    /* (a result of bf16 has no use for more than 8-bit instructions give; its slots' rows are rounded to bf16 themselves, which halves the bytes
-     * between the two kernels and adds half a step of each weighted row: 2048 tokens on 64 experts 1363 -> 1217 us) */
+    /* (a result of bf16 has no use for more than 8-bit instructions give) */
     a.wide = out_type == K3D_F32;
-    a.y_type = out_type;
     a.xs = w.hs;
     a.Ws = s2;
     a.x_rows = NULL;
     a.y_rows = w.perm;
-    a.ldy = hidden;
+    a.ldy = (hidden + 63L) / 64 * 64;
     a.ldx = blocks(inter) * 128L;
     a.ldxs = blocks(inter);
     a.ldws = blocks(inter);
@@ -427,15 +425,18 @@ int k3d_moe_f8(void *out, int out_type, long ldo, const int *idx, const float *w
     a.out = hidden;
     a.x_div = 1;
     a.x_cap = N;
-    if (k3k_grouped_f8(&a, stream)) return fail(fn);
+    float *ys;
+    if (k3k_slots_f8(&a, &ys, stream)) return fail(fn);
     k3k_prof_mark(stream, K3D_STAGE_DOWN);
     K3kSum s;
     s.out = out;
     s.y = w.y;
+    s.ys = ys;
+    s.ldy = a.ldy;
     s.wt = wt;
     s.idx = idx;
     s.ldo = ldo;
-    s.out_type = s.y_type = out_type;
+    s.out_type = out_type;
     s.T = T;
     s.topk = topk;
     s.n = hidden;

@@ -21,6 +21,7 @@ namespace {
 /* (16 bytes at any alignment of their elements: as one vector, where a copy of eight elements became smaller stores, 51 against 47 us at
  * 4096 rows of 7168) */
 typedef uint32_t u32x4a __attribute__((ext_vector_type(4), aligned(2)));
+typedef int16_t i16x8 __attribute__((ext_vector_type(8)));
 
 /* Elements i ..+8 of a row of n, zeros behind its end; any alignment of the elements. */
 template <int TYPE>
@@ -179,7 +180,8 @@ __global__ __launch_bounds__(256) void quant_kernel(K3kQuant a, unsigned t0, int
     put_codes<!GATED>(a.q, a.qs, t * a.ldq, t * a.ldqs, i, u, kb < nb);
 }
 
-/* Eight columns of one token to a thread; the slots' rows are requested four at a time. */
+/* Eight columns of one token to a thread; the slots' rows are requested four at a time. INTS: as integers with scales. */
+template <bool INTS>
 __global__ __launch_bounds__(256) void sum_slots_kernel(K3kSum a, unsigned t0, unsigned per)
 {
     const size_t t = t0 + blockIdx.x / per;
@@ -188,19 +190,24 @@ __global__ __launch_bounds__(256) void sum_slots_kernel(K3kSum a, unsigned t0, u
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (int j = 0; j < a.topk; j += 4) {
         float v[4][8], w[4];
+        i16x8 h[4];
         bool on[4];
 #pragma unroll
         for (int u = 0; u < 4; u++) {
             const size_t k = t * a.topk + min(j + u, a.topk - 1);
             on[u] = j + u < a.topk && (unsigned)a.idx[k] < (unsigned)a.n_experts;
             w[u] = a.wt[k];
-            load8_of(v[u], a.y, a.y_type, k * a.n, i, on[u] ? a.n : 0);
+            if (!on[u]) continue;
+            if constexpr (INTS) {
+                h[u] = *(const i16x8 *)((const int16_t *)a.y + k * a.ldy + i);
+                w[u] *= a.ys[k * (a.ldy / 64) + i / 64];
+            } else load8<K3D_F32>(v[u], (const float *)a.y + k * a.ldy, i, a.n);
         }
 #pragma unroll
         for (int u = 0; u < 4; u++)
             if (on[u])
 #pragma unroll
-                for (int c = 0; c < 8; c++) s[c] = fmaf(w[u], v[u][c], s[c]);
+                for (int c = 0; c < 8; c++) s[c] = fmaf(w[u], INTS ? (float)h[u][c] : v[u][c], s[c]);
     }
     store8_of(a.out, a.out_type, t * a.ldo, i, a.n, s);
 }
@@ -242,7 +249,10 @@ extern "C" int k3k_add_norm(const K3kNorm *a, void *stream)
 extern "C" int k3k_sum_slots(const K3kSum *a, void *stream)
 {
     const unsigned per = ((unsigned)a->n + 2047) / 2048;
-    each_launch(a->T, 256 * per, [&](unsigned t0, unsigned n) { sum_slots_kernel<<<n * per, 256, 0, (hipStream_t)stream>>>(*a, t0, per); });
+    each_launch(a->T, 256 * per, [&](unsigned t0, unsigned n) {
+        if (a->ys) sum_slots_kernel<true><<<n * per, 256, 0, (hipStream_t)stream>>>(*a, t0, per);
+        else sum_slots_kernel<false><<<n * per, 256, 0, (hipStream_t)stream>>>(*a, t0, per);
+    });
     K3K_LAUNCH_CHECK("sum_slots");
     return 0;
 }

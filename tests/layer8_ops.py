@@ -245,6 +245,9 @@ def moe64(X, idx, wt, W1, W3, W2, act, b1, b2, out_type):
             v, vt = product64(h, W2[e], out_type == BF16)
             vt = vt * 1.1 + ht @ np.abs(W2[e]).T
             y[t] += wt[t, j] * v[0]
-            # (bf16: each slot's row is rounded, by half a step, before it is weighted)
-            tol[t] += abs(wt[t, j]) * (vt[0] + np.abs(v[0]) * k * 2.0 ** -22 + (HALF[BF16] * (np.abs(v[0]) + vt[0]) if out_type == BF16 else 0.0))
+            tol[t] += abs(wt[t, j]) * (vt[0] + np.abs(v[0]) * k * 2.0 ** -22)
+            if out_type == BF16:        # a slot's row as 16-bit integers: a step of its 64 columns' largest / 32767, and the scale's own roundings
+                m = np.zeros(-(-v.shape[1] // 64) * 64)
+                m[:v.shape[1]] = np.abs(v[0]) + vt[0]
+                tol[t] += abs(wt[t, j]) * (np.repeat(np.maximum(m.reshape(-1, 64).max(1), LEAST), 64)[:v.shape[1]] * 2.0 ** -15 * 1.001)
     return y, tol
