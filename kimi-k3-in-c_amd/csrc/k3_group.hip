@@ -14,32 +14,32 @@ namespace {
 
 constexpr int GR_C = 1024, GR_ONE = 4, GR_MAXE = 2048;
 
-/* this slot's place among the wave's slots of its expert, their number, and whether it is the first of them */
-__device__ __forceinline__ void rank_wave(int e, bool valid, int &rank, int &count, bool &first)
+/* This slot's place among the wave's slots of its expert, their number, and whether it is the first of them: the lanes whose expert agrees in
+ * each bit (a ballot a bit; one for each expert that the wave holds would be up to 64). */
+__device__ __forceinline__ void rank_wave(int e, bool valid, int bits, int &rank, int &count, bool &first)
 {
-    const int lane = threadIdx.x & 63;
-    rank = count = 0;
-    first = false;
-    for (uint64_t todo = __ballot(valid); todo;) {
-        const int l = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)todo) - 1);
-        const uint64_t same = __ballot(valid && e == __builtin_amdgcn_readlane(e, l));
-        if (same >> lane & 1) {
-            rank = __popcll(same & ((1ull << lane) - 1));
-            count = __popcll(same);
-            first = lane == l;
-        }
-        todo &= ~same;
+    const uint64_t below = (1ull << (threadIdx.x & 63)) - 1;
+    uint64_t same = __ballot(valid);
+    for (int b = 0; b < bits; b++) {
+        const bool on = e >> b & 1;
+        const uint64_t m = __ballot(on);
+        same &= on ? m : ~m;
     }
+    rank = __popcll(same & below);
+    count = __popcll(same);
+    first = valid && rank == 0;
 }
 
-/* the slot's place among its expert's slots up to here: cnt counts them, wave after wave */
-__device__ __forceinline__ int rank_chunk(int *cnt, int e, bool valid)
+__device__ __forceinline__ int bits_of(int E) { return E < 2 ? 0 : 32 - __clz(E - 1); }
+
+/* the slot's place among its expert's slots up to here: cnt counts them, wave after wave of those that hold the chunk's n slots */
+__device__ __forceinline__ int rank_chunk(int *cnt, int e, bool valid, int bits, int n)
 {
     int rank, count;
     bool first;
-    rank_wave(e, valid, rank, count, first);
+    rank_wave(e, valid, bits, rank, count, first);
     const int wv = threadIdx.x >> 6;
-    for (int w = 0; w < GR_C / 64; w++) {
+    for (int w = 0; w < GR_C / 64 && w * 64 < n; w++) {
         if (w == wv && valid) {
             const int base = cnt[e];
             __builtin_amdgcn_wave_barrier();
@@ -84,7 +84,7 @@ __global__ __launch_bounds__(GR_C) void group_one_kernel(int *offsets, int *perm
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < GR_ONE; u++)
-        if (u * GR_C < N) rank[u] = rank_chunk(cnt, e[u], (unsigned)e[u] < (unsigned)E);
+        if (u * GR_C < N) rank[u] = rank_chunk(cnt, e[u], (unsigned)e[u] < (unsigned)E, bits_of(E), N - u * GR_C);
     const int total = scan_experts(cnt, off, waves);
     for (int i = tid; i <= E; i += GR_C) offsets[i] = i < E ? off[i] : total;
 #pragma unroll
@@ -140,7 +140,7 @@ __global__ __launch_bounds__(GR_C) void group_place_kernel(int *perm, const int 
     for (int k = tid; k < E; k += GR_C) cnt[k] = hist[(size_t)blockIdx.x * E + k];
     __syncthreads();
     const bool valid = (unsigned)e < (unsigned)E;
-    const int at = rank_chunk(cnt, e, valid);
+    const int at = rank_chunk(cnt, e, valid, bits_of(E), N - (int)blockIdx.x * GR_C);
     if (valid) perm[at] = i;
 }
 
