@@ -3,9 +3,10 @@
  * k3_group.hip -- a routing's slots by expert (k3d_group): offsets[e] .. offsets[e + 1] of perm are the slots t * topk + j
  * whose expert is e, ascending; slots without an expert are in none.
  *
- * A counting sort, the same order every time: a wave ranks its slots among equal experts by ballots, its workgroup's waves
- * add their counts to the experts' one after another. Up to 4096 slots in one workgroup; more in chunks of 1024, whose
- * counts are summed by chunk before the slots take their places. Bound by latency: barriers and launches.
+ * A counting sort, the same order every time: a wave ranks its slots among equal experts by ballots, each expert's counts are summed over
+ * the workgroup's waves in their order. Up to 4096 slots in one workgroup; more in chunks of 1024, whose
+ * counts are summed by chunk before the slots take their places. Bound by latency: barriers and launches (one token of 8 3.3 us, 64 3.9, 512
+ * 8.0, 2048 in three launches 8.4; 20000 23.4).
  */
 #include "k3_common.h"
 #include "k3k.h"
@@ -32,23 +33,32 @@ __device__ __forceinline__ void rank_wave(int e, bool valid, int bits, int &rank
 
 __device__ __forceinline__ int bits_of(int E) { return E < 2 ? 0 : 32 - __clz(E - 1); }
 
-/* the slot's place among its expert's slots up to here: cnt counts them, wave after wave of those that hold the chunk's n slots */
-__device__ __forceinline__ int rank_chunk(int *cnt, int e, bool valid, int bits, int n)
+/* The slot's place among its expert's slots up to here: cnt counts them, over the chunk's n slots; by: counts of each wave, [waves][E up to a
+ * pair]. (Waves that add to cnt one after another, with a barrier each, took twice as long: 4096 slots 13.4 us.) */
+__device__ __forceinline__ int rank_chunk(int *cnt, uint16_t *by, int e, bool valid, int E, int n)
 {
     int rank, count;
     bool first;
-    rank_wave(e, valid, bits, rank, count, first);
-    const int wv = threadIdx.x >> 6;
-    for (int w = 0; w < GR_C / 64 && w * 64 < n; w++) {
-        if (w == wv && valid) {
-            const int base = cnt[e];
-            __builtin_amdgcn_wave_barrier();
-            if (first) cnt[e] = base + count;
-            rank += base;
+    const int waves = min(GR_C / 64, (n + 63) / 64), S = (E + 1) / 2 * 2;
+    for (int k = threadIdx.x; k < waves * S / 2; k += GR_C) reinterpret_cast<uint32_t *>(by)[k] = 0;
+    rank_wave(e, valid, bits_of(E), rank, count, first);
+    uint16_t *const mine = by + (threadIdx.x >> 6) * S;
+    __syncthreads();
+    if (first) mine[e] = (uint16_t)count;
+    __syncthreads();
+    for (int k = threadIdx.x; k < E; k += GR_C) {
+        int s = cnt[k];
+        for (int w = 0; w < waves; w++) {
+            const int c = by[w * S + k];
+            by[w * S + k] = (uint16_t)s;
+            s += c;
         }
-        __syncthreads();
+        cnt[k] = s;
     }
-    return rank;
+    __syncthreads();
+    const int at = valid ? mine[e] + rank : 0;
+    __syncthreads();            /* (the next chunk's counts take the same place) */
+    return at;
 }
 
 /* off[e]: the sum of n[0 .. e) of GR_MAXE entries, two a thread; the whole sum returned */
@@ -77,6 +87,7 @@ __device__ __forceinline__ int scan_experts(const int *n, int *off, int *waves)
 __global__ __launch_bounds__(GR_C) void group_one_kernel(int *offsets, int *perm, const int *idx, int N, int E)
 {
     __shared__ int cnt[GR_MAXE], off[GR_MAXE], waves[GR_C / 64];
+    __shared__ uint32_t by[GR_C / 64 * GR_MAXE / 2];
     const int tid = threadIdx.x;
     int e[GR_ONE], rank[GR_ONE];
     for (int u = 0; u < GR_ONE; u++) e[u] = u * GR_C + tid < N ? idx[u * GR_C + tid] : -1;
@@ -84,7 +95,7 @@ __global__ __launch_bounds__(GR_C) void group_one_kernel(int *offsets, int *perm
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < GR_ONE; u++)
-        if (u * GR_C < N) rank[u] = rank_chunk(cnt, e[u], (unsigned)e[u] < (unsigned)E, bits_of(E), N - u * GR_C);
+        if (u * GR_C < N) rank[u] = rank_chunk(cnt, (uint16_t *)by, e[u], (unsigned)e[u] < (unsigned)E, E, N - u * GR_C);
     const int total = scan_experts(cnt, off, waves);
     for (int i = tid; i <= E; i += GR_C) offsets[i] = i < E ? off[i] : total;
 #pragma unroll
@@ -135,13 +146,15 @@ __global__ __launch_bounds__(GR_C) void group_scan_kernel(int *offsets, int *his
 __global__ __launch_bounds__(GR_C) void group_place_kernel(int *perm, const int *hist, const int *idx, int N, int E)
 {
     __shared__ int cnt[GR_MAXE];
+    __shared__ uint32_t by[GR_C / 64 * GR_MAXE / 2];
     const int tid = threadIdx.x, i = blockIdx.x * GR_C + tid;
     const int e = i < N ? idx[i] : -1;
-    for (int k = tid; k < E; k += GR_C) cnt[k] = hist[(size_t)blockIdx.x * E + k];
-    __syncthreads();
     const bool valid = (unsigned)e < (unsigned)E;
-    const int at = rank_chunk(cnt, e, valid, bits_of(E), N - (int)blockIdx.x * GR_C);
-    if (valid) perm[at] = i;
+    const int from = valid ? hist[(size_t)blockIdx.x * E + e] : 0;
+    for (int k = tid; k < E; k += GR_C) cnt[k] = 0;
+    __syncthreads();
+    const int at = rank_chunk(cnt, (uint16_t *)by, e, valid, E, N - (int)blockIdx.x * GR_C);
+    if (valid) perm[from + at] = i;
 }
 
 }  // namespace
