@@ -312,7 +312,8 @@ __global__ __launch_bounds__(64 * SK_NW) void f8_skinny_kernel(K3kF8 a, int o0, 
     auto buf_of = [&](auto slot) -> uint32_t * { return stage_of<decltype(slot)::value, NW * XW>() + wv * XW; };
     u32x4 wr[R][RW][2];
     int at = 0;                                 /* the block requested next */
-    auto load = [&](auto slot) {
+    /* (inlined in any case: a call would put what the bodies share in memory, 64 tokens of 7168 -> 12288 to fp32 in 360 us) */
+    auto load = [&](auto slot) __attribute__((always_inline)) {
         constexpr int S = decltype(slot)::value;
         const uint32_t none = at < n ? 0u : F8_OOB, kb = k0 + at;
 #pragma unroll
@@ -329,7 +330,7 @@ __global__ __launch_bounds__(64 * SK_NW) void f8_skinny_kernel(K3kF8 a, int o0, 
 #pragma unroll
         for (int j = 0; j < NT; j++) acc[q][j] = k3_f32x4{0.f, 0.f, 0.f, 0.f};
     int i = 0;
-    auto use = [&](auto slot) {
+    auto use = [&](auto slot) __attribute__((always_inline)) {
         constexpr int S = decltype(slot)::value;
         const uint32_t *const b = buf_of(slot);
         const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wsc), i & 63));
@@ -345,12 +346,12 @@ __global__ __launch_bounds__(64 * SK_NW) void f8_skinny_kernel(K3kF8 a, int o0, 
             for (int h = 0; h < 2; h++) xf[j][h] = *reinterpret_cast<const u32x4 *>(b + (16 * j + r16) * 32 + (((4 * h + g) ^ sw(r16)) & 7) * 4);
         Wide ww[WIDE ? RW : 1];
         if constexpr (WIDE) each_of<0, RW>([&](auto q) { ww[decltype(q)::value] = widen(wr[S][decltype(q)::value][0], wr[S][decltype(q)::value][1]); });
-        each_of<0, NT>([&](auto jj) {
+        each_of<0, NT>([&](auto jj) __attribute__((always_inline)) {
             constexpr int j = decltype(jj)::value;
             const float xs = __uint_as_float(sc[(i & 15) * NT * 16 + 16 * j + r16]);
             Wide xw;
             if constexpr (WIDE) xw = widen(xf[j][0], xf[j][1]);
-            each_of<0, RW>([&](auto qq) {
+            each_of<0, RW>([&](auto qq) __attribute__((always_inline)) {
                 constexpr int q = decltype(qq)::value;
                 const float f = xs * (TWO && (rt0 + q) / F8_G != rb ? w2 : w);
                 k3_f32x4 v;
@@ -374,18 +375,18 @@ __global__ __launch_bounds__(64 * SK_NW) void f8_skinny_kernel(K3kF8 a, int o0, 
     int left = n;
     /* block k is used while block k + R - 1 is requested, into the stage that block k - 1 left */
     for (; left >= R; left -= R)
-        each_of<0, R>([&](auto slot) {
+        each_of<0, R>([&](auto slot) __attribute__((always_inline)) {
             load(std::integral_constant<int, (decltype(slot)::value + R - 1) % R>{});
             use(slot);
         });
-    each_of<0, R - 1>([&](auto slot) {
+    each_of<0, R - 1>([&](auto slot) __attribute__((always_inline)) {
         if (decltype(slot)::value < left) use(slot);
     });
 
     /* the waves' sums, in their order, 16 rows of W at a time, where the last requests (of zeros) have landed */
     __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));
     float4 *const part = reinterpret_cast<float4 *>(buf_of(std::integral_constant<int, 0>{}));
-    each_of<0, RW>([&](auto qq) {
+    each_of<0, RW>([&](auto qq) __attribute__((always_inline)) {
         constexpr int q = decltype(qq)::value;
         __syncthreads();
 #pragma unroll
@@ -831,6 +832,10 @@ __device__ __forceinline__ void tile_run(const F8Tile &p, const Job &job, int to
     });
 }
 
+/* Bound by the matrix cores and the clock under their power where rows are many (4096 tokens of 7168 -> 12288 with silu 316 to 328 us, 2.2 PFLOP/s at some
+ * 1.95 GHz; without the scales a library's product takes 263), 13 us of a tile's first requests and epilogue with nothing beside them among it. Experts of about a
+ * tile's rows ask for W, 8 MB a step of all workgroups, as fast as memory gives it, and wait: gate and up of 64 experts of 256 rows 606 us, the same
+ * rows on 32 experts 447. Tiles of 128 rows there, with three stages, took 10 % more at 256 rows and 4 % less at 264. */
 /* DUAL: passes of at most half the rows by a kernel of half the rows and three stages, which takes little over half the time (2048 tokens, eight of 64
  * experts each: half of the experts have a pass of some 16 rows behind one of 256) */
 template <int BT, int BO, int WT, int WO, int NST, bool WIDE, bool PAIR, bool DUAL>
