@@ -202,6 +202,7 @@ __device__ __forceinline__ Job find_job(const K3kF8 &a, const Jobs &s, int j, in
 /* the row of x of a job's i-th row, -1 for none */
 __device__ __forceinline__ int x_row(const K3kF8 &a, int r)
 {
+    if (a.slot_e) return r / a.x_div;
     if (!a.offsets) return r;
     int t = r;
     if (a.x_rows) {
@@ -246,7 +247,7 @@ __global__ __launch_bounds__(64 * SK_NW) void f8_skinny_kernel(K3kF8 a, int o0, 
     __shared__ uint32_t SC[NW * NT * 256];
     Job job = {0, 0, a.T};
     int o = blockIdx.x;
-    if (a.offsets) {
+    if (a.offsets || a.slot_e) {
         const int j = blockIdx.x / (unsigned)og;
         o -= j * og;
         if (a.W2 && 2 * o >= og) {              /* the second matrix, its outputs behind the first's */
@@ -255,7 +256,10 @@ __global__ __launch_bounds__(64 * SK_NW) void f8_skinny_kernel(K3kF8 a, int o0, 
             a.Ws = a.Ws2;
             a.y = (float *)a.y + a.out;
         }
-        job = find_job(a, count_jobs(a, 8 * NP), j, 8 * NP);
+        if (a.slot_e) {
+            const int e = a.slot_e[j];
+            job = Job{e, j, (unsigned)e < (unsigned)a.n_experts ? 1 : 0};
+        } else job = find_job(a, count_jobs(a, 8 * NP), j, 8 * NP);
         if (job.n == 0) return;
     }
     const int rt0 = (o0 + o) * RW;
@@ -913,7 +917,7 @@ void skinny_go(const K3kF8 *a, long jobs, hipStream_t st)
 {
     /* (a launch takes under 2^32 work-items) */
     const long og = ((a->out + 15) / 16 + RW - 1) / RW, mats = a->W2 ? 2 : 1, most = ((1L << 32) - 1) / (64 * SK_NW) / (jobs * mats);
-    const bool nt = tiled_bytes(a->out, a->in) * (a->offsets ? a->n_experts * mats : 1) >= F8_NT_BYTES;
+    const bool nt = tiled_bytes(a->out, a->in) * (a->offsets || a->slot_e ? a->n_experts * mats : 1) >= F8_NT_BYTES;
     for (long o = 0; o < og; o += most) {
         const int n = (int)(og - o < most ? og - o : most) * mats;
         const unsigned grid = (unsigned)(jobs * n);
@@ -929,7 +933,8 @@ void skinny_rows(const K3kF8 *a, hipStream_t st)
 {
     /* The rows of W of a workgroup: a CU takes in 46 KB/us, W and x for each of its workgroups (64 tokens of 7168 -> 12288: 256 workgroups of 48 rows
      * 24.5 us, 384 of 32 33, 192 of 64 26.7). By expert: as if each expert had one pass. */
-    const long jobs = a->offsets ? most_jobs(a, 8 * NP) : 1, about = a->offsets ? (a->rows < a->n_experts ? a->rows : a->n_experts) * (a->W2 ? 2 : 1) : 1;
+    const bool by = a->offsets || a->slot_e;
+    const long jobs = a->slot_e ? a->rows : a->offsets ? most_jobs(a, 8 * NP) : 1, about = by ? (a->rows < a->n_experts ? a->rows : a->n_experts) * (a->W2 ? 2 : 1) : 1;
     const long tiles = (a->out + 15) / 16, cus = k3k_cu_count();
     int rw = 1;
     long best = 0;

@@ -371,9 +371,10 @@ int k3d_moe_f8(void *out, int out_type, long ldo, const int *idx, const float *w
     if (!aligned(ws, 16)) return refuse(fn, "the workspace must be 16-byte aligned");
     if (out == (const void *)x || out == ws || out == (const void *)wt || out == (const void *)idx || out == (const void *)xs)
         return refuse(fn, "out lies in an operand's place");
-    const int N = T * topk;
+    const int N = T * topk, one = T == 1 && topk <= n_experts;
     k3k_prof_mark(stream, K3D_STAGE_BEGIN);
-    if (k3k_group(w.offsets, w.perm, idx, N, n_experts, w.hist, stream)) return fail(fn);
+    /* (one token's slots are rows of experts of their own: no launch to sort them, and no offsets to search) */
+    if (!one && k3k_group(w.offsets, w.perm, idx, N, n_experts, w.hist, stream)) return fail(fn);
     k3k_prof_mark(stream, K3D_STAGE_GATHER);
     K3kF8 a;
     memset(&a, 0, sizeof a);
@@ -383,8 +384,9 @@ int k3d_moe_f8(void *out, int out_type, long ldo, const int *idx, const float *w
     a.xs = xs;
     a.Ws = s1;
     a.Ws2 = s3;
-    a.offsets = w.offsets;
-    a.x_rows = w.perm;
+    a.offsets = one ? NULL : w.offsets;
+    a.slot_e = one ? idx : NULL;
+    a.x_rows = one ? NULL : w.perm;
     a.ldx = ldx;
     a.ldxs = ldxs;
     a.ldws = blocks(hidden);
@@ -414,7 +416,7 @@ int k3d_moe_f8(void *out, int out_type, long ldo, const int *idx, const float *w
     a.xs = w.hs;
     a.Ws = s2;
     a.x_rows = NULL;
-    a.y_rows = w.perm;
+    a.y_rows = one ? NULL : w.perm;
     a.ldy = (hidden + 63L) / 64 * 64;
     a.ldx = blocks(inter) * 128L;
     a.ldxs = blocks(inter);

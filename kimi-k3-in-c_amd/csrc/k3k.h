@@ -410,6 +410,7 @@ typedef struct {
     int y_type, T, in, out, act, rows, x_div, x_cap, n_experts;
     void *ws;
     int wide;                   /* products as exact as fp32 (else 8-bit instructions) */
+    const int *slot_e;          /* in place of offsets, few rows: row r's expert (none outside [0, n_experts)), its row of x r / x_div, of y r */
     float *ys;                  /* k3k_slots_f8: y is 16-bit integers, whole groups of 64 columns, these their scales [T][ldy / 64] */
     /* k3k_gateup_f8 */
     const uint8_t *W2;

@@ -305,3 +305,46 @@ def test_two_graphs(gpu, k3, T):
             if ex:
                 L.k3d_graph_destroy(ex)
             L.k3d_stream_destroy(st)
+
+
+def test_past_32_bits(gpu, k3):
+    """Rows, results and weights that lie more than 2^32 bytes from the first."""
+    g = lo.gen(3)
+    T, n = 530000, 4160
+    say("case: rows past 2^32 bytes")
+    x = torch.zeros(T, n, device="cuda", dtype=BF16)
+    some = [0, T // 2, T - 1]
+    x[some] = torch.randn(3, n, device="cuda", generator=g).to(BF16)
+    q, qs = torch.empty(T, l8.nb(n) * 128, device="cuda", dtype=torch.uint8), torch.empty(T, l8.nb(n), device="cuda")
+    s = torch.empty_like(x)
+    l8.add_norm(k3, x, None, None, EPS, y=None, q=q, qs=qs, sum_=s)
+    _, u, tol = l8.norm64(x[some], None, None, EPS)
+    l8.check_codes(q[some], qs[some], u, tol, n)
+    assert torch.equal(s, x)
+    q.zero_()
+    l8.quant(k3, x, q=q, qs=qs)
+    l8.check_codes(q[some], qs[some], lo.f64(x[some]), 0 * u, n)
+    del x, s, q, qs
+    say("case: weights and results past 2^32 bytes")
+    experts, inn, out, rows = 300, 2048, 8192, 150000
+    w = torch.randint(0, 0x70, (1, out, inn), device="cuda", generator=g, dtype=torch.uint8)
+    size = k3.lib().k3d_f8_tiled_bytes(out, inn)
+    W = torch.zeros(experts * size, device="cuda", dtype=torch.uint8)
+    W[-size:] = l8.tile(k3, w)
+    ws = torch.rand(experts, l8.nb(out), l8.nb(inn), device="cuda", generator=g) * 1e-3
+    assert W.numel() > 1 << 32 and rows * out * 4 > 1 << 32
+    xq, xs = l8.acts(g, rows, inn)
+    for last in (5, 140):                       # rows of the last expert
+        off = torch.full((experts + 1,), rows - last, device="cuda", dtype=torch.int32)
+        off[0], off[-1] = rows - last, rows
+        for n_rows in (rows, 299 * 3):          # (what is chosen by: many rows an expert, or few)
+            y = torch.full((rows, out), 7.0, device="cuda")
+            o = off if n_rows == rows else off - (rows - last) + n_rows - last
+            sl = slice(rows - n_rows, rows)     # (x from its start on, so that row numbers fit)
+            yr = torch.arange(rows - n_rows, rows, device="cuda", dtype=torch.int32)
+            l8.grouped(k3, y, xq[sl], xs[sl], o, n_rows, W, ws, inn, out, y_rows=yr)
+            X = l8.rows64(xq[rows - last:], xs[rows - last:], inn)
+            v, tol = l8.product64(X[[0, last - 1]], l8.weights64(w[0], ws[-1]))
+            lo.within(y[[rows - last, rows - 1]], (v, tol + np.abs(v) * lo.HALF[F32]))
+            assert (y[:rows - last] == 7).all()
+    torch.cuda.synchronize()

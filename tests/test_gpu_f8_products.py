@@ -221,7 +221,7 @@ def rng_counts(g, e, most):
     return torch.randint(0, 2 * most, (e,), device="cuda", generator=g).tolist()
 
 
-MOE = [(1, 8, 16, 256, 128, SILU), (1, 1, 1, 100, 30, SITU), (5, 2, 4, 130, 200, SITU), (33, 8, 12, 512, 384, SILU), (64, 4, 3, 384, 256, SITU),
+MOE = [(1, 8, 16, 256, 128, SILU), (1, 1, 1, 100, 30, SITU), (1, 8, 3, 200, 130, SITU), (1, 64, 70, 300, 200, SILU), (5, 2, 4, 130, 200, SITU), (33, 8, 12, 512, 384, SILU), (64, 4, 3, 384, 256, SITU),
        (200, 2, 3, 256, 300, SILU)]
 
 
@@ -250,7 +250,7 @@ def test_moe_is_its_parts(gpu):
     """The layer gives what its parts give one after another, rounded alike (sums of integers, exact in every instruction)."""
     from layer8_ops import quant
     g = gen(2)
-    for T in (3, 70, 400):
+    for T in (1, 3, 70, 400):
         k, experts, hidden, inter = 4, 6, 512, 256
         x, xs = acts(g, T, hidden, True)
         w = [weights(g, experts, o, i, True) for o, i in ((inter, hidden), (inter, hidden), (hidden, inter))]
