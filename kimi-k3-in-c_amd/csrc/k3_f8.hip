@@ -137,6 +137,7 @@ struct Job {
  * experts. Offsets out of order or range count as no rows. */
 struct Jobs {
     int total, before, mine, per;       /* passes; of the lanes before; of this lane; experts a lane */
+    int n, r0;                          /* (one expert a lane) its rows, the first */
 };
 
 __device__ __forceinline__ int rows_of(const K3kF8 &a, int e, int &r0)
@@ -159,6 +160,7 @@ __device__ __forceinline__ Jobs count_jobs(const K3kF8 &a, int most)
         for (int u = 0; u < 4; u++) {
             int r0 = 0;
             n[u] = i + u < s.per ? rows_of(a, lane * s.per + i + u, r0) : 0;
+            if (u == 0) s.n = n[0], s.r0 = r0;
         }
 #pragma unroll
         for (int u = 0; u < 4; u++) s.mine += (n[u] + most - 1) / most;
@@ -182,6 +184,10 @@ __device__ __forceinline__ Job find_job(const K3kF8 &a, const Jobs &s, int j, in
     if (!who) return job;
     const int l = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)who) - 1);
     int left = j - __builtin_amdgcn_readlane(s.before, l);
+    if (s.per == 1) {           /* (no second look at the offsets: 2048 tokens on 64 experts 1229 -> 1214 us) */
+        const int n = __builtin_amdgcn_readlane(s.n, l);
+        return Job{l, __builtin_amdgcn_readlane(s.r0, l) + left * most, min(most, n - left * most)};
+    }
     /* the lane's experts, one to a lane now */
     int r0 = 0, n = lane < s.per ? rows_of(a, l * s.per + lane, r0) : 0;
     const int p = (n + most - 1) / most;
