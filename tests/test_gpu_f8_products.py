@@ -268,3 +268,33 @@ def test_moe_is_its_parts(gpu):
         want = f64(y).reshape(T, k, hidden) * f64(wt)[:, :, None]
         S = np.abs(want).sum(1)
         assert (np.abs(f64(out) - want.sum(1)) <= S * 2.0 ** -20).all()
+
+
+@pytest.mark.parametrize("T", [1, 5, 300])
+@pytest.mark.parametrize("out_type", [F32, BF16])
+def test_moe_values(gpu, T, out_type):
+    """A token that is no number stays alone with it, a token without experts is zero, and the same expert twice counts twice."""
+    g = gen(T)
+    k, experts, hidden, inter = 3, 4, 384, 256
+    x, xs = acts(g, T, hidden)
+    bank = [(tile(gpu, q), s) for q, s in (weights(g, experts, o, i) for o, i in ((inter, hidden), (inter, hidden), (hidden, inter)))]
+    idx = torch.randint(0, experts, (T, k), device="cuda", generator=g, dtype=torch.int32)
+    wt = torch.rand(T, k, device="cuda", generator=g)
+    at = T // 2
+    idx[at] = torch.tensor([-1, experts, -2 ** 31], dtype=torch.int32)
+    assert (moe8(gpu, x, xs, idx, wt, bank, hidden, inter, out_type=out_type)[at] == 0).all()
+    idx[at] = torch.tensor([1, 1, -1], dtype=torch.int32)
+    clean = moe8(gpu, x, xs, idx, wt, bank, hidden, inter, out_type=out_type)
+    once, both = idx.clone(), wt.clone()
+    once[at, 1], both[at, 0] = -1, wt[at, 0] + wt[at, 1]
+    y = moe8(gpu, x, xs, once, both, bank, hidden, inter, out_type=out_type)
+    # (the two weights' sum and the two products are rounded, and then the result)
+    d = np.abs(f64(y[at]) - f64(clean[at]))
+    assert (d <= np.abs(f64(clean[at])) * (2.0 ** -22 + 2 * HALF[out_type])).all()
+    for bad in (float("nan"), float("inf")):
+        s = xs.clone()
+        s[at, 1] = bad
+        y = moe8(gpu, x, s, idx, wt, bank, hidden, inter, out_type=out_type)
+        assert torch.isnan(y[at]).all()
+        y[at] = clean[at]
+        assert torch.equal(y, clean)
