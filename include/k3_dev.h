@@ -327,7 +327,7 @@ int k3d_grouped_f8(void *y, int y_type, long ldy, const int *y_rows, int y_cap, 
 /* The experts' layer for a routing in idx/wt [T][topk] (k3d_route's), weights in 8 bits: out[t] = sum_j wt[t][j] W2_e (act(W1_e x[t]) * (W3_e x[t])),
  * e = idx[t][j], act and b1, b2 as in k3d_quant_f8. The gated activation goes through 8 bits as k3d_quant_f8 rounds it; gate and up, and
  * with out_type K3D_BF16 the down products, are formed by 8-bit instructions, as k3d_linear_f8's of bf16 are; many tokens' down products for a bf16 out
- * wait for their sum as 16-bit integers with a scale for each 64 columns (within 2^-15 of the largest of them; one that is no number makes the 64 none). The weighted sum
+ * wait for their sum as 16-bit floats with a power of two for each 64 columns (within 2^-11 of the value, or 2^-39 of the largest of them). The weighted sum
  * is fp32, rounded once to out_type. Slots whose idx lies outside [0, n_experts) contribute nothing; a token without any becomes 0. w1, w3 [n_experts] matrices [inter][hidden], w2
  * [hidden][inter] from k3d_f8_tile, s1, s3, s2 their scales as in k3d_grouped_f8. ws (k3d_moe_f8_ws bytes; 16-byte aligned) is scratch of one call. */
 size_t k3d_moe_f8_ws(int T, int hidden, int inter, int n_experts, int topk);

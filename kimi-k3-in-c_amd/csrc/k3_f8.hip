@@ -26,6 +26,7 @@ namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));     /* (a load of uint4 loses what tells LDS arrays apart) */
 constexpr uint32_t F8_OOB = 0x80000000u;        /* a buffer offset past any descriptor used here */
 
@@ -524,31 +525,30 @@ __device__ __forceinline__ uint32_t max8_bits(uint32_t v)
     return max(v, dpp_u32<0x141, 0xf, 0u>(v));  /* row_half_mirror */
 }
 
-/* outputs o ..+8 of row t as 16-bit integers, 8 lanes to a group of 64 columns and its scale, max(largest magnitude, 2^-100) / 32767 (NaN or
- * infinite as that is); every lane of the 8 takes part. Within 2^-15 of the group's largest: halves the bytes of fp32, where rows of bf16 would
- * double the error of a bf16 result. */
-__device__ __forceinline__ void put8_ints(const K3kF8 &a, int t, int o, const float (&v)[8])
+/* outputs o ..+8 of row t as 16-bit floats, 8 lanes to a group of 64 columns and its scale, the power of two that brings the largest finite magnitude
+ * (2^-100 at least) to 2^14 ..+2^14; every lane of the 8 takes part. Within 2^-11 of the value, down to 2^-28 of the group's largest; half the bytes of fp32
+ * (16-bit integers, as exact beside the largest, left an output 2^11 below it four bits). What is no number stays alone. */
+__device__ __forceinline__ void put8_halves(const K3kF8 &a, int t, int o, const float (&v)[8])
 {
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) m = max(m, abs_bits(v[i]));
-    const float most = __uint_as_float(max(max8_bits(m), __float_as_uint(0x1p-100f))), r = 1.0f / most;
+    for (int i = 0; i < 8; i++) m = max(m, abs_bits(v[i]) < 0x7f800000u ? abs_bits(v[i]) : 0u);
+    const uint32_t e = max(max8_bits(m) >> 23, 27u);            /* (biased) */
+    const float r = __uint_as_float((268 - e) << 23);
     if (t >= a.T || o >= a.ldy) return;
-    uint4 q;
-    q.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_i16(v[0] * r, v[1] * r));
-    q.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_i16(v[2] * r, v[3] * r));
-    q.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_i16(v[4] * r, v[5] * r));
-    q.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_i16(v[6] * r, v[7] * r));
-    *reinterpret_cast<uint4 *>((int16_t *)a.y + (size_t)t * a.ldy + o) = q;
-    if (o % 64 == 0) a.ys[(size_t)t * (a.ldy / 64) + o / 64] = most / 32767.0f;
+    f16x8 h;
+#pragma unroll
+    for (int i = 0; i < 8; i++) h[i] = (_Float16)(v[i] * r);
+    *reinterpret_cast<f16x8 *>((_Float16 *)a.y + (size_t)t * a.ldy + o) = h;
+    if (o % 64 == 0) a.ys[(size_t)t * (a.ldy / 64) + o / 64] = __uint_as_float((e - 14) << 23);
 }
 
 /* bytes of LDS: the stages, the scales of x for 16 column blocks, and where each row's lie */
 constexpr int tile_lds(int bt, int bo, int nw, int nst) { return nst * (bt + bo) * 128 + 3 * ((bt / 8 + nw - 1) / nw * nw) * 256; }
 
 /* PAIR: the tile is 128 rows of W (gate) and the same of W2 (up), a wave has 32 of both, and what leaves is act(gate) up in 8 bits: a
- * row's 128 columns are one block of it, so its scale is the workgroup's own business. INTS: a.ys may ask for 16-bit integers. */
-template <int BT, int BO, int WT, int WO, int NST, bool WIDE, bool PAIR, bool INTS>
+ * row's 128 columns are one block of it, so its scale is the workgroup's own business. HALVES: a.ys may ask for 16-bit floats. */
+template <int BT, int BO, int WT, int WO, int NST, bool WIDE, bool PAIR, bool HALVES>
 __device__ __forceinline__ void tile_run(const F8Tile &p, const Job &job, int to, int sl, uint32_t *lds)
 {
     constexpr int NW = WT * WO, FT = BT / WT / 16, FO = BO / WO / 16;
@@ -795,7 +795,7 @@ __device__ __forceinline__ void tile_run(const F8Tile &p, const Job &job, int to
     constexpr int RB1 = 16 * WOUT;              /* 4-byte units of one fragment of rows */
     constexpr int LR = NST * SZ / NW;           /* of a wave's region */
     constexpr int JR = LR >= FT * RB1 ? FT : LR >= FT / 2 * RB1 ? FT / 2 : FT / 4, RB = JR * RB1;
-    static_assert(!INTS || WOUT == 64, "a group of 64 columns");
+    static_assert(!HALVES || WOUT == 64, "a group of 64 columns");
     static_assert(JR >= 1 && FT % JR == 0 && RB <= LR && 128 % C == 0, "epilogue regions");
     float4 *const reg = reinterpret_cast<float4 *>(lds + wv * RB);
     constexpr int RI = 128 / C, IT = 16 * JR / RI;              /* rows of a round of the wave, rounds */
@@ -833,7 +833,7 @@ __device__ __forceinline__ void tile_run(const F8Tile &p, const Job &job, int to
                 const int r = lane / (C / 2) + (i0 + i) * RI, x = r & 15 & (C - 1);
                 const float4 v0 = reg[r * C + (2 * c ^ x)], v1 = reg[r * C + ((2 * c + 1) ^ x)];
                 float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-                if (INTS && a.ys) put8_ints(a, t[i], o, v);
+                if (HALVES && a.ys) put8_halves(a, t[i], o, v);
                 else if (p.nsl == 1) put8(a, t[i], o, v, bs, res[i]);
                 else if (t[i] < a.T && o < a.out) part8(p.part + ((size_t)sl * a.T + t[i]) * a.out + o, v, a.out - o);
             }
@@ -1081,7 +1081,7 @@ extern "C" int k3k_slots_f8(const K3kF8 *a, float **ys, void *stream)
 {
     K3kF8 s = *a;
     s.y_type = K3D_F32;
-    *ys = s.ys = a->wide || few_rows(a) ? NULL : (float *)((int16_t *)a->y + (size_t)a->T * a->ldy);
+    *ys = s.ys = a->wide || few_rows(a) ? NULL : (float *)((_Float16 *)a->y + (size_t)a->T * a->ldy);
     return k3k_grouped_f8(&s, stream);
 }
 

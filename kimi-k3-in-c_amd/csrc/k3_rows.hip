@@ -21,7 +21,7 @@ namespace {
 /* (16 bytes at any alignment of their elements: as one vector, where a copy of eight elements became smaller stores, 51 against 47 us at
  * 4096 rows of 7168) */
 typedef uint32_t u32x4a __attribute__((ext_vector_type(4), aligned(2)));
-typedef int16_t i16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 /* Elements i ..+8 of a row of n, zeros behind its end; any alignment of the elements. */
 template <int TYPE>
@@ -181,9 +181,9 @@ __global__ __launch_bounds__(256) void quant_kernel(K3kQuant a, unsigned t0, int
     put_codes<!GATED>(a.q, a.qs, t * a.ldq, t * a.ldqs, i, u, kb < nb);
 }
 
-/* Eight columns of one token to a thread; the slots' rows are requested four at a time. INTS: as integers with scales (2048
+/* Eight columns of one token to a thread; the slots' rows are requested four at a time. HALVES: as 16-bit floats with scales (2048
  * tokens of 8 slots of 7168 51 us, 5.4 TB/s; as fp32 113). */
-template <bool INTS>
+template <bool HALVES>
 __global__ __launch_bounds__(256) void sum_slots_kernel(K3kSum a, unsigned t0, unsigned per)
 {
     const size_t t = t0 + blockIdx.x / per;
@@ -192,7 +192,8 @@ __global__ __launch_bounds__(256) void sum_slots_kernel(K3kSum a, unsigned t0, u
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (int j = 0; j < a.topk; j += 4) {
         float v[4][8], w[4];
-        i16x8 h[4];
+        f16x8 h[4];
+        float sc[4];
         bool on[4];
 #pragma unroll
         for (int u = 0; u < 4; u++) {
@@ -200,16 +201,16 @@ __global__ __launch_bounds__(256) void sum_slots_kernel(K3kSum a, unsigned t0, u
             on[u] = j + u < a.topk && (unsigned)a.idx[k] < (unsigned)a.n_experts;
             w[u] = a.wt[k];
             if (!on[u]) continue;
-            if constexpr (INTS) {
-                h[u] = *(const i16x8 *)((const int16_t *)a.y + k * a.ldy + i);
-                w[u] *= a.ys[k * (a.ldy / 64) + i / 64];
+            if constexpr (HALVES) {
+                h[u] = *(const f16x8 *)((const _Float16 *)a.y + k * a.ldy + i);
+                sc[u] = a.ys[k * (a.ldy / 64) + i / 64];
             } else load8<K3D_F32>(v[u], (const float *)a.y + k * a.ldy, i, a.n);
         }
 #pragma unroll
         for (int u = 0; u < 4; u++)
             if (on[u])
 #pragma unroll
-                for (int c = 0; c < 8; c++) s[c] = fmaf(w[u], INTS ? (float)h[u][c] : v[u][c], s[c]);
+                for (int c = 0; c < 8; c++) s[c] = fmaf(w[u], HALVES ? (float)h[u][c] * sc[u] : v[u][c], s[c]);
     }
     store8_of(a.out, a.out_type, t * a.ldo, i, a.n, s);
 }

@@ -411,7 +411,7 @@ typedef struct {
     void *ws;
     int wide;                   /* products as exact as fp32 (else 8-bit instructions) */
     const int *slot_e;          /* in place of offsets, few rows: row r's expert (none outside [0, n_experts)), its row of x r / x_div, of y r */
-    float *ys;                  /* k3k_slots_f8: y is 16-bit integers, whole groups of 64 columns, these their scales [T][ldy / 64] */
+    float *ys;                  /* k3k_slots_f8: y is 16-bit floats, whole groups of 64 columns, these their scales [T][ldy / 64] */
     /* k3k_gateup_f8 */
     const uint8_t *W2;
     const float *Ws2;
@@ -425,8 +425,8 @@ int k3k_f8_tile(uint8_t *t, const uint8_t *W, long ldw, int rows, int in, int ma
 size_t k3k_linear_f8_ws(int T, int in, int out);
 int k3k_linear_f8(const K3kF8 *a, void *stream);
 int k3k_grouped_f8(const K3kF8 *a, void *stream);
-/* k3k_grouped_f8 into fp32 or, where the rows are many and `wide` is not asked for, into 16-bit integers and scales (ys) that take half the bytes:
- * what k3k_sum_slots reads. y: 4 bytes for each of [T][columns up to 64]; *ys is set to where the scales lie behind the integers, NULL for fp32. */
+/* k3k_grouped_f8 into fp32 or, where the rows are many and `wide` is not asked for, into 16-bit floats and scales (ys) that take half the bytes:
+ * what k3k_sum_slots reads. y: 4 bytes for each of [T][columns up to 64]; *ys is set to where the scales lie behind them, NULL for fp32. */
 int k3k_slots_f8(const K3kF8 *a, float **ys, void *stream);
 /* act(W x) (W2 x) of sorted rows in 8 bits; gu: [rows][2 out] of scratch. */
 int k3k_gateup_f8(const K3kF8 *a, float *gu, void *stream);
@@ -438,7 +438,7 @@ int k3k_group(int *offsets, int *perm, const int *idx, int N, int n_experts, int
 /* out[t] = sum_j wt[t][j] y[t * topk + j], j ascending, over slots with 0 <= idx < n_experts; out of out_type. */
 typedef struct {
     void *out;
-    const void *y;              /* [T * topk][ldy]: fp32, or with ys 16-bit integers, a scale to 64 columns */
+    const void *y;              /* [T * topk][ldy]: fp32, or with ys 16-bit floats, a scale to 64 columns */
     const float *ys;
     const float *wt;
     const int *idx;
