@@ -325,8 +325,9 @@ int k3d_grouped_f8(void *y, int y_type, long ldy, const int *y_rows, int y_cap, 
                    const uint8_t *W, const float *Ws, int in, int out, void *stream);
 
 /* The experts' layer for a routing in idx/wt [T][topk] (k3d_route's), weights in 8 bits: out[t] = sum_j wt[t][j] W2_e (act(W1_e x[t]) * (W3_e x[t])),
- * e = idx[t][j], act and b1, b2 as in k3d_quant_f8. The gated activation goes through 8 bits as k3d_quant_f8 rounds it; gate and up, and
- * with out_type K3D_BF16 the down products, are formed by 8-bit instructions, as k3d_linear_f8's of bf16 are; many tokens' down products for a bf16 out
+ * e = idx[t][j], act and b1, b2 as in k3d_quant_f8. The gated activation goes through 8 bits as k3d_quant_f8 rounds it. With out_type K3D_F32 every product is
+ * formed as k3d_linear_f8's of fp32 are. With K3D_BF16 the down products are formed by 8-bit instructions, as k3d_linear_f8's of bf16 are, and so are gate and up where the experts have more than
+ * about 10 rows each (16 of hidden >= 4096): some of their codes fall a step aside there, 1.1e-3 of the result beside the 1.7e-3 of its rounding; and many tokens' down products
  * wait for their sum as 16-bit floats with a power of two for each 64 columns (within 2^-11 of the value, or 2^-39 of the largest of them). The weighted sum
  * is fp32, rounded once to out_type. Slots whose idx lies outside [0, n_experts) contribute nothing; a token without any becomes 0. w1, w3 [n_experts] matrices [inter][hidden], w2
  * [hidden][inter] from k3d_f8_tile, s1, s3, s2 their scales as in k3d_grouped_f8. ws (k3d_moe_f8_ws bytes; 16-byte aligned) is scratch of one call. */

@@ -7,9 +7,9 @@
  * A block's 128 columns are one 8-bit matrix instruction (16 x 16 x 128), so each instruction starts from zero and its sums enter the
  * fp32 accumulators through one multiplication by the two scales' product: four vector FMAs to 32 cycles of the matrix cores. The
  * 8-bit instructions (all shapes of them alike, as measured) add each 8 neighbouring products after aligning them to the largest's exponent, and what is more
- * than 13 bits below that is cut off: 1.5 * 2^-16 of a sum of random products. That is far under the rounding of a bf16 result or of the next 8-bit
- * row, but not of an fp32 one; those products (WIDE) are formed by the bf16 instruction out of the codes widened to bf16 (exactly),
- * at half the rate.
+ * than 13 bits below that is cut off: 1.5 * 2^-16 of a sum of random products. That is far under the rounding of a bf16 result, but not of an fp32 one,
+ * nor harmless in front of 8-bit codes, which it turns (k3k_gateup_f8); those products (WIDE) are formed by the bf16 instruction out of the codes
+ * widened to bf16 (exactly), at half the rate.
  *
  * W is laid out once, by k3d_f8_tile: tiles of 16 rows x 128 columns in the operand's own order, 2 KB, F8_G row tiles side by side,
  * column block after column block, zeros where rows or columns end. So every load of W is contiguous at any size.
@@ -1085,11 +1085,15 @@ extern "C" int k3k_slots_f8(const K3kF8 *a, float **ys, void *stream)
     return k3k_grouped_f8(&s, stream);
 }
 
-/* gate and up: W, W2 [experts], into hq / hs; gu: room for their sums, where few rows make them a launch of their own */
+/* Gate and up: W, W2 [experts], into hq / hs; gu: room for their sums where they are formed as fp32 first. A code is a choice: what a sum's cut turns
+ * is a whole step of it. So the 8-bit instructions' cut (2e-5 of a sum) shows as 1.1e-3 of the layer's result, and they are for many rows alone, where they
+ * halve the time, and for a result that is rounded to bf16 (1.7e-3) anyway. Few rows wait for W: exact products cost
+ * them nothing (one token on 8 of 64 experts 69.7 us, 70.1 cut; its error 1.66e-3 as bf16's own, 2.12e-3 cut). An fp32 result of 2048 tokens takes 2003 us, 1497 cut. */
 extern "C" int k3k_gateup_f8(const K3kF8 *a, float *gu, void *stream_)
 {
     hipStream_t st = (hipStream_t)stream_;
-    if (!few_rows(a)) {
+    const bool few = few_rows(a);
+    if (!few && !a->wide) {
         F8Tile p;
         p.a = *a;
         p.part = NULL;
@@ -1101,7 +1105,15 @@ extern "C" int k3k_gateup_f8(const K3kF8 *a, float *gu, void *stream_)
     s.y = gu;
     s.ldy = 2L * a->out;
     s.T = a->rows;
+    s.wide = 1;
+    if (!few) s.W2 = NULL;              /* (tiles have one matrix to a launch) */
     if (k3k_grouped_f8(&s, stream_)) return -1;
+    if (!few) {
+        s.W = a->W2;
+        s.Ws = a->Ws2;
+        s.y = gu + a->out;
+        if (k3k_grouped_f8(&s, stream_)) return -1;
+    }
     K3kQuant q = {a->hq, a->hs, gu, blocks(a->out) * 128L, blocks(a->out), 2L * a->out, K3D_F32, a->rows, a->out, a->glu, a->b1, a->b2};
     return k3k_quant_f8(&q, stream_);
 }

@@ -405,14 +405,13 @@ int k3d_moe_f8(void *out, int out_type, long ldo, const int *idx, const float *w
     a.glu = act;
     a.b1 = b1;
     a.b2 = b2;
+    a.wide = out_type == K3D_F32;
     if (k3k_gateup_f8(&a, w.gu, stream)) return fail(fn);
     k3k_prof_mark(stream, K3D_STAGE_GATEUP);
     a.y = w.y;
     a.x = w.hq;
     a.W = w2;
     a.W2 = NULL;
-    /* (a result of bf16 has no use for more than 8-bit instructions give) */
-    a.wide = out_type == K3D_F32;
     a.xs = w.hs;
     a.Ws = s2;
     a.x_rows = NULL;

@@ -428,7 +428,7 @@ int k3k_grouped_f8(const K3kF8 *a, void *stream);
 /* k3k_grouped_f8 into fp32 or, where the rows are many and `wide` is not asked for, into 16-bit floats and scales (ys) that take half the bytes:
  * what k3k_sum_slots reads. y: 4 bytes for each of [T][columns up to 64]; *ys is set to where the scales lie behind them, NULL for fp32. */
 int k3k_slots_f8(const K3kF8 *a, float **ys, void *stream);
-/* act(W x) (W2 x) of sorted rows in 8 bits; gu: [rows][2 out] of scratch. */
+/* act(W x) (W2 x) of sorted rows in 8 bits, W x and W2 x as exact as fp32 where `wide` or few rows ask for it; gu: [rows][2 out] of scratch. */
 int k3k_gateup_f8(const K3kF8 *a, float *gu, void *stream);
 
 /* The slots of idx [N] by expert (k3_group.hip; up to 2048 experts); hist: k3k_group_ws bytes. */

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from layer8_ops import (BF16, F8, HALF, LEAST, SILU, SITU, acts, codes_of, f64, group, grouped, moe8, nb, quant, tile, weights)
+from layer8_ops import (BF16, F32, F8, HALF, LEAST, SILU, SITU, acts, codes_of, f64, group, grouped, moe8, nb, quant, tile, weights)
 from layer_ops import gen
 
 pytestmark = pytest.mark.gpu
@@ -78,6 +78,26 @@ def check(c, out, out_type, sixteen):
     tol = 1.001 * (tol + (np.abs(want) + tol) * HALF[out_type])
     off = np.abs(f64(out) - want)
     assert (off <= tol).all(), (float((off / np.maximum(tol, 1e-300)).max()), int((off > tol).sum()), off.size)
+
+
+FEW = [(1, 4, 6, 1024, 256), (1, 8, 64, 584, 384), (3, 4, 6, 1024, 256), (12, 4, 6, 1001, 200), (20, 4, 6, 4224, 256)]
+MANY = [(70, 4, 6, 584, 384), (400, 4, 6, 1160, 328), (300, 2, 3, 256, 129)]
+
+
+@pytest.mark.parametrize("T,k,experts,hidden,inter", FEW + MANY)
+@pytest.mark.parametrize("act", [SILU, SITU])
+def test_fp32(gpu, T, k, experts, hidden, inter, act):
+    """An fp32 result: every product as exact as fp32, at any number of rows."""
+    c = Case(gpu, T, k, experts, hidden, inter, act, False)
+    check(c, c.layer(F32), F32, False)
+
+
+@pytest.mark.parametrize("T,k,experts,hidden,inter", FEW)
+@pytest.mark.parametrize("act", [SILU, SITU])
+def test_bf16_few_rows(gpu, T, k, experts, hidden, inter, act):
+    """A bf16 result of few rows an expert: gate and up as exact as fp32."""
+    c = Case(gpu, T, k, experts, hidden, inter, act, False)
+    check(c, c.layer(BF16), BF16, T * k > 10 * experts)
 
 
 def counted(counts, k, g):
