@@ -315,14 +315,15 @@ typedef struct {
     void *y;
 } MoeF8Ws;
 
-/* where each part lies in ws; the bytes of all (256-byte aligned parts) */
+/* where each part lies in ws; the bytes of all (256-byte aligned parts). gu (gate and up as fp32, where they do not become codes at once) is done with
+ * before y (the slots' rows) begins: one place. */
 static size_t moe_layout(MoeF8Ws *w, void *ws, int T, int hidden, int inter, int n_experts, int topk)
 {
     const size_t N = (size_t)T * topk, nb = blocks(inter), wide = ((size_t)hidden + 63) / 64 * 64;
-    const size_t sizes[7] = {((size_t)n_experts + 1) * 4, N * 4, k3k_group_ws((int)N, n_experts), N * nb * 128, N * nb * 4,
-                             N * 2 * inter * 4, N * wide * 4};
-    size_t off = 0, at[7];
-    for (int i = 0; i < 7; i++) {
+    const size_t gu = N * 2 * inter * 4, y = N * wide * 4;
+    const size_t sizes[6] = {((size_t)n_experts + 1) * 4, N * 4, k3k_group_ws((int)N, n_experts), N * nb * 128, N * nb * 4, gu > y ? gu : y};
+    size_t off = 0, at[6];
+    for (int i = 0; i < 6; i++) {
         at[i] = off;
         off += (sizes[i] + 255) / 256 * 256;
     }
@@ -334,7 +335,7 @@ static size_t moe_layout(MoeF8Ws *w, void *ws, int T, int hidden, int inter, int
         w->hq = (uint8_t *)(b + at[3]);
         w->hs = (float *)(b + at[4]);
         w->gu = (float *)(b + at[5]);
-        w->y = b + at[6];
+        w->y = w->gu;
     }
     return off;
 }

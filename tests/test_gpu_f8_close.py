@@ -136,3 +136,16 @@ def test_outputs_apart(gpu):
         else:
             assert not torch.isfinite(y[:, 70]).any()
             assert torch.equal(y[:, 128:], clean[:, 128:])
+
+
+@pytest.mark.parametrize("T,k,experts,hidden,inter", [(1, 4, 6, 584, 384), (7, 4, 6, 100, 500), (300, 2, 5, 200, 129), (700, 8, 9, 129, 200)])
+@pytest.mark.parametrize("out_type", [F32, BF16])
+def test_workspace(gpu, T, k, experts, hidden, inter, out_type):
+    """The layer stays within its workspace, and takes nothing of what lay there."""
+    c = Case(gpu, T, k, experts, hidden, inter, SILU, False)
+    need = gpu.lib().k3d_moe_f8_ws(T, hidden, inter, experts, k)
+    want = c.layer(out_type)
+    for fill in (0x00, 0xff, 0x7f):
+        ws = torch.full((need + 4096,), fill, device="cuda", dtype=torch.uint8)
+        assert torch.equal(moe8(gpu, c.x, c.xs, c.idx, c.wt, c.bank, hidden, inter, SILU, out_type=out_type, ws=ws[:need]), want)
+        assert (ws[need:] == fill).all()
