@@ -301,7 +301,7 @@ int k3d_f8_tile(uint8_t *t, const uint8_t *W, long ldw, int rows, int in, int ma
  * sums; for K3D_BF16 by 8-bit matrix instructions, which align each 8 neighbouring products to the largest of them and cut 13 bits below it (1.5 * 2^-16 of a
  * sum of random products, a 70th of what y's own rounding adds) and take half the time. The two scales' product is formed
  * in fp32, as are the sum over blocks, bias, activation and residual; one rounding to y_type. Which kernel runs, and with it the order of the
- * sum over blocks, goes by the shape; a call's bits repeat. ws (k3d_linear_f8_ws bytes, which hold any fewer tokens too; 16-byte aligned) is
+ * sum over blocks, goes by the shape; a call's bits repeat. ws (k3d_linear_f8_ws bytes, which hold any fewer tokens too, none up to 64; 16-byte aligned) is
  * scratch of one call: calls and graphs that may run at the same time need one each. y must not overlap an operand, nor res unless
  * it is y itself. */
 size_t k3d_linear_f8_ws(int T, int in, int out);

@@ -898,6 +898,7 @@ __global__ __launch_bounds__(64) void f8_join_kernel(K3kF8 a, const float *part,
 }
 
 /* ---- launches -------------------------------------------------------------------------------- */
+constexpr int F8_FEW = 64;              /* rows of a dense product that f8_skinny_kernel takes, without slices */
 constexpr int F8_MAX_SLICES = 16;
 constexpr size_t F8_PART_CAP = (size_t)64 << 20;
 
@@ -1010,13 +1011,13 @@ extern "C" int k3k_f8_tile(uint8_t *t, const uint8_t *W, long ldw, int rows, int
 extern "C" size_t k3k_linear_f8_ws(int T, int in, int out)
 {
     (void)in;
-    return part_bytes(T, out);
+    return T <= F8_FEW ? 0 : part_bytes(T, out);
 }
 
 extern "C" int k3k_linear_f8(const K3kF8 *a, void *stream_)
 {
     hipStream_t st = (hipStream_t)stream_;
-    if (a->T <= 64) {
+    if (a->T <= F8_FEW) {
         skinny(a, a->T, st);
         K3K_LAUNCH_CHECK("linear_f8: few rows");
         return 0;

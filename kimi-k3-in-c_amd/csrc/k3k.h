@@ -422,7 +422,7 @@ typedef struct {
 } K3kF8;
 size_t k3k_f8_tiled_bytes(int rows, int in);
 int k3k_f8_tile(uint8_t *t, const uint8_t *W, long ldw, int rows, int in, int mats, void *stream);
-size_t k3k_linear_f8_ws(int T, int in, int out);
+size_t k3k_linear_f8_ws(int T, int in, int out);        /* (0: no use of ws) */
 int k3k_linear_f8(const K3kF8 *a, void *stream);
 int k3k_grouped_f8(const K3kF8 *a, void *stream);
 /* k3k_grouped_f8 into fp32 or, where the rows are many and `wide` is not asked for, into 16-bit floats and scales (ys) that take half the bytes:

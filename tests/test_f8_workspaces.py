@@ -15,3 +15,11 @@ def test_moe(k3, T, hidden, inter, experts, topk):
     parts = [(experts + 1) * 4, N * 4, L.k3d_group_ws(T, topk, experts), N * up(inter, 128), N * up(inter, 128) // 32,
              N * max(2 * inter, up(hidden, 64)) * 4]
     assert L.k3d_moe_f8_ws(T, hidden, inter, experts, topk) == sum(up(p, 256) for p in parts)
+
+
+def test_linear(k3):
+    """Up to 64 tokens a dense product has no sums of slices."""
+    L = k3.lib()
+    for inn, out in ((7168, 12288), (128, 16), (1 << 20, 1 << 18)):
+        assert all(L.k3d_linear_f8_ws(T, inn, out) == 0 for T in (1, 16, 17, 63, 64))
+        assert L.k3d_linear_f8_ws(65, inn, out) > 0
