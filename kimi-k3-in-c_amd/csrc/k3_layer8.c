@@ -26,6 +26,15 @@ static size_t type_size(int t) { return t == K3D_F32 ? 4 : 2; }
 static int aligned(const void *p, size_t n) { return ((uintptr_t)p % n) == 0; }
 static int blocks(int n) { return (n + 127) / 128; }
 
+/* p is one of the n places at q (none is no place) */
+static int among(const void *p, const void *const *q, size_t n)
+{
+    for (size_t i = 0; p && i < n; i++)
+        if (p == q[i]) return 1;
+    return 0;
+}
+#define AMONG(p, ...) among(p, (const void *const[]){__VA_ARGS__}, sizeof((const void *const[]){__VA_ARGS__}) / sizeof(void *))
+
 /* 8-bit rows of n columns and their scales: NULL, or what is wrong with them */
 static const char *rows_bad(const void *q, long ldq, const void *s, long lds, int n)
 {
@@ -69,8 +78,8 @@ int k3d_add_norm(void *y, int y_type, long ldy, uint8_t *q, long ldq, float *qs,
     if (sum && sum == x && (ldsum != ldx || r_type != x_type)) return refuse(fn, "sum in x's place needs its stride and type");
     if (y && y == x && (ldy != ldx || y_type != x_type)) return refuse(fn, "y in x's place needs its stride and type");
     if (y && y == res && (ldy != ldr || y_type != r_type)) return refuse(fn, "y in res's place needs its stride and type");
-    if ((y && (y == sum || y == (void *)q)) || (sum && sum == (void *)q)) return refuse(fn, "two outputs are one place");
-    if ((q && ((void *)q == x || (void *)q == res))) return refuse(fn, "codes lie in an operand's place");
+    if (AMONG(y, sum, q) || AMONG(sum, q) || (q && AMONG(qs, y, sum, q))) return refuse(fn, "two outputs are one place");
+    if (AMONG(q, x, res, w) || (q && AMONG(qs, x, res, w)) || AMONG(w, y, sum)) return refuse(fn, "an output lies in an operand's place");
     K3kNorm a;
     a.y = y;
     a.sum = sum;
@@ -113,7 +122,8 @@ int k3d_quant_f8(uint8_t *q, long ldq, float *qs, long ldqs, const void *x, int 
     if (!aligned(x, type_size(x_type))) return refuse(fn, "a pointer is not aligned to its elements");
     const char *bad = rows_bad(q, ldq, qs, ldqs, n);
     if (bad) return refuse(fn, bad);
-    if ((const void *)q == x) return refuse(fn, "codes lie in an operand's place");
+    if ((const void *)q == qs) return refuse(fn, "two outputs are one place");
+    if (AMONG(x, q, qs)) return refuse(fn, "an output lies in an operand's place");
     K3kQuant a;
     a.q = q;
     a.qs = qs;
@@ -191,8 +201,8 @@ int k3d_linear_f8(void *y, int y_type, long ldy, const uint8_t *x, long ldx, con
     const size_t need = k3k_linear_f8_ws(T, in, out);
     if (need && (!ws || ws_bytes < need)) return refuse(fn, "workspace too small");
     if (need && !aligned(ws, 16)) return refuse(fn, "the workspace must be 16-byte aligned");
-    if (y == (const void *)x || y == (const void *)xs || y == (const void *)W || y == (const void *)Ws || y == ws || y == (const void *)bias)
-        return refuse(fn, "y lies in an operand's place");
+    if (AMONG(y, x, xs, W, Ws, ws, bias)) return refuse(fn, "y lies in an operand's place");
+    if (need && AMONG(ws, x, xs, W, Ws, bias, res)) return refuse(fn, "the workspace lies in an operand's place");
     K3kF8 a;
     memset(&a, 0, sizeof a);
     a.y = y;
@@ -246,6 +256,7 @@ int k3d_group(int *offsets, int *perm, const int *idx, int T, int topk, int n_ex
     const size_t need = k3k_group_ws(T * topk, n_experts);
     if (need && (!ws || ws_bytes < need)) return refuse(fn, "workspace too small");
     if (need && !aligned(ws, 4)) return refuse(fn, "a pointer is not aligned to its elements");
+    if (need && AMONG(ws, offsets, perm, idx)) return refuse(fn, "the workspace lies in another argument's place");
     if (k3k_group(offsets, perm, idx, T * topk, n_experts, (int *)ws, stream)) return fail(fn);
     return 0;
 }
@@ -273,9 +284,7 @@ int k3d_grouped_f8(void *y, int y_type, long ldy, const int *y_rows, int y_cap, 
     if (!aligned(y, type_size(y_type)) || !aligned(Ws, 4) || !aligned(offsets, 4) || !aligned(x_rows, 4) || !aligned(y_rows, 4))
         return refuse(fn, "a pointer is not aligned to its elements");
     if (!aligned(W, 16)) return refuse(fn, "W must be 16-byte aligned");
-    if (y == (const void *)x || y == (const void *)xs || y == (const void *)W || y == (const void *)Ws || y == (const void *)offsets ||
-        y == (const void *)x_rows || y == (const void *)y_rows)
-        return refuse(fn, "y lies in an operand's place");
+    if (AMONG(y, x, xs, W, Ws, offsets, x_rows, y_rows)) return refuse(fn, "y lies in an operand's place");
     K3kF8 a;
     memset(&a, 0, sizeof a);
     a.y = y;
@@ -370,8 +379,8 @@ int k3d_moe_f8(void *out, int out_type, long ldo, const int *idx, const float *w
     MoeF8Ws w;
     if (!ws || ws_bytes < moe_layout(&w, ws, T, hidden, inter, n_experts, topk)) return refuse(fn, "workspace too small");
     if (!aligned(ws, 16)) return refuse(fn, "the workspace must be 16-byte aligned");
-    if (out == (const void *)x || out == ws || out == (const void *)wt || out == (const void *)idx || out == (const void *)xs)
-        return refuse(fn, "out lies in an operand's place");
+    if (AMONG(out, x, xs, wt, idx, w1, s1, w3, s3, w2, s2, ws)) return refuse(fn, "out lies in an operand's place");
+    if (AMONG(ws, x, xs, wt, idx, w1, s1, w3, s3, w2, s2)) return refuse(fn, "the workspace lies in an operand's place");
     const int N = T * topk, one = T == 1 && topk <= n_experts;
     k3k_prof_mark(stream, K3D_STAGE_BEGIN);
     /* (one token's slots are rows of experts of their own: no launch to sort them, and no offsets to search) */
