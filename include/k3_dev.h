@@ -277,14 +277,15 @@ enum { K3D_GLU_NONE = -1, K3D_GLU_SITU = 0, K3D_GLU_SILU = 1 };
  *   v = x[t][i] + res[t][i] (res may be NULL);  sum = v, rounded to r_type (sum may be NULL);
  *   u = v / sqrt(mean_i(v^2) + eps) * w[i]  (w fp32 or NULL for ones);  y = u, rounded to y_type (y may be NULL);
  *   q, qs (may be NULL): scale = max(max |u| over 128 columns, 2^-100) / 448, code = u / scale to nearest, ties to even.
- * All in fp32, v unrounded (the squares too: a row whose sum of them passes fp32's range becomes 0). x is of x_type, res and sum of r_type; res, sum and y at any alignment of
+ * All in fp32, v unrounded (the squares too: a row whose sum of them passes fp32's range becomes 0, and squares under 2^-126 lose bits, which an eps of 1e-37 or less
+ * does not hide: such a row's u is inexact, infinite where they vanish beside eps 0, and NaN where it is zeros). x is of x_type, res and sum of r_type; res, sum and y at any alignment of
  * their elements. sum may be res or x itself, y too (same type and stride). A NaN in a block of u makes its scale and codes NaN; an infinity the scale infinite. */
 int k3d_add_norm(void *y, int y_type, long ldy, uint8_t *q, long ldq, float *qs, long ldqs, void *sum, long ldsum,
                  const void *x, int x_type, long ldx, const void *res, int r_type, long ldr, int T, int n, const float *w,
                  float eps, void *stream);
 
 /* The rows of x in 8 bits (act K3D_GLU_NONE), or of act(gate) * up: row t of x is gate [n], then up [n]. Scales and codes as above;
- * the activation in fp32. b1, b2 from 2^-64 to 2^64 for K3D_GLU_SITU. */
+ * the activation in fp32; behind one a code is the nearest to u times the scale's rounded reciprocal, within 2^-23 of u / scale. b1, b2 from 2^-64 to 2^64 for K3D_GLU_SITU. */
 int k3d_quant_f8(uint8_t *q, long ldq, float *qs, long ldqs, const void *x, int x_type, long ldx, int T, int n, int act,
                  float b1, float b2, void *stream);
 
@@ -319,7 +320,8 @@ int k3d_group(int *offsets, int *perm, const int *idx, int T, int topk, int n_ex
  *   y[Y(r)][o] = sum_b xs[X(r)][b] Ws[e][o / 128][b] p[..],  X(r) = x_rows ? x_rows[r] / x_div : r,  Y(r) = y_rows ? y_rows[r] : r.
  * with p as in k3d_linear_f8, by y_type too. W: n_experts matrices [out][in] from k3d_f8_tile, Ws [n_experts][ceil(out / 128)][ceil(in / 128)]. With k3d_group's perm as x_rows and x_div = topk a
  * row takes its token of x; as y_rows it returns to its slot. x has x_cap rows, y y_cap; a row with X(r) or Y(r) outside them is left as it was,
- * and so is every row of y that no r has. No Y(r) may come twice. Experts without rows cost nothing; offsets that fall or leave [0, rows] count as no rows there. */
+ * and so is every row of y that no r has. No Y(r) may come twice. Experts without rows cost nothing; an expert's end past `rows` counts as `rows`, and one whose offsets fall,
+ * or begin below 0, has none. */
 int k3d_grouped_f8(void *y, int y_type, long ldy, const int *y_rows, int y_cap, const uint8_t *x, long ldx, const float *xs,
                    long ldxs, const int *x_rows, int x_div, int x_cap, const int *offsets, int rows, int n_experts,
                    const uint8_t *W, const float *Ws, int in, int out, void *stream);

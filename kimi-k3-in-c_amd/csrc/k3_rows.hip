@@ -51,7 +51,8 @@ __device__ __forceinline__ void load8_of(float (&f)[8], const void *p, int type,
     else load8<K3D_BF16>(f, (const uint16_t *)p + row, i, n);
 }
 
-/* NT: not to be read again soon */
+/* NT: not to be read again soon (rows of bf16; the sum of 4096 rows of 7168 41.0 against 46.2 us, of 1024 11.6 against 12.7, the same up to 256 and in fp32;
+ * where the next call reads it at once 4096 take 39.9 against 36.9) */
 template <bool NT = false>
 __device__ __forceinline__ void store8_of(void *p, int type, size_t row, int i, int n, const float (&f)[8])
 {
