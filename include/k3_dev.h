@@ -278,7 +278,7 @@ enum { K3D_GLU_NONE = -1, K3D_GLU_SITU = 0, K3D_GLU_SILU = 1 };
  *   u = v / sqrt(mean_i(v^2) + eps) * w[i]  (w fp32 or NULL for ones);  y = u, rounded to y_type (y may be NULL);
  *   q, qs (may be NULL): scale = max(max |u| over 128 columns, 2^-100) / 448, code = u / scale to nearest, ties to even.
  * All in fp32, v unrounded (the squares too: a row whose sum of them passes fp32's range becomes 0, and squares under 2^-126 lose bits, which an eps of 1e-37 or less
- * does not hide: such a row's u is inexact, infinite where they vanish beside eps 0, and NaN where it is zeros). x is of x_type, res and sum of r_type; res, sum and y at any alignment of
+ * does not hide: such a row's u is inexact, and NaN where all of them vanish beside an eps of 0, as of a row of zeros). x is of x_type, res and sum of r_type; res, sum and y at any alignment of
  * their elements. sum may be res or x itself, y too (same type and stride). A NaN in a block of u makes its scale and codes NaN; an infinity the scale infinite. */
 int k3d_add_norm(void *y, int y_type, long ldy, uint8_t *q, long ldq, float *qs, long ldqs, void *sum, long ldsum,
                  const void *x, int x_type, long ldx, const void *res, int r_type, long ldr, int T, int n, const float *w,

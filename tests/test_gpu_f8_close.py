@@ -1,6 +1,8 @@
 # SPDX-License-Identifier: Apache-2.0
 """k3d_moe_f8 held closely: its gated activation is k3d_quant_f8's of k3d_grouped_f8's fp32 products, code for code, and behind it only
 the down products' and the result's own roundings are left."""
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
@@ -149,3 +151,49 @@ def test_workspace(gpu, T, k, experts, hidden, inter, out_type):
         ws = torch.full((need + 4096,), fill, device="cuda", dtype=torch.uint8)
         assert torch.equal(moe8(gpu, c.x, c.xs, c.idx, c.wt, c.bank, hidden, inter, SILU, out_type=out_type, ws=ws[:need]), want)
         assert (ws[need:] == fill).all()
+
+
+@pytest.mark.parametrize("T", [5, 300])
+@pytest.mark.parametrize("out_type", [F32, BF16])
+def test_captured(gpu, k3, T, out_type):
+    """Captured once, replayed on other inputs and over other tensors' old values, beside eager calls."""
+    L, k, experts, hidden, inter = k3.lib(), 4, 6, 584, 384
+    c = Case(gpu, T, k, experts, hidden, inter, SITU, False)
+    others = [Case(gpu, T, k, experts, hidden, inter, SITU, True), c]
+    keep = [(o.x.clone(), o.xs.clone(), o.idx.clone(), o.wt.clone()) for o in others]
+    ws = torch.full((L.k3d_moe_f8_ws(T, hidden, inter, experts, k),), 0xff, device="cuda", dtype=torch.uint8)
+    out = torch.full((T, hidden), float("nan"), device="cuda", dtype=out_type)
+    run = lambda st=None: moe8(gpu, c.x, c.xs, c.idx, c.wt, c.bank, hidden, inter, SITU, out=out, st=st, ws=ws)    # noqa: E731
+    ex = C.c_void_p()
+    torch.cuda.synchronize()
+    st = L.k3d_stream_create()
+    try:
+        k3.check(L.k3d_graph_begin(st))
+        run(st)
+        k3.check(L.k3d_graph_end(st, C.byref(ex)))
+        for r in range(5):
+            for t, v in zip((c.x, c.xs, c.idx, c.wt), keep[r % 2]):
+                t.copy_(v)
+            want = run().clone()
+            ws.fill_(0xff)
+            out.fill_(float("nan"))
+            torch.cuda.synchronize()
+            k3.check(L.k3d_graph_launch(ex, st))
+            k3.check(L.k3d_sync(st))
+            assert torch.equal(out, want), r
+    finally:
+        torch.cuda.synchronize()
+        if ex:
+            L.k3d_graph_destroy(ex)
+        L.k3d_stream_destroy(st)
+
+
+@pytest.mark.parametrize("out_type", [F32, BF16])
+def test_past_32_bits(gpu, out_type):
+    """Slots' rows that lie more than 2^32 bytes from the first: copies of 64 tokens, whose results are one another's."""
+    c, copies = Case(gpu, 64, 8, 16, 8192, 128, SILU, True), 520
+    big = [t.repeat(copies, 1) for t in (c.x, c.xs, c.idx, c.wt)]
+    assert 64 * copies * 8 * 8192 * 2 > 1 << 32
+    out = moe8(gpu, *big, c.bank, 8192, 128, SILU, out_type=out_type).view(copies, 64, 8192)
+    check(c, out[0], out_type, out_type == BF16)
+    assert torch.equal(out, out[:1].expand_as(out))
